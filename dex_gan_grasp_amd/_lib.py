@@ -16,6 +16,9 @@ _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.environ.get("DGG_LIB", os.path.join(_HERE, "libdgg.so"))  # DGG_LIB: diagnostic builds only
 
 NET_GEN, NET_DISC, NET_EVA = 0, 1, 2
+F32, BF16, F16 = 0, 1, 2
+ACT_NONE, ACT_LEAKY_RELU, ACT_SILU = 0, 1, 2
+MUON_SPECTRAL, MUON_MATCH_RMS = 0, 1
 TRAIN, ACCUM_GRADS, SKIP_PARAM_GRADS, NEED_INPUT_GRADS = 1, 2, 4, 8
 # loss slots (include/dgg.h)
 L_TOTAL_DISC, L_BCE_REAL, L_BCE_FAKE, L_GEN_FAKE, L_TRANSL, L_ROT, L_CONF, L_TOTAL_GEN, L_TOTAL_EVA, L_BCE_EVA = range(10)
@@ -34,6 +37,13 @@ class Cfg(C.Structure):
 class Entry(C.Structure):
     _fields_ = [("name", C.c_char * 64), ("offset", C.c_int64), ("rows", C.c_int32), ("cols", C.c_int32),
                 ("kind", C.c_int32), ("pad_", C.c_int32)]
+
+
+class Matrix(C.Structure):
+    _fields_ = [("in_", C.c_void_p), ("out", C.c_void_p), ("momentum", C.c_void_p), ("batch", C.c_int64),
+                ("in_stride", C.c_int64), ("out_stride", C.c_int64), ("momentum_stride", C.c_int64), ("rows", C.c_int32),
+                ("cols", C.c_int32), ("ld_in", C.c_int32), ("ld_out", C.c_int32), ("ld_momentum", C.c_int32),
+                ("pad_", C.c_int32)]
 
 
 class HParams(C.Structure):
@@ -67,6 +77,11 @@ SIGNATURES = {
     "dgg_bps_encode_ws": (_I, [_VP, _I, _I, _VP, _I, _VP, _VP, _VP, _SZ, _VP]),
     "dgg_set_bps_algo": (_I, [_I]),
     "dgg_get_bps_algo": (_I, []),
+    "dgg_group_norm_workspace_bytes": (_I64, [_I64, _I64, _I, _I, _I, _I]),
+    "dgg_group_norm_act_forward": (_I, [_VP, _I64, _I64, _I64, _I64, _I, _I, _VP, _VP, _D, _I, _F, _I, _VP, _VP, _VP, _SZ,
+                                        _VP]),
+    "dgg_group_norm_act_backward": (_I, [_VP, _I64, _I64, _VP, _I64, _I64, _I64, _I64, _I, _I, _VP, _VP, _I, _F, _I, _VP,
+                                         _VP, _VP, _VP, _VP, _SZ, _VP]),
     "dgg_gen_forward": (_I, [_CFG, _VP, _VP, _VP, _SZ, _I, _U, _VP, _VP, _VP, _VP]),
     "dgg_gen_backward": (_I, [_CFG, _VP, _VP, _VP, _SZ, _I, _U, _VP, _VP, _VP, _VP, _VP, _VP]),
     "dgg_disc_forward": (_I, [_CFG, _VP, _VP, _VP, _SZ, _I, _U, _VP, _VP, _VP, _VP, _VP, _VP]),
@@ -77,6 +92,9 @@ SIGNATURES = {
     "dgg_ortho6d_backward": (_I, [_VP, _I, _I, _VP, _VP, _I, _VP]),
     "dgg_bce": (_I, [_VP, _VP, _F, _I, _F, _F, _VP, _VP, _VP]),
     "dgg_adam_l2": (_I, [_VP, _VP, _VP, _VP, _I64, _I, _D, _D, _D, _D, _D, _D, _VP]),
+    "dgg_orthogonalize_workspace_bytes": (_I64, [C.POINTER(Matrix), _I]),
+    "dgg_orthogonalize": (_I, [C.POINTER(Matrix), _I, _I, C.POINTER(_D), _I, _D, _VP, _SZ, _VP]),
+    "dgg_muon_step": (_I, [C.POINTER(Matrix), _I, _D, _D, _I, _D, _I, _D, C.POINTER(_D), _I, _D, _VP, _SZ, _VP]),
     "dgg_cgan_workspace_bytes": (_I64, [_CFG, _I]),
     "dgg_cgan_d_phase": (_I, [_CFG, C.POINTER(GanState), C.POINTER(HParams), _VP, _SZ, _I, _VP, _VP, _VP, _VP, _VP,
                               _VP, _VP]),

@@ -1,0 +1,731 @@
+// Group normalisation with an activation over channels-last data: x (N, S, C), S points (rows) of C channels per sample,
+// G groups of D = C / G channels.
+//   forward   mean, var over the S x D elements of (n, g);  xh = (x - mean) rstd;  z = w[c] xh + b[c];  y = act(z)
+//   backward  dz = dy act'(z);  dw[c] = sum_{n,s} dz xh;  db[c] = sum_{n,s} dz;
+//             dx = rstd (w dz - mean(w dz) - xh mean(w dz xh))          (means over the group)
+// act: none, LeakyReLU(slope) — the ResBlock's — or SiLU.
+//
+// Bound: HBM (2 E elements forward, 3 E backward), a few dozen vector instructions per 16 bytes beside it.
+//
+// Arithmetic.  Statistics are accumulated in 64 bits, and so is the pre-activation z = (x - mean) rstd w + b: its
+// SIGN decides which side of LeakyReLU's kink an element lies on, i.e. a factor 1 / slope in its gradient, and an fp32 z
+// would take the wrong side for every element within its rounding error of zero.  (64-bit vector instructions run at the
+// rate of the fp32 ones here; per element they are 4 to 6 of them.)  What follows the sign is fp32, rounded once to the output type.
+//
+// Two routes, chosen by gn_run:
+//  * "unit": a group's S x D elements fit the registers of at most one wave.  L = 2^k lanes own one (n, g): one read of x,
+//    mean and centred variance by lane shuffles, no LDS, no barrier.
+//  * "tile": a workgroup owns a range of the rows of one sample and a block of channels (a thread keeps ITS channels while
+//    it walks down the rows), leaves per-channel partial sums in the workspace, and a small launch merges them in a fixed
+//    order into the groups' statistics (and dw, db); a last launch applies them.  No atomics: results do not depend on the
+//    order in which workgroups run.
+#include <initializer_list>
+
+#include "dgg_internal.h"
+
+namespace dgg {
+namespace {
+
+constexpr int kGnThreads = 256;
+constexpr int kUnitItems = 8;   // vectors of a group one lane holds, at most
+
+template <typename T, int V> struct alignas(sizeof(T) * V) Vec { T e[V]; };
+
+template <typename T, int V> __device__ __forceinline__ void load_vec(const T* p, float (&v)[V]) {
+    const Vec<T, V> r = *reinterpret_cast<const Vec<T, V>*>(p);
+#pragma unroll
+    for (int i = 0; i < V; ++i) v[i] = (float)r.e[i];
+}
+template <typename T, int V> __device__ __forceinline__ void store_vec(T* p, const float (&v)[V]) {
+    Vec<T, V> r;
+#pragma unroll
+    for (int i = 0; i < V; ++i) r.e[i] = (T)v[i];   // the one rounding to the output type (nearest even)
+    *reinterpret_cast<Vec<T, V>*>(p) = r;
+}
+
+// act(z) and act'(z) of a 64-bit pre-activation
+__device__ __forceinline__ float act_value(double z, int act, float slope) {
+    const float zf = (float)z;
+    if (act == DGG_ACT_LEAKY_RELU) return z > 0.0 ? zf : zf * slope;
+    if (act == DGG_ACT_SILU) return zf / (1.f + expf(-zf));
+    return zf;
+}
+__device__ __forceinline__ float act_slope(double z, int act, float slope) {
+    if (act == DGG_ACT_LEAKY_RELU) return z > 0.0 ? 1.f : slope;
+    if (act == DGG_ACT_SILU) {
+        const float zf = (float)z, s = 1.f / (1.f + expf(-zf));
+        return s * (1.f + zf * (1.f - s));
+    }
+    return 1.f;
+}
+
+struct GnArgs {
+    const void* x;
+    const void* dy;
+    void* out;              // y (forward) or dx (backward), contiguous
+    const float* w;         // NULL: 1
+    const float* b;         // NULL: 0
+    double* stats;          // [N][G][2]: mean, rstd
+    double* part;           // tile: [N][chunks][C][2]; unit backward: float [rows of partials][C][2]
+    double* coef;           // tile backward: [N][G][2]: mean(w dz), mean(w dz xh)
+    float* dw;
+    float* db;
+    long long x_sn, x_ss, dy_sn, dy_ss;   // strides in elements; the channel stride is 1
+    long long N, S;
+    int C, G, D;
+    int act;
+    float slope;
+    double eps;
+    int chunks;             // tile: row ranges per sample
+    long long chunk_rows;
+    int tx;                 // tile: vectors of a row a workgroup covers
+    int lanes;              // unit: lanes per group
+    int blocks_g, blocks_n; // unit backward: grid
+};
+
+__device__ __forceinline__ double lane_sum(double v, int lanes) {
+    for (int o = lanes >> 1; o > 0; o >>= 1) v += __shfl_xor(v, o);
+    return v;
+}
+
+// ------------------------------------------------------------------------------------------------ unit route
+template <typename T, int V, int I>
+__global__ __launch_bounds__(kGnThreads) void gn_unit_fwd_kernel(GnArgs a) {
+    const int L = a.lanes, lane = threadIdx.x & (L - 1);
+    const long long u = ((long long)blockIdx.x * kGnThreads + threadIdx.x) / L;
+    if (u >= a.N * a.G) return;   // whole groups of L lanes leave together: the shuffles below stay inside a group
+    const unsigned n = (unsigned)u / (unsigned)a.G, g = (unsigned)u - n * (unsigned)a.G;
+    const int dv = a.D / V, nv = (int)a.S * dv;
+    const T* x = (const T*)a.x + (long long)n * a.x_sn + (long long)g * a.D;
+    float v[I][V];
+    double sum = 0.0;
+#pragma unroll
+    for (int i = 0; i < I; ++i) {
+        const int e = lane + i * L;
+        if (e < nv) {
+            const int s = e / dv;
+            load_vec<T, V>(x + (long long)s * a.x_ss + (e - s * dv) * V, v[i]);
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < I; ++i)
+        if (lane + i * L < nv)
+#pragma unroll
+            for (int k = 0; k < V; ++k) sum += (double)v[i][k];
+    const double count = (double)nv * V;
+    const double mean = lane_sum(sum, L) / count;   // (a constant group's mean is exact: z = bias there, not beside it)
+    double m2 = 0.0;
+#pragma unroll
+    for (int i = 0; i < I; ++i)
+        if (lane + i * L < nv)
+#pragma unroll
+            for (int k = 0; k < V; ++k) {
+                const double d = (double)v[i][k] - mean;
+                m2 = fma(d, d, m2);
+            }
+    const double rstd = 1.0 / sqrt(lane_sum(m2, L) / count + a.eps);
+    if (a.stats && lane == 0) {
+        a.stats[2 * u] = mean;
+        a.stats[2 * u + 1] = rstd;
+    }
+#pragma unroll
+    for (int i = 0; i < I; ++i) {
+        const int e = lane + i * L;
+        if (e >= nv) continue;
+        const int s = e / dv, c = (int)g * a.D + (e - s * dv) * V;
+        float y[V];
+#pragma unroll
+        for (int k = 0; k < V; ++k) {
+            const double sc = rstd * (a.w ? (double)a.w[c + k] : 1.0);
+            y[k] = act_value(fma((double)v[i][k] - mean, sc, a.b ? (double)a.b[c + k] : 0.0), a.act, a.slope);
+        }
+        store_vec<T, V>((T*)a.out + ((long long)n * a.S + s) * a.C + c, y);
+    }
+}
+
+// Backward for S = 1 (rows): a lane keeps its channels while it walks over the samples n, so that dw and db need no
+// exchange between lanes; every workgroup row leaves one partial (64-bit sums, stored as fp32) per channel.
+template <typename T, int V, int I>
+__global__ __launch_bounds__(kGnThreads) void gn_unit_bwd_kernel(GnArgs a) {
+    const int L = a.lanes, lane = threadIdx.x & (L - 1), slot = threadIdx.x / L, slots = kGnThreads / L;
+    const int per = a.G < slots ? slots / a.G : 1;             // samples side by side in a workgroup
+    const int g = a.G < slots ? slot % a.G : (int)(blockIdx.x % a.blocks_g) * slots + slot;
+    const int side = a.G < slots ? slot / a.G : 0;
+    if (side >= per || g >= a.G) return;
+    const int nb = (int)(blockIdx.x / a.blocks_g);
+    const int nv = a.D / V;
+    float w[I][V], b[I][V];
+    double dw[I][V], db[I][V];
+#pragma unroll
+    for (int i = 0; i < I; ++i)
+#pragma unroll
+        for (int k = 0; k < V; ++k) {
+            const int e = lane + i * L, c = g * a.D + e * V + k;
+            w[i][k] = a.w && e < nv ? a.w[c] : 1.f;
+            b[i][k] = a.b && e < nv ? a.b[c] : 0.f;
+            dw[i][k] = db[i][k] = 0.0;
+        }
+    const double inv = 1.0 / ((double)nv * V);
+    for (long long n = (long long)nb * per + side; n < a.N; n += (long long)a.blocks_n * per) {
+        const T* x = (const T*)a.x + n * a.x_sn + (long long)g * a.D;
+        const T* dy = (const T*)a.dy + n * a.dy_sn + (long long)g * a.D;
+        const double mean = a.stats[2 * (n * a.G + g)], rstd = a.stats[2 * (n * a.G + g) + 1];
+        float xv[I][V], dv[I][V];
+#pragma unroll
+        for (int i = 0; i < I; ++i) {
+            const int e = lane + i * L;
+            if (e < nv) {
+                load_vec<T, V>(x + e * V, xv[i]);
+                load_vec<T, V>(dy + e * V, dv[i]);
+            }
+        }
+        double s1 = 0.0, s2 = 0.0;
+#pragma unroll
+        for (int i = 0; i < I; ++i)
+            if (lane + i * L < nv)
+#pragma unroll
+                for (int k = 0; k < V; ++k) {
+                    const double xh = ((double)xv[i][k] - mean) * rstd;
+                    const double dz = (double)(dv[i][k] * act_slope(fma(xh, (double)w[i][k], (double)b[i][k]), a.act, a.slope));
+                    dw[i][k] = fma(dz, xh, dw[i][k]);
+                    db[i][k] += dz;
+                    const double wd = dz * w[i][k];
+                    s1 += wd;
+                    s2 = fma(wd, xh, s2);
+                    xv[i][k] = (float)xh;
+                    dv[i][k] = (float)wd;
+                }
+        const double m1 = lane_sum(s1, L) * inv, m2 = lane_sum(s2, L) * inv;
+        const float f1 = (float)m1, f2 = (float)m2, fr = (float)rstd;
+#pragma unroll
+        for (int i = 0; i < I; ++i) {
+            const int e = lane + i * L;
+            if (e >= nv) continue;
+            float o[V];
+#pragma unroll
+            for (int k = 0; k < V; ++k) o[k] = fr * (dv[i][k] - f1 - xv[i][k] * f2);
+            store_vec<T, V>((T*)a.out + n * a.C + g * a.D + e * V, o);
+        }
+    }
+    if (!a.part) return;
+    float* p = (float*)a.part + 2ll * a.C * ((long long)nb * per + side);
+#pragma unroll
+    for (int i = 0; i < I; ++i) {
+        const int e = lane + i * L;
+        if (e < nv)
+#pragma unroll
+            for (int k = 0; k < V; ++k) {
+                p[2 * (g * a.D + e * V + k)] = (float)dw[i][k];
+                p[2 * (g * a.D + e * V + k) + 1] = (float)db[i][k];
+            }
+    }
+}
+
+// ------------------------------------------------------------------------------------------------ tile route
+// thread -> (vector of the row, row): tx vectors side by side, 256 / tx rows at a time; threads left over idle
+struct Tile { int vx, ty, rows; bool on; };
+__device__ __forceinline__ Tile tile_of(const GnArgs& a, int vecs, int by) {
+    Tile t;
+    t.rows = kGnThreads / a.tx;
+    t.ty = threadIdx.x / a.tx;
+    t.vx = by * a.tx + (int)threadIdx.x - t.ty * a.tx;
+    t.on = t.ty < t.rows && t.vx < vecs;
+    return t;
+}
+
+// sums a per-thread (p, q)[V] over the workgroup's rows in a fixed order; row 0 of each column holds the result
+template <int V> __device__ __forceinline__ void column_sum(double (&p)[V], double (&q)[V], const GnArgs& a, const Tile& t) {
+    __shared__ double sh[kGnThreads * 2];
+    for (int k = 0; k < V; ++k) {
+        __syncthreads();
+        sh[2 * threadIdx.x] = p[k];
+        sh[2 * threadIdx.x + 1] = q[k];
+        __syncthreads();
+        if (t.on && t.ty == 0) {
+            double s = 0.0, r = 0.0;
+            for (int y = 0; y < t.rows; ++y) {
+                s += sh[2 * (y * a.tx + threadIdx.x)];
+                r += sh[2 * (y * a.tx + threadIdx.x) + 1];
+            }
+            p[k] = s;
+            q[k] = r;
+        }
+    }
+}
+
+// per channel: sums of (x - k) and (x - k)^2 over a range of rows, k = the sample's first row: a shift that keeps the
+// variance of data far from zero, removed again by gn_stats_kernel
+template <typename T, int V>
+__global__ __launch_bounds__(kGnThreads) void gn_tile_sum_kernel(GnArgs a) {
+    const unsigned n = blockIdx.x / (unsigned)a.chunks, ch = blockIdx.x - n * (unsigned)a.chunks;
+    const Tile t = tile_of(a, a.C / V, blockIdx.y);
+    double p[V], q[V];
+#pragma unroll
+    for (int k = 0; k < V; ++k) p[k] = q[k] = 0.0;
+    if (t.on) {
+        const T* x = (const T*)a.x + (long long)n * a.x_sn + t.vx * V;
+        const long long s0 = (long long)ch * a.chunk_rows, s1 = s0 + a.chunk_rows < a.S ? s0 + a.chunk_rows : a.S;
+        float piv[V];
+        load_vec<T, V>(x, piv);
+        for (long long s = s0 + t.ty; s < s1; s += t.rows) {
+            float v[V];
+            load_vec<T, V>(x + s * a.x_ss, v);
+#pragma unroll
+            for (int k = 0; k < V; ++k) {
+                const double d = (double)v[k] - (double)piv[k];
+                p[k] += d;
+                q[k] = fma(d, d, q[k]);
+            }
+        }
+    }
+    column_sum<V>(p, q, a, t);
+    if (t.on && t.ty == 0)
+#pragma unroll
+        for (int k = 0; k < V; ++k) {
+            double* o = a.part + 2ll * ((long long)blockIdx.x * a.C + t.vx * V + k);
+            o[0] = p[k];
+            o[1] = q[k];
+        }
+}
+
+// sum of v over the workgroup, in a fixed order, for every thread
+__device__ __forceinline__ double block_sum(double v, double* sh /* kGnThreads / 64 */) {
+    v = lane_sum(v, 64);
+    __syncthreads();
+    if ((threadIdx.x & 63) == 0) sh[threadIdx.x >> 6] = v;
+    __syncthreads();
+    double s = 0.0;
+#pragma unroll
+    for (int i = 0; i < kGnThreads / 64; ++i) s += sh[i];
+    return s;
+}
+
+// One workgroup per (n, g) merges the shifted sums of its channels and row ranges: with d = x - k_c,
+//   mean = (sum_c k_c + sum d / S) / D,   sum (x - mean)^2 = sum d^2 + 2 (k_c - mean) sum d + S sum_c (k_c - mean)^2
+template <typename T>
+__global__ __launch_bounds__(kGnThreads) void gn_stats_kernel(GnArgs a) {
+    __shared__ double sh[kGnThreads / 64];
+    const unsigned n = blockIdx.x / (unsigned)a.G, g = blockIdx.x - n * (unsigned)a.G;
+    const T* x0 = (const T*)a.x + (long long)n * a.x_sn + (long long)g * a.D;
+    const double* part = a.part + 2ll * ((long long)n * a.chunks * a.C + (long long)g * a.D);
+    const long long items = (long long)a.D * a.chunks;
+    const double rs = 1.0 / (double)a.S;
+    double sum = 0.0;
+    for (long long e = threadIdx.x; e < items; e += kGnThreads) {
+        const unsigned ch = (unsigned)(e / a.D), c = (unsigned)(e - (long long)ch * a.D);
+        sum += part[2ll * ((long long)ch * a.C + c)] * rs;
+        if (ch == 0) sum += (double)(float)x0[c];
+    }
+    const double mean = block_sum(sum, sh) / (double)a.D;
+    double m2 = 0.0;
+    for (long long e = threadIdx.x; e < items; e += kGnThreads) {
+        const unsigned ch = (unsigned)(e / a.D), c = (unsigned)(e - (long long)ch * a.D);
+        const double* o = part + 2ll * ((long long)ch * a.C + c);
+        const double k = (double)(float)x0[c] - mean;
+        m2 += fma(2.0 * k, o[0], o[1]) * rs;
+        if (ch == 0) m2 = fma(k, k, m2);
+    }
+    const double var = block_sum(m2, sh) / (double)a.D;
+    if (threadIdx.x == 0) {
+        double* o = a.stats + 2ll * blockIdx.x;
+        o[0] = mean;
+        o[1] = 1.0 / sqrt((var < 0.0 ? 0.0 : var) + a.eps);   // (rounding may leave a constant group below 0; a NaN stays)
+    }
+}
+
+template <typename T, int V>
+__global__ __launch_bounds__(kGnThreads) void gn_tile_apply_kernel(GnArgs a) {
+    const unsigned n = blockIdx.x / (unsigned)a.chunks, ch = blockIdx.x - n * (unsigned)a.chunks;
+    const Tile t = tile_of(a, a.C / V, blockIdx.y);
+    if (!t.on) return;
+    double mean[V], sc[V], sh[V];
+#pragma unroll
+    for (int k = 0; k < V; ++k) {
+        const int c = t.vx * V + k;
+        const double* st = a.stats + 2ll * ((long long)n * a.G + c / a.D);
+        mean[k] = st[0];
+        sc[k] = st[1] * (a.w ? (double)a.w[c] : 1.0);
+        sh[k] = a.b ? (double)a.b[c] : 0.0;
+    }
+    const T* x = (const T*)a.x + (long long)n * a.x_sn + t.vx * V;
+    T* y = (T*)a.out + (long long)n * a.S * a.C + t.vx * V;
+    const long long s0 = (long long)ch * a.chunk_rows, s1 = s0 + a.chunk_rows < a.S ? s0 + a.chunk_rows : a.S;
+    for (long long s = s0 + t.ty; s < s1; s += t.rows) {
+        float v[V];
+        load_vec<T, V>(x + s * a.x_ss, v);
+#pragma unroll
+        for (int k = 0; k < V; ++k) v[k] = act_value(fma((double)v[k] - mean[k], sc[k], sh[k]), a.act, a.slope);
+        store_vec<T, V>(y + s * a.C, v);
+    }
+}
+
+// per channel: sums of dz xh and dz over a range of rows
+template <typename T, int V>
+__global__ __launch_bounds__(kGnThreads) void gn_tile_bwd_sum_kernel(GnArgs a) {
+    const unsigned n = blockIdx.x / (unsigned)a.chunks, ch = blockIdx.x - n * (unsigned)a.chunks;
+    const Tile t = tile_of(a, a.C / V, blockIdx.y);
+    double p[V], q[V];
+#pragma unroll
+    for (int k = 0; k < V; ++k) p[k] = q[k] = 0.0;
+    if (t.on) {
+        double mean[V], rstd[V];
+        float w[V], b[V];
+#pragma unroll
+        for (int k = 0; k < V; ++k) {
+            const int c = t.vx * V + k;
+            const double* st = a.stats + 2ll * ((long long)n * a.G + c / a.D);
+            mean[k] = st[0];
+            rstd[k] = st[1];
+            w[k] = a.w ? a.w[c] : 1.f;
+            b[k] = a.b ? a.b[c] : 0.f;
+        }
+        const T* x = (const T*)a.x + (long long)n * a.x_sn + t.vx * V;
+        const T* dy = (const T*)a.dy + (long long)n * a.dy_sn + t.vx * V;
+        const long long s0 = (long long)ch * a.chunk_rows, s1 = s0 + a.chunk_rows < a.S ? s0 + a.chunk_rows : a.S;
+        for (long long s = s0 + t.ty; s < s1; s += t.rows) {
+            float v[V], d[V];
+            load_vec<T, V>(x + s * a.x_ss, v);
+            load_vec<T, V>(dy + s * a.dy_ss, d);
+#pragma unroll
+            for (int k = 0; k < V; ++k) {
+                const double xh = ((double)v[k] - mean[k]) * rstd[k];
+                const double dz = (double)(d[k] * act_slope(fma(xh, (double)w[k], (double)b[k]), a.act, a.slope));
+                p[k] = fma(dz, xh, p[k]);
+                q[k] += dz;
+            }
+        }
+    }
+    column_sum<V>(p, q, a, t);
+    if (t.on && t.ty == 0)
+#pragma unroll
+        for (int k = 0; k < V; ++k) {
+            double* o = a.part + 2ll * ((long long)blockIdx.x * a.C + t.vx * V + k);
+            o[0] = p[k];
+            o[1] = q[k];
+        }
+}
+
+__global__ __launch_bounds__(kGnThreads) void gn_bwd_coef_kernel(GnArgs a) {
+    __shared__ double sh[kGnThreads / 64];
+    const unsigned n = blockIdx.x / (unsigned)a.G, g = blockIdx.x - n * (unsigned)a.G;
+    const double* part = a.part + 2ll * ((long long)n * a.chunks * a.C + (long long)g * a.D);
+    const long long items = (long long)a.D * a.chunks;
+    double s1 = 0.0, s2 = 0.0;
+    for (long long e = threadIdx.x; e < items; e += kGnThreads) {
+        const unsigned ch = (unsigned)(e / a.D), c = (unsigned)(e - (long long)ch * a.D);
+        const double* o = part + 2ll * ((long long)ch * a.C + c);
+        const double w = a.w ? (double)a.w[(long long)g * a.D + c] : 1.0;
+        s1 = fma(w, o[1], s1);
+        s2 = fma(w, o[0], s2);
+    }
+    const double inv = 1.0 / ((double)a.S * a.D);
+    s1 = block_sum(s1, sh) * inv;
+    s2 = block_sum(s2, sh) * inv;
+    if (threadIdx.x == 0) {
+        a.coef[2ll * blockIdx.x] = s1;
+        a.coef[2ll * blockIdx.x + 1] = s2;
+    }
+}
+
+template <typename T, int V>
+__global__ __launch_bounds__(kGnThreads) void gn_tile_bwd_apply_kernel(GnArgs a) {
+    const unsigned n = blockIdx.x / (unsigned)a.chunks, ch = blockIdx.x - n * (unsigned)a.chunks;
+    const Tile t = tile_of(a, a.C / V, blockIdx.y);
+    if (!t.on) return;
+    double mean[V], rstd[V];
+    float w[V], b[V], f1[V], f2[V];
+#pragma unroll
+    for (int k = 0; k < V; ++k) {
+        const int c = t.vx * V + k;
+        const long long u = (long long)n * a.G + c / a.D;
+        mean[k] = a.stats[2 * u];
+        rstd[k] = a.stats[2 * u + 1];
+        f1[k] = (float)a.coef[2 * u];
+        f2[k] = (float)a.coef[2 * u + 1];
+        w[k] = a.w ? a.w[c] : 1.f;
+        b[k] = a.b ? a.b[c] : 0.f;
+    }
+    const T* x = (const T*)a.x + (long long)n * a.x_sn + t.vx * V;
+    const T* dy = (const T*)a.dy + (long long)n * a.dy_sn + t.vx * V;
+    T* o = (T*)a.out + (long long)n * a.S * a.C + t.vx * V;
+    const long long s0 = (long long)ch * a.chunk_rows, s1 = s0 + a.chunk_rows < a.S ? s0 + a.chunk_rows : a.S;
+    for (long long s = s0 + t.ty; s < s1; s += t.rows) {
+        float v[V], d[V];
+        load_vec<T, V>(x + s * a.x_ss, v);
+        load_vec<T, V>(dy + s * a.dy_ss, d);
+#pragma unroll
+        for (int k = 0; k < V; ++k) {
+            const double xh = ((double)v[k] - mean[k]) * rstd[k];
+            const float wd = w[k] * (d[k] * act_slope(fma(xh, (double)w[k], (double)b[k]), a.act, a.slope));
+            v[k] = (float)rstd[k] * (wd - f1[k] - (float)xh * f2[k]);
+        }
+        store_vec<T, V>(o + s * a.C, v);
+    }
+}
+
+// dw, db: the partials [rows][C][2] summed over their rows, 64 channels and 16 row walkers per workgroup
+template <typename P>
+__global__ __launch_bounds__(1024) void gn_param_grad_kernel(const P* part, long long rows, int C, float* dw, float* db) {
+    __shared__ double sh[1024 * 2];
+    const int col = threadIdx.x & 63, ty = threadIdx.x >> 6, c = (int)blockIdx.x * 64 + col;
+    double p = 0.0, q = 0.0;
+    if (c < C)
+        for (long long r = ty; r < rows; r += 16) {
+            p += (double)part[2 * (r * C + c)];
+            q += (double)part[2 * (r * C + c) + 1];
+        }
+    sh[2 * threadIdx.x] = p;
+    sh[2 * threadIdx.x + 1] = q;
+    __syncthreads();
+    if (ty == 0 && c < C) {
+        p = q = 0.0;
+        for (int y = 0; y < 16; ++y) {
+            p += sh[2 * (y * 64 + col)];
+            q += sh[2 * (y * 64 + col) + 1];
+        }
+        dw[c] = (float)p;
+        db[c] = (float)q;
+    }
+}
+
+// ------------------------------------------------------------------------------------------------ host side
+struct GnPlan {
+    int V;                // elements per access
+    bool unit;
+    int items, lanes;     // unit
+    int per, blocks_g, blocks_n;
+    int tx, blocks_c, chunks;
+    long long chunk_rows;
+};
+
+int elem_bytes(int dtype) { return dtype == DGG_F32 ? 4 : 2; }
+
+// The widest access (at most 16 bytes) that every row allows; unit: that a group's row also divides into.
+int gn_width(int dtype, int unit_d, int C, std::initializer_list<long long> strides, std::initializer_list<const void*> ptrs) {
+    const int es = elem_bytes(dtype);
+    for (int V = 16 / es; V > 1; V >>= 1) {
+        if (V == 2) continue;   // no 2-element kernels: rows that allow no more go element by element
+        bool ok = C % V == 0 && (unit_d == 0 || unit_d % V == 0);
+        for (long long s : strides) ok = ok && s % V == 0;
+        for (const void* p : ptrs) ok = ok && ((uintptr_t)p % (V * es)) == 0;
+        if (ok) return V;
+    }
+    return 1;
+}
+
+void gn_tile_plan(GnPlan& P, long long N, long long S, int C) {
+    const int vecs = C / P.V;
+    P.blocks_c = (vecs + kGnThreads - 1) / kGnThreads;
+    P.tx = (vecs + P.blocks_c - 1) / P.blocks_c;
+    // about 2048 workgroups, of at least 64 rows each (the partial sums stay small beside the data)
+    long long want = 2048 / (N * P.blocks_c);
+    const long long most = (S + 63) / 64;
+    if (want > most) want = most;
+    if (want < 1) want = 1;
+    P.chunk_rows = (S + want - 1) / want;
+    P.chunks = (int)((S + P.chunk_rows - 1) / P.chunk_rows);
+}
+
+bool gn_unit_plan(GnPlan& P, long long S, int D, bool backward) {
+    if (backward ? S != 1 : S * D > 64ll * kUnitItems * P.V) return false;
+    const long long nv = S * (D / P.V);
+    if (nv > 64 * kUnitItems) return false;
+    P.lanes = 1;
+    while (P.lanes < 64 && P.lanes < nv) P.lanes *= 2;
+    P.items = 1;
+    while (P.items * P.lanes < nv) P.items *= 2;
+    return true;
+}
+
+void gn_unit_bwd_grid(GnPlan& P, long long N, int G) {
+    const int slots = kGnThreads / P.lanes;
+    P.per = G < slots ? slots / G : 1;
+    P.blocks_g = G < slots ? 1 : (G + slots - 1) / slots;
+    long long nb = (N + P.per - 1) / P.per, most = 1024 / P.blocks_g;
+    if (most < 1) most = 1;
+    P.blocks_n = (int)(nb < most ? nb : most);
+}
+
+int gn_check(long long N, long long S, int C, int G, int act, int dtype, const char* who) {
+    if (N < 1 || S < 1 || C < 1 || G < 1 || C % G != 0) {
+        set_error_text("%s: N, S, C, groups must be positive and groups must divide C (N = %lld, S = %lld, C = %d, groups = %d)",
+                       who, N, S, C, G);
+        return DGG_ERR_INVALID;
+    }
+    if (dtype < DGG_F32 || dtype > DGG_F16 || act < DGG_ACT_NONE || act > DGG_ACT_SILU) {
+        set_error_text("%s: unknown type %d or activation %d", who, dtype, act);
+        return DGG_ERR_INVALID;
+    }
+    // 32-bit workgroup and unit numbers; element offsets are 64 bits wide
+    if (N > 0x7fffffffll / G || S > 0x7fffffffll || C > (1 << 24)) {
+        set_error_text("%s: N * groups and S must stay below 2^31, C up to 2^24 (N = %lld, S = %lld, C = %d)", who, N, S, C);
+        return DGG_ERR_INVALID;
+    }
+    return DGG_OK;
+}
+
+// What both directions need at most, for whatever alignment the tensors turn out to have.
+int64_t gn_ws_bytes(long long N, long long S, int C, int G, int dtype, bool backward) {
+    int64_t need = 0;
+    for (int V : {16 / elem_bytes(dtype), 4, 1}) {
+        if (C % V) continue;
+        GnPlan P;
+        P.V = V;
+        int64_t n = 0;
+        if ((C / G) % V == 0 && gn_unit_plan(P, S, C / G, backward)) {
+            if (backward) {
+                gn_unit_bwd_grid(P, N, G);
+                n = (int64_t)P.blocks_n * P.per * C * 2 * sizeof(float);
+            } else {
+                n = 0;
+            }
+        } else {
+            gn_tile_plan(P, N, S, C);
+            n = (int64_t)N * P.chunks * C * 2 * sizeof(double) + (int64_t)N * G * 2 * sizeof(double);
+        }
+        if (n > need) need = n;
+    }
+    return need;
+}
+
+template <typename T, int V> int gn_forward_v(const GnPlan& P, GnArgs& a, hipStream_t st) {
+    if (P.unit) {
+        const long long threads = a.N * a.G * P.lanes;
+        const dim3 grid((unsigned)((threads + kGnThreads - 1) / kGnThreads)), block(kGnThreads);
+        switch (P.items) {
+            case 1: hipLaunchKernelGGL((gn_unit_fwd_kernel<T, V, 1>), grid, block, 0, st, a); break;
+            case 2: hipLaunchKernelGGL((gn_unit_fwd_kernel<T, V, 2>), grid, block, 0, st, a); break;
+            case 4: hipLaunchKernelGGL((gn_unit_fwd_kernel<T, V, 4>), grid, block, 0, st, a); break;
+            default: hipLaunchKernelGGL((gn_unit_fwd_kernel<T, V, 8>), grid, block, 0, st, a); break;
+        }
+        return check_launch("group_norm forward");
+    }
+    const dim3 grid((unsigned)(a.N * P.chunks), P.blocks_c), block(kGnThreads);
+    hipLaunchKernelGGL((gn_tile_sum_kernel<T, V>), grid, block, 0, st, a);
+    hipLaunchKernelGGL((gn_stats_kernel<T>), dim3((unsigned)(a.N * a.G)), block, 0, st, a);
+    hipLaunchKernelGGL((gn_tile_apply_kernel<T, V>), grid, block, 0, st, a);
+    return check_launch("group_norm forward");
+}
+
+template <typename T, int V> int gn_backward_v(const GnPlan& P, GnArgs& a, hipStream_t st) {
+    const dim3 block(kGnThreads), cols((unsigned)((a.C + 63) / 64));
+    if (P.unit) {
+        if (!a.dw) a.part = nullptr;
+        const dim3 grid((unsigned)P.blocks_g * P.blocks_n);
+        switch (P.items) {
+            case 1: hipLaunchKernelGGL((gn_unit_bwd_kernel<T, V, 1>), grid, block, 0, st, a); break;
+            case 2: hipLaunchKernelGGL((gn_unit_bwd_kernel<T, V, 2>), grid, block, 0, st, a); break;
+            case 4: hipLaunchKernelGGL((gn_unit_bwd_kernel<T, V, 4>), grid, block, 0, st, a); break;
+            default: hipLaunchKernelGGL((gn_unit_bwd_kernel<T, V, 8>), grid, block, 0, st, a); break;
+        }
+        if (a.dw)
+            hipLaunchKernelGGL((gn_param_grad_kernel<float>), cols, dim3(1024), 0, st, (const float*)a.part,
+                               (long long)P.blocks_n * P.per, a.C, a.dw, a.db);
+        return check_launch("group_norm backward");
+    }
+    const dim3 grid((unsigned)(a.N * P.chunks), P.blocks_c);
+    hipLaunchKernelGGL((gn_tile_bwd_sum_kernel<T, V>), grid, block, 0, st, a);
+    hipLaunchKernelGGL(gn_bwd_coef_kernel, dim3((unsigned)(a.N * a.G)), block, 0, st, a);
+    if (a.dw)
+        hipLaunchKernelGGL((gn_param_grad_kernel<double>), cols, dim3(1024), 0, st, (const double*)a.part,
+                           a.N * P.chunks, a.C, a.dw, a.db);
+    hipLaunchKernelGGL((gn_tile_bwd_apply_kernel<T, V>), grid, block, 0, st, a);
+    return check_launch("group_norm backward");
+}
+
+template <typename T> int gn_dispatch(bool backward, const GnPlan& P, GnArgs& a, hipStream_t st) {
+    constexpr int W = 16 / sizeof(T);
+    if (P.V == W) return backward ? gn_backward_v<T, W>(P, a, st) : gn_forward_v<T, W>(P, a, st);
+    if (W > 4 && P.V == 4) return backward ? gn_backward_v<T, 4>(P, a, st) : gn_forward_v<T, 4>(P, a, st);
+    return backward ? gn_backward_v<T, 1>(P, a, st) : gn_forward_v<T, 1>(P, a, st);
+}
+
+int gn_run(bool backward, GnArgs& a, int dtype, void* ws, size_t ws_bytes, hipStream_t st, const char* who) {
+    a.D = a.C / a.G;
+    GnPlan P;
+    std::initializer_list<long long> fs = {a.x_sn, a.x_ss}, bs = {a.x_sn, a.x_ss, a.dy_sn, a.dy_ss};
+    P.V = gn_width(dtype, a.D, a.C, backward ? bs : fs, {a.x, a.out, backward ? a.dy : a.x});
+    P.unit = gn_unit_plan(P, a.S, a.D, backward);
+    if (!P.unit) {
+        P.V = gn_width(dtype, 0, a.C, backward ? bs : fs, {a.x, a.out, backward ? a.dy : a.x});
+        gn_tile_plan(P, a.N, a.S, a.C);
+        if (P.blocks_c > 65535) return DGG_ERR_INVALID;
+        a.chunks = P.chunks;
+        a.chunk_rows = P.chunk_rows;
+        a.tx = P.tx;
+    } else {
+        a.lanes = P.lanes;
+        if (backward) {
+            gn_unit_bwd_grid(P, a.N, a.G);
+            a.blocks_g = P.blocks_g;
+            a.blocks_n = P.blocks_n;
+        }
+    }
+    size_t need = 0;
+    if (P.unit) {
+        need = backward && a.dw ? (size_t)P.blocks_n * P.per * a.C * 2 * sizeof(float) : 0;
+    } else {
+        const size_t part = (size_t)a.N * P.chunks * a.C * 2 * sizeof(double);
+        need = part + (size_t)a.N * a.G * 2 * sizeof(double);
+        a.coef = (double*)((char*)ws + part);
+        if (!a.stats) a.stats = a.coef;   // a forward without a backward keeps its statistics in the workspace
+    }
+    if (need && (!ws || ws_bytes < need || (uintptr_t)ws % 8)) {
+        set_error_text("%s: the workspace has %zu bytes, %zu (8-byte aligned) are needed", who, ws_bytes, need);
+        return DGG_ERR_WORKSPACE;
+    }
+    a.part = (double*)ws;
+    return dtype == DGG_F32 ? gn_dispatch<float>(backward, P, a, st)
+         : dtype == DGG_BF16 ? gn_dispatch<__bf16>(backward, P, a, st) : gn_dispatch<_Float16>(backward, P, a, st);
+}
+
+}  // namespace
+}  // namespace dgg
+
+using namespace dgg;
+
+extern "C" {
+
+int64_t dgg_group_norm_workspace_bytes(int64_t N, int64_t S, int C, int groups, int dtype, int backward) {
+    const int rc = gn_check(N, S, C, groups, DGG_ACT_NONE, dtype, "dgg_group_norm_workspace_bytes");
+    return rc != DGG_OK ? rc : gn_ws_bytes(N, S, C, groups, dtype, backward != 0);
+}
+
+int dgg_group_norm_act_forward(const void* x, int64_t x_stride_n, int64_t x_stride_s, int64_t N, int64_t S, int C, int groups,
+                               const float* weight, const float* bias, double eps, int act, float slope, int dtype, void* y,
+                               double* stats, void* ws, size_t ws_bytes, void* stream) {
+    const char* who = "dgg_group_norm_act_forward";
+    const int rc = gn_check(N, S, C, groups, act, dtype, who);
+    if (rc != DGG_OK) return rc;
+    if (!x || !y || x_stride_n < 0 || x_stride_s < 0 || !(eps >= 0.0)) {
+        set_error_text("%s: x, y, strides >= 0 and eps >= 0 are needed", who);
+        return DGG_ERR_INVALID;
+    }
+    GnArgs a = {};
+    a.x = x; a.out = y; a.w = weight; a.b = bias; a.stats = stats;
+    a.x_sn = x_stride_n; a.x_ss = x_stride_s;
+    a.N = N; a.S = S; a.C = C; a.G = groups;
+    a.act = act; a.slope = slope; a.eps = eps;
+    return gn_run(false, a, dtype, ws, ws_bytes, (hipStream_t)stream, who);
+}
+
+int dgg_group_norm_act_backward(const void* dy, int64_t dy_stride_n, int64_t dy_stride_s, const void* x, int64_t x_stride_n,
+                                int64_t x_stride_s, int64_t N, int64_t S, int C, int groups, const float* weight,
+                                const float* bias, int act, float slope, int dtype, const double* stats, void* dx,
+                                float* dweight, float* dbias, void* ws, size_t ws_bytes, void* stream) {
+    const char* who = "dgg_group_norm_act_backward";
+    const int rc = gn_check(N, S, C, groups, act, dtype, who);
+    if (rc != DGG_OK) return rc;
+    if (!dy || !x || !stats || !dx || x_stride_n < 0 || x_stride_s < 0 || dy_stride_n < 0 || dy_stride_s < 0 || !dweight != !dbias) {
+        set_error_text("%s: dy, x, stats, dx, strides >= 0, and both or none of dweight and dbias are needed", who);
+        return DGG_ERR_INVALID;
+    }
+    GnArgs a = {};
+    a.dy = dy; a.x = x; a.out = dx; a.w = weight; a.b = bias; a.stats = const_cast<double*>(stats);
+    a.dy_sn = dy_stride_n; a.dy_ss = dy_stride_s; a.x_sn = x_stride_n; a.x_ss = x_stride_s;
+    a.N = N; a.S = S; a.C = C; a.G = groups;
+    a.act = act; a.slope = slope; a.dw = dweight; a.db = dbias;
+    return gn_run(true, a, dtype, ws, ws_bytes, (hipStream_t)stream, who);
+}
+
+}  // extern "C"

@@ -4,6 +4,7 @@ here: every function is one or two library calls on the current HIP stream."""
 from __future__ import annotations
 
 import ctypes as C
+from contextlib import nullcontext
 
 import torch
 
@@ -170,6 +171,196 @@ def eva_forward_objects(fn, bps_obj, rot9, transl, n_per):
                                         ptr(bps_obj), ptr(rot9), ptr(transl), ptr(out), stream_ptr(dev)),
           "dgg_eva_forward_objects")
     return out
+
+
+# ------------------------------------------------------------------------------------------ group normalisation
+_DTYPES = {torch.float32: _lib.F32, torch.bfloat16: _lib.BF16, torch.float16: _lib.F16}
+_ACTS = {"none": _lib.ACT_NONE, "leaky_relu": _lib.ACT_LEAKY_RELU, "silu": _lib.ACT_SILU}
+
+
+def _on(dev):
+    """The context in which kernels for `dev` are launched: launches go to the current device."""
+    return torch.cuda.device(dev) if dev.index is not None and dev.index != torch.cuda.current_device() else nullcontext()
+
+
+def _rows(t):
+    """t (N, .., C) as (tensor, N, S, C, stride of n, stride of s): the dimensions between the first and the last are one
+    axis of S points.  A tensor whose channels do not lie side by side, or whose points are not evenly spaced, is copied."""
+    n, c = t.shape[0], t.shape[-1]
+    s = t.numel() // (n * c) if n * c else 0
+    mid = [(size, stride) for size, stride in zip(t.shape[1:-1], t.stride()[1:-1]) if size != 1]
+    even = all(mid[i][1] == mid[i + 1][0] * mid[i + 1][1] for i in range(len(mid) - 1))
+    if (c > 1 and t.stride(-1) != 1) or not even:
+        t = t.contiguous()
+        return t, n, s, c, s * c, c
+    return t, n, s, c, (t.stride(0) if n > 1 else s * c), (mid[-1][1] if mid else c)
+
+
+def _group_norm_args(who, x, num_groups, weight, bias, act):
+    dev = _dev(x)
+    if x.dtype not in _DTYPES or x.dim() < 2:
+        raise _lib.DggError("%s: x must be (N, .., C) of float32, bfloat16 or float16; got %s %s"
+                            % (who, x.dtype, tuple(x.shape)))
+    if act not in _ACTS:
+        raise _lib.DggError("%s: act must be one of %s; got %r" % (who, sorted(_ACTS), act))
+    c = x.shape[-1]
+    if num_groups < 1 or c < 1 or c % num_groups:
+        raise _lib.DggError("%s: %d groups do not divide %d channels" % (who, num_groups, c))
+    for name, t in (("weight", weight), ("bias", bias)):
+        if t is not None and (t.device != dev or t.dtype != torch.float32 or t.shape != (c,)):
+            raise _lib.DggError("%s: %s must be a float32 (%d,) tensor on %s; got %s %s on %s"
+                                % (who, name, c, dev, t.dtype, tuple(t.shape), t.device))
+    return dev, (None if weight is None else weight.contiguous()), (None if bias is None else bias.contiguous())
+
+
+def _group_norm_ws(n, s, c, g, dtype, backward, dev):
+    nb = int(lib().dgg_group_norm_workspace_bytes(n, s, c, g, dtype, backward))
+    if nb < 0:
+        check(nb, "dgg_group_norm_workspace_bytes")
+    return _lib.new_workspace(nb, dev) if nb else None, nb
+
+
+def group_norm_act_forward(x, num_groups, weight=None, bias=None, eps=1e-5, act="leaky_relu", slope=0.2):
+    """act(group_norm(x)) over channels-last data: x (N, .., C) float32 / bfloat16 / float16 (a column block of a wider
+    product is read in place), num_groups groups of C / num_groups channels, statistics over a sample's points and a group's
+    channels; weight / bias float32 (C,) or None; act "none", "leaky_relu" (`slope` for z <= 0) or "silu".
+    Returns (y contiguous, of x's shape and type; stats (N, num_groups, 2) float64 = mean and 1 / sqrt(var + eps), which
+    group_norm_act_backward takes)."""
+    dev, weight, bias = _group_norm_args("group_norm_act_forward", x, num_groups, weight, bias, act)
+    y = torch.empty(x.shape, dtype=x.dtype, device=dev)
+    stats = torch.empty((x.shape[0], num_groups, 2), dtype=torch.float64, device=dev)
+    if x.numel() == 0:
+        return y, stats.zero_()
+    x, n, s, c, sn, ss = _rows(x)
+    dt = _DTYPES[x.dtype]
+    with _on(dev):
+        ws, nb = _group_norm_ws(n, s, c, num_groups, dt, 0, dev)
+        check(lib().dgg_group_norm_act_forward(ptr(x), sn, ss, n, s, c, num_groups, ptr(weight), ptr(bias), float(eps),
+                                               _ACTS[act], float(slope), dt, ptr(y), ptr(stats), ptr(ws), nb,
+                                               stream_ptr(dev)), "dgg_group_norm_act_forward")
+    return y, stats
+
+
+def group_norm_act_backward(dy, x, num_groups, weight, bias, eps, act, slope, stats, param_grads=True):
+    """Gradients of group_norm_act_forward with the same arguments and its `stats`: (dx contiguous, of x's type; dweight,
+    dbias float32 (C,), None with param_grads=False)."""
+    dev, weight, bias = _group_norm_args("group_norm_act_backward", x, num_groups, weight, bias, act)
+    if dy.shape != x.shape or dy.dtype != x.dtype or dy.device != dev:
+        raise _lib.DggError("group_norm_act_backward: dy must be like x: %s %s; got %s %s on %s"
+                            % (x.dtype, tuple(x.shape), dy.dtype, tuple(dy.shape), dy.device))
+    if (stats.shape != (x.shape[0], num_groups, 2) or stats.dtype != torch.float64 or stats.device != dev
+            or not stats.is_contiguous()):
+        raise _lib.DggError("group_norm_act_backward: stats must be what the forward of the same x returned")
+    c = x.shape[-1]
+    dx = torch.empty(x.shape, dtype=x.dtype, device=dev)
+    dw = db = None
+    if param_grads:
+        dw, db = (torch.empty((c,), dtype=torch.float32, device=dev) for _ in range(2))
+    if x.numel() == 0:
+        return dx, (dw.zero_() if param_grads else None), (db.zero_() if param_grads else None)
+    x, n, s, c, sn, ss = _rows(x)
+    dy, _, _, _, dsn, dss = _rows(dy)
+    dt = _DTYPES[x.dtype]
+    with _on(dev):
+        ws, nb = _group_norm_ws(n, s, c, num_groups, dt, 1, dev)
+        check(lib().dgg_group_norm_act_backward(ptr(dy), dsn, dss, ptr(x), sn, ss, n, s, c, num_groups, ptr(weight),
+                                                ptr(bias), _ACTS[act], float(slope), dt, ptr(stats), ptr(dx), ptr(dw),
+                                                ptr(db), ptr(ws), nb, stream_ptr(dev)), "dgg_group_norm_act_backward")
+    return dx, dw, db
+
+
+# ------------------------------------------------------------------------------------------ Newton-Schulz, Muon
+NS_COEFFICIENTS = (3.4445, -4.7750, 2.0315)   # the quintic whose iterates bring singular values near 1 fast, not exactly to it
+_ADJUST = {"spectral": _lib.MUON_SPECTRAL, "match_rms": _lib.MUON_MATCH_RMS}
+
+
+def _coefficients(who, steps, coefficients):
+    """`coefficients`: one (a, b, c) for all steps or a sequence of `steps` of them -> a C array of doubles."""
+    rows = [coefficients] * steps if len(coefficients) == 3 and not hasattr(coefficients[0], "__len__") else list(coefficients)
+    if steps < 1 or len(rows) != steps or any(len(r) != 3 for r in rows):
+        raise _lib.DggError("%s: %d steps need one (a, b, c) or one for each step; got %r" % (who, steps, coefficients))
+    return (C.c_double * (3 * steps))(*[float(v) for r in rows for v in r])
+
+
+def _matrix_rows(t):
+    """A matrix or a stack (B, rows, cols) whose rows are contiguous, as (tensor, batch, rows, cols, pitch, stride)."""
+    if t.stride(-1) != 1 and t.shape[-1] > 1 or t.shape[-2] > 1 and t.stride(-2) < t.shape[-1]:
+        t = t.contiguous()
+    b, r, c = (1,) * (3 - t.dim()) + tuple(t.shape)
+    return t, b, r, c, (t.stride(-2) if r > 1 else c), (t.stride(0) if t.dim() == 3 and b > 1 else r * c)
+
+
+def _ns_workspace(mats, n, dev):
+    nb = int(lib().dgg_orthogonalize_workspace_bytes(mats, n))
+    if nb < 0:
+        check(nb, "dgg_orthogonalize_workspace_bytes")
+    return _lib.new_workspace(nb, dev), nb
+
+
+def orthogonalize(grad, steps=5, coefficients=NS_COEFFICIENTS, eps=1e-7):
+    """The orthogonalised form of a matrix (rows, cols), of every matrix of a stack (B, rows, cols), or of each of a list of
+    them (one set of launches for the whole list): X_0 = grad / (|grad|_F + eps), then `steps` times
+    X <- a X + (b A + c A^2) X with A = X X^T over the shorter side.  float32, bfloat16 or float16 (one type per call);
+    returns contiguous tensors of the same shape and type.  No gradient: an optimiser's operator."""
+    single = torch.is_tensor(grad)
+    grads = [grad] if single else list(grad)
+    coef = _coefficients("orthogonalize", steps, coefficients)
+    for t in grads:
+        dev = _dev(t)
+        if t.dtype not in _DTYPES or t.dim() not in (2, 3) or t.dtype != grads[0].dtype or dev != grads[0].device:
+            raise _lib.DggError("orthogonalize: matrices (rows, cols) or stacks (B, rows, cols) of one type (float32, bfloat16, "
+                                "float16) on one device; got %s %s on %s" % (t.dtype, tuple(t.shape), dev))
+    outs = [torch.empty(t.shape, dtype=t.dtype, device=t.device) for t in grads]
+    work = [(_matrix_rows(t.detach()), o) for t, o in zip(grads, outs) if t.numel()]
+    if work:
+        dev = grads[0].device
+        mats = (_lib.Matrix * len(work))()
+        for m, ((t, b, r, c, ld, st), o) in zip(mats, work):
+            m.in_, m.out, m.batch, m.rows, m.cols, m.ld_in, m.ld_out = t.data_ptr(), o.data_ptr(), b, r, c, ld, c
+            m.in_stride, m.out_stride = st, r * c
+        with _on(dev):
+            ws, nb = _ns_workspace(mats, len(work), dev)
+            check(lib().dgg_orthogonalize(mats, len(work), _DTYPES[grads[0].dtype], coef, steps, float(eps), ptr(ws), nb,
+                                          stream_ptr(dev)), "dgg_orthogonalize")
+    return outs[0] if single else outs
+
+
+def muon_step(params, grads, momentum, lr, mu=0.95, nesterov=True, weight_decay=0.0, steps=5, coefficients=NS_COEFFICIENTS,
+              eps=1e-7, adjust="spectral", grad_scale=1.0):
+    """One Muon step over lists of float32 matrices (or stacks of them), params and momentum in place:
+        M <- mu M + grad_scale G;   U = grad_scale G + mu M (nesterov) or M;   W <- (1 - lr weight_decay) W - lr f orthogonalize(U)
+    with f = sqrt(max(1, rows / cols)) (adjust="spectral") or 0.2 sqrt(max(rows, cols)) ("match_rms")."""
+    who = "muon_step"
+    params, grads, momentum = list(params), list(grads), list(momentum)
+    if not (len(params) == len(grads) == len(momentum)):
+        raise _lib.DggError("%s: %d parameters, %d gradients, %d momenta" % (who, len(params), len(grads), len(momentum)))
+    if adjust not in _ADJUST:
+        raise _lib.DggError("%s: adjust must be one of %s; got %r" % (who, sorted(_ADJUST), adjust))
+    coef = _coefficients(who, steps, coefficients)
+    keep, mats, n = [], (_lib.Matrix * max(len(params), 1))(), 0
+    for w, g, m in zip(params, grads, momentum):
+        dev = _dev(w)
+        for t in (w, g, m):
+            if (t.dtype != torch.float32 or t.dim() not in (2, 3) or t.shape != w.shape or t.device != dev
+                    or dev != params[0].device):
+                raise _lib.DggError("%s: float32 matrices of equal shape on one device are needed; got %s %s on %s"
+                                    % (who, t.dtype, tuple(t.shape), t.device))
+        if not w.numel():
+            continue
+        (wt, b, r, c, ldw, sw), (mt, _, _, _, ldm, sm), (gt, _, _, _, ldg, sg) = (_matrix_rows(t.detach()) for t in (w, m, g))
+        if wt.data_ptr() != w.data_ptr() or mt.data_ptr() != m.data_ptr() or (b > 1 and min(sw, sm) < r * c):
+            raise _lib.DggError("%s: parameters and momentum are updated in place: their rows must be contiguous and apart" % who)
+        keep.append(gt)
+        e = mats[n]
+        n += 1
+        e.in_, e.out, e.momentum, e.batch, e.rows, e.cols = gt.data_ptr(), wt.data_ptr(), mt.data_ptr(), b, r, c
+        e.ld_in, e.ld_out, e.ld_momentum, e.in_stride, e.out_stride, e.momentum_stride = ldg, ldw, ldm, sg, sw, sm
+    if n:
+        dev = params[0].device
+        with _on(dev):
+            ws, nb = _ns_workspace(mats, n, dev)
+            check(lib().dgg_muon_step(mats, n, float(lr), float(mu), int(bool(nesterov)), float(weight_decay), _ADJUST[adjust],
+                                      float(grad_scale), coef, steps, float(eps), ptr(ws), nb, stream_ptr(dev)), "dgg_muon_step")
 
 
 # ------------------------------------------------------------------------------------------ small ops

@@ -1,0 +1,276 @@
+"""Newton-Schulz orthogonalisation (ops.orthogonalize) and the Muon step (ops.muon_step) against the iteration in 64 bits on the CPU,
+at the sizes, layouts and values where they can go wrong, and their refusals.
+
+Tolerances.  A step multiplies operands of 22 bits (two fp16 planes: 2^-23 of a value at most, the dropped lo lo 2^-22 of a term) and
+sums in fp32, and b A + c A^2 is a difference of terms a few times its size: 2^-21 of |X| is allowed a step.  Later steps pass an error on
+with the iteration's derivative, whose largest value from X_0 on is kappa = max(|p'(s)|, |p(s) / s|) over the singular values s of X_0
+(p: the composed polynomial; 0 belongs to them where the rank is short).  So |error|_F <= 2^-21 (steps |X|_F + kappa |X_0|_F); a single
+element is allowed 20 times the root mean square of that.  Outputs of 16 bits: half a step of the type more."""
+import math
+
+import pytest
+import torch
+
+from dex_gan_grasp_amd import _lib, ops
+
+COEF = ops.NS_COEFFICIENTS
+EPS = 1e-7
+U = 2.0 ** -24
+
+
+def reference(g, steps=5, coef=COEF, eps=EPS):
+    """The iteration in doubles on the CPU for one matrix, and the Frobenius error allowed."""
+    g = g.double().cpu()
+    turned = g.shape[0] > g.shape[1]
+    x = g.t() if turned else g
+    x = x / (x.norm() + eps)
+    rows = [coef] * steps if not hasattr(coef[0], "__len__") else coef
+    s = torch.linalg.svdvals(x)
+    if x.shape[0] > 1:
+        s = torch.cat([s, torch.zeros(1, dtype=torch.float64)])
+    p, dp, over, x0 = s.clone(), torch.ones_like(s), torch.ones_like(s), float(x.norm())
+    for a, b, c in rows:
+        dp = dp * (a + 3 * b * p ** 2 + 5 * c * p ** 4)
+        over = over * (a + b * p ** 2 + c * p ** 4)      # p(s) / s, also at 0
+        p = p * (a + b * p ** 2 + c * p ** 4)
+        gram = x @ x.t()
+        x = a * x + (b * gram + c * gram @ gram) @ x
+    kappa = float(torch.maximum(dp.abs(), over.abs()).max())
+    tol = 2.0 ** -21 * (steps * float(x.norm()) + kappa * x0)
+    return (x.t() if turned else x), tol
+
+
+def close(got, g, dtype=torch.float32, **kw):
+    ref, tol = reference(g, **kw)
+    got = got.double().cpu()
+    half = torch.finfo(dtype).eps / 2 if dtype != torch.float32 else U
+    err = (got - ref).abs()
+    rms = tol / math.sqrt(ref.numel())
+    tiny = 2.0 ** -25 if dtype == torch.float16 else 0.0
+    assert float((got - ref).norm()) <= tol + half * float(ref.norm()) + tiny * math.sqrt(ref.numel()), (
+        float((got - ref).norm()), tol, float(ref.norm()))
+    assert bool((err <= 20 * rms + half * ref.abs() + tiny).all()), float((err / (20 * rms + half * ref.abs() + tiny)).max())
+
+
+def matrix(rows, cols, seed, dtype=torch.float32, kind="gradient"):
+    g = torch.Generator().manual_seed(seed)
+    if kind == "gradient":      # dy^T x over a batch of 300, scales spread over a decade
+        dy = torch.randn(300, rows, generator=g) * torch.logspace(0, -1, rows)
+        m = dy.t() @ torch.randn(300, cols, generator=g) / 300
+    elif kind == "low rank":
+        m = torch.randn(rows, 3, generator=g) @ torch.randn(3, cols, generator=g)
+    else:
+        m = torch.randn(rows, cols, generator=g)
+    return m.to(dtype)
+
+
+SHAPES = [(1, 1), (1, 7), (7, 1), (1, 300), (2, 2), (12, 512), (3, 512), (31, 33), (63, 65), (64, 64), (65, 63), (66, 200), (128, 128),
+          (129, 257), (200, 100), (257, 771), (512, 256), (320, 700), (100, 4101), (4613, 40)]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("shape", SHAPES, ids=lambda s: "%dx%d" % s)
+def test_matches_the_iteration(shape):
+    for dtype in (torch.float32, torch.bfloat16, torch.float16):
+        g = matrix(*shape, seed=sum(shape), dtype=dtype)
+        out = ops.orthogonalize(g.cuda())
+        assert out.dtype == dtype and out.shape == g.shape and out.is_contiguous()
+        close(out, g, dtype)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kind", ["low rank", "normal"])
+@pytest.mark.parametrize("shape", [(40, 90), (256, 512), (300, 130)], ids=lambda s: "%dx%d" % s)
+def test_spectra(shape, kind):
+    g = matrix(*shape, seed=3, kind=kind)
+    close(ops.orthogonalize(g.cuda()), g)
+    if kind == "normal":        # what it is for: singular values near 1
+        s = torch.linalg.svdvals(ops.orthogonalize(g.cuda()).double().cpu())
+        assert 0.6 < float(s.min()) and float(s.max()) < 1.25
+
+
+@pytest.mark.gpu
+def test_scales_and_special_values():
+    g = matrix(70, 130, 4)
+    for scale in (1e-4, 1e-12, 1e-16, 1e15, 1e30):      # (from 1e-12 down eps is larger than the norm)
+        close(ops.orthogonalize((g * scale).cuda()), g * scale)
+    assert not ops.orthogonalize(torch.zeros(70, 130, device="cuda")).any()
+    spike = torch.zeros(70, 130)
+    spike[5, 7] = -3.0
+    close(ops.orthogonalize(spike.cuda()), spike)
+    close(ops.orthogonalize((g * 1e-30).cuda(), eps=0.0), g * 1e-30, eps=0.0)
+    stack = torch.stack([g, g, g, g])
+    stack[1, 69, 129] = float("nan")
+    stack[2, 0, 3] = float("inf")
+    out = ops.orthogonalize(stack.cuda())
+    one = ops.orthogonalize(g.cuda())
+    assert torch.equal(out[0], one) and torch.equal(out[3], one) and out[1].isnan().all() and out[2].isnan().all()
+
+
+@pytest.mark.gpu
+def test_steps_and_coefficients():
+    g = matrix(48, 100, 6)
+    for steps in (1, 2, 10):
+        close(ops.orthogonalize(g.cuda(), steps), g, steps=steps)
+    rows = [(3.0, -3.2, 1.2), (2.5, -2.0, 0.6), (1.875, -1.25, 0.375)]
+    close(ops.orthogonalize(g.cuda(), 3, rows), g, steps=3, coef=rows)
+    close(ops.orthogonalize(g.cuda(), 8, (1.5, -0.5, 0.0)), g, steps=8, coef=(1.5, -0.5, 0.0))
+
+
+@pytest.mark.gpu
+def test_stacks_lists_and_strides():
+    stack = torch.stack([matrix(33, 65, s) for s in range(5)])
+    out = ops.orthogonalize(stack.cuda())
+    for o, g in zip(out, stack):
+        close(o, g)
+    # more entries than one set of launches takes, of all shapes; an empty one among them
+    shapes = [(1 + 7 * i % 40, 1 + 13 * i % 90) for i in range(19)] + [(0, 5), (300, 200)]
+    many = [matrix(*s, seed=i) for i, s in enumerate(shapes)]
+    outs = ops.orthogonalize([m.cuda() for m in many])
+    for o, g in zip(outs, many):
+        assert o.shape == g.shape
+        if g.numel():
+            close(o, g)
+    g = matrix(40, 100, 8)
+    want = ops.orthogonalize(g.cuda())
+    wide = torch.full((40, 131), 9.0, device="cuda")
+    wide[:, 17:117] = g.cuda()
+    assert torch.equal(ops.orthogonalize(wide[:, 17:117]), want)
+    assert torch.equal(ops.orthogonalize(g.t().contiguous().cuda().t()), want)
+    assert torch.equal(ops.orthogonalize(stack.cuda().transpose(0, 1).contiguous().transpose(0, 1)), out)
+    row = matrix(1, 100, 9)
+    close(ops.orthogonalize(row.cuda().expand(6, 100)), row.expand(6, 100))
+
+
+def muon_reference(w, g, m, lr, mu, nesterov, wd, f, gs):
+    m64 = mu * m.double() + gs * g.double()
+    ref, tol = reference(gs * g.double() + mu * m64 if nesterov else m64)
+    return (1 - lr * wd) * w.double() - lr * f * ref, m64, lr * f * tol
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("nesterov,adjust,gs", [(True, "spectral", 1.0), (False, "match_rms", 0.125)], ids=["nesterov", "plain"])
+def test_muon_step(nesterov, adjust, gs):
+    shapes = [(256, 300), (512, 256), (12, 512), (1, 9), (65, 64), (130, 40)]
+    lr, mu, wd = 0.02, 0.95, 0.1
+    ws = [matrix(*s, seed=1, kind="normal") for s in shapes]
+    gs_ = [matrix(*s, seed=2) for s in shapes]
+    ms = [matrix(*s, seed=3) for s in shapes]
+    # parameters as column blocks of wider tensors: what lies beside them stays
+    wide = [torch.full((s[0], s[1] + 5), 4.0, device="cuda") for s in shapes]
+    dw = [t[:, 2:2 + s[1]].copy_(w) for t, s, w in zip(wide, shapes, ws)]
+    dg, dm = [t.cuda() for t in gs_], [t.cuda() for t in ms]
+    ops.muon_step(dw, dg, dm, lr, mu, nesterov, wd, adjust=adjust, grad_scale=gs)
+    for s, w, g, m, nw, ng, nm, t in zip(shapes, ws, gs_, ms, dw, dg, dm, wide):
+        f = math.sqrt(max(1.0, s[0] / s[1])) if adjust == "spectral" else 0.2 * math.sqrt(max(s))
+        rw, rm, tol = muon_reference(w, g, m, lr, mu, nesterov, wd, f, gs)
+        assert torch.equal(ng.cpu(), g)
+        # M: mu rounded to fp32, one product and one sum rounded
+        assert bool(((nm.cpu().double() - rm).abs() <= 3 * U * (m.double().abs() + gs * g.double().abs() + rm.abs())).all())
+        err = (nw.cpu().double() - rw).abs()
+        # W: decay and step rounded, one fma; u's own roundings (3 U) pass through the iteration like its 2^-21 of a step
+        assert float(err.norm()) <= 2 * tol + 4 * U * float(w.norm()) and bool((err <= 40 * tol / math.sqrt(w.numel())
+                                                                                 + 4 * U * (w.double().abs() + rw.abs())).all())
+        assert bool((t[:, :2] == 4).all()) and bool((t[:, 2 + s[1]:] == 4).all())
+
+
+@pytest.mark.gpu
+def test_muon_of_a_zero_gradient_and_of_stacks():
+    w = torch.randn(3, 20, 30, device="cuda")
+    m = torch.zeros_like(w)
+    was = w.clone()
+    ops.muon_step([w], [torch.zeros_like(w)], [m], 0.1, weight_decay=0.5)
+    assert not m.any() and bool(((w - 0.95 * was).abs() <= 2 * U * was.abs()).all())
+    g = torch.stack([matrix(20, 30, s) for s in range(3)]).cuda()
+    one = [t.clone() for t in w]
+    ops.muon_step([w], [g], [m], 0.1)
+    for i in range(3):
+        ops.muon_step([one[i]], [g[i]], [torch.zeros(20, 30, device="cuda")], 0.1)
+        assert torch.equal(one[i], w[i])
+
+
+@pytest.mark.gpu
+def test_other_streams_and_graph_replays():
+    shapes = [(200, 300), (12, 512), (256, 64)]
+    gs = [matrix(*s, seed=5).cuda() for s in shapes]
+    want = ops.orthogonalize(gs)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        got = ops.orthogonalize(gs)
+        again = ops.orthogonalize(gs)
+    both = ops.orthogonalize(gs)          # beside the other stream's: a workspace of its own
+    torch.cuda.synchronize()
+    for e, a, b, c in zip(want, got, again, both):
+        assert torch.equal(e, a) and torch.equal(e, b) and torch.equal(e, c)
+    ws, ms = [torch.randn_like(g) for g in gs], [torch.zeros_like(g) for g in gs]
+    ew, em = [w.clone() for w in ws], [m.clone() for m in ms]
+    graph, second = torch.cuda.CUDAGraph(), torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        ops.muon_step(ws, gs, ms, 0.02, weight_decay=0.01)
+    with torch.cuda.graph(second):
+        out = ops.orthogonalize(gs)
+    for k in range(4):
+        for g, s in zip(gs, shapes):
+            g.copy_(matrix(*s, seed=30 + k))
+        graph.replay()
+        second.replay()
+        ops.muon_step(ew, gs, em, 0.02, weight_decay=0.01)
+        eager = ops.orthogonalize(gs)
+        torch.cuda.synchronize()
+        for a, b in zip(ws + ms + list(out), ew + em + list(eager)):
+            assert torch.equal(a, b), k
+
+
+def test_refusals_without_a_gpu():
+    with pytest.raises(_lib.DggError):
+        ops.orthogonalize(torch.zeros(4, 4))
+    with pytest.raises(_lib.DggError):
+        ops.muon_step([torch.zeros(4, 4)], [torch.zeros(4, 4)], [torch.zeros(4, 4)], 0.1)
+    lib = _lib.lib()
+    C = _lib.C
+    coef = (C.c_double * 15)(*(COEF * 5))
+
+    def mat(**kw):
+        m = (_lib.Matrix * 1)()
+        base = dict(in_=4096, out=4096, momentum=4096, batch=1, rows=8, cols=8, ld_in=8, ld_out=8, ld_momentum=8)
+        for k, v in {**base, **kw}.items():
+            setattr(m[0], k, v)
+        return m
+
+    need = lib.dgg_orthogonalize_workspace_bytes(mat(), 1)
+    assert need > 0 and lib.dgg_orthogonalize_workspace_bytes(mat(), 0) == -1
+    for bad in (dict(rows=0), dict(cols=-1), dict(batch=0), dict(rows=16385, cols=16385), dict(cols=(1 << 20) + 1), dict(batch=1 << 30)):
+        assert lib.dgg_orthogonalize_workspace_bytes(mat(**bad), 1) == -1, bad
+
+    def orth(m=None, dtype=0, c=coef, steps=5, eps=1e-7, ws=4096, n=need):
+        return lib.dgg_orthogonalize(mat() if m is None else m, 1, dtype, c, steps, eps, ws, n, None)
+
+    def muon(m=None, lr=0.1, mu=0.9, adjust=0, gs=1.0):
+        return lib.dgg_muon_step(mat() if m is None else m, 1, lr, mu, 1, 0.0, adjust, gs, coef, 5, 1e-7, 4096, 0, None)
+
+    assert orth(dtype=3) == orth(c=None) == orth(steps=0) == orth(steps=17) == orth(eps=-1.0) == orth(eps=float("nan")) == -1
+    assert orth(c=(C.c_double * 15)(*([9.0] * 15))) == -1                       # iterates that run away
+    assert orth(c=(C.c_double * 15)(*([float("nan")] * 15))) == -1
+    for bad in (dict(in_=None), dict(out=None), dict(ld_in=7), dict(ld_out=7), dict(in_stride=-1)):
+        assert orth(mat(**bad)) == -1, bad
+    assert orth(ws=None) == orth(ws=4100) == orth(n=need - 1) == -3
+    assert muon(adjust=2) == muon(lr=float("inf")) == muon(mu=float("nan")) == muon(gs=float("nan")) == -1
+    assert muon(mat(momentum=None)) == muon(mat(ld_momentum=7)) == -1
+    assert muon() == -3                                                         # no workspace
+
+
+@pytest.mark.gpu
+def test_refusals():
+    g = torch.zeros(4, 6, device="cuda")
+    f = torch.zeros(4, 6, device="cuda")
+    for call in (lambda: ops.orthogonalize(g[0]), lambda: ops.orthogonalize(g.double()), lambda: ops.orthogonalize([g, g.half()]),
+                 lambda: ops.orthogonalize([g, g.cpu()]), lambda: ops.orthogonalize(g, 0), lambda: ops.orthogonalize(g, 17),
+                 lambda: ops.orthogonalize(g, 3, [COEF, COEF]), lambda: ops.orthogonalize(g, 5, (30.0, 0.0, 0.0)),
+                 lambda: ops.muon_step([g], [f], [], 0.1), lambda: ops.muon_step([g], [f[:2]], [f], 0.1),
+                 lambda: ops.muon_step([g], [f.half()], [f], 0.1), lambda: ops.muon_step([g.t()], [f.t()], [f.t()], 0.1),
+                 lambda: ops.muon_step([g], [f], [f], 0.1, adjust="none"),
+                 lambda: ops.muon_step([g[:1].expand(4, 6)], [f], [f], 0.1)):
+        with pytest.raises(_lib.DggError):
+            call()
+    assert ops.orthogonalize([]) == []
