@@ -1,5 +1,5 @@
 // Orthogonalisation of matrices by Newton-Schulz products, and the Muon step built on it.
-//   X_0 = U / (|U|_F + eps);   X <- a X + B X,  B = b A + c A^2,  A = X X^T      over the shorter side, `steps` times
+//   X_0 = U / (|U|_F + eps);   X <- B X,  B = a + b A + c A^2,  A = X X^T      over the shorter side, `steps` times
 //   orthogonalize: out = X.   muon step: M <- mu M + s G;  U = s G + mu M (Nesterov) or M;
 //                             W <- (1 - lr wd) W - lr f X      (f: a factor by the matrix' shape)
 // X is m x n with m <= n: a matrix taller than wide is read and written transposed.
@@ -12,12 +12,13 @@
 // plane in every step).  Every operand is kept as TWO fp16 planes, hi = fp16(x), lo = fp16(x - hi), 22 bits together, and a
 // product is hi hi + (hi lo + lo hi) on v_mfma_f32_32x32x16_f16 with fp32 accumulators: what fp32 products give (the dropped
 // lo lo is 2^-22 of a term at most) at a third of the fp16 rate instead of a sixteenth.  fp16's range is no limit: X_0 is U times a power of
-// two (exact: the factor that is left of 1 / (|U| + eps) goes into the first step's coefficients), and every later operand has
+// two (exact: the factor that is left of 1 / (|U| + eps) is applied to the first step's results), and every later operand has
 // a bound that follows from |X_0| and the coefficients (ns_bounds) and is scaled by a power of two to stay below 2^15.
 //
 // Layout.  All products are C[i][j] = sum_k P[i][k] Q[j][k] with k contiguous in both operands: A = X X^T from X stored by rows,
-// A^2 from A (symmetric), B X from B and X stored by columns.  So X is kept in both layouts.  A row is cut into blocks of 32 k, a
-// block is 128 bytes: 32 hi, 32 lo.  Both sizes are padded to multiples of 64 with zeros, which stay zeros in every product.
+// A^2 from A (symmetric), B X from B and X stored by columns.  So X is kept in both layouts.  Planes lie in the order in which the
+// matrix instruction reads them (plane_at): a product's operands go through LDS as they are, and an epilogue's lanes write 512 bytes
+// in a row.  Both sizes are padded to multiples of 64 with zeros, which stay zeros in every product.
 #include <math.h>
 
 #include "dgg_internal.h"
@@ -51,18 +52,21 @@ struct NsMat {
     float step;              // muon: lr f
     // workspace (bytes from its start, for the whole stack)
     size_t xr, xt, a, b, slab, part, scal;
-    int at_norm, at_split, at_gram, at_sum, at_square, at_apply;   // first workgroup in each launch
 };
 
-// One step's coefficients and the bounds that follow from them (ns_bounds): |X| <= r, |b A + c A^2| <= mb, |X'| <= grow |X|
-struct NsStep { float a, b, c, r, mb, grow; };
+// One step's coefficients and the bounds that follow from them (ns_bounds): |X| <= r, |B| <= grow, so |X'| <= grow |X|
+struct NsStep { float a, b, c, r, grow; };
 
 // The powers of two of one matrix in one step: X = planes * sx, planes of A, B and the next X = value * sa, sb, sx_next
 struct NsScale { float sx, sa, sb, sx_next; };
 
+enum { kNorm, kSplit, kGram, kSum, kSquare, kApply, kPhases };
+
+// first workgroup of each matrix in one of the launches (none: INT_MAX)
+struct NsFirst { int at[kNsMats]; };
+
 struct NsArgs {
     NsMat mat[kNsMats];
-    int count;
     char* ws;
     int dtype;               // of in / out
     int muon, nesterov;
@@ -71,23 +75,37 @@ struct NsArgs {
     double lr, eps;
     int steps;
     NsStep step[kNsSteps];
-    int k;                   // the current step
 };
 
-static_assert(sizeof(NsArgs) <= 4096, "kernel arguments");
+static_assert(sizeof(NsArgs) <= 4096 && sizeof(NsArgs) % 8 == 0, "kernel arguments");
 
-__device__ __forceinline__ const NsMat& find(const NsArgs& a, int NsMat::*at, int& local) {
-    int d = 0;
-    for (int i = 1; i < a.count; ++i)
-        if ((int)blockIdx.x >= a.mat[i].*at) d = i;
-    local = (int)blockIdx.x - a.mat[d].*at;
-    return a.mat[d];
+// the matrix a workgroup works on, and its number among the matrix' workgroups
+__device__ __forceinline__ int find(const NsFirst& f, int block, int& local) {
+    int d = 0, at = 0;
+#pragma unroll
+    for (int i = 1; i < kNsMats; ++i)
+        if (block >= f.at[i]) {
+            d = i;
+            at = f.at[i];
+        }
+    local = block - at;
+    return d;
 }
 
-// bytes of one matrix' planes with r rows of k columns
+// Workgroups go to the 8 dies in turn; work items that follow each other share operands: each die takes a run of them, so that
+// they meet in its L2.  (A grid is a permutation of its items for any size.)
+__device__ __forceinline__ int by_die() {
+    const int n = (int)gridDim.x, q = n >> 3, r = n & 7, die = (int)blockIdx.x & 7;
+    return die * q + min(die, r) + ((int)blockIdx.x >> 3);
+}
+
+// Fragment order: the planes of a matrix with rows of k are cut into blocks of 32 rows x 16 k, 2 KB each: hi, then lo; in a plane
+// lane l of the matrix instruction finds its 8 k (16 bytes) at l * 16.  A row group's blocks follow each other along k.
 __host__ __device__ __forceinline__ size_t plane_bytes(int r, int k) { return (size_t)r * k * 4; }
-// halfs from the start of a row's planes to (hi of) column k; lo lies 32 further on
-__device__ __forceinline__ int plane_at(int k) { return (k >> 5) * 64 + (k & 31); }
+// byte offset of (row, k) in the hi plane; lo: 1024 further on
+__device__ __forceinline__ size_t plane_at(int row, int k, int kp) {
+    return ((size_t)(row >> 5) * (kp >> 4) + (k >> 4)) * 2048 + ((k >> 3) & 1) * 512 + (row & 31) * 16 + (k & 7) * 2;
+}
 
 __device__ __forceinline__ float load_as_float(const void* p, long long i, int dtype) {
     if (dtype == DGG_F32) return ((const float*)p)[i];
@@ -110,26 +128,54 @@ __device__ __forceinline__ double block_sum(double v, double* sh /* kThreads / 6
 __device__ __forceinline__ float muon_u(const NsArgs& a, float g, float m) { return a.nesterov ? fmaf(a.mu, m, a.gscale * g) : m; }
 
 // ------------------------------------------------------------------------------------------------ norm
-// sum of squares in 64 bits, one partial a workgroup (muon: M is updated on the way)
-__global__ __launch_bounds__(kThreads) void ns_norm_kernel(NsArgs a) {
+// sum of squares in 64 bits, one partial a workgroup (muon: M is updated on the way).  Rows without gaps are one long row.
+__global__ __launch_bounds__(kThreads) void ns_norm_kernel(NsArgs a, NsFirst first) {
     __shared__ double sh[kThreads / 64];
+    // the launches that follow find the arguments in device memory: 3 KB through the kernel arguments of each would be copied
+    // by the host and read back over the bus every time
+    if (blockIdx.x == 0)
+        for (int i = threadIdx.x; i < (int)(sizeof(NsArgs) / 8); i += kThreads) ((uint64_t*)a.ws)[i] = ((const uint64_t*)&a)[i];
     int local;
-    const NsMat& M = find(a, &NsMat::at_norm, local);
+    const NsMat& M = a.mat[find(first, (int)blockIdx.x, local)];
     const int bat = local / M.parts, part = local - bat * M.parts;
     const char* in = (const char*)M.in + (size_t)bat * M.in_stride * (a.dtype == DGG_F32 ? 4 : 2);
     float* mom = a.muon ? M.mom + (size_t)bat * M.mom_stride : nullptr;
+    const bool flat = M.ld_in == M.cols && (!a.muon || M.ld_mom == M.cols);
     const long long total = (long long)M.rows * M.cols;
+    // a workgroup's share: a range of the long row, or whole rows
+    const long long per = flat ? ((total + M.parts - 1) / M.parts + 63) / 64 * 64 : 0;
+    const int row0 = flat ? 0 : part, rows = flat ? 1 : M.rows, drow = flat ? 1 : M.parts;
+    const long long c0 = flat ? part * per : 0, c1 = flat ? (c0 + per < total ? c0 + per : total) : M.cols;
     double s = 0.0;
-    for (long long e = (long long)part * kThreads + threadIdx.x; e < total; e += (long long)M.parts * kThreads) {
-        const long long r = e / M.cols, c = e - r * M.cols;
-        float u = load_as_float(in, r * M.ld_in + c, a.dtype);
-        if (a.muon) {
-            float* mp = mom + r * M.ld_mom + c;
-            const float m = fmaf(a.mu, *mp, a.gscale * u);
-            *mp = m;
-            u = muon_u(a, u, m);
+    for (int r = row0; r < rows; r += drow) {
+        const long long gi = (long long)r * M.ld_in, mi = (long long)r * M.ld_mom;
+        long long c = c0 + threadIdx.x;
+        for (; c + 3 * kThreads < c1; c += 4 * kThreads) {   // four loads in flight
+            float u[4], m[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                u[e] = load_as_float(in, gi + c + e * kThreads, a.dtype);
+                if (a.muon) m[e] = mom[mi + c + e * kThreads];
+            }
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                if (a.muon) {
+                    m[e] = fmaf(a.mu, m[e], a.gscale * u[e]);
+                    mom[mi + c + e * kThreads] = m[e];
+                    u[e] = muon_u(a, u[e], m[e]);
+                }
+                s = fma((double)u[e], (double)u[e], s);
+            }
         }
-        s = fma((double)u, (double)u, s);
+        for (; c < c1; c += kThreads) {
+            float u = load_as_float(in, gi + c, a.dtype);
+            if (a.muon) {
+                const float m = fmaf(a.mu, mom[mi + c], a.gscale * u);
+                mom[mi + c] = m;
+                u = muon_u(a, u, m);
+            }
+            s = fma((double)u, (double)u, s);
+        }
     }
     s = block_sum(s, sh);
     if (threadIdx.x == 0) ((double*)(a.ws + M.part))[(size_t)bat * M.parts + part] = s;
@@ -141,173 +187,206 @@ __device__ __forceinline__ void split2(float x, _Float16& hi, _Float16& lo) {
     lo = (_Float16)(x - (float)hi);
 }
 
+// eight k of a row, at their place in the hi plane
+__device__ __forceinline__ void store8(char* p, const float (&v)[8]) {
+    half8 hi, lo;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+        _Float16 h, l;
+        split2(v[e], h, l);
+        hi[e] = h;
+        lo[e] = l;
+    }
+    *(half8*)p = hi;
+    *(half8*)(p + 1024) = lo;
+}
+
 // the power of two that brings `bound` into [2^14, 2^15)
 __device__ __forceinline__ float below(float bound) { return ldexpf(1.f, 14 - ilogbf(bound)); }
 
+// every operand's bound: the one of the coefficients, or, for a norm far below eps, what |X_0| can have grown to
+__device__ __forceinline__ void scales(const NsArgs& a, double norm, int k, NsScale* o) {
+    float r = (float)(norm / (norm + a.eps));
+    if (!(r > 0x1p-40f)) r = 0x1p-40f;
+    float sx = (float)(1.0 / ldexp(norm + a.eps, k));
+    for (int i = 0; i < a.steps; ++i) {
+        const NsStep S = a.step[i];
+        r = fminf(1.01f * r, S.r);
+        const float next = S.grow * r;
+        NsScale z;
+        z.sx = sx;
+        z.sa = below(r * r);
+        z.sb = below(S.grow);
+        z.sx_next = below(i + 1 < a.steps ? fminf(next, a.step[i + 1].r) : next);
+        o[i] = z;
+        sx = 1.f / z.sx_next;
+        r = next;
+    }
+}
+
 // 64 x 64 of X: U read along its rows, written by rows and by columns of X as planes of U * 2^k
-__global__ __launch_bounds__(kThreads) void ns_split_kernel(NsArgs a) {
+__global__ __launch_bounds__(kThreads) void ns_split_kernel(const NsArgs* args, NsFirst first) {
+    const NsArgs& a = *args;
     __shared__ double sh[kThreads / 64];
     __shared__ float t[64][65];   // [i][j] of X
     int local;
-    const NsMat& M = find(a, &NsMat::at_split, local);
+    const NsMat M = a.mat[find(first, (int)blockIdx.x, local)];
     const int ti = M.mp / 64, tj = M.np / 64;
     const int bat = local / (ti * tj), tile = local - bat * ti * tj, i0 = tile / tj * 64, j0 = tile % tj * 64;
+    const char* in = (const char*)M.in + (size_t)bat * M.in_stride * (a.dtype == DGG_F32 ? 4 : 2);
+    const float* mom = a.muon ? M.mom + (size_t)bat * M.mom_stride : nullptr;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int r0 = M.turned ? j0 : i0, c0 = M.turned ? i0 : j0;   // of U
+    float u[16], m[16];   // all of the tile is in flight while the norm is summed
+#pragma unroll
+    for (int q = 0; q < 16; ++q) {
+        const int r = r0 + q * 4 + wave, c = c0 + lane;
+        const bool in_u = r < M.rows && c < M.cols;
+        u[q] = in_u ? load_as_float(in, (long long)r * M.ld_in + c, a.dtype) : 0.f;
+        m[q] = in_u && a.muon ? mom[(long long)r * M.ld_mom + c] : 0.f;
+    }
     double s = 0.0;
     for (int p = threadIdx.x; p < M.parts; p += kThreads) s += ((const double*)(a.ws + M.part))[(size_t)bat * M.parts + p];
     const double norm = sqrt(block_sum(s, sh));
     // 2^k |U| in [2^14, 2^15): no element of the planes is larger.  A zero, infinite or NaN norm keeps k = 0.
     const int k = norm > 0.0 && norm < INFINITY ? 14 - ilogb(norm) : 0;
-    if (tile == 0 && threadIdx.x == 0) {
-        // every operand's bound: the one of the coefficients, or, for a norm far below eps, what |X_0| can have grown to
-        NsScale* o = (NsScale*)(a.ws + M.scal) + (size_t)bat * kNsSteps;
-        float r = (float)(norm / (norm + a.eps));
-        if (!(r > 0x1p-40f)) r = 0x1p-40f;
-        float sx = (float)(1.0 / ldexp(norm + a.eps, k));
-        for (int i = 0; i < a.steps; ++i) {
-            const NsStep& S = a.step[i];
-            r = fminf(1.01f * r, S.r);
-            const float next = S.grow * r;
-            NsScale z;
-            z.sx = sx;
-            z.sa = below(r * r);
-            z.sb = below(fmaxf(fminf(S.mb, (fabsf(S.b) + fabsf(S.c) * r * r) * r * r), 0x1p-100f));
-            z.sx_next = below(i + 1 < a.steps ? fminf(next, a.step[i + 1].r) : next);
-            o[i] = z;
-            sx = 1.f / z.sx_next;
-            r = next;
-        }
-    }
-    const char* in = (const char*)M.in + (size_t)bat * M.in_stride * (a.dtype == DGG_F32 ? 4 : 2);
-    const float* mom = a.muon ? M.mom + (size_t)bat * M.mom_stride : nullptr;
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const int r0 = M.turned ? j0 : i0, c0 = M.turned ? i0 : j0;   // of U
-    for (int q = wave; q < 64; q += 4) {
-        const int r = r0 + q, c = c0 + lane;
-        float u = 0.f;
-        if (r < M.rows && c < M.cols) {
-            u = load_as_float(in, (long long)r * M.ld_in + c, a.dtype);
-            if (a.muon) u = muon_u(a, u, mom[(long long)r * M.ld_mom + c]);
-            u = (float)ldexp((double)u, k);
-        }
-        if (M.turned) t[lane][q] = u;
-        else t[q][lane] = u;
+    if (tile == 0 && threadIdx.x == 0) scales(a, norm, k, (NsScale*)(a.ws + M.scal) + (size_t)bat * kNsSteps);
+#pragma unroll
+    for (int q = 0; q < 16; ++q) {
+        const float v = ldexpf(a.muon ? muon_u(a, u[q], m[q]) : u[q], k);
+        if (M.turned) t[lane][q * 4 + wave] = v;
+        else t[q * 4 + wave][lane] = v;
     }
     __syncthreads();
-    _Float16* xr = (_Float16*)(a.ws + M.xr + (size_t)bat * plane_bytes(M.mp, M.np));
-    _Float16* xt = (_Float16*)(a.ws + M.xt + (size_t)bat * 2 * plane_bytes(M.np, M.mp));
+    char* xr = a.ws + M.xr + (size_t)bat * plane_bytes(M.mp, M.np);
+    char* xt = a.ws + M.xt + (size_t)bat * 2 * plane_bytes(M.np, M.mp);
     // 64 rows of 64 k: 8 k a thread, twice per layout
     for (int q = threadIdx.x; q < 512; q += kThreads) {
-        const int row = q >> 3, k8 = (q & 7) * 8;
-        half8 hi, lo, thi, tlo;
+        const int row = q & 63, k8 = (q >> 6) * 8;
+        float v[8], w[8];
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
-            _Float16 h, l;
-            split2(t[row][k8 + e], h, l);
-            hi[e] = h; lo[e] = l;
-            split2(t[k8 + e][row], h, l);
-            thi[e] = h; tlo[e] = l;
+            v[e] = t[row][k8 + e];
+            w[e] = t[k8 + e][row];
         }
-        _Float16* o = xr + (size_t)(i0 + row) * M.np * 2 + plane_at(j0 + k8);
-        *(half8*)o = hi;
-        *(half8*)(o + 32) = lo;
-        o = xt + (size_t)(j0 + row) * M.mp * 2 + plane_at(i0 + k8);
-        *(half8*)o = thi;
-        *(half8*)(o + 32) = tlo;
+        store8(xr + plane_at(i0 + row, j0 + k8, M.np), v);
+        store8(xt + plane_at(j0 + row, i0 + k8, M.mp), w);
     }
 }
 
 // ------------------------------------------------------------------------------------------------ product
-// acc[64 x 64 per wave: 2 x 2 blocks of 32 x 32] of C[i][j] = sum_k P[i][k] Q[j][k], TM x TN = 32 fi * 2 x 32 fj * 2 per workgroup,
-// waves 2 x 2.  P, Q: row 0's planes; rows beyond the last are read as the last (their results are not stored).
-// LDS: two stages of (TM + TN) rows x 128 bytes.  The 16-byte chunk q of row r lies at chunk q ^ ((r >> 1) & 7): a fragment's 16
-// rows then fall on 16 different groups of banks.  The swizzle is in the GLOBAL address: LDS-DMA writes lane by lane.
-template <int FI, int FJ>
+// C[i][j] = sum_k P[i][k] Q[j][k]: a workgroup of 2 x 2 waves owns a tile of 64 F x 64 F of C, a wave F x F blocks of 32 x 32.  P, Q: row
+// group 0 of planes in fragment order; row groups beyond the last are read as the last (their results are not stored).
+// A stage is 32 k of both operands, 16 F KB, copied by LDS-DMA as it lies (a fragment is 1 KB in a row, lane by lane: no bank
+// conflicts, no swizzle).  S stages, S - 1 of them in flight; the fragments of the next 16 k are read while the current ones are
+// multiplied.  F = 1 is bound by LDS (1.3 KB read a matrix instruction and as much again written every third, 128 B a cycle),
+// F = 2 by half of that.  hi hi and the two cross terms have accumulators of their own: the small ones are not rounded at the
+// size of the large.
+template <int F, int S>
 struct Prod {
-    static constexpr int TM = 64 * FI, TN = 64 * FJ, kStage = (TM + TN) * 128;
-    static constexpr int kLds = 2 * kStage;
+    static constexpr int kTile = 64 * F, kStage = 16384 * F, kLds = S * kStage, kPieces = 4 * F;   // pieces a wave and stage
+    f32x16 hh[F][F], cross[F][F];
+    struct Frags { half8 ph[F], pl[F], qh[F], ql[F]; };
 
-    __device__ static __forceinline__ void run(const char* P, int prow, int prows, const char* Q, int qrow, int qrows,
-                                               size_t pitch, int kb0, int kb1, f32x16 (&acc)[FI][FJ]) {
+    template <int N> __device__ static __forceinline__ void wait() {   // all but the newest N pieces have landed; everyone's
+        asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(N) : "memory");
+    }
+    __device__ __forceinline__ void multiply(const Frags& x) {
+#pragma unroll
+        for (int i = 0; i < F; ++i)
+#pragma unroll
+            for (int j = 0; j < F; ++j) cross[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(x.ph[i], x.ql[j], cross[i][j], 0, 0, 0);
+#pragma unroll
+        for (int i = 0; i < F; ++i)
+#pragma unroll
+            for (int j = 0; j < F; ++j) hh[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(x.ph[i], x.qh[j], hh[i][j], 0, 0, 0);
+#pragma unroll
+        for (int i = 0; i < F; ++i)
+#pragma unroll
+            for (int j = 0; j < F; ++j) cross[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(x.pl[i], x.qh[j], cross[i][j], 0, 0, 0);
+    }
+
+    __device__ __forceinline__ void run(const char* P, int prow, int prows, const char* Q, int qrow, int qrows, int kp, int kb0, int kb1) {
         extern __shared__ char smem[];
         const unsigned lds = (unsigned)(size_t)(lds_char*)smem;
-        const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, wi = wave >> 1, wj = wave & 1;
-        const int c = tid & 7, rr = tid >> 3;
-        constexpr int NP = TM / 32, NQ = TN / 32;
-        const char* src[NP + NQ];
+        const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6), wi = wave >> 1, wj = wave & 1;
+        // of every row group a wave fetches one piece: a plane of 16 k
+        const char* src[4 * F];
 #pragma unroll
-        for (int t = 0; t < NP + NQ; ++t) {
-            const int row = (t < NP ? t : t - NP) * 32 + rr;
-            const int at = t < NP ? min(prow + row, prows - 1) : min(qrow + row, qrows - 1);
-            src[t] = (t < NP ? P : Q) + (size_t)at * pitch + (size_t)((c ^ ((row >> 1) & 7)) * 16);
+        for (int g = 0; g < 4 * F; ++g) {
+            const int at = g < 2 * F ? min(prow / 32 + g, prows / 32 - 1) : min(qrow / 32 + g - 2 * F, qrows / 32 - 1);
+            src[g] = (g < 2 * F ? P : Q) + (size_t)at * kp * 128 + wave * 1024 + lane * 16;
         }
-        auto fetch = [&](int kb, int stage) {
+        const int n = kb1 - kb0;
+        auto fetch = [&](int s) {
+            const unsigned to = lds + wave * 1024 + (unsigned)(s % S) * kStage;
 #pragma unroll
-            for (int t = 0; t < NP + NQ; ++t)
-                __builtin_amdgcn_global_load_lds(
-                    reinterpret_cast<const float*>(src[t] + (size_t)kb * 128),
-                    (lds_f32*)(size_t)__builtin_amdgcn_readfirstlane(lds + stage * kStage + t * 4096 + wave * 1024), 16, 0, 0);
+            for (int g = 0; g < 4 * F; ++g)
+                __builtin_amdgcn_global_load_lds(reinterpret_cast<const float*>(src[g] + (size_t)(kb0 + s) * 4096),
+                                                 (lds_f32*)(size_t)(to + g * 4096), 16, 0, 0);
         };
-        const int fr = lane & 31, fk = lane >> 5;
-        auto frag = [&](int stage, int base_row, int plane, int kk) {
-            const int row = base_row + fr, chunk = (plane * 4 + kk * 2 + fk) ^ ((row >> 1) & 7);
-            return *(lds_half8*)(size_t)(lds + stage * kStage + row * 128 + chunk * 16);
-        };
-        fetch(kb0, 0);
-        for (int kb = kb0; kb < kb1; ++kb) {
-            const int st = (kb - kb0) & 1;
-            asm volatile("s_waitcnt vmcnt(0)" ::: "memory");   // this stage's pieces have landed (LDS-DMA is counted by vmcnt)
-            __syncthreads();                                   // .. everyone's; and everyone is done with the other stage
-            if (kb + 1 < kb1) fetch(kb + 1, st ^ 1);
+        const unsigned at_p = lds + lane * 16 + wi * F * 4096, at_q = lds + lane * 16 + (2 + wj) * F * 4096;
+        auto read = [&](int s, int kk, Frags& x) {
+            const unsigned o = (unsigned)(s % S) * kStage + kk * 2048;
 #pragma unroll
-            for (int kk = 0; kk < 2; ++kk) {
-                half8 ph[FI], pl[FI], qh[FJ], ql[FJ];
-#pragma unroll
-                for (int i = 0; i < FI; ++i) {
-                    ph[i] = frag(st, (wi * FI + i) * 32, 0, kk);
-                    pl[i] = frag(st, (wi * FI + i) * 32, 1, kk);
-                }
-#pragma unroll
-                for (int j = 0; j < FJ; ++j) {
-                    qh[j] = frag(st, TM + (wj * FJ + j) * 32, 0, kk);
-                    ql[j] = frag(st, TM + (wj * FJ + j) * 32, 1, kk);
-                }
-#pragma unroll
-                for (int i = 0; i < FI; ++i)
-#pragma unroll
-                    for (int j = 0; j < FJ; ++j) {
-                        acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(ph[i], ql[j], acc[i][j], 0, 0, 0);
-                        acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(pl[i], qh[j], acc[i][j], 0, 0, 0);
-                        acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(ph[i], qh[j], acc[i][j], 0, 0, 0);
-                    }
+            for (int i = 0; i < F; ++i) {
+                x.ph[i] = *(lds_half8*)(size_t)(at_p + o + i * 4096);
+                x.ql[i] = *(lds_half8*)(size_t)(at_q + o + i * 4096 + 1024);
+                x.qh[i] = *(lds_half8*)(size_t)(at_q + o + i * 4096);
+                x.pl[i] = *(lds_half8*)(size_t)(at_p + o + i * 4096 + 1024);
             }
+        };
+#pragma unroll
+        for (int i = 0; i < F; ++i)
+#pragma unroll
+            for (int j = 0; j < F; ++j)
+#pragma unroll
+                for (int e = 0; e < 16; ++e) hh[i][j][e] = cross[i][j][e] = 0.f;
+#pragma unroll
+        for (int s = 0; s < S; ++s)
+            if (s < n) fetch(s);
+        if (n >= S) wait<(S - 1) * kPieces>();
+        else wait<0>();
+        Frags even, odd;
+        read(0, 0, even);
+        for (int s = 0; s < n; ++s) {
+            read(s, 1, odd);
+            multiply(even);
+            if (s + 1 < n) {
+                // stage s + 1 has landed, and everyone has read all of stage s (their reads have returned: lgkmcnt): its place is free
+                if (s + S <= n) wait<(S - 2) * kPieces>();
+                else wait<0>();
+                if (s + S < n) fetch(s + S);
+                read(s + 1, 0, even);
+            }
+            multiply(odd);
         }
+        wait<0>();   // the LDS is free for the epilogue
     }
 
-    // calls f(i, j, v) for the thread's elements, four consecutive i at a time: v[0..3] at rows i .. i + 3, column j
-    template <typename F> __device__ static __forceinline__ void each(const f32x16 (&acc)[FI][FJ], F f) {
-        const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, wi = wave >> 1, wj = wave & 1;
+    // The lane's elements of block (f, g): four runs q of four consecutive i, (i0 + 32 f + 8 q + e, j0 + 32 g).
+    __device__ static __forceinline__ int i0() { return ((threadIdx.x >> 7) & 1) * 32 * F + ((threadIdx.x >> 5) & 1) * 4; }
+    __device__ static __forceinline__ int j0() { return ((threadIdx.x >> 6) & 1) * 32 * F + (threadIdx.x & 31); }
+    __device__ __forceinline__ float value(int f, int g, int q, int e) const { return hh[f][g][4 * q + e] + cross[f][g][4 * q + e]; }
+
+    // v[q][e] -> w[q][0..7] at row ti() + 32 f, columns tj() + 32 g + 16 q ..: a 32 x 32 block is turned in 4.5 KB of LDS of the wave's
+    // own (pitch 36: 16-byte stores, and reads of 32 rows on 32 banks)
+    __device__ static __forceinline__ int ti() { return ((threadIdx.x >> 7) & 1) * 32 * F + (threadIdx.x & 31); }
+    __device__ static __forceinline__ int tj() { return ((threadIdx.x >> 6) & 1) * 32 * F + ((threadIdx.x >> 5) & 1) * 8; }
+    __device__ static __forceinline__ void turn(const float (&v)[4][4], float (&w)[2][8]) {
+        extern __shared__ char smem[];
+        const int lane = threadIdx.x & 63, r = lane & 31, h = lane >> 5;
+        float* t = reinterpret_cast<float*>(smem) + (threadIdx.x >> 6) * (32 * 36);
 #pragma unroll
-        for (int i = 0; i < FI; ++i)
+        for (int q = 0; q < 4; ++q) *reinterpret_cast<float4*>(t + r * 36 + 8 * q + 4 * h) = make_float4(v[q][0], v[q][1], v[q][2], v[q][3]);
+        __builtin_amdgcn_wave_barrier();   // (the wave's own LDS, in order: no workgroup barrier)
 #pragma unroll
-            for (int j = 0; j < FJ; ++j)
+        for (int q = 0; q < 2; ++q)
 #pragma unroll
-                for (int q = 0; q < 4; ++q) {
-                    float v[4];
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) v[e] = acc[i][j][4 * q + e];
-                    f((wi * FI + i) * 32 + 8 * q + 4 * (lane >> 5), (wj * FJ + j) * 32 + (lane & 31), v);
-                }
+            for (int e = 0; e < 8; ++e) w[q][e] = t[(16 * q + 8 * h + e) * 36 + r];
+        __builtin_amdgcn_wave_barrier();
     }
 };
-
-template <int FI, int FJ> __device__ __forceinline__ void zero(f32x16 (&acc)[FI][FJ]) {
-#pragma unroll
-    for (int i = 0; i < FI; ++i)
-#pragma unroll
-        for (int j = 0; j < FJ; ++j)
-#pragma unroll
-            for (int e = 0; e < 16; ++e) acc[i][j][e] = 0.f;
-}
 
 // tile number -> (ti, tj) with ti <= tj, of a t x t grid, row by row
 __device__ __forceinline__ void upper(int tile, int t, int& ti, int& tj) {
@@ -319,12 +398,12 @@ __device__ __forceinline__ void upper(int tile, int t, int& ti, int& tj) {
     tj = ti + tile;
 }
 
-__device__ __forceinline__ NsScale scale_of(const NsArgs& a, const NsMat& M, int bat) {
-    return ((const NsScale*)(a.ws + M.scal))[(size_t)bat * kNsSteps + a.k];
+__device__ __forceinline__ NsScale scale_of(const NsArgs& a, const NsMat& M, int bat, int k) {
+    return ((const NsScale*)(a.ws + M.scal))[(size_t)bat * kNsSteps + k];
 }
 
-// four values at rows i .. i + 3 of column j into planes stored by columns (row j, k = i ..): 8 bytes each
-__device__ __forceinline__ void store_planes_t(_Float16* base, size_t pitch, int i, int j, const float (&v)[4]) {
+// four k of a row, at their place in the hi plane: written, and read as the values they stand for
+__device__ __forceinline__ void store4(char* p, const float (&v)[4]) {
     half4 hi, lo;
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
@@ -333,116 +412,106 @@ __device__ __forceinline__ void store_planes_t(_Float16* base, size_t pitch, int
         hi[e] = h;
         lo[e] = l;
     }
-    _Float16* o = base + (size_t)j * pitch + plane_at(i);
-    *(half4*)o = hi;
-    *(half4*)(o + 32) = lo;
+    *(half4*)p = hi;
+    *(half4*)(p + 1024) = lo;
 }
-// .. and stored by rows (row i + e, k = j)
-__device__ __forceinline__ void store_planes(_Float16* base, size_t pitch, int i, int j, const float (&v)[4]) {
+__device__ __forceinline__ void load4(const char* p, float (&v)[4]) {
+    const half4 hi = *(const half4*)p, lo = *(const half4*)(p + 1024);
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {
-        _Float16 h, l;
-        split2(v[e], h, l);
-        _Float16* o = base + (size_t)(i + e) * pitch + plane_at(j);
-        o[0] = h;
-        o[32] = l;
-    }
-}
-__device__ __forceinline__ float load_plane(const _Float16* base, size_t pitch, int r, int k) {
-    const _Float16* p = base + (size_t)r * pitch + plane_at(k);
-    return (float)p[0] + (float)p[32];
+    for (int e = 0; e < 4; ++e) v[e] = (float)hi[e] + (float)lo[e];
 }
 
 // A = X X^T, tiles on and above the diagonal, a range of k each: fp32 slabs [split][mp][mp]
-template <int F>
-__global__ __launch_bounds__(kThreads) void ns_gram_kernel(NsArgs a) {
+template <int S>
+__global__ __launch_bounds__(kThreads) void ns_gram_kernel(const NsArgs* args, NsFirst first, int k) {
+    using Pr = Prod<1, S>;
+    const NsArgs& a = *args;
     int local;
-    const NsMat& M = find(a, &NsMat::at_gram, local);
-    const int t = (M.mp + 64 * F - 1) / (64 * F), tiles = t * (t + 1) / 2, per = tiles * M.splits;
+    const NsMat M = a.mat[find(first, by_die(), local)];
+    const int t = M.mp / Pr::kTile, tiles = t * (t + 1) / 2, per = tiles * M.splits;
     const int bat = local / per, rest = local - bat * per, split = rest / tiles;
     int ti, tj;
     upper(rest - split * tiles, t, ti, tj);
     const char* x = a.ws + M.xr + (size_t)bat * plane_bytes(M.mp, M.np);
-    f32x16 acc[F][F];
-    zero(acc);
-    const int kb0 = split * M.kblocks, kb1 = min(kb0 + M.kblocks, M.np / 32);
-    Prod<F, F>::run(x, ti * 64 * F, M.mp, x, tj * 64 * F, M.mp, (size_t)M.np * 4, kb0, kb1, acc);
-    float* slab = (float*)(a.ws + M.slab) + ((size_t)bat * M.splits + split) * M.mp * M.mp;
-    Prod<F, F>::each(acc, [&](int i, int j, const float (&v)[4]) {
-        i += ti * 64 * F;
-        j += tj * 64 * F;
-        if (j >= M.mp) return;
+    Pr p;
+    p.run(x, ti * Pr::kTile, M.mp, x, tj * Pr::kTile, M.mp, M.np, split * M.kblocks, min((split + 1) * M.kblocks, M.np / 32));
+    const int i0 = ti * Pr::kTile + p.i0(), j0 = tj * Pr::kTile + p.j0();
+    float* slab = (float*)(a.ws + M.slab) + ((size_t)bat * M.splits + split) * M.mp * M.mp + (size_t)i0 * M.mp + j0;
 #pragma unroll
-        for (int e = 0; e < 4; ++e)
-            if (i + e < M.mp) slab[(size_t)(i + e) * M.mp + j] = v[e];
-    });
+    for (int q = 0; q < 4; ++q)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) slab[(size_t)(8 * q + e) * M.mp] = p.value(0, 0, q, e);
 }
 
 // sums the slabs in order: planes of A, both triangles; 32 x 32 elements a workgroup
-__global__ __launch_bounds__(kThreads) void ns_sum_kernel(NsArgs a) {
+__global__ __launch_bounds__(kThreads) void ns_sum_kernel(const NsArgs* args, NsFirst first, int k) {
+    const NsArgs& a = *args;
     __shared__ float t[32][33];
     int local;
-    const NsMat& M = find(a, &NsMat::at_sum, local);
+    const NsMat M = a.mat[find(first, by_die(), local)];
     const int n32 = M.mp / 32, tiles = n32 * (n32 + 1) / 2, bat = local / tiles;
     int ti, tj;
     upper(local - bat * tiles, n32, ti, tj);
-    const NsScale z = scale_of(a, M, bat);
-    const float* slab = (const float*)(a.ws + M.slab) + (size_t)bat * M.splits * M.mp * M.mp;
-    _Float16* A = (_Float16*)(a.ws + M.a + (size_t)bat * plane_bytes(M.mp, M.mp));
-    const int c = threadIdx.x & 31;
-    for (int r = threadIdx.x >> 5; r < 32; r += 8) {
-        const size_t at = (size_t)(ti * 32 + r) * M.mp + tj * 32 + c;
-        float v = 0.f;
-        for (int sp = 0; sp < M.splits; ++sp) v += slab[(size_t)sp * M.mp * M.mp + at];
-        t[r][c] = v * z.sx * z.sx * z.sa;   // (in this order: sx * sx alone may be below fp32's range)
+    const NsScale z = scale_of(a, M, bat, k);
+    const size_t slab = (size_t)M.mp * M.mp;
+    const int r0 = threadIdx.x >> 3, c0 = (threadIdx.x & 7) * 4;
+    const float* p = (const float*)(a.ws + M.slab) + (size_t)bat * M.splits * slab + (size_t)(ti * 32 + r0) * M.mp + tj * 32 + c0;
+    float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 8
+    for (int sp = 0; sp < M.splits; ++sp) {
+        const float4 w = *reinterpret_cast<const float4*>(p + sp * slab);
+        v.x += w.x;
+        v.y += w.y;
+        v.z += w.z;
+        v.w += w.w;
     }
-    __syncthreads();
-    // a 32 x 32 block is one 128-byte piece of each row: 4 threads x 8 k of hi and lo; then the block's mirror image
-    const int row = threadIdx.x >> 2, k8 = (threadIdx.x & 3) * 8;
-    if (row < 64) {
-        const int r = row & 31, mirror = row >> 5;
-        half8 hi, lo;
+    const float* pv = &v.x;
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-            _Float16 h, l;
-            split2(mirror || (ti == tj && k8 + e < r) ? t[k8 + e][r] : t[r][k8 + e], h, l);
-            hi[e] = h;
-            lo[e] = l;
-        }
-        if (!mirror || ti != tj) {
-            _Float16* o = A + (size_t)((mirror ? tj : ti) * 32 + r) * M.mp * 2 + (mirror ? ti : tj) * 64 + k8;
-            *(half8*)o = hi;
-            *(half8*)(o + 32) = lo;
-        }
-    }
+    for (int e = 0; e < 4; ++e) t[r0][c0 + e] = pv[e] * z.sx * z.sx * z.sa;   // (in this order: sx * sx alone may be below fp32's range)
+    __syncthreads();
+    // 8 k of a row a thread: the block, then its mirror image
+    const int r = threadIdx.x & 31, k8 = ((threadIdx.x >> 5) & 3) * 8, mirror = threadIdx.x >> 7;
+    if (mirror && ti == tj) return;
+    float w[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) w[e] = mirror || (ti == tj && k8 + e < r) ? t[k8 + e][r] : t[r][k8 + e];
+    char* A = a.ws + M.a + (size_t)bat * plane_bytes(M.mp, M.mp);
+    store8(A + plane_at((mirror ? tj : ti) * 32 + r, (mirror ? ti : tj) * 32 + k8, M.mp), w);
 }
 
-// B = b A + c A^2, tiles on and above the diagonal and their mirror images
-template <int F>
-__global__ __launch_bounds__(kThreads) void ns_square_kernel(NsArgs a) {
+// B = a + b A + c A^2, tiles on and above the diagonal and their mirror images
+template <int S>
+__global__ __launch_bounds__(kThreads) void ns_square_kernel(const NsArgs* args, NsFirst first, int k) {
+    using Pr = Prod<1, S>;
+    const NsArgs& a = *args;
     int local;
-    const NsMat& M = find(a, &NsMat::at_square, local);
-    const int t = (M.mp + 64 * F - 1) / (64 * F), tiles = t * (t + 1) / 2, bat = local / tiles;
+    const NsMat M = a.mat[find(first, by_die(), local)];
+    const int t = M.mp / Pr::kTile, tiles = t * (t + 1) / 2, bat = local / tiles;
     int ti, tj;
     upper(local - bat * tiles, t, ti, tj);
-    const _Float16* A = (const _Float16*)(a.ws + M.a + (size_t)bat * plane_bytes(M.mp, M.mp));
-    _Float16* B = (_Float16*)(a.ws + M.b + (size_t)bat * plane_bytes(M.mp, M.mp));
-    f32x16 acc[F][F];
-    zero(acc);
-    Prod<F, F>::run((const char*)A, ti * 64 * F, M.mp, (const char*)A, tj * 64 * F, M.mp, (size_t)M.mp * 4, 0, M.mp / 32, acc);
-    const NsScale z = scale_of(a, M, bat);
-    const float ratio = z.sb / z.sa, fb = a.step[a.k].b * ratio, fc = a.step[a.k].c * ratio / z.sa;
-    const size_t pitch = (size_t)M.mp * 2;
-    Prod<F, F>::each(acc, [&](int i, int j, const float (&v)[4]) {
-        i += ti * 64 * F;
-        j += tj * 64 * F;
-        if (i >= M.mp || j >= M.mp) return;
-        float w[4];
+    const char* A = a.ws + M.a + (size_t)bat * plane_bytes(M.mp, M.mp);
+    char* B = a.ws + M.b + (size_t)bat * plane_bytes(M.mp, M.mp);
+    Pr p;
+    const int i0 = ti * Pr::kTile, j0 = tj * Pr::kTile, i = i0 + p.i0(), j = j0 + p.j0();
+    const size_t at = plane_at(j, i, M.mp);   // row j, k = i: A and B are symmetric
+    float v[4][4];
 #pragma unroll
-        for (int e = 0; e < 4; ++e) w[e] = fmaf(fc, v[e], fb * load_plane(A, pitch, j, i + e));
-        if (ti != tj) store_planes_t(B, pitch, i, j, w);
-        store_planes(B, pitch, i, j, w);
-    });
+    for (int q = 0; q < 4; ++q) load4(A + at + (q >> 1) * 2048 + (q & 1) * 512, v[q]);
+    const NsScale z = scale_of(a, M, bat, k);
+    const float ratio = z.sb / z.sa, fa = a.step[k].a * z.sb, fb = a.step[k].b * ratio, fc = a.step[k].c * ratio / z.sa;
+    p.run(A, i0, M.mp, A, j0, M.mp, M.mp, 0, M.mp / 32);
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+            v[q][e] = fmaf(fc, p.value(0, 0, q, e), fmaf(fb, v[q][e], i + 8 * q + e == j ? fa : 0.f));
+        store4(B + at + (q >> 1) * 2048 + (q & 1) * 512, v[q]);
+    }
+    if (ti == tj) return;
+    float w[2][8];
+    p.turn(v, w);
+#pragma unroll
+    for (int q = 0; q < 2; ++q) store8(B + plane_at(i0 + p.ti(), j0 + p.tj() + 16 * q, M.mp), w[q]);
 }
 
 __device__ __forceinline__ void store_as(void* p, long long i, float v, int dtype) {
@@ -451,76 +520,91 @@ __device__ __forceinline__ void store_as(void* p, long long i, float v, int dtyp
     else ((_Float16*)p)[i] = (_Float16)v;
 }
 
-// X <- a X + B X: planes in both layouts, or (last step) the result
-template <int FI, int FJ>
-__global__ __launch_bounds__(kThreads) void ns_apply_kernel(NsArgs a) {
+// X <- B X: planes in both layouts, or (last step) the result
+template <int F, int S>
+__global__ __launch_bounds__(kThreads, 2) void ns_apply_kernel(const NsArgs* args, NsFirst first, int k) {
+    using Pr = Prod<F, S>;
+    const NsArgs& a = *args;
     int local;
-    const NsMat& M = find(a, &NsMat::at_apply, local);
-    using Pr = Prod<FI, FJ>;
-    const int ti = (M.mp + Pr::TM - 1) / Pr::TM, tj = (M.np + Pr::TN - 1) / Pr::TN;
-    const int bat = local / (ti * tj), tile = local - bat * ti * tj, i0 = tile % ti * Pr::TM, j0 = tile / ti * Pr::TN;
+    const NsMat M = a.mat[find(first, by_die(), local)];
+    const int ti = (M.mp + Pr::kTile - 1) / Pr::kTile, tj = (M.np + Pr::kTile - 1) / Pr::kTile;
+    const int bat = local / (ti * tj), tile = local - bat * ti * tj, i0 = tile % ti * Pr::kTile, j0 = tile / ti * Pr::kTile;
     const char* B = a.ws + M.b + (size_t)bat * plane_bytes(M.mp, M.mp);
     const size_t xtb = plane_bytes(M.np, M.mp);
-    const int flip = a.k & 1;   // which half of xt holds X
-    const _Float16* xt = (const _Float16*)(a.ws + M.xt + ((size_t)bat * 2 + flip) * xtb);
-    _Float16* xt_next = (_Float16*)(a.ws + M.xt + ((size_t)bat * 2 + (flip ^ 1)) * xtb);
-    _Float16* xr = (_Float16*)(a.ws + M.xr + (size_t)bat * plane_bytes(M.mp, M.np));
-    f32x16 acc[FI][FJ];
-    zero(acc);
-    Pr::run(B, i0, M.mp, (const char*)xt, j0, M.np, (size_t)M.mp * 4, 0, M.mp / 32, acc);
-    const NsScale z = scale_of(a, M, bat);
-    const float fx = a.step[a.k].a * z.sx, fb = z.sx / z.sb;
-    const size_t pt = (size_t)M.mp * 2, pr = (size_t)M.np * 2;
-    const size_t es = a.dtype == DGG_F32 ? 4 : 2;
-    char* out = (char*)M.out + (size_t)bat * M.out_stride * es;
-    Pr::each(acc, [&](int i, int j, const float (&v)[4]) {
-        i += i0;
-        j += j0;
-        if (i >= M.mp || j >= M.np) return;
-        float y[4];
+    const int flip = k & 1;   // which half of xt holds X
+    const char* xt = a.ws + M.xt + ((size_t)bat * 2 + flip) * xtb;
+    char* xt_next = a.ws + M.xt + ((size_t)bat * 2 + (flip ^ 1)) * xtb;
+    char* xr = a.ws + M.xr + (size_t)bat * plane_bytes(M.mp, M.np);
+    const NsScale z = scale_of(a, M, bat, k);
+    const bool last = k + 1 == a.steps;
+    const float fb = z.sx / z.sb * (last ? 1.f : z.sx_next);
+    Pr p;
+    p.run(B, i0, M.mp, xt, j0, M.np, M.mp, 0, M.mp / 32);
 #pragma unroll
-        for (int e = 0; e < 4; ++e) y[e] = fmaf(fb, v[e], fx * load_plane(xt, pt, j, i + e));
-        if (a.k + 1 < a.steps) {
+    for (int f = 0; f < F; ++f)
 #pragma unroll
-            for (int e = 0; e < 4; ++e) y[e] *= z.sx_next;
-            store_planes_t(xt_next, pt, i, j, y);
-            store_planes(xr, pr, i, j, y);
-            return;
-        }
+        for (int g = 0; g < F; ++g) {
+            const int i = i0 + p.i0() + 32 * f, j = j0 + p.j0() + 32 * g;
+            if (i >= M.mp || j >= M.np) continue;   // (the same for all of a wave: sizes are multiples of 64)
+            float v[4][4];
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-            if (i + e >= M.m || j >= M.n) continue;
-            const long long at = M.turned ? (long long)j * M.ld_out + i + e : (long long)(i + e) * M.ld_out + j;
+            for (int q = 0; q < 4; ++q)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) v[q][e] = fb * p.value(f, g, q, e);
+            if (!last) {
+                char* o = xt_next + plane_at(j, i, M.mp);
+#pragma unroll
+                for (int q = 0; q < 4; ++q) store4(o + (q >> 1) * 2048 + (q & 1) * 512, v[q]);
+                float w[2][8];
+                p.turn(v, w);
+                o = xr + plane_at(i0 + p.ti() + 32 * f, j0 + p.tj() + 32 * g, M.np);
+#pragma unroll
+                for (int q = 0; q < 2; ++q) store8(o + q * 2048, w[q]);
+                continue;
+            }
+            const long long di = M.turned ? 1 : M.ld_out;
+            const long long at = M.turned ? (long long)j * M.ld_out + i : (long long)i * M.ld_out + j;
             if (a.muon) {
-                float* w = (float*)out + at;
-                *w = fmaf(-M.step, y[e], a.decay * *w);
+                float* W = (float*)M.out + (size_t)bat * M.out_stride + at;
+                float w[4][4];
+#pragma unroll
+                for (int q = 0; q < 4; ++q)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) w[q][e] = i + 8 * q + e < M.m && j < M.n ? W[(8 * q + e) * di] : 0.f;
+#pragma unroll
+                for (int q = 0; q < 4; ++q)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e)
+                        if (i + 8 * q + e < M.m && j < M.n) W[(8 * q + e) * di] = fmaf(-M.step, v[q][e], a.decay * w[q][e]);
             } else {
-                store_as(out, at, y[e], a.dtype);
+                char* out = (char*)M.out + (size_t)bat * M.out_stride * (a.dtype == DGG_F32 ? 4 : 2);
+#pragma unroll
+                for (int q = 0; q < 4; ++q)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e)
+                        if (i + 8 * q + e < M.m && j < M.n) store_as(out, at + (8 * q + e) * di, v[q][e], a.dtype);
             }
         }
-    });
 }
 
 // ------------------------------------------------------------------------------------------------ host side
 // Bounds of every step's operands from the coefficients alone.  |X_0| <= 1 in the 2-norm; with r = |X| the singular values lie in
-// [0, r], so |A| <= r^2, |B| <= max |b s^2 + c s^4|, |X'| <= max |a s + b s^3 + c s^5| over [0, r], and no element exceeds its
-// matrix' norm.  1 % is added for the roundings.
+// [0, r], so |A| <= r^2, |B| <= max |a + b s^2 + c s^4|, |X'| <= max |a s + b s^3 + c s^5| over [0, r], and no element exceeds
+// its matrix' norm.  1 % is added for the roundings.
 bool ns_bounds(const double* coef, int steps, NsStep* out) {
     double r = 1.0;
     for (int k = 0; k < steps; ++k) {
         const double a = coef[3 * k], b = coef[3 * k + 1], c = coef[3 * k + 2];
         r *= 1.01;
-        double mb = 0.0, mx = 0.0, mg = 0.0;
+        double mx = 0.0, mg = 0.0;
         for (int i = 0; i <= 4096; ++i) {
-            const double s = r * i / 4096.0, s2 = s * s, g = a + b * s2 + c * s2 * s2;
-            mb = fmax(mb, fabs(b * s2 + c * s2 * s2));
+            const double s = r * i / 4096.0, g = a + b * s * s + c * s * s * s * s;
             mx = fmax(mx, fabs(s * g));
             mg = fmax(mg, fabs(g));
         }
-        mb *= 1.01;
         mx *= 1.01;
-        if (!isfinite(a + b + c) || !(mb < 1e6) || !(mx < 1e6) || !(mx > 1e-6) || !(mg < 1e6)) return false;
-        out[k] = {(float)a, (float)b, (float)c, (float)r, (float)fmax(mb, 1e-6), (float)(1.01 * mg)};
+        if (!isfinite(a + b + c) || !(mx < 1e6) || !(mx > 1e-6) || !(mg < 1e6)) return false;
+        out[k] = {(float)a, (float)b, (float)c, (float)r, (float)(1.01 * mg)};
         r = mx;
     }
     return true;
@@ -547,11 +631,25 @@ int ns_check(const dgg_matrix* mats, int count, const char* who) {
     return DGG_OK;
 }
 
-// Sizes, workspace places and first workgroups of up to kNsMats matrices; returns the workspace bytes.
-size_t ns_plan(const dgg_matrix* mats, int count, NsArgs& a, int grids[6]) {
-    size_t at = 0;
-    for (int k = 0; k < 6; ++k) grids[k] = 0;
-    a.count = count;
+// Sizes, workspace places and first workgroups of up to kNsMats matrices.
+struct NsPlan {
+    int grid[kPhases];
+    NsFirst first[kPhases];
+    int f_apply;   // tiles of 64 f in B X
+    size_t bytes;
+};
+
+void ns_plan(const dgg_matrix* mats, int count, NsArgs& a, NsPlan& P) {
+    size_t at = up(sizeof(NsArgs));   // (its device copy)
+    for (int k = 0; k < kPhases; ++k) {
+        P.grid[k] = 0;
+        for (int i = 0; i < kNsMats; ++i) P.first[k].at[i] = 0x7fffffff;
+    }
+    // B X in tiles of 128 x 128 where they give every CU one (a generator's hidden matrices, 436 tiles: 31.5 us a launch against 34.4
+    // with tiles of 64 x 64), else of 64 x 64 (512 x 4620, 148 against 584 tiles: 16.8 against 19.4 us)
+    long long wide = 0;
+    for (int i = 0; i < count; ++i) wide += mats[i].batch * ceil_div(mats[i].rows, 128) * ceil_div(mats[i].cols, 128);
+    P.f_apply = wide >= 256 ? 2 : 1;
     for (int i = 0; i < count; ++i) {
         const dgg_matrix& in = mats[i];
         NsMat& M = a.mat[i];
@@ -568,8 +666,10 @@ size_t ns_plan(const dgg_matrix* mats, int count, NsArgs& a, int grids[6]) {
         M.step = (float)(a.lr * f);
         M.parts = ceil_div((long long)M.m * M.n, kThreads * 16);
         if (M.parts > kNsParts) M.parts = kNsParts;
-        const int t = ceil_div(M.mp, 128), tiles = t * (t + 1) / 2;
-        int splits = ceil_div(128, (long long)tiles * M.batch);
+        const int t = M.mp / 64, tiles = t * (t + 1) / 2;
+        // two workgroups a CU share the k of A = X X^T, 256 k or more each (192 .. 768 workgroups: 26.8, 21.8 (256), 19.6 (512), 19.0 us
+        // for the generator's matrices, 10.8 .. 11.6 for 512 x 4620; 128 x 128 tiles: 18.9 and 11.6)
+        int splits = ceil_div(512, (long long)tiles * M.batch);
         if (splits > M.np / 256) splits = M.np / 256;
         if (splits < 1) splits = 1;
         M.kblocks = ceil_div(M.np / 32, splits);
@@ -583,15 +683,14 @@ size_t ns_plan(const dgg_matrix* mats, int count, NsArgs& a, int grids[6]) {
         M.part = at; at = up(at + b * M.parts * 8);
         M.scal = at; at = up(at + b * kNsSteps * sizeof(NsScale));
         const int n32 = M.mp / 32;
-        int* first[6] = {&M.at_norm, &M.at_split, &M.at_gram, &M.at_sum, &M.at_square, &M.at_apply};
-        const int blocks[6] = {M.parts, (M.mp / 64) * (M.np / 64), tiles * M.splits, n32 * (n32 + 1) / 2, tiles,
-                               t * ceil_div(M.np, 128)};
-        for (int k = 0; k < 6; ++k) {
-            *first[k] = grids[k];
-            grids[k] += blocks[k] * M.batch;
+        const int blocks[kPhases] = {M.parts, t * (M.np / 64), tiles * M.splits, n32 * (n32 + 1) / 2, tiles,
+                                       ceil_div(M.mp, 64 * P.f_apply) * ceil_div(M.np, 64 * P.f_apply)};
+        for (int k = 0; k < kPhases; ++k) {
+            P.first[k].at[i] = P.grid[k];
+            P.grid[k] += blocks[k] * M.batch;
         }
     }
-    return at;
+    P.bytes = at;
 }
 
 int ns_run(const dgg_matrix* mats, int count, NsArgs& a, const double* coef, int steps, void* ws, size_t ws_bytes,
@@ -614,23 +713,29 @@ int ns_run(const dgg_matrix* mats, int count, NsArgs& a, const double* coef, int
     }
     a.ws = (char*)ws;
     a.steps = steps;
-    int g[6];
-    for (int at = 0; at < count; at += kNsMats)
-        if (ns_plan(mats + at, count - at < kNsMats ? count - at : kNsMats, a, g) > ws_bytes) {
-            set_error_text("%s: the workspace of %zu bytes is too small", who, ws_bytes);
+    NsPlan P;
+    for (int at = 0; at < count; at += kNsMats) {
+        ns_plan(mats + at, count - at < kNsMats ? count - at : kNsMats, a, P);
+        if (P.bytes > ws_bytes) {
+            set_error_text("%s: the workspace has %zu bytes, %zu are needed", who, ws_bytes, P.bytes);
             return DGG_ERR_WORKSPACE;
         }
+    }
     for (int at = 0; at < count; at += kNsMats) {
-        ns_plan(mats + at, count - at < kNsMats ? count - at : kNsMats, a, g);
+        ns_plan(mats + at, count - at < kNsMats ? count - at : kNsMats, a, P);
         const dim3 block(kThreads);
-        hipLaunchKernelGGL(ns_norm_kernel, dim3(g[0]), block, 0, st, a);
-        hipLaunchKernelGGL(ns_split_kernel, dim3(g[1]), block, 0, st, a);
+        const NsArgs* args = (const NsArgs*)ws;
+        hipLaunchKernelGGL(ns_norm_kernel, dim3(P.grid[kNorm]), block, 0, st, a, P.first[kNorm]);
+        hipLaunchKernelGGL(ns_split_kernel, dim3(P.grid[kSplit]), block, 0, st, args, P.first[kSplit]);
+        constexpr int lds1 = Prod<1, 3>::kLds, lds2 = Prod<2, 2>::kLds;
         for (int k = 0; k < steps; ++k) {
-            a.k = k;
-            hipLaunchKernelGGL((ns_gram_kernel<2>), dim3(g[2]), block, (Prod<2, 2>::kLds), st, a);
-            hipLaunchKernelGGL(ns_sum_kernel, dim3(g[3]), block, 0, st, a);
-            hipLaunchKernelGGL((ns_square_kernel<2>), dim3(g[4]), block, (Prod<2, 2>::kLds), st, a);
-            hipLaunchKernelGGL((ns_apply_kernel<2, 2>), dim3(g[5]), block, (Prod<2, 2>::kLds), st, a);
+            hipLaunchKernelGGL((ns_gram_kernel<3>), dim3(P.grid[kGram]), block, lds1, st, args, P.first[kGram], k);
+            hipLaunchKernelGGL(ns_sum_kernel, dim3(P.grid[kSum]), block, 0, st, args, P.first[kSum], k);
+            hipLaunchKernelGGL((ns_square_kernel<3>), dim3(P.grid[kSquare]), block, lds1, st, args, P.first[kSquare], k);
+            if (P.f_apply == 2)
+                hipLaunchKernelGGL((ns_apply_kernel<2, 2>), dim3(P.grid[kApply]), block, lds2, st, args, P.first[kApply], k);
+            else
+                hipLaunchKernelGGL((ns_apply_kernel<1, 3>), dim3(P.grid[kApply]), block, lds1, st, args, P.first[kApply], k);
         }
     }
     return check_launch(who);
@@ -642,9 +747,9 @@ int64_t ns_ws(const dgg_matrix* mats, int count, const char* who) {
     size_t need = 0;
     for (int at = 0; at < count; at += kNsMats) {
         NsArgs a = {};
-        int g[6];
-        const size_t n = ns_plan(mats + at, count - at < kNsMats ? count - at : kNsMats, a, g);
-        if (n > need) need = n;
+        NsPlan P;
+        ns_plan(mats + at, count - at < kNsMats ? count - at : kNsMats, a, P);
+        if (P.bytes > need) need = P.bytes;
     }
     return (int64_t)need;
 }
