@@ -21,12 +21,15 @@
 // in a row.  Both sizes are padded to multiples of 64 with zeros, which stay zeros in every product.
 #include <math.h>
 
+#include <type_traits>
+
 #include "dgg_internal.h"
 
 namespace dgg {
 namespace {
 
 typedef _Float16 half8 __attribute__((ext_vector_type(8)));
+typedef _Float16 half2 __attribute__((ext_vector_type(2)));
 typedef _Float16 half4 __attribute__((ext_vector_type(4)));
 typedef float f32x16 __attribute__((ext_vector_type(16)));
 typedef __attribute__((address_space(3))) char lds_char;
@@ -54,8 +57,8 @@ struct NsMat {
     size_t xr, xt, a, b, slab, part, scal;
 };
 
-// One step's coefficients and the bounds that follow from them (ns_bounds): |X| <= r, |B| <= grow, so |X'| <= grow |X|
-struct NsStep { float a, b, c, r, grow; };
+// One step's coefficients and the bounds that follow from them (ns_bounds): |B| <= grow, |X| <= r and <= times |X_0|; the same of the next X
+struct NsStep { float a, b, c, grow, r, times, r_next, times_next; };
 
 // The powers of two of one matrix in one step: X = planes * sx, planes of A, B and the next X = value * sa, sb, sx_next
 struct NsScale { float sx, sa, sb, sx_next; };
@@ -68,8 +71,7 @@ struct NsFirst { int at[kNsMats]; };
 struct NsArgs {
     NsMat mat[kNsMats];
     char* ws;
-    int dtype;               // of in / out
-    int muon, nesterov;
+    int nesterov;
     float mu, gscale, decay;
     int adjust;
     double lr, eps;
@@ -107,20 +109,19 @@ __device__ __forceinline__ size_t plane_at(int row, int k, int kp) {
     return ((size_t)(row >> 5) * (kp >> 4) + (k >> 4)) * 2048 + ((k >> 3) & 1) * 512 + (row & 31) * 16 + (k & 7) * 2;
 }
 
-__device__ __forceinline__ float load_as_float(const void* p, long long i, int dtype) {
-    if (dtype == DGG_F32) return ((const float*)p)[i];
-    if (dtype == DGG_BF16) return (float)((const __bf16*)p)[i];
-    return (float)((const _Float16*)p)[i];
-}
+// A pointer that was read from memory could point anywhere, to the compiler: as a pointer to global memory it is not accessed by flat
+// instructions, which also wait for LDS.
+template <typename T> using Global = T __attribute__((address_space(1)));
 
-__device__ __forceinline__ double block_sum(double v, double* sh /* kThreads / 64 */) {
+// sum of v over the workgroup's N threads, in a fixed order, for every thread
+template <int N> __device__ __forceinline__ double block_sum(double v, double* sh /* N / 64 */) {
     for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o);
     __syncthreads();
     if ((threadIdx.x & 63) == 0) sh[threadIdx.x >> 6] = v;
     __syncthreads();
     double s = 0.0;
 #pragma unroll
-    for (int i = 0; i < kThreads / 64; ++i) s += sh[i];
+    for (int i = 0; i < N / 64; ++i) s += sh[i];
     return s;
 }
 
@@ -129,18 +130,19 @@ __device__ __forceinline__ float muon_u(const NsArgs& a, float g, float m) { ret
 
 // ------------------------------------------------------------------------------------------------ norm
 // sum of squares in 64 bits, one partial a workgroup (muon: M is updated on the way).  Rows without gaps are one long row.
+template <typename T, bool MUON>
 __global__ __launch_bounds__(kThreads) void ns_norm_kernel(NsArgs a, NsFirst first) {
     __shared__ double sh[kThreads / 64];
     // the launches that follow find the arguments in device memory: 3 KB through the kernel arguments of each would be copied
     // by the host and read back over the bus every time
     if (blockIdx.x == 0)
-        for (int i = threadIdx.x; i < (int)(sizeof(NsArgs) / 8); i += kThreads) ((uint64_t*)a.ws)[i] = ((const uint64_t*)&a)[i];
+        for (int i = threadIdx.x; i < (int)(sizeof(NsArgs) / 8); i += kThreads) ((Global<uint64_t>*)a.ws)[i] = ((const uint64_t*)&a)[i];
     int local;
     const NsMat& M = a.mat[find(first, (int)blockIdx.x, local)];
     const int bat = local / M.parts, part = local - bat * M.parts;
-    const char* in = (const char*)M.in + (size_t)bat * M.in_stride * (a.dtype == DGG_F32 ? 4 : 2);
-    float* mom = a.muon ? M.mom + (size_t)bat * M.mom_stride : nullptr;
-    const bool flat = M.ld_in == M.cols && (!a.muon || M.ld_mom == M.cols);
+    const Global<T>* in = (const Global<T>*)M.in + (size_t)bat * M.in_stride;
+    Global<float>* mom = MUON ? (Global<float>*)M.mom + (size_t)bat * M.mom_stride : nullptr;
+    const bool flat = M.ld_in == M.cols && (!MUON || M.ld_mom == M.cols);
     const long long total = (long long)M.rows * M.cols;
     // a workgroup's share: a range of the long row, or whole rows
     const long long per = flat ? ((total + M.parts - 1) / M.parts + 63) / 64 * 64 : 0;
@@ -148,118 +150,109 @@ __global__ __launch_bounds__(kThreads) void ns_norm_kernel(NsArgs a, NsFirst fir
     const long long c0 = flat ? part * per : 0, c1 = flat ? (c0 + per < total ? c0 + per : total) : M.cols;
     double s = 0.0;
     for (int r = row0; r < rows; r += drow) {
-        const long long gi = (long long)r * M.ld_in, mi = (long long)r * M.ld_mom;
-        long long c = c0 + threadIdx.x;
-        for (; c + 3 * kThreads < c1; c += 4 * kThreads) {   // four loads in flight
-            float u[4], m[4];
+        const Global<T>* g = in + (long long)r * M.ld_in;
+        Global<float>* mr = MUON ? mom + (long long)r * M.ld_mom : nullptr;
+        for (long long c = c0 + threadIdx.x; c < c1; c += 8 * kThreads) {   // eight elements in flight
+            float u[8], m[8];
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                u[e] = load_as_float(in, gi + c + e * kThreads, a.dtype);
-                if (a.muon) m[e] = mom[mi + c + e * kThreads];
+            for (int e = 0; e < 8; ++e) {
+                const long long at = c + e * kThreads < c1 ? c + e * kThreads : c;   // (beyond the end: the first once more, not used)
+                u[e] = (float)g[at];
+                if (MUON) m[e] = mr[at];
             }
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                if (a.muon) {
+            for (int e = 0; e < 8; ++e) {
+                if (c + e * kThreads >= c1) break;
+                if (MUON) {
                     m[e] = fmaf(a.mu, m[e], a.gscale * u[e]);
-                    mom[mi + c + e * kThreads] = m[e];
+                    mr[c + e * kThreads] = m[e];
                     u[e] = muon_u(a, u[e], m[e]);
                 }
                 s = fma((double)u[e], (double)u[e], s);
             }
         }
-        for (; c < c1; c += kThreads) {
-            float u = load_as_float(in, gi + c, a.dtype);
-            if (a.muon) {
-                const float m = fmaf(a.mu, mom[mi + c], a.gscale * u);
-                mom[mi + c] = m;
-                u = muon_u(a, u, m);
-            }
-            s = fma((double)u, (double)u, s);
-        }
     }
-    s = block_sum(s, sh);
-    if (threadIdx.x == 0) ((double*)(a.ws + M.part))[(size_t)bat * M.parts + part] = s;
+    s = block_sum<kThreads>(s, sh);
+    if (threadIdx.x == 0) ((Global<double>*)(a.ws + M.part))[(size_t)bat * M.parts + part] = s;
 }
 
 // ------------------------------------------------------------------------------------------------ planes of X_0
-__device__ __forceinline__ void split2(float x, _Float16& hi, _Float16& lo) {
-    hi = (_Float16)x;
-    lo = (_Float16)(x - (float)hi);
+// x, y as hi + lo, rounded to nearest.  hi is one value, behind the compiler's back: fused into the product that x came from, the
+// conversion that is stored and the one that lo is taken from could round apart (a step of fp16 where they do).
+__device__ __forceinline__ void split2(float x, float y, half2& hi, half2& lo) {
+    hi = half2{(_Float16)x, (_Float16)y};
+    asm("" : "+v"(hi));
+    lo = half2{(_Float16)fmaf(-1.f, (float)hi.x, x), (_Float16)fmaf(-1.f, (float)hi.y, y)};
+}
+template <int N> struct Halves { half2 e[N / 2]; };
+template <int N> __device__ __forceinline__ void store_planes(char* p, const float (&v)[N]) {
+    Halves<N> hi, lo;
+#pragma unroll
+    for (int e = 0; e < N / 2; ++e) split2(v[2 * e], v[2 * e + 1], hi.e[e], lo.e[e]);
+    typedef uint32_t Bits __attribute__((ext_vector_type(N / 2)));
+    *(Bits*)p = __builtin_bit_cast(Bits, hi);
+    *(Bits*)(p + 1024) = __builtin_bit_cast(Bits, lo);
 }
 
 // eight k of a row, at their place in the hi plane
-__device__ __forceinline__ void store8(char* p, const float (&v)[8]) {
-    half8 hi, lo;
-#pragma unroll
-    for (int e = 0; e < 8; ++e) {
-        _Float16 h, l;
-        split2(v[e], h, l);
-        hi[e] = h;
-        lo[e] = l;
-    }
-    *(half8*)p = hi;
-    *(half8*)(p + 1024) = lo;
-}
+__device__ __forceinline__ void store8(char* p, const float (&v)[8]) { store_planes<8>(p, v); }
 
 // the power of two that brings `bound` into [2^14, 2^15)
 __device__ __forceinline__ float below(float bound) { return ldexpf(1.f, 14 - ilogbf(bound)); }
 
-// every operand's bound: the one of the coefficients, or, for a norm far below eps, what |X_0| can have grown to
-__device__ __forceinline__ void scales(const NsArgs& a, double norm, int k, NsScale* o) {
-    float r = (float)(norm / (norm + a.eps));
-    if (!(r > 0x1p-40f)) r = 0x1p-40f;
-    float sx = (float)(1.0 / ldexp(norm + a.eps, k));
-    for (int i = 0; i < a.steps; ++i) {
-        const NsStep S = a.step[i];
-        r = fminf(1.01f * r, S.r);
-        const float next = S.grow * r;
-        NsScale z;
-        z.sx = sx;
-        z.sa = below(r * r);
-        z.sb = below(S.grow);
-        z.sx_next = below(i + 1 < a.steps ? fminf(next, a.step[i + 1].r) : next);
-        o[i] = z;
-        sx = 1.f / z.sx_next;
-        r = next;
-    }
+// one step's powers of two, from every operand's bound: the one of the coefficients, or, for a norm far below eps, what |X_0| can
+// have grown to (a thread a step: none waits for the one before)
+__device__ __forceinline__ void scales(const NsArgs& a, double norm, int k0, int k, NsScale* o) {
+    const NsStep S = a.step[k];
+    float r0 = (float)(norm / (norm + a.eps));
+    if (!(r0 > 0x1p-40f)) r0 = 0x1p-40f;
+    const float r = fminf(S.r, S.times * r0);
+    NsScale z;
+    z.sx = k ? 1.f / below(r) : (float)(1.0 / ldexp(norm + a.eps, k0));
+    z.sa = below(r * r);
+    z.sb = below(S.grow);
+    z.sx_next = below(fminf(S.r_next, S.times_next * r0));
+    o[k] = z;
 }
 
 // 64 x 64 of X: U read along its rows, written by rows and by columns of X as planes of U * 2^k
+template <typename T, bool MUON>
 __global__ __launch_bounds__(kThreads) void ns_split_kernel(const NsArgs* args, NsFirst first) {
     const NsArgs& a = *args;
+    char* const ws = (char*)args;   // (they lie at its start)
     __shared__ double sh[kThreads / 64];
     __shared__ float t[64][65];   // [i][j] of X
     int local;
     const NsMat M = a.mat[find(first, (int)blockIdx.x, local)];
     const int ti = M.mp / 64, tj = M.np / 64;
     const int bat = local / (ti * tj), tile = local - bat * ti * tj, i0 = tile / tj * 64, j0 = tile % tj * 64;
-    const char* in = (const char*)M.in + (size_t)bat * M.in_stride * (a.dtype == DGG_F32 ? 4 : 2);
-    const float* mom = a.muon ? M.mom + (size_t)bat * M.mom_stride : nullptr;
+    const Global<T>* in = (const Global<T>*)M.in + (size_t)bat * M.in_stride;
+    const Global<float>* mom = MUON ? (Global<float>*)M.mom + (size_t)bat * M.mom_stride : nullptr;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const int r0 = M.turned ? j0 : i0, c0 = M.turned ? i0 : j0;   // of U
     float u[16], m[16];   // all of the tile is in flight while the norm is summed
 #pragma unroll
     for (int q = 0; q < 16; ++q) {
-        const int r = r0 + q * 4 + wave, c = c0 + lane;
-        const bool in_u = r < M.rows && c < M.cols;
-        u[q] = in_u ? load_as_float(in, (long long)r * M.ld_in + c, a.dtype) : 0.f;
-        m[q] = in_u && a.muon ? mom[(long long)r * M.ld_mom + c] : 0.f;
+        const int r = min(r0 + q * 4 + wave, M.rows - 1), c = min(c0 + lane, M.cols - 1);   // (beyond: not used)
+        u[q] = (float)in[(long long)r * M.ld_in + c];
+        if (MUON) m[q] = mom[(long long)r * M.ld_mom + c];
     }
     double s = 0.0;
-    for (int p = threadIdx.x; p < M.parts; p += kThreads) s += ((const double*)(a.ws + M.part))[(size_t)bat * M.parts + p];
-    const double norm = sqrt(block_sum(s, sh));
+    for (int p = threadIdx.x; p < M.parts; p += kThreads) s += ((const double*)(ws + M.part))[(size_t)bat * M.parts + p];
+    const double norm = sqrt(block_sum<kThreads>(s, sh));
     // 2^k |U| in [2^14, 2^15): no element of the planes is larger.  A zero, infinite or NaN norm keeps k = 0.
     const int k = norm > 0.0 && norm < INFINITY ? 14 - ilogb(norm) : 0;
-    if (tile == 0 && threadIdx.x == 0) scales(a, norm, k, (NsScale*)(a.ws + M.scal) + (size_t)bat * kNsSteps);
+    if (tile == 0 && (int)threadIdx.x < a.steps) scales(a, norm, k, threadIdx.x, (NsScale*)(ws + M.scal) + (size_t)bat * kNsSteps);
 #pragma unroll
     for (int q = 0; q < 16; ++q) {
-        const float v = ldexpf(a.muon ? muon_u(a, u[q], m[q]) : u[q], k);
+        const bool in_u = r0 + q * 4 + wave < M.rows && c0 + lane < M.cols;
+        const float v = in_u ? ldexpf(MUON ? muon_u(a, u[q], m[q]) : u[q], k) : 0.f;
         if (M.turned) t[lane][q * 4 + wave] = v;
         else t[q * 4 + wave][lane] = v;
     }
     __syncthreads();
-    char* xr = a.ws + M.xr + (size_t)bat * plane_bytes(M.mp, M.np);
-    char* xt = a.ws + M.xt + (size_t)bat * 2 * plane_bytes(M.np, M.mp);
+    char* xr = ws + M.xr + (size_t)bat * plane_bytes(M.mp, M.np);
+    char* xt = ws + M.xt + (size_t)bat * 2 * plane_bytes(M.np, M.mp);
     // 64 rows of 64 k: 8 k a thread, twice per layout
     for (int q = threadIdx.x; q < 512; q += kThreads) {
         const int row = q & 63, k8 = (q >> 6) * 8;
@@ -398,23 +391,12 @@ __device__ __forceinline__ void upper(int tile, int t, int& ti, int& tj) {
     tj = ti + tile;
 }
 
-__device__ __forceinline__ NsScale scale_of(const NsArgs& a, const NsMat& M, int bat, int k) {
-    return ((const NsScale*)(a.ws + M.scal))[(size_t)bat * kNsSteps + k];
+__device__ __forceinline__ NsScale scale_of(const char* ws, const NsMat& M, int bat, int k) {
+    return ((const NsScale*)(ws + M.scal))[(size_t)bat * kNsSteps + k];
 }
 
 // four k of a row, at their place in the hi plane: written, and read as the values they stand for
-__device__ __forceinline__ void store4(char* p, const float (&v)[4]) {
-    half4 hi, lo;
-#pragma unroll
-    for (int e = 0; e < 4; ++e) {
-        _Float16 h, l;
-        split2(v[e], h, l);
-        hi[e] = h;
-        lo[e] = l;
-    }
-    *(half4*)p = hi;
-    *(half4*)(p + 1024) = lo;
-}
+__device__ __forceinline__ void store4(char* p, const float (&v)[4]) { store_planes<4>(p, v); }
 __device__ __forceinline__ void load4(const char* p, float (&v)[4]) {
     const half4 hi = *(const half4*)p, lo = *(const half4*)(p + 1024);
 #pragma unroll
@@ -426,17 +408,18 @@ template <int S>
 __global__ __launch_bounds__(kThreads) void ns_gram_kernel(const NsArgs* args, NsFirst first, int k) {
     using Pr = Prod<1, S>;
     const NsArgs& a = *args;
+    char* const ws = (char*)args;   // (they lie at its start)
     int local;
     const NsMat M = a.mat[find(first, by_die(), local)];
     const int t = M.mp / Pr::kTile, tiles = t * (t + 1) / 2, per = tiles * M.splits;
     const int bat = local / per, rest = local - bat * per, split = rest / tiles;
     int ti, tj;
     upper(rest - split * tiles, t, ti, tj);
-    const char* x = a.ws + M.xr + (size_t)bat * plane_bytes(M.mp, M.np);
+    const char* x = ws + M.xr + (size_t)bat * plane_bytes(M.mp, M.np);
     Pr p;
     p.run(x, ti * Pr::kTile, M.mp, x, tj * Pr::kTile, M.mp, M.np, split * M.kblocks, min((split + 1) * M.kblocks, M.np / 32));
     const int i0 = ti * Pr::kTile + p.i0(), j0 = tj * Pr::kTile + p.j0();
-    float* slab = (float*)(a.ws + M.slab) + ((size_t)bat * M.splits + split) * M.mp * M.mp + (size_t)i0 * M.mp + j0;
+    float* slab = (float*)(ws + M.slab) + ((size_t)bat * M.splits + split) * M.mp * M.mp + (size_t)i0 * M.mp + j0;
 #pragma unroll
     for (int q = 0; q < 4; ++q)
 #pragma unroll
@@ -446,16 +429,17 @@ __global__ __launch_bounds__(kThreads) void ns_gram_kernel(const NsArgs* args, N
 // sums the slabs in order: planes of A, both triangles; 32 x 32 elements a workgroup
 __global__ __launch_bounds__(kThreads) void ns_sum_kernel(const NsArgs* args, NsFirst first, int k) {
     const NsArgs& a = *args;
+    char* const ws = (char*)args;   // (they lie at its start)
     __shared__ float t[32][33];
     int local;
     const NsMat M = a.mat[find(first, by_die(), local)];
     const int n32 = M.mp / 32, tiles = n32 * (n32 + 1) / 2, bat = local / tiles;
     int ti, tj;
     upper(local - bat * tiles, n32, ti, tj);
-    const NsScale z = scale_of(a, M, bat, k);
+    const NsScale z = scale_of(ws, M, bat, k);
     const size_t slab = (size_t)M.mp * M.mp;
     const int r0 = threadIdx.x >> 3, c0 = (threadIdx.x & 7) * 4;
-    const float* p = (const float*)(a.ws + M.slab) + (size_t)bat * M.splits * slab + (size_t)(ti * 32 + r0) * M.mp + tj * 32 + c0;
+    const float* p = (const float*)(ws + M.slab) + (size_t)bat * M.splits * slab + (size_t)(ti * 32 + r0) * M.mp + tj * 32 + c0;
     float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll 8
     for (int sp = 0; sp < M.splits; ++sp) {
@@ -475,7 +459,7 @@ __global__ __launch_bounds__(kThreads) void ns_sum_kernel(const NsArgs* args, Ns
     float w[8];
 #pragma unroll
     for (int e = 0; e < 8; ++e) w[e] = mirror || (ti == tj && k8 + e < r) ? t[k8 + e][r] : t[r][k8 + e];
-    char* A = a.ws + M.a + (size_t)bat * plane_bytes(M.mp, M.mp);
+    char* A = ws + M.a + (size_t)bat * plane_bytes(M.mp, M.mp);
     store8(A + plane_at((mirror ? tj : ti) * 32 + r, (mirror ? ti : tj) * 32 + k8, M.mp), w);
 }
 
@@ -484,20 +468,21 @@ template <int S>
 __global__ __launch_bounds__(kThreads) void ns_square_kernel(const NsArgs* args, NsFirst first, int k) {
     using Pr = Prod<1, S>;
     const NsArgs& a = *args;
+    char* const ws = (char*)args;   // (they lie at its start)
     int local;
     const NsMat M = a.mat[find(first, by_die(), local)];
     const int t = M.mp / Pr::kTile, tiles = t * (t + 1) / 2, bat = local / tiles;
     int ti, tj;
     upper(local - bat * tiles, t, ti, tj);
-    const char* A = a.ws + M.a + (size_t)bat * plane_bytes(M.mp, M.mp);
-    char* B = a.ws + M.b + (size_t)bat * plane_bytes(M.mp, M.mp);
+    const char* A = ws + M.a + (size_t)bat * plane_bytes(M.mp, M.mp);
+    char* B = ws + M.b + (size_t)bat * plane_bytes(M.mp, M.mp);
     Pr p;
     const int i0 = ti * Pr::kTile, j0 = tj * Pr::kTile, i = i0 + p.i0(), j = j0 + p.j0();
     const size_t at = plane_at(j, i, M.mp);   // row j, k = i: A and B are symmetric
     float v[4][4];
 #pragma unroll
     for (int q = 0; q < 4; ++q) load4(A + at + (q >> 1) * 2048 + (q & 1) * 512, v[q]);
-    const NsScale z = scale_of(a, M, bat, k);
+    const NsScale z = scale_of(ws, M, bat, k);
     const float ratio = z.sb / z.sa, fa = a.step[k].a * z.sb, fb = a.step[k].b * ratio, fc = a.step[k].c * ratio / z.sa;
     p.run(A, i0, M.mp, A, j0, M.mp, M.mp, 0, M.mp / 32);
 #pragma unroll
@@ -514,29 +499,27 @@ __global__ __launch_bounds__(kThreads) void ns_square_kernel(const NsArgs* args,
     for (int q = 0; q < 2; ++q) store8(B + plane_at(i0 + p.ti(), j0 + p.tj() + 16 * q, M.mp), w[q]);
 }
 
-__device__ __forceinline__ void store_as(void* p, long long i, float v, int dtype) {
-    if (dtype == DGG_F32) ((float*)p)[i] = v;
-    else if (dtype == DGG_BF16) ((__bf16*)p)[i] = (__bf16)v;
-    else ((_Float16*)p)[i] = (_Float16)v;
-}
+// What the last step writes: X in a type of the caller's, or the parameters
+struct ToMuon {};
 
-// X <- B X: planes in both layouts, or (last step) the result
-template <int F, int S>
+// X <- B X: planes in both layouts (Out = void), or (last step) the result
+template <int F, int S, typename Out>
 __global__ __launch_bounds__(kThreads, 2) void ns_apply_kernel(const NsArgs* args, NsFirst first, int k) {
     using Pr = Prod<F, S>;
     const NsArgs& a = *args;
+    char* const ws = (char*)args;   // (they lie at its start)
     int local;
     const NsMat M = a.mat[find(first, by_die(), local)];
     const int ti = (M.mp + Pr::kTile - 1) / Pr::kTile, tj = (M.np + Pr::kTile - 1) / Pr::kTile;
     const int bat = local / (ti * tj), tile = local - bat * ti * tj, i0 = tile % ti * Pr::kTile, j0 = tile / ti * Pr::kTile;
-    const char* B = a.ws + M.b + (size_t)bat * plane_bytes(M.mp, M.mp);
+    const char* B = ws + M.b + (size_t)bat * plane_bytes(M.mp, M.mp);
     const size_t xtb = plane_bytes(M.np, M.mp);
     const int flip = k & 1;   // which half of xt holds X
-    const char* xt = a.ws + M.xt + ((size_t)bat * 2 + flip) * xtb;
-    char* xt_next = a.ws + M.xt + ((size_t)bat * 2 + (flip ^ 1)) * xtb;
-    char* xr = a.ws + M.xr + (size_t)bat * plane_bytes(M.mp, M.np);
-    const NsScale z = scale_of(a, M, bat, k);
-    const bool last = k + 1 == a.steps;
+    const char* xt = ws + M.xt + ((size_t)bat * 2 + flip) * xtb;
+    char* xt_next = ws + M.xt + ((size_t)bat * 2 + (flip ^ 1)) * xtb;
+    char* xr = ws + M.xr + (size_t)bat * plane_bytes(M.mp, M.np);
+    const NsScale z = scale_of(ws, M, bat, k);
+    constexpr bool last = !std::is_same<Out, void>::value;
     const float fb = z.sx / z.sb * (last ? 1.f : z.sx_next);
     Pr p;
     p.run(B, i0, M.mp, xt, j0, M.np, M.mp, 0, M.mp / 32);
@@ -551,7 +534,7 @@ __global__ __launch_bounds__(kThreads, 2) void ns_apply_kernel(const NsArgs* arg
             for (int q = 0; q < 4; ++q)
 #pragma unroll
                 for (int e = 0; e < 4; ++e) v[q][e] = fb * p.value(f, g, q, e);
-            if (!last) {
+            if constexpr (!last) {
                 char* o = xt_next + plane_at(j, i, M.mp);
 #pragma unroll
                 for (int q = 0; q < 4; ++q) store4(o + (q >> 1) * 2048 + (q & 1) * 512, v[q]);
@@ -560,31 +543,258 @@ __global__ __launch_bounds__(kThreads, 2) void ns_apply_kernel(const NsArgs* arg
                 o = xr + plane_at(i0 + p.ti() + 32 * f, j0 + p.tj() + 32 * g, M.np);
 #pragma unroll
                 for (int q = 0; q < 2; ++q) store8(o + q * 2048, w[q]);
-                continue;
-            }
-            const long long di = M.turned ? 1 : M.ld_out;
-            const long long at = M.turned ? (long long)j * M.ld_out + i : (long long)i * M.ld_out + j;
-            if (a.muon) {
-                float* W = (float*)M.out + (size_t)bat * M.out_stride + at;
-                float w[4][4];
-#pragma unroll
-                for (int q = 0; q < 4; ++q)
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) w[q][e] = i + 8 * q + e < M.m && j < M.n ? W[(8 * q + e) * di] : 0.f;
-#pragma unroll
-                for (int q = 0; q < 4; ++q)
-#pragma unroll
-                    for (int e = 0; e < 4; ++e)
-                        if (i + 8 * q + e < M.m && j < M.n) W[(8 * q + e) * di] = fmaf(-M.step, v[q][e], a.decay * w[q][e]);
             } else {
-                char* out = (char*)M.out + (size_t)bat * M.out_stride * (a.dtype == DGG_F32 ? 4 : 2);
+                const long long di = M.turned ? 1 : M.ld_out;
+                const long long at = (size_t)bat * M.out_stride + (M.turned ? (long long)j * M.ld_out + i : (long long)i * M.ld_out + j);
+                if constexpr (std::is_same<Out, ToMuon>::value) {
+                    Global<float>* W = (Global<float>*)M.out + at;
+                    float w[4][4];
+                    const int jn = min(j, M.n - 1) - j;   // (beyond the end: an element inside, not used)
+                    const long long dj = M.turned ? (long long)jn * M.ld_out : jn;
 #pragma unroll
-                for (int q = 0; q < 4; ++q)
+                    for (int q = 0; q < 4; ++q)
 #pragma unroll
-                    for (int e = 0; e < 4; ++e)
-                        if (i + 8 * q + e < M.m && j < M.n) store_as(out, at + (8 * q + e) * di, v[q][e], a.dtype);
+                        for (int e = 0; e < 4; ++e) w[q][e] = W[(min(i + 8 * q + e, M.m - 1) - i) * di + dj];
+#pragma unroll
+                    for (int q = 0; q < 4; ++q)
+#pragma unroll
+                        for (int e = 0; e < 4; ++e)
+                            if (i + 8 * q + e < M.m && j < M.n) W[(8 * q + e) * di] = fmaf(-M.step, v[q][e], a.decay * w[q][e]);
+                } else {
+                    Global<Out>* o = (Global<Out>*)M.out + at;
+#pragma unroll
+                    for (int q = 0; q < 4; ++q)
+#pragma unroll
+                        for (int e = 0; e < 4; ++e)
+                            if (i + 8 * q + e < M.m && j < M.n) o[(8 * q + e) * di] = (Out)v[q][e];
+                }
             }
         }
+}
+
+// ------------------------------------------------------------------------------------------------ small matrices
+// A matrix whose planes fit the LDS of one workgroup (short side <= 32 and long side <= 512, or 64 and 192): the whole step in one
+// launch, 16 waves.  What bounds it is the chain of 5 barriers a step; the launches of the other route alone take 100 us.
+// The same planes in the same order and scales as there: A = X X^T in ranges of k that meet in LDS, A^2 and B X one 32 x 32 block a wave.
+constexpr int kSmallThreads = 1024, kPart = 32 * 36;
+
+__host__ __device__ __forceinline__ int small_splits(int mp) { return mp == 32 ? 4 : 2; }
+__host__ __device__ __forceinline__ int small_tiles(int mp) { return mp == 32 ? 1 : 3; }
+int small_lds(int mp, int np) { return mp * np * 8 + mp * mp * 8 + small_tiles(mp) * small_splits(mp) * kPart * 4; }
+
+struct SmallFrags { half8 ph, pl, qh, ql; };
+__device__ __forceinline__ void small_read(const char* p, const char* q, SmallFrags& x) {
+    x.ph = *(const half8*)p;
+    x.ql = *(const half8*)(q + 1024);
+    x.qh = *(const half8*)q;
+    x.pl = *(const half8*)(p + 1024);
+}
+__device__ __forceinline__ void small_multiply(const SmallFrags& x, f32x16& hh, f32x16& cross) {
+    cross = __builtin_amdgcn_mfma_f32_32x32x16_f16(x.ph, x.ql, cross, 0, 0, 0);
+    hh = __builtin_amdgcn_mfma_f32_32x32x16_f16(x.ph, x.qh, hh, 0, 0, 0);
+    cross = __builtin_amdgcn_mfma_f32_32x32x16_f16(x.pl, x.qh, cross, 0, 0, 0);
+}
+__device__ __forceinline__ void zero(f32x16& hh, f32x16& cross) {
+#pragma unroll
+    for (int e = 0; e < 16; ++e) hh[e] = cross[e] = 0.f;
+}
+
+template <typename In, bool MUON>
+__global__ __launch_bounds__(kSmallThreads) void ns_small_kernel(NsArgs a, NsFirst first) {
+    extern __shared__ char smem[];
+    __shared__ double sh[kSmallThreads / 64];
+    __shared__ NsScale sc[kNsSteps];
+    int bat;
+    const NsMat& M = a.mat[find(first, (int)blockIdx.x, bat)];
+    const int mp = M.mp, np = M.np, T = mp / 32, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    char* xr = smem;
+    char* xt = xr + mp * np * 4;
+    char* A = xt + mp * np * 4;
+    char* B = A + mp * mp * 4;
+    float* part = (float*)(B + mp * mp * 4);
+    const Global<In>* in = (const Global<In>*)M.in + (size_t)bat * M.in_stride;
+    Global<float>* mom = MUON ? (Global<float>*)M.mom + (size_t)bat * M.mom_stride : nullptr;
+    // U as it lies in memory, 16 elements a thread at most, through LDS (fp32 [mp][np + 4], in the place of X by columns and the start of A)
+    float* stage = (float*)xt;
+    const int total = M.rows * M.cols, pitch = np + 4, units = mp * np / 8;
+    const float per_col = 1.f / (float)M.cols;
+    for (int e = threadIdx.x; e < mp * pitch / 4; e += kSmallThreads) ((float4*)stage)[e] = make_float4(0.f, 0.f, 0.f, 0.f);
+    float u[16], m[16];
+#pragma unroll
+    for (int t = 0; t < 16; ++t) {
+        const int e = min((int)threadIdx.x + t * kSmallThreads, total - 1), r = (int)(((float)e + 0.5f) * per_col), c = e - r * M.cols;
+        u[t] = (float)in[(long long)r * M.ld_in + c];   // (e below 2^14: the quotient's error stays below the half)
+        if (MUON) m[t] = mom[(long long)r * M.ld_mom + c];
+    }
+    __syncthreads();
+    double s = 0.0;
+#pragma unroll
+    for (int t = 0; t < 16; ++t) {
+        const int e = (int)threadIdx.x + t * kSmallThreads, r = (int)(((float)e + 0.5f) * per_col), c = e - r * M.cols;
+        if (e >= total) break;
+        if (MUON) {
+            m[t] = fmaf(a.mu, m[t], a.gscale * u[t]);
+            mom[(long long)r * M.ld_mom + c] = m[t];
+            u[t] = muon_u(a, u[t], m[t]);
+        }
+        s = fma((double)u[t], (double)u[t], s);
+        stage[M.turned ? c * pitch + r : r * pitch + c] = u[t];
+    }
+    const double norm = sqrt(block_sum<kSmallThreads>(s, sh));
+    const int k0 = norm > 0.0 && norm < INFINITY ? 14 - ilogb(norm) : 0;   // (as in ns_split_kernel)
+    if ((int)threadIdx.x < a.steps) scales(a, norm, k0, threadIdx.x, sc);
+    // 8 k of a row a thread, two rounds at most: X by rows, and by columns once everyone has read
+    float v[2][8];
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+        const int q = threadIdx.x + t * kSmallThreads, i = q & (mp - 1), j = q / mp * 8, groups = np / 32;
+        if (q >= units) break;
+        float w[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) w[e] = ldexpf(stage[i * pitch + j + e], k0);
+        store8(xr + plane_at(i, j, np), w);
+        const int g = (q >> 5) / groups, i8 = g * 8, col = ((q >> 5) - g * groups) * 32 + (q & 31);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[t][e] = ldexpf(stage[(i8 + e) * pitch + col], k0);
+    }
+    __syncthreads();
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+        const int q = threadIdx.x + t * kSmallThreads, groups = np / 32, g = (q >> 5) / groups;
+        if (q < units) store8(xt + plane_at(((q >> 5) - g * groups) * 32 + (q & 31), g * 8, mp), v[t]);
+    }
+    __syncthreads();
+    const int splits = small_splits(mp), tiles = small_tiles(mp), r = lane & 31, h = lane >> 5;
+    // B X: the block of this wave; the lane's elements are (i + 8 q + e, j)
+    const bool mine = wave < T * (np / 32);
+    const int bj = wave / T, bi = wave - bj * T, i = bi * 32 + 4 * h, j = bj * 32 + r;
+    const long long di = M.turned ? 1 : M.ld_out, at = M.turned ? (long long)j * M.ld_out + i : (long long)i * M.ld_out + j;
+    Global<float>* W = (Global<float>*)M.out + (size_t)bat * M.out_stride;
+    float w[4][4];
+    for (int k = 0; k < a.steps; ++k) {
+        const NsScale z = sc[k];
+        const bool last = k + 1 == a.steps;
+        if (MUON && last) {   // the parameters are on their way during the last step
+#pragma unroll
+            for (int q = 0; q < 4; ++q)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const int ic = min(i + 8 * q + e, M.m - 1), jc = min(j, M.n - 1);   // (beyond: not used)
+                    w[q][e] = W[M.turned ? (long long)jc * M.ld_out + ic : (long long)ic * M.ld_out + jc];
+                }
+        }
+        f32x16 hh, cross;
+        if (wave < tiles * splits) {   // A: tiles (0, 0), (0, 1), (1, 1), a range of k each
+            const int tile = wave / splits, ti = tile >> 1, tj = (tile + 1) >> 1, n = np / 16, per = ((n + splits - 1) / splits + 1) & ~1;
+            const int b = (wave - tile * splits) * per, e = min(b + per, n);   // (an even number of 16 k)
+            const char *p = xr + ti * n * 2048 + lane * 16, *q = xr + tj * n * 2048 + lane * 16;
+            zero(hh, cross);
+            for (int x = b; x < e; x += 2) {
+                SmallFrags f[2];
+                small_read(p + x * 2048, q + x * 2048, f[0]);
+                small_read(p + x * 2048 + 2048, q + x * 2048 + 2048, f[1]);
+                small_multiply(f[0], hh, cross);
+                small_multiply(f[1], hh, cross);
+            }
+            float* o = part + wave * kPart + r * 36 + 4 * h;   // [j][i]
+#pragma unroll
+            for (int y = 0; y < 4; ++y)
+                *(float4*)(o + 8 * y) = make_float4(hh[4 * y] + cross[4 * y], hh[4 * y + 1] + cross[4 * y + 1],
+                                                    hh[4 * y + 2] + cross[4 * y + 2], hh[4 * y + 3] + cross[4 * y + 3]);
+        }
+        __syncthreads();
+        if ((int)threadIdx.x < tiles * 128) {   // 8 i of a row j a thread
+            const int tile = threadIdx.x >> 7, ti = tile >> 1, tj = (tile + 1) >> 1, aj = threadIdx.x & 31, i8 = ((threadIdx.x >> 5) & 3) * 8;
+            float v[8];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) v[e] = 0.f;
+            for (int sp = 0; sp < splits; ++sp) {
+                const float* o = part + (tile * splits + sp) * kPart + aj * 36 + i8;
+                const float4 lo = *(const float4*)o, hi = *(const float4*)(o + 4);
+                v[0] += lo.x; v[1] += lo.y; v[2] += lo.z; v[3] += lo.w;
+                v[4] += hi.x; v[5] += hi.y; v[6] += hi.z; v[7] += hi.w;
+            }
+#pragma unroll
+            for (int e = 0; e < 8; ++e) v[e] = v[e] * z.sx * z.sx * z.sa;
+            store8(A + plane_at(tj * 32 + aj, ti * 32 + i8, mp), v);
+            if (ti != tj)
+#pragma unroll
+                for (int e = 0; e < 8; e += 2) {
+                    half2 hi, lo;
+                    split2(v[e], v[e + 1], hi, lo);
+                    char* o = A + plane_at(ti * 32 + i8 + e, tj * 32 + aj, mp);
+                    *(_Float16*)o = hi.x;
+                    *(_Float16*)(o + 1024) = lo.x;
+                    *(_Float16*)(o + 16) = hi.y;   // (the next row)
+                    *(_Float16*)(o + 1040) = lo.y;
+                }
+        }
+        __syncthreads();
+        if (wave < T * T) {   // B
+            const int ti = wave / T, tj = wave - ti * T, n = mp / 16, bcol = tj * 32 + r;
+            const float ratio = z.sb / z.sa, fa = a.step[k].a * z.sb, fb = a.step[k].b * ratio, fc = a.step[k].c * ratio / z.sa;
+            zero(hh, cross);
+            for (int x = 0; x < n; x += 2) {
+                SmallFrags f[2];
+#pragma unroll
+                for (int y = 0; y < 2; ++y)
+                    small_read(A + (ti * n + x + y) * 2048 + lane * 16, A + (tj * n + x + y) * 2048 + lane * 16, f[y]);
+                small_multiply(f[0], hh, cross);
+                small_multiply(f[1], hh, cross);
+            }
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+                const int row = ti * 32 + 8 * q + 4 * h;
+                float v[4];
+                load4(A + plane_at(bcol, row, mp), v);
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                    v[e] = fmaf(fc, hh[4 * q + e] + cross[4 * q + e], fmaf(fb, v[e], row + e == bcol ? fa : 0.f));
+                store4(B + plane_at(bcol, row, mp), v);
+            }
+        }
+        __syncthreads();
+        // B X, and once more with the operands exchanged: the same values lane by row, as X by rows is written
+        f32x16 hh2, cross2;
+        zero(hh, cross);
+        zero(hh2, cross2);
+        if (mine)
+            for (int x = 0, n = mp / 16; x < n; x += 2) {
+                SmallFrags f[2];
+#pragma unroll
+                for (int y = 0; y < 2; ++y)
+                    small_read(B + (bi * n + x + y) * 2048 + lane * 16, xt + (bj * n + x + y) * 2048 + lane * 16, f[y]);
+#pragma unroll
+                for (int y = 0; y < 2; ++y) {
+                    small_multiply(f[y], hh, cross);
+                    small_multiply({f[y].qh, f[y].ql, f[y].ph, f[y].pl}, hh2, cross2);
+                }
+            }
+        const float f = z.sx / z.sb * (last ? 1.f : z.sx_next);
+        __syncthreads();   // everyone has read X: its place takes the next
+        if (mine)
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+                float v[4], x[4];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    v[e] = f * (hh[4 * q + e] + cross[4 * q + e]);
+                    x[e] = f * (hh2[4 * q + e] + cross2[4 * q + e]);
+                }
+                if (!last) {
+                    store4(xt + plane_at(j, i + 8 * q, mp), v);
+                    store4(xr + plane_at(bi * 32 + r, bj * 32 + 8 * q + 4 * h, np), x);
+                    continue;
+                }
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    if (i + 8 * q + e >= M.m || j >= M.n) continue;
+                    if (MUON) W[at + (8 * q + e) * di] = fmaf(-M.step, v[e], a.decay * w[q][e]);
+                    else ((Global<In>*)M.out)[(size_t)bat * M.out_stride + at + (8 * q + e) * di] = (In)v[e];
+                }
+            }
+        __syncthreads();
+    }
 }
 
 // ------------------------------------------------------------------------------------------------ host side
@@ -592,20 +802,30 @@ __global__ __launch_bounds__(kThreads, 2) void ns_apply_kernel(const NsArgs* arg
 // [0, r], so |A| <= r^2, |B| <= max |a + b s^2 + c s^4|, |X'| <= max |a s + b s^3 + c s^5| over [0, r], and no element exceeds
 // its matrix' norm.  1 % is added for the roundings.
 bool ns_bounds(const double* coef, int steps, NsStep* out) {
-    double r = 1.0;
+    double r = 1.0, times = 1.0;
     for (int k = 0; k < steps; ++k) {
         const double a = coef[3 * k], b = coef[3 * k + 1], c = coef[3 * k + 2];
-        r *= 1.01;
-        double mx = 0.0, mg = 0.0;
-        for (int i = 0; i <= 4096; ++i) {
-            const double s = r * i / 4096.0, g = a + b * s * s + c * s * s * s * s;
-            mx = fmax(mx, fabs(s * g));
-            mg = fmax(mg, fabs(g));
+        // largest |g| and |s g| with g = a + b t + c t^2, t = s^2, over t in [0, r^2]: at its ends and where g' or (s g)' is 0
+        double t[5] = {0.0, r * r, -b / (2.0 * c), -1.0, -1.0}, mx = 0.0, mg = 0.0;
+        const double d = 9.0 * b * b - 20.0 * a * c;
+        if (d >= 0.0) {   // 5 c t^2 + 3 b t + a = 0, both roots without cancellation
+            const double q = -0.5 * (3.0 * b + copysign(sqrt(d), b));
+            t[3] = q / (5.0 * c);
+            t[4] = a / q;
         }
+        for (double v : t)
+            if (v >= 0.0 && v <= r * r) {   // (also leaves out infinities and NaN of c = 0)
+                const double g = fabs(a + (b + c * v) * v);
+                mg = fmax(mg, g);
+                mx = fmax(mx, sqrt(v) * g);
+            }
         mx *= 1.01;
+        mg *= 1.01;
         if (!isfinite(a + b + c) || !(mx < 1e6) || !(mx > 1e-6) || !(mg < 1e6)) return false;
-        out[k] = {(float)a, (float)b, (float)c, (float)r, (float)(1.01 * mg)};
+        const double most = fmin(times * mg, 1e30);
+        out[k] = {(float)a, (float)b, (float)c, (float)mg, (float)r, (float)times, (float)mx, (float)most};
         r = mx;
+        times = most;
     }
     return true;
 }
@@ -631,6 +851,26 @@ int ns_check(const dgg_matrix* mats, int count, const char* who) {
     return DGG_OK;
 }
 
+bool ns_small(const dgg_matrix& m) {
+    const int lo = m.rows < m.cols ? m.rows : m.cols, hi = m.rows < m.cols ? m.cols : m.rows;
+    return lo <= 32 ? hi <= 512 : lo <= 64 && hi <= 192;
+}
+
+// What both routes need to know of one matrix.
+void ns_fill(const dgg_matrix& in, const NsArgs& a, int pad, NsMat& M) {
+    M.in = in.in; M.out = in.out; M.mom = in.momentum;
+    M.in_stride = in.in_stride; M.out_stride = in.out_stride; M.mom_stride = in.momentum_stride;
+    M.ld_in = in.ld_in; M.ld_out = in.ld_out; M.ld_mom = in.ld_momentum;
+    M.rows = in.rows; M.cols = in.cols; M.batch = (int)in.batch;
+    M.turned = in.rows > in.cols;
+    M.m = M.turned ? in.cols : in.rows;
+    M.n = M.turned ? in.rows : in.cols;
+    M.mp = ceil_div(M.m, pad) * pad;
+    M.np = ceil_div(M.n, pad) * pad;
+    const double f = a.adjust == DGG_MUON_SPECTRAL ? sqrt(fmax(1.0, (double)in.rows / in.cols)) : 0.2 * sqrt((double)M.n);
+    M.step = (float)(a.lr * f);
+}
+
 // Sizes, workspace places and first workgroups of up to kNsMats matrices.
 struct NsPlan {
     int grid[kPhases];
@@ -639,7 +879,7 @@ struct NsPlan {
     size_t bytes;
 };
 
-void ns_plan(const dgg_matrix* mats, int count, NsArgs& a, NsPlan& P) {
+void ns_plan(const dgg_matrix* const* mats, int count, NsArgs& a, NsPlan& P) {
     size_t at = up(sizeof(NsArgs));   // (its device copy)
     for (int k = 0; k < kPhases; ++k) {
         P.grid[k] = 0;
@@ -648,22 +888,12 @@ void ns_plan(const dgg_matrix* mats, int count, NsArgs& a, NsPlan& P) {
     // B X in tiles of 128 x 128 where they give every CU one (a generator's hidden matrices, 436 tiles: 31.5 us a launch against 34.4
     // with tiles of 64 x 64), else of 64 x 64 (512 x 4620, 148 against 584 tiles: 16.8 against 19.4 us)
     long long wide = 0;
-    for (int i = 0; i < count; ++i) wide += mats[i].batch * ceil_div(mats[i].rows, 128) * ceil_div(mats[i].cols, 128);
+    for (int i = 0; i < count; ++i) wide += mats[i]->batch * ceil_div(mats[i]->rows, 128) * ceil_div(mats[i]->cols, 128);
     P.f_apply = wide >= 256 ? 2 : 1;
     for (int i = 0; i < count; ++i) {
-        const dgg_matrix& in = mats[i];
+        const dgg_matrix& in = *mats[i];
         NsMat& M = a.mat[i];
-        M.in = in.in; M.out = in.out; M.mom = in.momentum;
-        M.in_stride = in.in_stride; M.out_stride = in.out_stride; M.mom_stride = in.momentum_stride;
-        M.ld_in = in.ld_in; M.ld_out = in.ld_out; M.ld_mom = in.ld_momentum;
-        M.rows = in.rows; M.cols = in.cols; M.batch = (int)in.batch;
-        M.turned = in.rows > in.cols;
-        M.m = M.turned ? in.cols : in.rows;
-        M.n = M.turned ? in.rows : in.cols;
-        M.mp = ceil_div(M.m, 64) * 64;
-        M.np = ceil_div(M.n, 64) * 64;
-        const double f = a.adjust == DGG_MUON_SPECTRAL ? sqrt(fmax(1.0, (double)in.rows / in.cols)) : 0.2 * sqrt((double)M.n);
-        M.step = (float)(a.lr * f);
+        ns_fill(in, a, 64, M);
         M.parts = ceil_div((long long)M.m * M.n, kThreads * 16);
         if (M.parts > kNsParts) M.parts = kNsParts;
         const int t = M.mp / 64, tiles = t * (t + 1) / 2;
@@ -693,6 +923,27 @@ void ns_plan(const dgg_matrix* mats, int count, NsArgs& a, NsPlan& P) {
     P.bytes = at;
 }
 
+// up to kNsMats matrices of one route, from mats[at] on; at moves behind them
+int ns_group(const dgg_matrix* mats, int count, bool small, int& at, const dgg_matrix** group) {
+    int n = 0;
+    for (; at < count && n < kNsMats; ++at)
+        if (ns_small(mats[at]) == small) group[n++] = mats + at;
+    return n;
+}
+
+int64_t ns_need(const dgg_matrix* mats, int count) {
+    const dgg_matrix* group[kNsMats];
+    size_t need = 256;
+    for (int at = 0, n; (n = ns_group(mats, count, false, at, group)) > 0;) {
+        NsArgs a = {};
+        NsPlan P;
+        ns_plan(group, n, a, P);
+        if (P.bytes > need) need = P.bytes;
+    }
+    return (int64_t)need;
+}
+
+template <typename T, bool MUON>
 int ns_run(const dgg_matrix* mats, int count, NsArgs& a, const double* coef, int steps, void* ws, size_t ws_bytes,
            hipStream_t st, const char* who) {
     if (steps < 1 || steps > kNsSteps || !coef || !(a.eps >= 0.0) || !ns_bounds(coef, steps, a.step)) {
@@ -701,7 +952,7 @@ int ns_run(const dgg_matrix* mats, int count, NsArgs& a, const double* coef, int
     }
     for (int i = 0; i < count; ++i) {
         const dgg_matrix& m = mats[i];
-        const bool mom = !a.muon || (m.momentum && m.ld_momentum >= m.cols && m.momentum_stride >= 0);
+        const bool mom = !MUON || (m.momentum && m.ld_momentum >= m.cols && m.momentum_stride >= 0);
         if (!m.in || !m.out || !mom || m.ld_in < m.cols || m.ld_out < m.cols || m.in_stride < 0 || m.out_stride < 0) {
             set_error_text("%s: matrix %d: null pointer, a pitch below %d columns or a negative stride", who, i, m.cols);
             return DGG_ERR_INVALID;
@@ -714,28 +965,54 @@ int ns_run(const dgg_matrix* mats, int count, NsArgs& a, const double* coef, int
     a.ws = (char*)ws;
     a.steps = steps;
     NsPlan P;
-    for (int at = 0; at < count; at += kNsMats) {
-        ns_plan(mats + at, count - at < kNsMats ? count - at : kNsMats, a, P);
-        if (P.bytes > ws_bytes) {
-            set_error_text("%s: the workspace has %zu bytes, %zu are needed", who, ws_bytes, P.bytes);
-            return DGG_ERR_WORKSPACE;
-        }
+    const dgg_matrix* group[kNsMats];
+    int64_t need = ns_need(mats, count);
+    if ((int64_t)ws_bytes < need) {
+        set_error_text("%s: the workspace has %zu bytes, %lld are needed", who, ws_bytes, (long long)need);
+        return DGG_ERR_WORKSPACE;
     }
-    for (int at = 0; at < count; at += kNsMats) {
-        ns_plan(mats + at, count - at < kNsMats ? count - at : kNsMats, a, P);
+    for (int at = 0, n; (n = ns_group(mats, count, true, at, group)) > 0;) {
+        NsFirst first;
+        int grid = 0, lds = 0;
+        for (int i = 0; i < kNsMats; ++i) {
+            first.at[i] = 0x7fffffff;
+            if (i >= n) continue;
+            ns_fill(*group[i], a, 32, a.mat[i]);
+            const int bytes = small_lds(a.mat[i].mp, a.mat[i].np);
+            if (bytes > lds) lds = bytes;
+            first.at[i] = grid;
+            grid += a.mat[i].batch;
+        }
+        // (more than 64 KB of LDS has to be asked for, on every device that launches)
+        const hipError_t e = hipFuncSetAttribute((const void*)ns_small_kernel<T, MUON>, hipFuncAttributeMaxDynamicSharedMemorySize, lds);
+        if (e != hipSuccess) {
+            set_error(who, e);
+            return DGG_ERR_LAUNCH;
+        }
+        hipLaunchKernelGGL((ns_small_kernel<T, MUON>), dim3(grid), dim3(kSmallThreads), lds, st, a, first);
+    }
+    for (int at = 0, n; (n = ns_group(mats, count, false, at, group)) > 0;) {
+        ns_plan(group, n, a, P);
         const dim3 block(kThreads);
         const NsArgs* args = (const NsArgs*)ws;
-        hipLaunchKernelGGL(ns_norm_kernel, dim3(P.grid[kNorm]), block, 0, st, a, P.first[kNorm]);
-        hipLaunchKernelGGL(ns_split_kernel, dim3(P.grid[kSplit]), block, 0, st, args, P.first[kSplit]);
+        hipLaunchKernelGGL((ns_norm_kernel<T, MUON>), dim3(P.grid[kNorm]), block, 0, st, a, P.first[kNorm]);
+        hipLaunchKernelGGL((ns_split_kernel<T, MUON>), dim3(P.grid[kSplit]), block, 0, st, args, P.first[kSplit]);
         constexpr int lds1 = Prod<1, 3>::kLds, lds2 = Prod<2, 2>::kLds;
         for (int k = 0; k < steps; ++k) {
             hipLaunchKernelGGL((ns_gram_kernel<3>), dim3(P.grid[kGram]), block, lds1, st, args, P.first[kGram], k);
             hipLaunchKernelGGL(ns_sum_kernel, dim3(P.grid[kSum]), block, 0, st, args, P.first[kSum], k);
             hipLaunchKernelGGL((ns_square_kernel<3>), dim3(P.grid[kSquare]), block, lds1, st, args, P.first[kSquare], k);
-            if (P.f_apply == 2)
-                hipLaunchKernelGGL((ns_apply_kernel<2, 2>), dim3(P.grid[kApply]), block, lds2, st, args, P.first[kApply], k);
-            else
-                hipLaunchKernelGGL((ns_apply_kernel<1, 3>), dim3(P.grid[kApply]), block, lds1, st, args, P.first[kApply], k);
+            using Last = typename std::conditional<MUON, ToMuon, T>::type;
+            const bool last = k + 1 == steps;
+            const dim3 grid(P.grid[kApply]);
+            const NsFirst& f = P.first[kApply];
+            if (P.f_apply == 2) {
+                if (last) hipLaunchKernelGGL((ns_apply_kernel<2, 2, Last>), grid, block, lds2, st, args, f, k);
+                else hipLaunchKernelGGL((ns_apply_kernel<2, 2, void>), grid, block, lds2, st, args, f, k);
+            } else {
+                if (last) hipLaunchKernelGGL((ns_apply_kernel<1, 3, Last>), grid, block, lds1, st, args, f, k);
+                else hipLaunchKernelGGL((ns_apply_kernel<1, 3, void>), grid, block, lds1, st, args, f, k);
+            }
         }
     }
     return check_launch(who);
@@ -743,15 +1020,7 @@ int ns_run(const dgg_matrix* mats, int count, NsArgs& a, const double* coef, int
 
 int64_t ns_ws(const dgg_matrix* mats, int count, const char* who) {
     const int rc = ns_check(mats, count, who);
-    if (rc != DGG_OK) return rc;
-    size_t need = 0;
-    for (int at = 0; at < count; at += kNsMats) {
-        NsArgs a = {};
-        NsPlan P;
-        ns_plan(mats + at, count - at < kNsMats ? count - at : kNsMats, a, P);
-        if (P.bytes > need) need = P.bytes;
-    }
-    return (int64_t)need;
+    return rc != DGG_OK ? rc : ns_need(mats, count);
 }
 
 }  // namespace
@@ -775,9 +1044,11 @@ int dgg_orthogonalize(const dgg_matrix* mats, int count, int dtype, const double
         return DGG_ERR_INVALID;
     }
     NsArgs a = {};
-    a.dtype = dtype;
     a.eps = eps;
-    return ns_run(mats, count, a, coefficients, steps, ws, ws_bytes, (hipStream_t)stream, who);
+    hipStream_t st = (hipStream_t)stream;
+    return dtype == DGG_F32 ? ns_run<float, false>(mats, count, a, coefficients, steps, ws, ws_bytes, st, who)
+         : dtype == DGG_BF16 ? ns_run<__bf16, false>(mats, count, a, coefficients, steps, ws, ws_bytes, st, who)
+                             : ns_run<_Float16, false>(mats, count, a, coefficients, steps, ws, ws_bytes, st, who);
 }
 
 int dgg_muon_step(const dgg_matrix* mats, int count, double lr, double momentum, int nesterov, double weight_decay, int adjust,
@@ -791,8 +1062,6 @@ int dgg_muon_step(const dgg_matrix* mats, int count, double lr, double momentum,
         return DGG_ERR_INVALID;
     }
     NsArgs a = {};
-    a.dtype = DGG_F32;
-    a.muon = 1;
     a.nesterov = nesterov != 0;
     a.mu = (float)momentum;
     a.gscale = (float)grad_scale;
@@ -800,7 +1069,7 @@ int dgg_muon_step(const dgg_matrix* mats, int count, double lr, double momentum,
     a.adjust = adjust;
     a.decay = (float)(1.0 - lr * weight_decay);
     a.eps = eps;
-    return ns_run(mats, count, a, coefficients, steps, ws, ws_bytes, (hipStream_t)stream, who);
+    return ns_run<float, true>(mats, count, a, coefficients, steps, ws, ws_bytes, (hipStream_t)stream, who);
 }
 
 }  // extern "C"

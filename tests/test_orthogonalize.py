@@ -118,6 +118,18 @@ def test_steps_and_coefficients():
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("shape", [(31, 200), (64, 100), (128, 128), (300, 170)], ids=lambda s: "%dx%d" % s)
+def test_operands_keep_22_bits(shape):
+    """With X <- X in every step what is left of each is taking X apart into two planes and putting it together again: hi is off by
+    2^-12 of a value at most, lo by 2^-12 of that, so 2^-23 a step (one more for the common factor) — element by element, where a hi
+    and a lo of two different roundings would differ by 2^-11."""
+    g = matrix(*shape, seed=11)
+    out = ops.orthogonalize(g.cuda(), 10, (1.0, 0.0, 0.0)).double().cpu()
+    ref = g.double() / (g.double().norm() + EPS)
+    assert bool(((out - ref).abs() <= 11 * 2.0 ** -23 * ref.abs() + 2.0 ** -38).all())   # 2^-38: fp16's smallest step under 2^14
+
+
+@pytest.mark.gpu
 def test_stacks_lists_and_strides():
     stack = torch.stack([matrix(33, 65, s) for s in range(5)])
     out = ops.orthogonalize(stack.cuda())
