@@ -43,20 +43,37 @@ template <typename T, int V> __device__ __forceinline__ void store_vec(T* p, con
     *reinterpret_cast<Vec<T, V>*>(p) = r;
 }
 
+// 1 / (1 + exp(-z)) by the hardware's exp2 and reciprocal (1 unit in the last place each).  The exponent is formed in 64 bits and
+// rounded once, so the result is off by (|z| + 6) 2^-24 of itself at most.  (With expf and a division, 30 instructions an element,
+// a forward pass over 64 M bf16 elements was bound by them: 77 us for the launch that moves 268 MB.)
+__device__ __forceinline__ float sigmoid(double z) {
+    return __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f((float)(z * -1.4426950408889634)));
+}
 // act(z) and act'(z) of a 64-bit pre-activation
 __device__ __forceinline__ float act_value(double z, int act, float slope) {
     const float zf = (float)z;
     if (act == DGG_ACT_LEAKY_RELU) return z > 0.0 ? zf : zf * slope;
-    if (act == DGG_ACT_SILU) return zf / (1.f + expf(-zf));
+    if (act == DGG_ACT_SILU) return zf * sigmoid(z);
     return zf;
 }
 __device__ __forceinline__ float act_slope(double z, int act, float slope) {
     if (act == DGG_ACT_LEAKY_RELU) return z > 0.0 ? 1.f : slope;
     if (act == DGG_ACT_SILU) {
-        const float zf = (float)z, s = 1.f / (1.f + expf(-zf));
+        const float zf = (float)z, s = sigmoid(z);
         return s * (1.f + zf * (1.f - s));
     }
     return 1.f;
+}
+
+// V consecutive channels of weight or bias, or what stands for one that is not there (one branch for all of them)
+template <int V> __device__ __forceinline__ void load_param(const float* p, long long c, float none, float (&v)[V]) {
+    if (p) {
+#pragma unroll
+        for (int k = 0; k < V; ++k) v[k] = p[c + k];
+    } else {
+#pragma unroll
+        for (int k = 0; k < V; ++k) v[k] = none;
+    }
 }
 
 struct GnArgs {
@@ -67,6 +84,7 @@ struct GnArgs {
     const float* b;         // NULL: 0
     double* stats;          // [N][G][2]: mean, rstd
     double* part;           // tile: [N][chunks][C][2]; unit backward: float [rows of partials][C][2]
+    double* chan;           // tile backward: [N][C][2], part summed over the chunks (part itself where there is one)
     double* coef;           // tile backward: [N][G][2]: mean(w dz), mean(w dz xh)
     float* dw;
     float* db;
@@ -97,15 +115,14 @@ __global__ __launch_bounds__(kGnThreads) void gn_unit_fwd_kernel(GnArgs a) {
     const unsigned n = (unsigned)u / (unsigned)a.G, g = (unsigned)u - n * (unsigned)a.G;
     const int dv = a.D / V, nv = (int)a.S * dv;
     const T* x = (const T*)a.x + (long long)n * a.x_sn + (long long)g * a.D;
-    float v[I][V];
+    float v[I][V], w[I][V], b[I][V];
     double sum = 0.0;
 #pragma unroll
-    for (int i = 0; i < I; ++i) {
-        const int e = lane + i * L;
-        if (e < nv) {
-            const int s = e / dv;
-            load_vec<T, V>(x + (long long)s * a.x_ss + (e - s * dv) * V, v[i]);
-        }
+    for (int i = 0; i < I; ++i) {   // (lanes beyond the end: the last vector once more, not used)
+        const int e = min(lane + i * L, nv - 1), s = a.S == 1 ? 0 : e / dv, cv = (e - s * dv) * V;
+        load_vec<T, V>(x + (long long)s * a.x_ss + cv, v[i]);
+        load_param<V>(a.w, (long long)g * a.D + cv, 1.f, w[i]);
+        load_param<V>(a.b, (long long)g * a.D + cv, 0.f, b[i]);
     }
 #pragma unroll
     for (int i = 0; i < I; ++i)
@@ -132,13 +149,10 @@ __global__ __launch_bounds__(kGnThreads) void gn_unit_fwd_kernel(GnArgs a) {
     for (int i = 0; i < I; ++i) {
         const int e = lane + i * L;
         if (e >= nv) continue;
-        const int s = e / dv, c = (int)g * a.D + (e - s * dv) * V;
+        const int s = a.S == 1 ? 0 : e / dv, c = (int)g * a.D + (e - s * dv) * V;
         float y[V];
 #pragma unroll
-        for (int k = 0; k < V; ++k) {
-            const double sc = rstd * (a.w ? (double)a.w[c + k] : 1.0);
-            y[k] = act_value(fma((double)v[i][k] - mean, sc, a.b ? (double)a.b[c + k] : 0.0), a.act, a.slope);
-        }
+        for (int k = 0; k < V; ++k) y[k] = act_value(fma((double)v[i][k] - mean, rstd * (double)w[i][k], (double)b[i][k]), a.act, a.slope);
         store_vec<T, V>((T*)a.out + ((long long)n * a.S + s) * a.C + c, y);
     }
 }
@@ -157,14 +171,13 @@ __global__ __launch_bounds__(kGnThreads) void gn_unit_bwd_kernel(GnArgs a) {
     float w[I][V], b[I][V];
     double dw[I][V], db[I][V];
 #pragma unroll
-    for (int i = 0; i < I; ++i)
+    for (int i = 0; i < I; ++i) {
+        const long long c = (long long)g * a.D + min(lane + i * L, nv - 1) * V;
+        load_param<V>(a.w, c, 1.f, w[i]);
+        load_param<V>(a.b, c, 0.f, b[i]);
 #pragma unroll
-        for (int k = 0; k < V; ++k) {
-            const int e = lane + i * L, c = g * a.D + e * V + k;
-            w[i][k] = a.w && e < nv ? a.w[c] : 1.f;
-            b[i][k] = a.b && e < nv ? a.b[c] : 0.f;
-            dw[i][k] = db[i][k] = 0.0;
-        }
+        for (int k = 0; k < V; ++k) dw[i][k] = db[i][k] = 0.0;
+    }
     const double inv = 1.0 / ((double)nv * V);
     for (long long n = (long long)nb * per + side; n < a.N; n += (long long)a.blocks_n * per) {
         const T* x = (const T*)a.x + n * a.x_sn + (long long)g * a.D;
@@ -173,11 +186,9 @@ __global__ __launch_bounds__(kGnThreads) void gn_unit_bwd_kernel(GnArgs a) {
         float xv[I][V], dv[I][V];
 #pragma unroll
         for (int i = 0; i < I; ++i) {
-            const int e = lane + i * L;
-            if (e < nv) {
-                load_vec<T, V>(x + e * V, xv[i]);
-                load_vec<T, V>(dy + e * V, dv[i]);
-            }
+            const int e = min(lane + i * L, nv - 1);
+            load_vec<T, V>(x + e * V, xv[i]);
+            load_vec<T, V>(dy + e * V, dv[i]);
         }
         double s1 = 0.0, s2 = 0.0;
 #pragma unroll
@@ -253,6 +264,23 @@ template <int V> __device__ __forceinline__ void column_sum(double (&p)[V], doub
     }
 }
 
+// load(s, v) and use(s, v) for the rows s, s + step, .. below s1, U loads ahead
+template <int U, int N, typename Load, typename Use>
+__device__ __forceinline__ void walk(long long s, long long s1, int step, Load load, Use use) {
+    for (; s + (U - 1) * step < s1; s += U * step) {
+        float v[U][N];
+#pragma unroll
+        for (int u = 0; u < U; ++u) load(s + u * step, v[u]);
+#pragma unroll
+        for (int u = 0; u < U; ++u) use(s + u * step, v[u]);
+    }
+    for (; s < s1; s += step) {
+        float v[N];
+        load(s, v);
+        use(s, v);
+    }
+}
+
 // per channel: sums of (x - k) and (x - k)^2 over a range of rows, k = the sample's first row: a shift that keeps the
 // variance of data far from zero, removed again by gn_stats_kernel
 template <typename T, int V>
@@ -267,16 +295,15 @@ __global__ __launch_bounds__(kGnThreads) void gn_tile_sum_kernel(GnArgs a) {
         const long long s0 = (long long)ch * a.chunk_rows, s1 = s0 + a.chunk_rows < a.S ? s0 + a.chunk_rows : a.S;
         float piv[V];
         load_vec<T, V>(x, piv);
-        for (long long s = s0 + t.ty; s < s1; s += t.rows) {
-            float v[V];
-            load_vec<T, V>(x + s * a.x_ss, v);
+        walk<4, V>(s0 + t.ty, s1, t.rows, [&](long long s, float (&v)[V]) { load_vec<T, V>(x + s * a.x_ss, v); },
+                   [&](long long, float (&v)[V]) {
 #pragma unroll
-            for (int k = 0; k < V; ++k) {
-                const double d = (double)v[k] - (double)piv[k];
-                p[k] += d;
-                q[k] = fma(d, d, q[k]);
-            }
-        }
+                       for (int k = 0; k < V; ++k) {
+                           const double d = (double)v[k] - (double)piv[k];
+                           p[k] += d;
+                           q[k] = fma(d, d, q[k]);
+                       }
+                   });
     }
     column_sum<V>(p, q, a, t);
     if (t.on && t.ty == 0)
@@ -333,34 +360,55 @@ __global__ __launch_bounds__(kGnThreads) void gn_stats_kernel(GnArgs a) {
     }
 }
 
-template <typename T, int V>
+// what a tile kernel keeps of its V channels
+template <int V> struct Channels {
+    double mean[V], rstd[V];
+    float w[V], b[V];
+    int group[V];
+    __device__ __forceinline__ Channels(const GnArgs& a, long long n, int c0) {
+        int g = c0 / a.D, r = c0 - g * a.D;
+#pragma unroll
+        for (int k = 0; k < V; ++k) {
+            group[k] = g;
+            if (++r == a.D) {
+                r = 0;
+                ++g;
+            }
+        }
+        const double* st = a.stats + 2ll * n * a.G;
+#pragma unroll
+        for (int k = 0; k < V; ++k) {
+            mean[k] = st[2 * group[k]];
+            rstd[k] = st[2 * group[k] + 1];
+        }
+        load_param<V>(a.w, c0, 1.f, w);
+        load_param<V>(a.b, c0, 0.f, b);
+    }
+};
+
+template <typename T, int V, int ACT>
 __global__ __launch_bounds__(kGnThreads) void gn_tile_apply_kernel(GnArgs a) {
     const unsigned n = blockIdx.x / (unsigned)a.chunks, ch = blockIdx.x - n * (unsigned)a.chunks;
     const Tile t = tile_of(a, a.C / V, blockIdx.y);
     if (!t.on) return;
-    double mean[V], sc[V], sh[V];
+    const Channels<V> c(a, n, t.vx * V);
+    double sc[V];
 #pragma unroll
-    for (int k = 0; k < V; ++k) {
-        const int c = t.vx * V + k;
-        const double* st = a.stats + 2ll * ((long long)n * a.G + c / a.D);
-        mean[k] = st[0];
-        sc[k] = st[1] * (a.w ? (double)a.w[c] : 1.0);
-        sh[k] = a.b ? (double)a.b[c] : 0.0;
-    }
+    for (int k = 0; k < V; ++k) sc[k] = c.rstd[k] * (double)c.w[k];
+    const float slope = a.slope;
     const T* x = (const T*)a.x + (long long)n * a.x_sn + t.vx * V;
     T* y = (T*)a.out + (long long)n * a.S * a.C + t.vx * V;
-    const long long s0 = (long long)ch * a.chunk_rows, s1 = s0 + a.chunk_rows < a.S ? s0 + a.chunk_rows : a.S;
-    for (long long s = s0 + t.ty; s < s1; s += t.rows) {
-        float v[V];
-        load_vec<T, V>(x + s * a.x_ss, v);
+    const long long s0 = (long long)ch * a.chunk_rows, s1 = s0 + a.chunk_rows < a.S ? s0 + a.chunk_rows : a.S, xs = a.x_ss, C = a.C;
+    walk<4, V>(s0 + t.ty, s1, t.rows, [&](long long s, float (&v)[V]) { load_vec<T, V>(x + s * xs, v); },
+               [&](long long s, float (&v)[V]) {
 #pragma unroll
-        for (int k = 0; k < V; ++k) v[k] = act_value(fma((double)v[k] - mean[k], sc[k], sh[k]), a.act, a.slope);
-        store_vec<T, V>(y + s * a.C, v);
-    }
+                   for (int k = 0; k < V; ++k) v[k] = act_value(fma((double)v[k] - c.mean[k], sc[k], (double)c.b[k]), ACT, slope);
+                   store_vec<T, V>(y + s * C, v);
+               });
 }
 
 // per channel: sums of dz xh and dz over a range of rows
-template <typename T, int V>
+template <typename T, int V, int ACT>
 __global__ __launch_bounds__(kGnThreads) void gn_tile_bwd_sum_kernel(GnArgs a) {
     const unsigned n = blockIdx.x / (unsigned)a.chunks, ch = blockIdx.x - n * (unsigned)a.chunks;
     const Tile t = tile_of(a, a.C / V, blockIdx.y);
@@ -368,32 +416,25 @@ __global__ __launch_bounds__(kGnThreads) void gn_tile_bwd_sum_kernel(GnArgs a) {
 #pragma unroll
     for (int k = 0; k < V; ++k) p[k] = q[k] = 0.0;
     if (t.on) {
-        double mean[V], rstd[V];
-        float w[V], b[V];
-#pragma unroll
-        for (int k = 0; k < V; ++k) {
-            const int c = t.vx * V + k;
-            const double* st = a.stats + 2ll * ((long long)n * a.G + c / a.D);
-            mean[k] = st[0];
-            rstd[k] = st[1];
-            w[k] = a.w ? a.w[c] : 1.f;
-            b[k] = a.b ? a.b[c] : 0.f;
-        }
+        const Channels<V> c(a, n, t.vx * V);
+        const float slope = a.slope;
         const T* x = (const T*)a.x + (long long)n * a.x_sn + t.vx * V;
         const T* dy = (const T*)a.dy + (long long)n * a.dy_sn + t.vx * V;
         const long long s0 = (long long)ch * a.chunk_rows, s1 = s0 + a.chunk_rows < a.S ? s0 + a.chunk_rows : a.S;
-        for (long long s = s0 + t.ty; s < s1; s += t.rows) {
-            float v[V], d[V];
-            load_vec<T, V>(x + s * a.x_ss, v);
-            load_vec<T, V>(dy + s * a.dy_ss, d);
+        walk<2, 2 * V>(s0 + t.ty, s1, t.rows,
+                       [&](long long s, float (&v)[2 * V]) {
+                           load_vec<T, V>(x + s * a.x_ss, reinterpret_cast<float(&)[V]>(v));
+                           load_vec<T, V>(dy + s * a.dy_ss, reinterpret_cast<float(&)[V]>(v[V]));
+                       },
+                       [&](long long, float (&v)[2 * V]) {
 #pragma unroll
-            for (int k = 0; k < V; ++k) {
-                const double xh = ((double)v[k] - mean[k]) * rstd[k];
-                const double dz = (double)(d[k] * act_slope(fma(xh, (double)w[k], (double)b[k]), a.act, a.slope));
-                p[k] = fma(dz, xh, p[k]);
-                q[k] += dz;
-            }
-        }
+                           for (int k = 0; k < V; ++k) {
+                               const double xh = ((double)v[k] - c.mean[k]) * c.rstd[k];
+                               const double dz = (double)(v[V + k] * act_slope(fma(xh, (double)c.w[k], (double)c.b[k]), ACT, slope));
+                               p[k] = fma(dz, xh, p[k]);
+                               q[k] += dz;
+                           }
+                       });
     }
     column_sum<V>(p, q, a, t);
     if (t.on && t.ty == 0)
@@ -405,18 +446,42 @@ __global__ __launch_bounds__(kGnThreads) void gn_tile_bwd_sum_kernel(GnArgs a) {
         }
 }
 
+// One workgroup per (n, g): the group's two means, and its channels' sums over the chunks on the way (T walkers a channel, in order)
 __global__ __launch_bounds__(kGnThreads) void gn_bwd_coef_kernel(GnArgs a) {
-    __shared__ double sh[kGnThreads / 64];
+    __shared__ double sh[kGnThreads / 64], col[kGnThreads * 2];
     const unsigned n = blockIdx.x / (unsigned)a.G, g = blockIdx.x - n * (unsigned)a.G;
-    const double* part = a.part + 2ll * ((long long)n * a.chunks * a.C + (long long)g * a.D);
-    const long long items = (long long)a.D * a.chunks;
+    const int wide = a.D < kGnThreads ? a.D : kGnThreads, T = kGnThreads / wide, w = (int)threadIdx.x / wide, c0 = (int)threadIdx.x - w * wide;
     double s1 = 0.0, s2 = 0.0;
-    for (long long e = threadIdx.x; e < items; e += kGnThreads) {
-        const unsigned ch = (unsigned)(e / a.D), c = (unsigned)(e - (long long)ch * a.D);
-        const double* o = part + 2ll * ((long long)ch * a.C + c);
-        const double w = a.w ? (double)a.w[(long long)g * a.D + c] : 1.0;
-        s1 = fma(w, o[1], s1);
-        s2 = fma(w, o[0], s2);
+    for (int base = 0; base < a.D; base += wide) {
+        const int c = base + c0;
+        const bool on = w < T && c < a.D;
+        double p = 0.0, q = 0.0;
+        if (on) {
+            const double* o = a.part + 2ll * ((long long)n * a.chunks * a.C + (long long)g * a.D + c);
+#pragma unroll 4
+            for (int ch = w; ch < a.chunks; ch += T) {
+                p += o[2ll * ch * a.C];
+                q += o[2ll * ch * a.C + 1];
+            }
+        }
+        __syncthreads();
+        col[2 * threadIdx.x] = p;
+        col[2 * threadIdx.x + 1] = q;
+        __syncthreads();
+        if (on && w == 0) {
+            for (int t = 1; t < T; ++t) {
+                p += col[2 * (t * wide + c0)];
+                q += col[2 * (t * wide + c0) + 1];
+            }
+            const long long at = 2ll * ((long long)n * a.C + (long long)g * a.D + c);
+            if (a.chan != a.part) {
+                a.chan[at] = p;
+                a.chan[at + 1] = q;
+            }
+            const double wt = a.w ? (double)a.w[(long long)g * a.D + c] : 1.0;
+            s1 = fma(wt, q, s1);
+            s2 = fma(wt, p, s2);
+        }
     }
     const double inv = 1.0 / ((double)a.S * a.D);
     s1 = block_sum(s1, sh) * inv;
@@ -427,50 +492,51 @@ __global__ __launch_bounds__(kGnThreads) void gn_bwd_coef_kernel(GnArgs a) {
     }
 }
 
-template <typename T, int V>
+template <typename T, int V, int ACT>
 __global__ __launch_bounds__(kGnThreads) void gn_tile_bwd_apply_kernel(GnArgs a) {
     const unsigned n = blockIdx.x / (unsigned)a.chunks, ch = blockIdx.x - n * (unsigned)a.chunks;
     const Tile t = tile_of(a, a.C / V, blockIdx.y);
     if (!t.on) return;
-    double mean[V], rstd[V];
-    float w[V], b[V], f1[V], f2[V];
+    const Channels<V> c(a, n, t.vx * V);
+    float f1[V], f2[V];
 #pragma unroll
     for (int k = 0; k < V; ++k) {
-        const int c = t.vx * V + k;
-        const long long u = (long long)n * a.G + c / a.D;
-        mean[k] = a.stats[2 * u];
-        rstd[k] = a.stats[2 * u + 1];
+        const long long u = (long long)n * a.G + c.group[k];
         f1[k] = (float)a.coef[2 * u];
         f2[k] = (float)a.coef[2 * u + 1];
-        w[k] = a.w ? a.w[c] : 1.f;
-        b[k] = a.b ? a.b[c] : 0.f;
     }
+    const float slope = a.slope;
     const T* x = (const T*)a.x + (long long)n * a.x_sn + t.vx * V;
     const T* dy = (const T*)a.dy + (long long)n * a.dy_sn + t.vx * V;
     T* o = (T*)a.out + (long long)n * a.S * a.C + t.vx * V;
     const long long s0 = (long long)ch * a.chunk_rows, s1 = s0 + a.chunk_rows < a.S ? s0 + a.chunk_rows : a.S;
-    for (long long s = s0 + t.ty; s < s1; s += t.rows) {
-        float v[V], d[V];
-        load_vec<T, V>(x + s * a.x_ss, v);
-        load_vec<T, V>(dy + s * a.dy_ss, d);
+    const long long xs = a.x_ss, ds = a.dy_ss, C = a.C;
+    walk<2, 2 * V>(s0 + t.ty, s1, t.rows,
+                   [&](long long s, float (&v)[2 * V]) {
+                       load_vec<T, V>(x + s * xs, reinterpret_cast<float(&)[V]>(v));
+                       load_vec<T, V>(dy + s * ds, reinterpret_cast<float(&)[V]>(v[V]));
+                   },
+                   [&](long long s, float (&v)[2 * V]) {
+                       float r[V];
 #pragma unroll
-        for (int k = 0; k < V; ++k) {
-            const double xh = ((double)v[k] - mean[k]) * rstd[k];
-            const float wd = w[k] * (d[k] * act_slope(fma(xh, (double)w[k], (double)b[k]), a.act, a.slope));
-            v[k] = (float)rstd[k] * (wd - f1[k] - (float)xh * f2[k]);
-        }
-        store_vec<T, V>(o + s * a.C, v);
-    }
+                       for (int k = 0; k < V; ++k) {
+                           const double xh = ((double)v[k] - c.mean[k]) * c.rstd[k];
+                           const float wd = c.w[k] * (v[V + k] * act_slope(fma(xh, (double)c.w[k], (double)c.b[k]), ACT, slope));
+                           r[k] = (float)c.rstd[k] * (wd - f1[k] - (float)xh * f2[k]);
+                       }
+                       store_vec<T, V>(o + s * C, r);
+                   });
 }
 
-// dw, db: the partials [rows][C][2] summed over their rows, 64 channels and 16 row walkers per workgroup
+// dw, db: the sums [rows][C][2] over their rows, 32 channels and 32 row walkers per workgroup
 template <typename P>
 __global__ __launch_bounds__(1024) void gn_param_grad_kernel(const P* part, long long rows, int C, float* dw, float* db) {
     __shared__ double sh[1024 * 2];
-    const int col = threadIdx.x & 63, ty = threadIdx.x >> 6, c = (int)blockIdx.x * 64 + col;
+    const int col = threadIdx.x & 31, ty = threadIdx.x >> 5, c = (int)blockIdx.x * 32 + col;
     double p = 0.0, q = 0.0;
     if (c < C)
-        for (long long r = ty; r < rows; r += 16) {
+#pragma unroll 8
+        for (long long r = ty; r < rows; r += 32) {
             p += (double)part[2 * (r * C + c)];
             q += (double)part[2 * (r * C + c) + 1];
         }
@@ -478,10 +544,9 @@ __global__ __launch_bounds__(1024) void gn_param_grad_kernel(const P* part, long
     sh[2 * threadIdx.x + 1] = q;
     __syncthreads();
     if (ty == 0 && c < C) {
-        p = q = 0.0;
-        for (int y = 0; y < 16; ++y) {
-            p += sh[2 * (y * 64 + col)];
-            q += sh[2 * (y * 64 + col) + 1];
+        for (int y = 1; y < 32; ++y) {
+            p += sh[2 * (y * 32 + col)];
+            q += sh[2 * (y * 32 + col) + 1];
         }
         dw[c] = (float)p;
         db[c] = (float)q;
@@ -541,7 +606,7 @@ void gn_unit_bwd_grid(GnPlan& P, long long N, int G) {
     const int slots = kGnThreads / P.lanes;
     P.per = G < slots ? slots / G : 1;
     P.blocks_g = G < slots ? 1 : (G + slots - 1) / slots;
-    long long nb = (N + P.per - 1) / P.per, most = 1024 / P.blocks_g;
+    long long nb = (N + P.per - 1) / P.per, most = 512 / P.blocks_g;
     if (most < 1) most = 1;
     P.blocks_n = (int)(nb < most ? nb : most);
 }
@@ -581,12 +646,17 @@ int64_t gn_ws_bytes(long long N, long long S, int C, int G, int dtype, bool back
             }
         } else {
             gn_tile_plan(P, N, S, C);
-            n = (int64_t)N * P.chunks * C * 2 * sizeof(double) + (int64_t)N * G * 2 * sizeof(double);
+            n = (int64_t)N * (P.chunks + (backward && P.chunks > 1)) * C * 2 * sizeof(double) + (int64_t)N * G * 2 * sizeof(double);
         }
         if (n > need) need = n;
     }
     return need;
 }
+
+#define GN_ACT(act, kernel, grid)                                                                                       \
+    if (act == DGG_ACT_LEAKY_RELU) hipLaunchKernelGGL((kernel<T, V, DGG_ACT_LEAKY_RELU>), grid, block, 0, st, a);       \
+    else if (act == DGG_ACT_SILU) hipLaunchKernelGGL((kernel<T, V, DGG_ACT_SILU>), grid, block, 0, st, a);              \
+    else hipLaunchKernelGGL((kernel<T, V, DGG_ACT_NONE>), grid, block, 0, st, a);
 
 template <typename T, int V> int gn_forward_v(const GnPlan& P, GnArgs& a, hipStream_t st) {
     if (P.unit) {
@@ -603,12 +673,12 @@ template <typename T, int V> int gn_forward_v(const GnPlan& P, GnArgs& a, hipStr
     const dim3 grid((unsigned)(a.N * P.chunks), P.blocks_c), block(kGnThreads);
     hipLaunchKernelGGL((gn_tile_sum_kernel<T, V>), grid, block, 0, st, a);
     hipLaunchKernelGGL((gn_stats_kernel<T>), dim3((unsigned)(a.N * a.G)), block, 0, st, a);
-    hipLaunchKernelGGL((gn_tile_apply_kernel<T, V>), grid, block, 0, st, a);
+    GN_ACT(a.act, gn_tile_apply_kernel, grid)
     return check_launch("group_norm forward");
 }
 
 template <typename T, int V> int gn_backward_v(const GnPlan& P, GnArgs& a, hipStream_t st) {
-    const dim3 block(kGnThreads), cols((unsigned)((a.C + 63) / 64));
+    const dim3 block(kGnThreads), cols((unsigned)((a.C + 31) / 32));
     if (P.unit) {
         if (!a.dw) a.part = nullptr;
         const dim3 grid((unsigned)P.blocks_g * P.blocks_n);
@@ -624,12 +694,11 @@ template <typename T, int V> int gn_backward_v(const GnPlan& P, GnArgs& a, hipSt
         return check_launch("group_norm backward");
     }
     const dim3 grid((unsigned)(a.N * P.chunks), P.blocks_c);
-    hipLaunchKernelGGL((gn_tile_bwd_sum_kernel<T, V>), grid, block, 0, st, a);
+    GN_ACT(a.act, gn_tile_bwd_sum_kernel, grid)
     hipLaunchKernelGGL(gn_bwd_coef_kernel, dim3((unsigned)(a.N * a.G)), block, 0, st, a);
     if (a.dw)
-        hipLaunchKernelGGL((gn_param_grad_kernel<double>), cols, dim3(1024), 0, st, (const double*)a.part,
-                           a.N * P.chunks, a.C, a.dw, a.db);
-    hipLaunchKernelGGL((gn_tile_bwd_apply_kernel<T, V>), grid, block, 0, st, a);
+        hipLaunchKernelGGL((gn_param_grad_kernel<double>), cols, dim3(1024), 0, st, (const double*)a.chan, a.N, a.C, a.dw, a.db);
+    GN_ACT(a.act, gn_tile_bwd_apply_kernel, grid)
     return check_launch("group_norm backward");
 }
 
@@ -665,9 +734,10 @@ int gn_run(bool backward, GnArgs& a, int dtype, void* ws, size_t ws_bytes, hipSt
     if (P.unit) {
         need = backward && a.dw ? (size_t)P.blocks_n * P.per * a.C * 2 * sizeof(float) : 0;
     } else {
-        const size_t part = (size_t)a.N * P.chunks * a.C * 2 * sizeof(double);
-        need = part + (size_t)a.N * a.G * 2 * sizeof(double);
-        a.coef = (double*)((char*)ws + part);
+        const size_t chan = (size_t)a.N * a.C * 2 * sizeof(double), part = chan * P.chunks, more = backward && P.chunks > 1 ? chan : 0;
+        need = part + more + (size_t)a.N * a.G * 2 * sizeof(double);
+        a.chan = (double*)((char*)ws + (more ? part : 0));
+        a.coef = (double*)((char*)ws + part + more);
         if (!a.stats) a.stats = a.coef;   // a forward without a backward keeps its statistics in the workspace
     }
     if (need && (!ws || ws_bytes < need || (uintptr_t)ws % 8)) {

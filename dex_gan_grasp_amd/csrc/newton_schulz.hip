@@ -68,11 +68,13 @@ enum { kNorm, kSplit, kGram, kSum, kSquare, kApply, kPhases };
 // first workgroup of each matrix in one of the launches (none: INT_MAX)
 struct NsFirst { int at[kNsMats]; };
 
+struct NsUpdate { float mu, gscale; int nesterov; };
+
 struct NsArgs {
     NsMat mat[kNsMats];
     char* ws;
-    int nesterov;
-    float mu, gscale, decay;
+    NsUpdate update;
+    float decay;
     int adjust;
     double lr, eps;
     int steps;
@@ -126,7 +128,7 @@ template <int N> __device__ __forceinline__ double block_sum(double v, double* s
 }
 
 // u of the muon step from the gradient and the momentum AFTER its update
-__device__ __forceinline__ float muon_u(const NsArgs& a, float g, float m) { return a.nesterov ? fmaf(a.mu, m, a.gscale * g) : m; }
+__device__ __forceinline__ float muon_u(const NsUpdate& a, float g, float m) { return a.nesterov ? fmaf(a.mu, m, a.gscale * g) : m; }
 
 // ------------------------------------------------------------------------------------------------ norm
 // sum of squares in 64 bits, one partial a workgroup (muon: M is updated on the way).  Rows without gaps are one long row.
@@ -148,6 +150,7 @@ __global__ __launch_bounds__(kThreads) void ns_norm_kernel(NsArgs a, NsFirst fir
     const long long per = flat ? ((total + M.parts - 1) / M.parts + 63) / 64 * 64 : 0;
     const int row0 = flat ? 0 : part, rows = flat ? 1 : M.rows, drow = flat ? 1 : M.parts;
     const long long c0 = flat ? part * per : 0, c1 = flat ? (c0 + per < total ? c0 + per : total) : M.cols;
+    const NsUpdate up = a.update;
     double s = 0.0;
     for (int r = row0; r < rows; r += drow) {
         const Global<T>* g = in + (long long)r * M.ld_in;
@@ -164,9 +167,9 @@ __global__ __launch_bounds__(kThreads) void ns_norm_kernel(NsArgs a, NsFirst fir
             for (int e = 0; e < 8; ++e) {
                 if (c + e * kThreads >= c1) break;
                 if (MUON) {
-                    m[e] = fmaf(a.mu, m[e], a.gscale * u[e]);
+                    m[e] = fmaf(up.mu, m[e], up.gscale * u[e]);
                     mr[c + e * kThreads] = m[e];
-                    u[e] = muon_u(a, u[e], m[e]);
+                    u[e] = muon_u(up, u[e], m[e]);
                 }
                 s = fma((double)u[e], (double)u[e], s);
             }
@@ -230,6 +233,7 @@ __global__ __launch_bounds__(kThreads) void ns_split_kernel(const NsArgs* args, 
     const Global<float>* mom = MUON ? (Global<float>*)M.mom + (size_t)bat * M.mom_stride : nullptr;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const int r0 = M.turned ? j0 : i0, c0 = M.turned ? i0 : j0;   // of U
+    const NsUpdate up = a.update;   // (read before anything is written: the compiler could not tell that it stays)
     float u[16], m[16];   // all of the tile is in flight while the norm is summed
 #pragma unroll
     for (int q = 0; q < 16; ++q) {
@@ -246,7 +250,7 @@ __global__ __launch_bounds__(kThreads) void ns_split_kernel(const NsArgs* args, 
 #pragma unroll
     for (int q = 0; q < 16; ++q) {
         const bool in_u = r0 + q * 4 + wave < M.rows && c0 + lane < M.cols;
-        const float v = in_u ? ldexpf(MUON ? muon_u(a, u[q], m[q]) : u[q], k) : 0.f;
+        const float v = in_u ? ldexpf(MUON ? muon_u(up, u[q], m[q]) : u[q], k) : 0.f;
         if (M.turned) t[lane][q * 4 + wave] = v;
         else t[q * 4 + wave][lane] = v;
     }
@@ -403,7 +407,7 @@ __device__ __forceinline__ void load4(const char* p, float (&v)[4]) {
     for (int e = 0; e < 4; ++e) v[e] = (float)hi[e] + (float)lo[e];
 }
 
-// A = X X^T, tiles on and above the diagonal, a range of k each: fp32 slabs [split][mp][mp]
+// A = X X^T, tiles on and above the diagonal, a range of k each: fp32 slabs [split][mp][mp], or A where one range is all of k
 template <int S>
 __global__ __launch_bounds__(kThreads) void ns_gram_kernel(const NsArgs* args, NsFirst first, int k) {
     using Pr = Prod<1, S>;
@@ -418,8 +422,26 @@ __global__ __launch_bounds__(kThreads) void ns_gram_kernel(const NsArgs* args, N
     const char* x = ws + M.xr + (size_t)bat * plane_bytes(M.mp, M.np);
     Pr p;
     p.run(x, ti * Pr::kTile, M.mp, x, tj * Pr::kTile, M.mp, M.np, split * M.kblocks, min((split + 1) * M.kblocks, M.np / 32));
-    const int i0 = ti * Pr::kTile + p.i0(), j0 = tj * Pr::kTile + p.j0();
-    float* slab = (float*)(ws + M.slab) + ((size_t)bat * M.splits + split) * M.mp * M.mp + (size_t)i0 * M.mp + j0;
+    if (M.splits == 1) {   // all of k: A itself, and its mirror image
+        const NsScale z = scale_of(ws, M, bat, k);
+        char* A = ws + M.a + (size_t)bat * plane_bytes(M.mp, M.mp);
+        const int i0 = ti * Pr::kTile, j0 = tj * Pr::kTile;
+        float v[4][4];
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) v[q][e] = p.value(0, 0, q, e) * z.sx * z.sx * z.sa;   // (in this order, as in ns_sum_kernel)
+            store4(A + plane_at(j0 + p.j0(), i0 + p.i0(), M.mp) + (q >> 1) * 2048 + (q & 1) * 512, v[q]);
+        }
+        if (ti == tj) return;
+        float w[2][8];
+        p.turn(v, w);
+#pragma unroll
+        for (int q = 0; q < 2; ++q) store8(A + plane_at(i0 + p.ti(), j0 + p.tj() + 16 * q, M.mp), w[q]);
+        return;
+    }
+    float* slab = (float*)(ws + M.slab) + ((size_t)bat * M.splits + split) * M.mp * M.mp +
+                  (size_t)(ti * Pr::kTile + p.i0()) * M.mp + tj * Pr::kTile + p.j0();
 #pragma unroll
     for (int q = 0; q < 4; ++q)
 #pragma unroll
@@ -520,7 +542,7 @@ __global__ __launch_bounds__(kThreads, 2) void ns_apply_kernel(const NsArgs* arg
     char* xr = ws + M.xr + (size_t)bat * plane_bytes(M.mp, M.np);
     const NsScale z = scale_of(ws, M, bat, k);
     constexpr bool last = !std::is_same<Out, void>::value;
-    const float fb = z.sx / z.sb * (last ? 1.f : z.sx_next);
+    const float fb = z.sx / z.sb * (last ? 1.f : z.sx_next), step = M.step, decay = a.decay;
     Pr p;
     p.run(B, i0, M.mp, xt, j0, M.np, M.mp, 0, M.mp / 32);
 #pragma unroll
@@ -559,7 +581,7 @@ __global__ __launch_bounds__(kThreads, 2) void ns_apply_kernel(const NsArgs* arg
                     for (int q = 0; q < 4; ++q)
 #pragma unroll
                         for (int e = 0; e < 4; ++e)
-                            if (i + 8 * q + e < M.m && j < M.n) W[(8 * q + e) * di] = fmaf(-M.step, v[q][e], a.decay * w[q][e]);
+                            if (i + 8 * q + e < M.m && j < M.n) W[(8 * q + e) * di] = fmaf(-step, v[q][e], decay * w[q][e]);
                 } else {
                     Global<Out>* o = (Global<Out>*)M.out + at;
 #pragma unroll
@@ -617,6 +639,7 @@ __global__ __launch_bounds__(kSmallThreads) void ns_small_kernel(NsArgs a, NsFir
     // U as it lies in memory, 16 elements a thread at most, through LDS (fp32 [mp][np + 4], in the place of X by columns and the start of A)
     float* stage = (float*)xt;
     const int total = M.rows * M.cols, pitch = np + 4, units = mp * np / 8;
+    const NsUpdate up = a.update;
     const float per_col = 1.f / (float)M.cols;
     for (int e = threadIdx.x; e < mp * pitch / 4; e += kSmallThreads) ((float4*)stage)[e] = make_float4(0.f, 0.f, 0.f, 0.f);
     float u[16], m[16];
@@ -633,9 +656,9 @@ __global__ __launch_bounds__(kSmallThreads) void ns_small_kernel(NsArgs a, NsFir
         const int e = (int)threadIdx.x + t * kSmallThreads, r = (int)(((float)e + 0.5f) * per_col), c = e - r * M.cols;
         if (e >= total) break;
         if (MUON) {
-            m[t] = fmaf(a.mu, m[t], a.gscale * u[t]);
+            m[t] = fmaf(up.mu, m[t], up.gscale * u[t]);
             mom[(long long)r * M.ld_mom + c] = m[t];
-            u[t] = muon_u(a, u[t], m[t]);
+            u[t] = muon_u(up, u[t], m[t]);
         }
         s = fma((double)u[t], (double)u[t], s);
         stage[M.turned ? c * pitch + r : r * pitch + c] = u[t];
@@ -666,6 +689,7 @@ __global__ __launch_bounds__(kSmallThreads) void ns_small_kernel(NsArgs a, NsFir
     __syncthreads();
     const int splits = small_splits(mp), tiles = small_tiles(mp), r = lane & 31, h = lane >> 5;
     // B X: the block of this wave; the lane's elements are (i + 8 q + e, j)
+    const float step = M.step, decay = a.decay;
     const bool mine = wave < T * (np / 32);
     const int bj = wave / T, bi = wave - bj * T, i = bi * 32 + 4 * h, j = bj * 32 + r;
     const long long di = M.turned ? 1 : M.ld_out, at = M.turned ? (long long)j * M.ld_out + i : (long long)i * M.ld_out + j;
@@ -789,7 +813,7 @@ __global__ __launch_bounds__(kSmallThreads) void ns_small_kernel(NsArgs a, NsFir
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
                     if (i + 8 * q + e >= M.m || j >= M.n) continue;
-                    if (MUON) W[at + (8 * q + e) * di] = fmaf(-M.step, v[e], a.decay * w[q][e]);
+                    if (MUON) W[at + (8 * q + e) * di] = fmaf(-step, v[e], decay * w[q][e]);
                     else ((Global<In>*)M.out)[(size_t)bat * M.out_stride + at + (8 * q + e) * di] = (In)v[e];
                 }
             }
@@ -901,7 +925,9 @@ void ns_plan(const dgg_matrix* const* mats, int count, NsArgs& a, NsPlan& P) {
         // for the generator's matrices, 10.8 .. 11.6 for 512 x 4620; 128 x 128 tiles: 18.9 and 11.6)
         int splits = ceil_div(512, (long long)tiles * M.batch);
         if (splits > M.np / 256) splits = M.np / 256;
-        if (splits < 1) splits = 1;
+        // one range of all k, and no launch that sums, for few k or where the tiles alone fill the chip (a call for 512 x 256: 108 -> 104 us,
+        // for 24 of 257 x 771: 272 -> 252 us)
+        if (splits < 1 || M.np <= 512 || (long long)tiles * M.batch >= 256) splits = 1;
         M.kblocks = ceil_div(M.np / 32, splits);
         M.splits = ceil_div(M.np / 32, M.kblocks);
         const size_t b = (size_t)M.batch;
@@ -909,11 +935,11 @@ void ns_plan(const dgg_matrix* const* mats, int count, NsArgs& a, NsPlan& P) {
         M.xt = at;   at = up(at + b * 2 * plane_bytes(M.np, M.mp));
         M.a = at;    at = up(at + b * plane_bytes(M.mp, M.mp));
         M.b = at;    at = up(at + b * plane_bytes(M.mp, M.mp));
-        M.slab = at; at = up(at + b * M.splits * M.mp * M.mp * 4);
+        M.slab = at; at = up(at + (M.splits > 1 ? b * M.splits * M.mp * M.mp * 4 : 0));
         M.part = at; at = up(at + b * M.parts * 8);
         M.scal = at; at = up(at + b * kNsSteps * sizeof(NsScale));
         const int n32 = M.mp / 32;
-        const int blocks[kPhases] = {M.parts, t * (M.np / 64), tiles * M.splits, n32 * (n32 + 1) / 2, tiles,
+        const int blocks[kPhases] = {M.parts, t * (M.np / 64), tiles * M.splits, M.splits > 1 ? n32 * (n32 + 1) / 2 : 0, tiles,
                                        ceil_div(M.mp, 64 * P.f_apply) * ceil_div(M.np, 64 * P.f_apply)};
         for (int k = 0; k < kPhases; ++k) {
             P.first[k].at[i] = P.grid[k];
@@ -1000,7 +1026,7 @@ int ns_run(const dgg_matrix* mats, int count, NsArgs& a, const double* coef, int
         constexpr int lds1 = Prod<1, 3>::kLds, lds2 = Prod<2, 2>::kLds;
         for (int k = 0; k < steps; ++k) {
             hipLaunchKernelGGL((ns_gram_kernel<3>), dim3(P.grid[kGram]), block, lds1, st, args, P.first[kGram], k);
-            hipLaunchKernelGGL(ns_sum_kernel, dim3(P.grid[kSum]), block, 0, st, args, P.first[kSum], k);
+            if (P.grid[kSum]) hipLaunchKernelGGL(ns_sum_kernel, dim3(P.grid[kSum]), block, 0, st, args, P.first[kSum], k);
             hipLaunchKernelGGL((ns_square_kernel<3>), dim3(P.grid[kSquare]), block, lds1, st, args, P.first[kSquare], k);
             using Last = typename std::conditional<MUON, ToMuon, T>::type;
             const bool last = k + 1 == steps;
@@ -1062,9 +1088,7 @@ int dgg_muon_step(const dgg_matrix* mats, int count, double lr, double momentum,
         return DGG_ERR_INVALID;
     }
     NsArgs a = {};
-    a.nesterov = nesterov != 0;
-    a.mu = (float)momentum;
-    a.gscale = (float)grad_scale;
+    a.update = {(float)momentum, (float)grad_scale, nesterov != 0};
     a.lr = lr;
     a.adjust = adjust;
     a.decay = (float)(1.0 - lr * weight_decay);
