@@ -98,7 +98,8 @@ struct GnArgs {
     long long chunk_rows;
     int tx;                 // tile: vectors of a row a workgroup covers
     int lanes;              // unit: lanes per group
-    int blocks_g, blocks_n; // unit backward: grid
+    int blocks_g, blocks_n; // unit backward: grid; resident: blocks_g blocks of
+    int res_groups;         // res_groups groups a sample
 };
 
 __device__ __forceinline__ double lane_sum(double v, int lanes) {
@@ -528,6 +529,246 @@ __global__ __launch_bounds__(kGnThreads) void gn_tile_bwd_apply_kernel(GnArgs a)
                    });
 }
 
+// ------------------------------------------------------------------------------------------------ resident route
+// A workgroup of up to 512 threads owns all S points of one sample in a block of whole groups and keeps them in registers: one
+// read, one launch.  Thread -> (vector of the row, row) as in the tile route, R rows a thread at most; a vector lies in one group
+// (V divides D).  The workgroups of neighbouring blocks share cache lines: consecutive numbers go to one die.
+constexpr int kResThreads = 512;
+
+__device__ __forceinline__ unsigned by_die() {   // a permutation of the grid's numbers that gives each of the 8 dies a run of them
+    const unsigned n = gridDim.x, q = n >> 3, r = n & 7, die = blockIdx.x & 7;
+    return die * q + min(die, r) + (blockIdx.x >> 3);
+}
+
+struct Res {
+    unsigned n, blk;
+    int tx, ty, rows, x, per;   // tx: vectors a row; rows: side by side; x: this thread's vector; per: vectors a group's row
+    bool on;
+    __device__ __forceinline__ Res(const GnArgs& a, int V) {
+        const unsigned id = by_die();
+        n = id / (unsigned)a.blocks_g;
+        blk = id - n * (unsigned)a.blocks_g;
+        per = a.D / V;
+        const int groups = min(a.res_groups, a.G - (int)blk * a.res_groups);
+        tx = groups * per;
+        rows = (int)blockDim.x / tx;
+        ty = (int)threadIdx.x / tx;
+        x = (int)threadIdx.x - ty * tx;
+        on = ty < rows;
+    }
+};
+
+// A vector of V elements as it lies in memory.  keep(): what has been made of it is forgotten — the compiler would rather hold the
+// unpacked fp32 values from one use to the next than unpack again, and spill them.
+template <typename T, int V> struct Raw {
+    typedef uint32_t Bits __attribute__((ext_vector_type(V * sizeof(T) / 4)));
+    Bits bits;
+    __device__ __forceinline__ void load(const T* p) { bits = *reinterpret_cast<const Bits*>(p); }
+    __device__ __forceinline__ void keep() { asm("" : "+v"(bits)); }
+    __device__ __forceinline__ void get(float (&v)[V]) const {
+        const Vec<T, V> r = __builtin_bit_cast(Vec<T, V>, bits);
+#pragma unroll
+        for (int k = 0; k < V; ++k) v[k] = (float)r.e[k];
+    }
+};
+
+// sums of sh[ty][x] over all rows and the `per` vectors of each group, a wave a group in turn, in a fixed order -> out[group]
+__device__ __forceinline__ void group_sums(const double* sh, double* out, const Res& t) {
+    __syncthreads();
+    const int lane = threadIdx.x & 63, waves = blockDim.x >> 6, groups = t.tx / t.per, n = t.rows * t.per;
+    for (int g = threadIdx.x >> 6; g < groups; g += waves) {
+        double s = 0.0;
+        for (int e = lane; e < n; e += 64) {
+            const int y = e / t.per;
+            s += sh[y * t.tx + g * t.per + e - y * t.per];
+        }
+        s = lane_sum(s, 64);
+        if (lane == 0) out[g] = s;
+    }
+    __syncthreads();
+}
+
+template <typename T, int V, int R, int ACT>
+__global__ __launch_bounds__(kResThreads) void gn_res_fwd_kernel(GnArgs a) {
+    __shared__ double sh[kResThreads], sums[kResThreads];
+    const Res t(a, V);
+    const int c0 = ((int)t.blk * a.res_groups * t.per + t.x) * V, S = (int)a.S, g = t.x / t.per;
+    const T* x = (const T*)a.x + (long long)t.n * a.x_sn + c0;
+    Raw<T, V> raw[R];
+    float w[V], b[V];
+    double s = 0.0;
+    if (t.on) {
+#pragma unroll
+        for (int r = 0; r < R; ++r) raw[r].load(x + (long long)min(t.ty + r * t.rows, S - 1) * a.x_ss);
+        load_param<V>(a.w, c0, 1.f, w);
+        load_param<V>(a.b, c0, 0.f, b);
+#pragma unroll
+        for (int r = 0; r < R; ++r)
+            if (t.ty + r * t.rows < S) {
+                float v[V];
+                raw[r].get(v);
+#pragma unroll
+                for (int k = 0; k < V; ++k) s += (double)v[k];
+            }
+    }
+    const double count = (double)S * a.D;
+    sh[threadIdx.x] = s;
+    group_sums(sh, sums, t);
+    const double mean = sums[g] / count;
+    s = 0.0;
+    if (t.on)
+#pragma unroll
+        for (int r = 0; r < R; ++r)
+            if (t.ty + r * t.rows < S) {
+                float v[V];
+                raw[r].keep();
+                raw[r].get(v);
+#pragma unroll
+                for (int k = 0; k < V; ++k) {
+                    const double d = (double)v[k] - mean;
+                    s = fma(d, d, s);
+                }
+            }
+    __syncthreads();   // (everyone has read sums)
+    sh[threadIdx.x] = s;
+    group_sums(sh, sums, t);
+    const double rstd = 1.0 / sqrt(sums[g] / count + a.eps);
+    if (!t.on) return;
+    if (a.stats && t.ty == 0 && t.x == g * t.per) {
+        double* o = a.stats + 2ll * ((long long)t.n * a.G + (long long)t.blk * a.res_groups + g);
+        o[0] = mean;
+        o[1] = rstd;
+    }
+    double sc[V];
+#pragma unroll
+    for (int k = 0; k < V; ++k) sc[k] = rstd * (double)w[k];
+    T* y = (T*)a.out + (long long)t.n * S * a.C + c0;
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+        const int row = t.ty + r * t.rows;
+        if (row >= S) break;
+        float v[V];
+        raw[r].keep();
+        raw[r].get(v);
+#pragma unroll
+        for (int k = 0; k < V; ++k) v[k] = act_value(fma((double)v[k] - mean, sc[k], (double)b[k]), ACT, a.slope);
+        store_vec<T, V>(y + (long long)row * a.C, v);
+    }
+}
+
+template <typename T, int V, int R, int ACT>
+__global__ __launch_bounds__(kResThreads) void gn_res_bwd_kernel(GnArgs a) {
+    __shared__ float sh[kResThreads * V * 2];
+    __shared__ double sums[2 * kResThreads];
+    const Res t(a, V);
+    const int c0 = ((int)t.blk * a.res_groups * t.per + t.x) * V, S = (int)a.S, g = t.x / t.per;
+    const T* x = (const T*)a.x + (long long)t.n * a.x_sn + c0;
+    const T* dy = (const T*)a.dy + (long long)t.n * a.dy_sn + c0;
+    Raw<T, V> rx[R], rd[R];
+    float w[V], b[V];
+    double p[V], q[V], mean = 0.0, rstd = 0.0;
+#pragma unroll
+    for (int k = 0; k < V; ++k) p[k] = q[k] = 0.0;
+    if (t.on) {
+#pragma unroll
+        for (int r = 0; r < R; ++r) {
+            const long long row = min(t.ty + r * t.rows, S - 1);
+            rx[r].load(x + row * a.x_ss);
+            rd[r].load(dy + row * a.dy_ss);
+        }
+        load_param<V>(a.w, c0, 1.f, w);
+        load_param<V>(a.b, c0, 0.f, b);
+        const double* st = a.stats + 2ll * ((long long)t.n * a.G + (long long)t.blk * a.res_groups + g);
+        mean = st[0];
+        rstd = st[1];
+#pragma unroll
+        for (int r = 0; r < R; ++r)
+            if (t.ty + r * t.rows < S) {
+                float v[V], d[V];
+                rx[r].get(v);
+                rd[r].get(d);
+#pragma unroll
+                for (int k = 0; k < V; ++k) {
+                    const double xh = ((double)v[k] - mean) * rstd;
+                    const double dz = (double)(d[k] * act_slope(fma(xh, (double)w[k], (double)b[k]), ACT, a.slope));
+                    p[k] = fma(dz, xh, p[k]);
+                    q[k] += dz;
+                }
+            }
+    }
+    // The columns' sums over the rows — a column: one of the two sums of one channel —, fp32 from each thread, added in 64 bits: `parts`
+    // threads a column, then a wave a group, which also has the group's two means from them.
+    const int cols = t.tx * V * 2, parts = cols < (int)blockDim.x ? (int)blockDim.x / cols : 1;
+    if (t.on)
+#pragma unroll
+        for (int k = 0; k < V; ++k) {
+            sh[((int)threadIdx.x * V + k) * 2] = (float)p[k];
+            sh[((int)threadIdx.x * V + k) * 2 + 1] = (float)q[k];
+        }
+    __syncthreads();
+    const int part = parts > 1 ? (int)threadIdx.x / cols : 0;
+    double sum = 0.0;
+    if (parts > 1) {
+        const int col = (int)threadIdx.x - part * cols;
+        if (part < parts)
+            for (int y = part; y < t.rows; y += parts) sum += (double)sh[y * cols + col];
+        __syncthreads();
+        if (part < parts) sh[part * cols + col] = (float)sum;
+        __syncthreads();
+    }
+    const int lane = threadIdx.x & 63, waves = blockDim.x >> 6, groups = t.tx / t.per, n = parts > 1 ? parts : t.rows;
+    for (int j = threadIdx.x >> 6; j < groups; j += waves) {
+        double s1 = 0.0, s2 = 0.0;
+        for (int e = lane; e < t.per * V; e += 64) {
+            const int ch = j * t.per * V + e;
+            double u = 0.0, v = 0.0;
+            for (int y = 0; y < n; ++y) {
+                const float2 o = *reinterpret_cast<const float2*>(sh + y * cols + 2 * ch);
+                u += (double)o.x;
+                v += (double)o.y;
+            }
+            const long long c = (long long)t.blk * a.res_groups * t.per * V + ch;
+            if (a.dw) {
+                double* o = a.chan + 2ll * ((long long)t.n * a.C + c);
+                o[0] = u;
+                o[1] = v;
+            }
+            const double wt = a.w ? (double)a.w[c] : 1.0;
+            s1 = fma(wt, v, s1);
+            s2 = fma(wt, u, s2);
+        }
+        s1 = lane_sum(s1, 64);
+        s2 = lane_sum(s2, 64);
+        if (lane == 0) {
+            sums[2 * j] = s1;
+            sums[2 * j + 1] = s2;
+        }
+    }
+    __syncthreads();
+    if (!t.on) return;
+    const double s1 = sums[2 * g], s2 = sums[2 * g + 1];
+    const double inv = 1.0 / ((double)S * a.D);
+    const float f1 = (float)(s1 * inv), f2 = (float)(s2 * inv), fr = (float)rstd;
+    T* o = (T*)a.out + (long long)t.n * S * a.C + c0;
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+        const int row = t.ty + r * t.rows;
+        if (row >= S) break;
+        float v[V], d[V];
+        rx[r].keep();
+        rd[r].keep();
+        rx[r].get(v);
+        rd[r].get(d);
+#pragma unroll
+        for (int k = 0; k < V; ++k) {
+            const double xh = ((double)v[k] - mean) * rstd;
+            const float wd = w[k] * (d[k] * act_slope(fma(xh, (double)w[k], (double)b[k]), ACT, a.slope));
+            v[k] = fr * (wd - f1 - (float)xh * f2);
+        }
+        store_vec<T, V>(o + (long long)row * a.C, v);
+    }
+}
+
 // dw, db: the sums [rows][C][2] over their rows, 32 channels and 32 row walkers per workgroup
 template <typename P>
 __global__ __launch_bounds__(1024) void gn_param_grad_kernel(const P* part, long long rows, int C, float* dw, float* db) {
@@ -555,8 +796,9 @@ __global__ __launch_bounds__(1024) void gn_param_grad_kernel(const P* part, long
 
 // ------------------------------------------------------------------------------------------------ host side
 struct GnPlan {
-    int V;                // elements per access
-    bool unit;
+    int V, es;            // elements per access, bytes of one
+    bool unit, res;
+    int res_rows, res_groups, res_blocks, res_threads;
     int items, lanes;     // unit
     int per, blocks_g, blocks_n;
     int tx, blocks_c, chunks;
@@ -600,6 +842,35 @@ bool gn_unit_plan(GnPlan& P, long long S, int D, bool backward) {
     P.items = 1;
     while (P.items * P.lanes < nv) P.items *= 2;
     return true;
+}
+
+// Resident: whole samples in registers, 16 vectors a thread (backward: of x and of dy) and 512 threads at most.
+bool gn_res_plan(GnPlan& P, long long N, long long S, int C, int G, bool backward) {
+    const int D = C / G;
+    if (P.V < 4 || D % P.V || S > 16 * kResThreads) return false;
+    const int per = D / P.V;
+    if (per > kResThreads) return false;
+    // as many groups side by side as leave every thread 16 rows ..
+    int groups = (int)(16ll * kResThreads / (S * per));
+    if (groups > kResThreads / per) groups = kResThreads / per;
+    while (groups > 0 && (long long)(kResThreads / (groups * per)) * 16 < S) --groups;
+    if (groups < 1) return false;
+    if (groups > G) groups = G;
+    // .. but 256 workgroups at least, down to 64 bytes of a row each (and 64 workgroups whatever it takes)
+    const int line = 64 / (P.V * P.es);
+    while (groups > 1 && N * ((G + groups - 1) / groups) < 256 && ((groups / 2) * per >= line || N * ((G + groups - 1) / groups) < 64))
+        groups /= 2;
+    P.res_groups = groups;
+    P.res_blocks = (G + groups - 1) / groups;
+    const int tx = groups * per;
+    long long rows = kResThreads / tx;
+    if (rows > S) rows = S;
+    P.res_threads = (int)((rows * tx + 63) / 64 * 64);
+    if (P.res_threads > kResThreads) P.res_threads = kResThreads;
+    rows = P.res_threads / tx;
+    const long long most = (S + rows - 1) / rows;
+    P.res_rows = most <= 4 ? 4 : most <= 8 ? 8 : 16;
+    return N * P.res_blocks < 0x7fffffff;
 }
 
 void gn_unit_bwd_grid(GnPlan& P, long long N, int G) {
@@ -658,6 +929,11 @@ int64_t gn_ws_bytes(long long N, long long S, int C, int G, int dtype, bool back
     else if (act == DGG_ACT_SILU) hipLaunchKernelGGL((kernel<T, V, DGG_ACT_SILU>), grid, block, 0, st, a);              \
     else hipLaunchKernelGGL((kernel<T, V, DGG_ACT_NONE>), grid, block, 0, st, a);
 
+#define GN_RES(act, kernel, R)                                                                                             \
+    if (act == DGG_ACT_LEAKY_RELU) hipLaunchKernelGGL((kernel<T, V, R, DGG_ACT_LEAKY_RELU>), grid, block, 0, st, a);       \
+    else if (act == DGG_ACT_SILU) hipLaunchKernelGGL((kernel<T, V, R, DGG_ACT_SILU>), grid, block, 0, st, a);              \
+    else hipLaunchKernelGGL((kernel<T, V, R, DGG_ACT_NONE>), grid, block, 0, st, a);
+
 template <typename T, int V> int gn_forward_v(const GnPlan& P, GnArgs& a, hipStream_t st) {
     if (P.unit) {
         const long long threads = a.N * a.G * P.lanes;
@@ -670,6 +946,14 @@ template <typename T, int V> int gn_forward_v(const GnPlan& P, GnArgs& a, hipStr
         }
         return check_launch("group_norm forward");
     }
+    if constexpr (V >= 4)
+        if (P.res) {
+            const dim3 grid((unsigned)(a.N * P.res_blocks)), block(P.res_threads);
+            if (P.res_rows == 4) { GN_RES(a.act, gn_res_fwd_kernel, 4) }
+            else if (P.res_rows == 8) { GN_RES(a.act, gn_res_fwd_kernel, 8) }
+            else { GN_RES(a.act, gn_res_fwd_kernel, 16) }
+            return check_launch("group_norm forward");
+        }
     const dim3 grid((unsigned)(a.N * P.chunks), P.blocks_c), block(kGnThreads);
     hipLaunchKernelGGL((gn_tile_sum_kernel<T, V>), grid, block, 0, st, a);
     hipLaunchKernelGGL((gn_stats_kernel<T>), dim3((unsigned)(a.N * a.G)), block, 0, st, a);
@@ -693,6 +977,16 @@ template <typename T, int V> int gn_backward_v(const GnPlan& P, GnArgs& a, hipSt
                                (long long)P.blocks_n * P.per, a.C, a.dw, a.db);
         return check_launch("group_norm backward");
     }
+    if constexpr (V >= 4)
+        if (P.res) {
+            const dim3 grid((unsigned)(a.N * P.res_blocks)), block(P.res_threads);
+            if (P.res_rows == 4) { GN_RES(a.act, gn_res_bwd_kernel, 4) }
+            else if (P.res_rows == 8) { GN_RES(a.act, gn_res_bwd_kernel, 8) }
+            else { GN_RES(a.act, gn_res_bwd_kernel, 16) }
+            if (a.dw)
+                hipLaunchKernelGGL((gn_param_grad_kernel<double>), cols, dim3(1024), 0, st, (const double*)a.chan, a.N, a.C, a.dw, a.db);
+            return check_launch("group_norm backward");
+        }
     const dim3 grid((unsigned)(a.N * P.chunks), P.blocks_c);
     GN_ACT(a.act, gn_tile_bwd_sum_kernel, grid)
     hipLaunchKernelGGL(gn_bwd_coef_kernel, dim3((unsigned)(a.N * a.G)), block, 0, st, a);
@@ -714,25 +1008,33 @@ int gn_run(bool backward, GnArgs& a, int dtype, void* ws, size_t ws_bytes, hipSt
     GnPlan P;
     std::initializer_list<long long> fs = {a.x_sn, a.x_ss}, bs = {a.x_sn, a.x_ss, a.dy_sn, a.dy_ss};
     P.V = gn_width(dtype, a.D, a.C, backward ? bs : fs, {a.x, a.out, backward ? a.dy : a.x});
+    P.es = elem_bytes(dtype);
     P.unit = gn_unit_plan(P, a.S, a.D, backward);
-    if (!P.unit) {
-        P.V = gn_width(dtype, 0, a.C, backward ? bs : fs, {a.x, a.out, backward ? a.dy : a.x});
-        gn_tile_plan(P, a.N, a.S, a.C);
-        if (P.blocks_c > 65535) return DGG_ERR_INVALID;
-        a.chunks = P.chunks;
-        a.chunk_rows = P.chunk_rows;
-        a.tx = P.tx;
-    } else {
+    P.res = !P.unit && gn_res_plan(P, a.N, a.S, a.C, a.G, backward);
+    if (P.unit) {
         a.lanes = P.lanes;
         if (backward) {
             gn_unit_bwd_grid(P, a.N, a.G);
             a.blocks_g = P.blocks_g;
             a.blocks_n = P.blocks_n;
         }
+    } else if (P.res) {
+        a.res_groups = P.res_groups;
+        a.blocks_g = P.res_blocks;
+    } else {
+        P.V = gn_width(dtype, 0, a.C, backward ? bs : fs, {a.x, a.out, backward ? a.dy : a.x});
+        gn_tile_plan(P, a.N, a.S, a.C);
+        if (P.blocks_c > 65535) return DGG_ERR_INVALID;
+        a.chunks = P.chunks;
+        a.chunk_rows = P.chunk_rows;
+        a.tx = P.tx;
     }
     size_t need = 0;
     if (P.unit) {
         need = backward && a.dw ? (size_t)P.blocks_n * P.per * a.C * 2 * sizeof(float) : 0;
+    } else if (P.res) {
+        need = backward && a.dw ? (size_t)a.N * a.C * 2 * sizeof(double) : 0;
+        a.chan = (double*)ws;
     } else {
         const size_t chan = (size_t)a.N * a.C * 2 * sizeof(double), part = chan * P.chunks, more = backward && P.chunks > 1 ? chan : 0;
         need = part + more + (size_t)a.N * a.G * 2 * sizeof(double);

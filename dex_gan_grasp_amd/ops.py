@@ -178,9 +178,23 @@ _DTYPES = {torch.float32: _lib.F32, torch.bfloat16: _lib.BF16, torch.float16: _l
 _ACTS = {"none": _lib.ACT_NONE, "leaky_relu": _lib.ACT_LEAKY_RELU, "silu": _lib.ACT_SILU}
 
 
+def _stream(dev):
+    """The current HIP stream of a tensor's device as an integer (stream_ptr without the Stream object it makes: 2 us a call)."""
+    return torch._C._cuda_getCurrentRawStream(dev.index)
+
+
 def _on(dev):
     """The context in which kernels for `dev` are launched: launches go to the current device."""
     return torch.cuda.device(dev) if dev.index is not None and dev.index != torch.cuda.current_device() else nullcontext()
+
+
+def _ptr(t):
+    return None if t is None else t.data_ptr()
+
+
+def _like(x):
+    """An uninitialised contiguous tensor of x's shape and type."""
+    return torch.empty_like(x) if x.is_contiguous() else torch.empty(x.shape, dtype=x.dtype, device=x.device)
 
 
 def _rows(t):
@@ -188,6 +202,8 @@ def _rows(t):
     axis of S points.  A tensor whose channels do not lie side by side, or whose points are not evenly spaced, is copied."""
     n, c = t.shape[0], t.shape[-1]
     s = t.numel() // (n * c) if n * c else 0
+    if t.is_contiguous():
+        return t, n, s, c, s * c, c
     mid = [(size, stride) for size, stride in zip(t.shape[1:-1], t.stride()[1:-1]) if size != 1]
     even = all(mid[i][1] == mid[i + 1][0] * mid[i + 1][1] for i in range(len(mid) - 1))
     if (c > 1 and t.stride(-1) != 1) or not even:
@@ -214,7 +230,7 @@ def _group_norm_args(who, x, num_groups, weight, bias, act):
 
 
 def _group_norm_ws(n, s, c, g, dtype, backward, dev):
-    nb = int(lib().dgg_group_norm_workspace_bytes(n, s, c, g, dtype, backward))
+    nb = lib().dgg_group_norm_workspace_bytes(n, s, c, g, dtype, backward)
     if nb < 0:
         check(nb, "dgg_group_norm_workspace_bytes")
     return _lib.new_workspace(nb, dev) if nb else None, nb
@@ -227,17 +243,17 @@ def group_norm_act_forward(x, num_groups, weight=None, bias=None, eps=1e-5, act=
     Returns (y contiguous, of x's shape and type; stats (N, num_groups, 2) float64 = mean and 1 / sqrt(var + eps), which
     group_norm_act_backward takes)."""
     dev, weight, bias = _group_norm_args("group_norm_act_forward", x, num_groups, weight, bias, act)
-    y = torch.empty(x.shape, dtype=x.dtype, device=dev)
-    stats = torch.empty((x.shape[0], num_groups, 2), dtype=torch.float64, device=dev)
+    y = _like(x)
+    stats = x.new_empty((x.shape[0], num_groups, 2), dtype=torch.float64)
     if x.numel() == 0:
         return y, stats.zero_()
     x, n, s, c, sn, ss = _rows(x)
     dt = _DTYPES[x.dtype]
     with _on(dev):
         ws, nb = _group_norm_ws(n, s, c, num_groups, dt, 0, dev)
-        check(lib().dgg_group_norm_act_forward(ptr(x), sn, ss, n, s, c, num_groups, ptr(weight), ptr(bias), float(eps),
-                                               _ACTS[act], float(slope), dt, ptr(y), ptr(stats), ptr(ws), nb,
-                                               stream_ptr(dev)), "dgg_group_norm_act_forward")
+        check(lib().dgg_group_norm_act_forward(x.data_ptr(), sn, ss, n, s, c, num_groups, _ptr(weight), _ptr(bias), eps,
+                                               _ACTS[act], slope, dt, y.data_ptr(), stats.data_ptr(), _ptr(ws), nb,
+                                               _stream(dev)), "dgg_group_norm_act_forward")
     return y, stats
 
 
@@ -252,10 +268,10 @@ def group_norm_act_backward(dy, x, num_groups, weight, bias, eps, act, slope, st
             or not stats.is_contiguous()):
         raise _lib.DggError("group_norm_act_backward: stats must be what the forward of the same x returned")
     c = x.shape[-1]
-    dx = torch.empty(x.shape, dtype=x.dtype, device=dev)
+    dx = _like(x)
     dw = db = None
     if param_grads:
-        dw, db = (torch.empty((c,), dtype=torch.float32, device=dev) for _ in range(2))
+        dw, db = x.new_empty((c,), dtype=torch.float32), x.new_empty((c,), dtype=torch.float32)
     if x.numel() == 0:
         return dx, (dw.zero_() if param_grads else None), (db.zero_() if param_grads else None)
     x, n, s, c, sn, ss = _rows(x)
@@ -263,9 +279,9 @@ def group_norm_act_backward(dy, x, num_groups, weight, bias, eps, act, slope, st
     dt = _DTYPES[x.dtype]
     with _on(dev):
         ws, nb = _group_norm_ws(n, s, c, num_groups, dt, 1, dev)
-        check(lib().dgg_group_norm_act_backward(ptr(dy), dsn, dss, ptr(x), sn, ss, n, s, c, num_groups, ptr(weight),
-                                                ptr(bias), _ACTS[act], float(slope), dt, ptr(stats), ptr(dx), ptr(dw),
-                                                ptr(db), ptr(ws), nb, stream_ptr(dev)), "dgg_group_norm_act_backward")
+        check(lib().dgg_group_norm_act_backward(dy.data_ptr(), dsn, dss, x.data_ptr(), sn, ss, n, s, c, num_groups, _ptr(weight),
+                                                _ptr(bias), _ACTS[act], slope, dt, stats.data_ptr(), dx.data_ptr(), _ptr(dw),
+                                                _ptr(db), _ptr(ws), nb, _stream(dev)), "dgg_group_norm_act_backward")
     return dx, dw, db
 
 
@@ -284,14 +300,17 @@ def _coefficients(who, steps, coefficients):
 
 def _matrix_rows(t):
     """A matrix or a stack (B, rows, cols) whose rows are contiguous, as (tensor, batch, rows, cols, pitch, stride)."""
-    if t.stride(-1) != 1 and t.shape[-1] > 1 or t.shape[-2] > 1 and t.stride(-2) < t.shape[-1]:
-        t = t.contiguous()
-    b, r, c = (1,) * (3 - t.dim()) + tuple(t.shape)
+    *stack, r, c = t.shape
+    b = stack[0] if stack else 1
+    if t.is_contiguous():
+        return t, b, r, c, c, r * c
+    if t.stride(-1) != 1 and c > 1 or r > 1 and t.stride(-2) < c:
+        t = t.detach().contiguous()
     return t, b, r, c, (t.stride(-2) if r > 1 else c), (t.stride(0) if t.dim() == 3 and b > 1 else r * c)
 
 
 def _ns_workspace(mats, n, dev):
-    nb = int(lib().dgg_orthogonalize_workspace_bytes(mats, n))
+    nb = lib().dgg_orthogonalize_workspace_bytes(mats, n)
     if nb < 0:
         check(nb, "dgg_orthogonalize_workspace_bytes")
     return _lib.new_workspace(nb, dev), nb
@@ -310,18 +329,16 @@ def orthogonalize(grad, steps=5, coefficients=NS_COEFFICIENTS, eps=1e-7):
         if t.dtype not in _DTYPES or t.dim() not in (2, 3) or t.dtype != grads[0].dtype or dev != grads[0].device:
             raise _lib.DggError("orthogonalize: matrices (rows, cols) or stacks (B, rows, cols) of one type (float32, bfloat16, "
                                 "float16) on one device; got %s %s on %s" % (t.dtype, tuple(t.shape), dev))
-    outs = [torch.empty(t.shape, dtype=t.dtype, device=t.device) for t in grads]
-    work = [(_matrix_rows(t.detach()), o) for t, o in zip(grads, outs) if t.numel()]
+    outs = [_like(t.detach()) for t in grads]
+    work = [(_matrix_rows(t), o) for t, o in zip(grads, outs) if t.numel()]
     if work:
         dev = grads[0].device
-        mats = (_lib.Matrix * len(work))()
-        for m, ((t, b, r, c, ld, st), o) in zip(mats, work):
-            m.in_, m.out, m.batch, m.rows, m.cols, m.ld_in, m.ld_out = t.data_ptr(), o.data_ptr(), b, r, c, ld, c
-            m.in_stride, m.out_stride = st, r * c
+        mats = (_lib.Matrix * len(work))(*[_lib.Matrix(t.data_ptr(), o.data_ptr(), None, b, st, r * c, 0, r, c, ld, c, 0, 0)
+                                           for (t, b, r, c, ld, st), o in work])
         with _on(dev):
             ws, nb = _ns_workspace(mats, len(work), dev)
-            check(lib().dgg_orthogonalize(mats, len(work), _DTYPES[grads[0].dtype], coef, steps, float(eps), ptr(ws), nb,
-                                          stream_ptr(dev)), "dgg_orthogonalize")
+            check(lib().dgg_orthogonalize(mats, len(work), _DTYPES[grads[0].dtype], coef, steps, eps, ws.data_ptr(), nb,
+                                          _stream(dev)), "dgg_orthogonalize")
     return outs[0] if single else outs
 
 
@@ -337,30 +354,31 @@ def muon_step(params, grads, momentum, lr, mu=0.95, nesterov=True, weight_decay=
     if adjust not in _ADJUST:
         raise _lib.DggError("%s: adjust must be one of %s; got %r" % (who, sorted(_ADJUST), adjust))
     coef = _coefficients(who, steps, coefficients)
-    keep, mats, n = [], (_lib.Matrix * max(len(params), 1))(), 0
+    mats, keep, seen = [], [], set()
+    dev = _dev(params[0]) if params else None
     for w, g, m in zip(params, grads, momentum):
-        dev = _dev(w)
         for t in (w, g, m):
-            if (t.dtype != torch.float32 or t.dim() not in (2, 3) or t.shape != w.shape or t.device != dev
-                    or dev != params[0].device):
+            if t.dtype != torch.float32 or t.dim() not in (2, 3) or t.shape != w.shape or t.device != dev:
                 raise _lib.DggError("%s: float32 matrices of equal shape on one device are needed; got %s %s on %s"
                                     % (who, t.dtype, tuple(t.shape), t.device))
         if not w.numel():
             continue
-        (wt, b, r, c, ldw, sw), (mt, _, _, _, ldm, sm), (gt, _, _, _, ldg, sg) = (_matrix_rows(t.detach()) for t in (w, m, g))
-        if wt.data_ptr() != w.data_ptr() or mt.data_ptr() != m.data_ptr() or (b > 1 and min(sw, sm) < r * c):
+        (wt, b, r, c, ldw, sw), (mt, _, _, _, ldm, sm), (gt, _, _, _, ldg, sg) = _matrix_rows(w), _matrix_rows(m), _matrix_rows(g)
+        at = (w.data_ptr(), m.data_ptr())
+        if wt is not w or mt is not m or (b > 1 and min(sw, sm) < r * c):
             raise _lib.DggError("%s: parameters and momentum are updated in place: their rows must be contiguous and apart" % who)
+        if at[0] == at[1] or at[0] in seen or at[1] in seen:
+            raise _lib.DggError("%s: a tensor is given twice: each is updated in place, once" % who)
+        seen.update(at)
         keep.append(gt)
-        e = mats[n]
-        n += 1
-        e.in_, e.out, e.momentum, e.batch, e.rows, e.cols = gt.data_ptr(), wt.data_ptr(), mt.data_ptr(), b, r, c
-        e.ld_in, e.ld_out, e.ld_momentum, e.in_stride, e.out_stride, e.momentum_stride = ldg, ldw, ldm, sg, sw, sm
-    if n:
-        dev = params[0].device
+        mats.append(_lib.Matrix(gt.data_ptr(), at[0], at[1], b, sg, sw, sm, r, c, ldg, ldw, ldm, 0))
+    if mats:
+        n = len(mats)
+        mats = (_lib.Matrix * n)(*mats)
         with _on(dev):
             ws, nb = _ns_workspace(mats, n, dev)
-            check(lib().dgg_muon_step(mats, n, float(lr), float(mu), int(bool(nesterov)), float(weight_decay), _ADJUST[adjust],
-                                      float(grad_scale), coef, steps, float(eps), ptr(ws), nb, stream_ptr(dev)), "dgg_muon_step")
+            check(lib().dgg_muon_step(mats, n, lr, mu, int(nesterov), weight_decay, _ADJUST[adjust], grad_scale, coef, steps, eps,
+                                      ws.data_ptr(), nb, _stream(dev)), "dgg_muon_step")
 
 
 # ------------------------------------------------------------------------------------------ small ops

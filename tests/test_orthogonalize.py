@@ -282,7 +282,8 @@ def test_refusals():
                  lambda: ops.muon_step([g], [f], [], 0.1), lambda: ops.muon_step([g], [f[:2]], [f], 0.1),
                  lambda: ops.muon_step([g], [f.half()], [f], 0.1), lambda: ops.muon_step([g.t()], [f.t()], [f.t()], 0.1),
                  lambda: ops.muon_step([g], [f], [f], 0.1, adjust="none"),
-                 lambda: ops.muon_step([g[:1].expand(4, 6)], [f], [f], 0.1)):
+                 lambda: ops.muon_step([g[:1].expand(4, 6)], [f], [f], 0.1), lambda: ops.muon_step([g], [f], [g], 0.1),
+                 lambda: ops.muon_step([g, g], [f, f], [torch.zeros_like(g), torch.zeros_like(g)], 0.1)):
         with pytest.raises(_lib.DggError):
             call()
     assert ops.orthogonalize([]) == []
