@@ -21,7 +21,10 @@
 // in a row.  Both sizes are padded to multiples of 64 with zeros, which stay zeros in every product.
 #include <math.h>
 
+#include <algorithm>
+#include <exception>
 #include <type_traits>
+#include <vector>
 
 #include "dgg_internal.h"
 
@@ -969,6 +972,51 @@ int64_t ns_need(const dgg_matrix* mats, int count) {
     return (int64_t)need;
 }
 
+// What one matrix or stack covers in memory (bytes), for the check below.
+struct NsSpan {
+    uintptr_t lo, hi, ld, stride, row;
+    int batch;
+    bool written;
+};
+
+// Two spans share no element: they lie apart, or they are column blocks of one wider buffer.
+bool ns_apart(const NsSpan& a, const NsSpan& b) {
+    if (a.hi <= b.lo || b.hi <= a.lo) return true;
+    if (a.ld != b.ld || (a.batch > 1 && a.stride % a.ld) || (b.batch > 1 && b.stride % b.ld)) return false;
+    const uintptr_t d = a.lo <= b.lo ? (b.lo - a.lo) % a.ld : (a.ld - (a.lo - b.lo) % a.ld) % a.ld;   // b's first column from a's
+    return d >= a.row && d + b.row <= a.ld;
+}
+
+// What a call writes is written once and read by nothing else in it, only an output may be its own matrix' input: launches read an
+// operand more than once and in no order between matrices.
+bool ns_disjoint(const dgg_matrix* mats, int count, size_t size, bool muon) {
+    std::vector<NsSpan> spans;
+    spans.reserve((size_t)count * 3);
+    for (int i = 0; i < count; ++i) {
+        const dgg_matrix& m = mats[i];
+        const auto put = [&](const void* p, int64_t ld, int64_t stride, bool written) {
+            const uintptr_t lo = (uintptr_t)p, row = (uintptr_t)m.cols * size, one = (uintptr_t)(m.rows - 1) * ld * size + row;
+            if (written && m.batch > 1) {   // the matrices of a stack: one behind the other, or side by side
+                const bool behind = (uintptr_t)stride * size >= one;
+                const bool beside = stride >= m.cols && (uintptr_t)(m.batch - 1) * stride * size + row <= (uintptr_t)ld * size;
+                if (!behind && !beside) return false;
+            }
+            spans.push_back({lo, lo + (uintptr_t)(m.batch - 1) * stride * size + one, (uintptr_t)ld * size, (uintptr_t)stride * size,
+                             row, (int)m.batch, written});
+            return true;
+        };
+        const bool same = !muon && m.in == m.out && m.ld_in == m.ld_out && (m.batch == 1 || m.in_stride == m.out_stride);
+        if (!put(m.out, m.ld_out, m.out_stride, true)) return false;
+        if (!same && !put(m.in, m.ld_in, m.in_stride, false)) return false;
+        if (muon && !put(m.momentum, m.ld_momentum, m.momentum_stride, true)) return false;
+    }
+    std::sort(spans.begin(), spans.end(), [](const NsSpan& a, const NsSpan& b) { return a.lo < b.lo; });
+    for (size_t i = 0; i < spans.size(); ++i)
+        for (size_t j = i + 1; j < spans.size() && spans[j].lo < spans[i].hi; ++j)
+            if ((spans[i].written || spans[j].written) && !ns_apart(spans[i], spans[j])) return false;
+    return true;
+}
+
 template <typename T, bool MUON>
 int ns_run(const dgg_matrix* mats, int count, NsArgs& a, const double* coef, int steps, void* ws, size_t ws_bytes,
            hipStream_t st, const char* who) {
@@ -996,6 +1044,17 @@ int ns_run(const dgg_matrix* mats, int count, NsArgs& a, const double* coef, int
     if ((int64_t)ws_bytes < need) {
         set_error_text("%s: the workspace has %zu bytes, %lld are needed", who, ws_bytes, (long long)need);
         return DGG_ERR_WORKSPACE;
+    }
+    bool apart = false;
+    try {
+        apart = ns_disjoint(mats, count, sizeof(T), MUON);
+    } catch (const std::exception& e) {
+        set_error_text("%s: %s", who, e.what());
+        return DGG_ERR_INVALID;
+    }
+    if (!apart) {
+        set_error_text("%s: what is written overlaps itself or another operand", who);
+        return DGG_ERR_INVALID;
     }
     for (int at = 0, n; (n = ns_group(mats, count, true, at, group)) > 0;) {
         NsFirst first;

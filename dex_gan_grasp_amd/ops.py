@@ -346,7 +346,8 @@ def muon_step(params, grads, momentum, lr, mu=0.95, nesterov=True, weight_decay=
               eps=1e-7, adjust="spectral", grad_scale=1.0):
     """One Muon step over lists of float32 matrices (or stacks of them), params and momentum in place:
         M <- mu M + grad_scale G;   U = grad_scale G + mu M (nesterov) or M;   W <- (1 - lr weight_decay) W - lr f orthogonalize(U)
-    with f = sqrt(max(1, rows / cols)) (adjust="spectral") or 0.2 sqrt(max(rows, cols)) ("match_rms")."""
+    with f = sqrt(max(1, rows / cols)) (adjust="spectral") or 0.2 sqrt(max(rows, cols)) ("match_rms").  A gradient may be
+    broadcast; parameters and momenta are written, so none of them may overlap another tensor of the call."""
     who = "muon_step"
     params, grads, momentum = list(params), list(grads), list(momentum)
     if not (len(params) == len(grads) == len(momentum)):
@@ -354,7 +355,7 @@ def muon_step(params, grads, momentum, lr, mu=0.95, nesterov=True, weight_decay=
     if adjust not in _ADJUST:
         raise _lib.DggError("%s: adjust must be one of %s; got %r" % (who, sorted(_ADJUST), adjust))
     coef = _coefficients(who, steps, coefficients)
-    mats, keep, seen = [], [], set()
+    mats, keep = [], []
     dev = _dev(params[0]) if params else None
     for w, g, m in zip(params, grads, momentum):
         for t in (w, g, m):
@@ -364,14 +365,10 @@ def muon_step(params, grads, momentum, lr, mu=0.95, nesterov=True, weight_decay=
         if not w.numel():
             continue
         (wt, b, r, c, ldw, sw), (mt, _, _, _, ldm, sm), (gt, _, _, _, ldg, sg) = _matrix_rows(w), _matrix_rows(m), _matrix_rows(g)
-        at = (w.data_ptr(), m.data_ptr())
-        if wt is not w or mt is not m or (b > 1 and min(sw, sm) < r * c):
+        if wt is not w or mt is not m:
             raise _lib.DggError("%s: parameters and momentum are updated in place: their rows must be contiguous and apart" % who)
-        if at[0] == at[1] or at[0] in seen or at[1] in seen:
-            raise _lib.DggError("%s: a tensor is given twice: each is updated in place, once" % who)
-        seen.update(at)
         keep.append(gt)
-        mats.append(_lib.Matrix(gt.data_ptr(), at[0], at[1], b, sg, sw, sm, r, c, ldg, ldw, ldm, 0))
+        mats.append(_lib.Matrix(gt.data_ptr(), w.data_ptr(), m.data_ptr(), b, sg, sw, sm, r, c, ldg, ldw, ldm, 0))
     if mats:
         n = len(mats)
         mats = (_lib.Matrix * n)(*mats)

@@ -263,14 +263,15 @@ int dgg_adam_l2(float* params, const float* grads, float* m, float* v, int64_t n
  * hidden matrices (everything else stays with Adam).
  * dgg_orthogonalize:  X_0 = in / (|in|_F + eps);  X <- a X + (b A + c A^2) X with A = X X^T (over the shorter side), `steps` times
  *   with the k-th (a, b, c) of `coefficients` (host, steps x 3);  out = X.  in / out of one type (DGG_F32 / BF16 / F16); a matrix
- *   taller than wide is treated as its transpose.  out may be in.
+ *   taller than wide is treated as its transpose.  out may be in, of the same pitch and stride.
  * dgg_muon_step (fp32, in place):  M <- momentum M + grad_scale G;  U = grad_scale G + momentum M (nesterov != 0) or M;
  *   W <- (1 - lr weight_decay) W - lr f X,  X the orthogonalised U and f = sqrt(max(1, rows / cols)) (DGG_MUON_SPECTRAL) or
  *   0.2 sqrt(max(rows, cols)) (DGG_MUON_MATCH_RMS: updates of Adam's size).  G = `in`, W = `out`, M = `momentum`.
  * `mats` (host): any number of entries, each a stack of `batch` matrices of one shape; all of them share the launches (16 entries
  * at a time).  Rows lie ld_* >= cols elements apart, the matrices of a stack *_stride elements.  Products are fp32-accurate
  * (two fp16 planes an operand, fp32 accumulators) for every type.  A NaN or infinity makes its own matrix NaN, no other; a zero
- * matrix stays zero (eps > 0).  The coefficients must keep the iterates bounded for singular values in [0, 1]: DGG_ERR_INVALID
+ * matrix stays zero (eps > 0).  What is written may overlap nothing else that the call reads or writes (column blocks of one
+ * wider buffer are apart): DGG_ERR_INVALID.  The coefficients must keep the iterates bounded for singular values in [0, 1]: DGG_ERR_INVALID
  * otherwise.  Short side <= 16384, long side <= 2^20, a stack <= 2^32 elements.  ws: dgg_orthogonalize_workspace_bytes, 256-byte
  * aligned, one per stream in flight. */
 typedef struct {

@@ -287,3 +287,60 @@ def test_refusals():
         with pytest.raises(_lib.DggError):
             call()
     assert ops.orthogonalize([]) == []
+
+
+def test_overlaps_are_refused_without_a_gpu():
+    """What a call writes may overlap nothing else in it.  (Layouts that share a buffer and are accepted: the test below.)"""
+    lib, C = _lib.lib(), _lib.C
+    coef = (C.c_double * 15)(*(COEF * 5))
+    base = 1 << 20
+
+    def call(*mats, muon=True, dtype=0):
+        arr = (_lib.Matrix * len(mats))()
+        for m, kw in zip(arr, mats):
+            d = dict(in_=base, out=2 * base, momentum=3 * base, batch=1, rows=8, cols=8, ld_in=8, ld_out=8, ld_momentum=8)
+            for k, v in {**d, **kw}.items():
+                setattr(m, k, v)
+        n = lib.dgg_orthogonalize_workspace_bytes(arr, len(mats))
+        if muon:
+            return lib.dgg_muon_step(arr, len(mats), 0.1, 0.9, 1, 0.0, 0, 1.0, coef, 5, 1e-7, 4096, n, None)
+        return lib.dgg_orthogonalize(arr, len(mats), dtype, coef, 5, 1e-7, 4096, n, None)
+
+    other = dict(in_=4 * base, out=5 * base, momentum=6 * base)
+    for bad in ([dict(in_=3 * base)], [dict(in_=2 * base)], [dict(momentum=2 * base)], [dict(momentum=2 * base + 252)],
+                [dict(in_=3 * base - 252)], [{}, {}], [{}, dict(other, out=2 * base + 4)], [{}, dict(other, in_=3 * base)],
+                [dict(batch=2, in_stride=64, out_stride=63, momentum_stride=64)], [dict(batch=2, in_stride=64, out_stride=64)],
+                [dict(batch=2, in_stride=64, out_stride=64, momentum_stride=8)],
+                [dict(ld_out=16), dict(other, out=2 * base + 28, ld_out=16)], [dict(ld_out=16), dict(other, out=2 * base + 32, ld_out=24)],
+                [dict(ld_out=16), dict(other, out=2 * base + 40, ld_out=16)]):
+        assert call(*bad) == -1, bad
+        assert b"overlaps" in lib.dgg_last_error(), bad
+    for bad in ([dict(out=base + 4)], [dict(out=base, ld_out=9)], [{}, {}], [{}, dict(in_=2 * base, out=5 * base)]):
+        assert call(*bad, muon=False) == -1, bad
+        assert b"overlaps" in lib.dgg_last_error(), bad
+
+
+@pytest.mark.gpu
+def test_layouts_that_share_a_buffer():
+    """Parameters that are column blocks of one buffer, stacks whose matrices lie side by side, one gradient for several matrices."""
+    g = torch.stack([matrix(20, 30, s) for s in range(3)]).cuda()
+    want = [torch.ones(20, 30, device="cuda") for _ in range(3)]
+    mom = [torch.zeros(20, 30, device="cuda") for _ in range(3)]
+    for i in range(3):
+        ops.muon_step([want[i]], [g[i]], [mom[i]], 0.1)
+    wide = torch.ones(20, 100, device="cuda")
+    ops.muon_step([wide[:, 30 * i:30 * i + 30] for i in range(3)], list(g), [torch.zeros(20, 30, device="cuda") for _ in range(3)], 0.1)
+    beside, m = torch.ones(20, 3, 30, device="cuda"), torch.zeros(20, 3, 30, device="cuda")
+    ops.muon_step([beside.transpose(0, 1)], [g], [m.transpose(0, 1)], 0.1)
+    for i in range(3):
+        assert torch.equal(wide[:, 30 * i:30 * i + 30], want[i]) and torch.equal(beside[:, i], want[i]) and torch.equal(m[:, i], mom[i])
+    assert bool((wide[:, 90:] == 1).all())
+    two = torch.ones(2, 20, 30, device="cuda")
+    ops.muon_step([two], [g[:1].expand(2, 20, 30)], [torch.zeros_like(two)], 0.1)
+    assert torch.equal(two[0], want[0]) and torch.equal(two[1], want[0])
+    w, m = torch.ones(20, 30, device="cuda"), torch.zeros(20, 30, device="cuda")
+    for call in (lambda: ops.muon_step([w], [m], [m], 0.1), lambda: ops.muon_step([w], [w], [m], 0.1),
+                 lambda: ops.muon_step([w, w[:10]], [g[0], g[0][:10]], [m, torch.zeros(10, 30, device="cuda")], 0.1)):
+        with pytest.raises(_lib.DggError):
+            call()
+    assert bool((w == 1).all()) and not m.any()
