@@ -341,3 +341,29 @@ class FlatNet:
         self.step += 1      # (the setter keeps the device-resident counter of the graph path in step)
         check(lib().dgg_adam_l2(ptr(self.params), ptr(self.grads), ptr(self.m), ptr(self.v), self.n_params, self.step,
                                 lr, beta1, beta2, eps, weight_decay, grad_scale, stream_ptr(self.device)), "dgg_adam_l2")
+
+    def muon_split(self):
+        """What Muon updates and what stays with Adam: (names of the hidden matrices — every ResBlock's fc1, fc2 and fc3 —,
+        [(lo, hi)] float ranges of everything else: biases, BatchNorm, heads)."""
+        hidden = [e for e in self.entries if e[4] == 0 and e[0].endswith((".fc1.weight", ".fc2.weight", ".fc3.weight"))]
+        rest, at = [], 0
+        for _, off, rows, cols, _ in sorted(hidden, key=lambda e: e[1]):
+            if off > at:
+                rest.append((at, off))
+            at = off + rows * cols
+        if at < self.n_params:
+            rest.append((at, self.n_params))
+        return [e[0] for e in hidden], rest
+
+    def muon_step(self, lr, beta1=0.9, beta2=0.999, eps=1e-8, weight_decay=5e-4, grad_scale=1.0, momentum=0.95, steps=5):
+        """An optimiser step with Muon for the hidden matrices (ops.muon_step: all of them in the same launches, `m` their
+        momentum, updates of Adam's size, weight decay decoupled) and Adam for the rest (dgg_adam_l2 on its ranges; the
+        other arguments are adam_step's)."""
+        from . import ops
+        names, rest = self.muon_split()
+        p, g, m = self.views("params"), self.views("grads"), self.views("m")
+        ops.muon_step([p[n] for n in names], [g[n] for n in names], [m[n] for n in names], lr, mu=momentum,
+                      weight_decay=weight_decay, steps=steps, adjust="match_rms", grad_scale=grad_scale)
+        self.adam_begin()
+        for lo, hi in rest:
+            self.adam_range(lo, hi, lr, beta1, beta2, eps, weight_decay, grad_scale)

@@ -56,12 +56,23 @@ class GraphStep:
         return self.loss_view
 
 
+def optimizer_of(cfg):
+    """cfg["optimizer"] (default "adam"), checked."""
+    kind = cfg.get("optimizer", "adam")
+    if kind not in ("adam", "muon"):
+        raise _lib.DggError('cfg["optimizer"] must be "adam" or "muon"; got %r' % (kind,))
+    return kind
+
+
 class TrainEngine:
     def __init__(self, cfg, flat_g, flat_d, flat_e, device):
         self.cfg = cfg
         self.G, self.D, self.E = flat_g, flat_d, flat_e
         self.device = torch.device(device)
         self.ccfg = _lib.make_cfg(cfg)
+        # cfg["optimizer"]: "adam" (the reference's) or "muon" — the hidden matrices by Muon (cfg["muon_momentum"],
+        # cfg["muon_steps"]), everything else by Adam, FlatNet.muon_step
+        self.muon = optimizer_of(cfg) == "muon"
         # The loss vector of a step (16 floats, slots _lib.L_*) is written by the kernels of that step into ONE slot of a
         # ring; every step takes the next slot and returns a VIEW of it — no copy kernel on the step's stream (until round 5:
         # `losses.clone()` per call, a launch + its gap on the chain; the reference only reads the values every print_freq
@@ -102,6 +113,14 @@ class TrainEngine:
         if lr_eva is not None:
             hp.lr_eva = lr_eva
         return hp
+
+    def _update(self, net, lr, hp):
+        """One optimiser step of a network on the current stream."""
+        kw = (lr, hp.beta1, hp.beta2, hp.eps, hp.weight_decay, hp.grad_scale)
+        if self.muon:
+            net.muon_step(*kw, momentum=float(self.cfg.get("muon_momentum", 0.95)), steps=int(self.cfg.get("muon_steps", 5)))
+        else:
+            net.adam_step(*kw)
 
     def _cgan_ws(self, B):
         ws = self._ws.get(B)
@@ -241,14 +260,14 @@ class TrainEngine:
         if getattr(self, "after_d_phase", None) is not None:   # tests: the fake pass' LeakyReLU sides (kink_sides)
             self.after_d_phase(self, B)
         self._reduce("D")
-        self.D.adam_step(hp.lr_dis, hp.beta1, hp.beta2, hp.eps, hp.weight_decay, hp.grad_scale)
+        self._update(self.D, hp.lr_dis, hp)
         self._mark("adam_d_end")
         if is_train_gen:
             check(lib().dgg_cgan_g_phase(cfg_p, C.byref(st), C.byref(hp), ptr(ws), ws.numel(), B, *args,
                                          ptr(L), stream_ptr(dev)), "dgg_cgan_g_phase")
             self._mark("g_phase_end")
             self._reduce("G")
-            self.G.adam_step(hp.lr_gen, hp.beta1, hp.beta2, hp.eps, hp.weight_decay, hp.grad_scale)
+            self._update(self.G, hp.lr_gen, hp)
             self._mark("adam_g_end")
         return L
 
@@ -283,12 +302,12 @@ class TrainEngine:
         check(lib().dgg_wgan_d_phase(cfg_p, C.byref(st), C.byref(hp), ptr(ws), ws.numel(), B, *args, ptr(alphas),
                                      float(penalty_gain), ptr(L), stream_ptr(dev)), "dgg_wgan_d_phase")
         parallel.allreduce_sum_(self.D.grads)
-        self.D.adam_step(hp.lr_dis, hp.beta1, hp.beta2, hp.eps, hp.weight_decay, hp.grad_scale)
+        self._update(self.D, hp.lr_dis, hp)
         if is_train_gen:
             check(lib().dgg_wgan_g_phase(cfg_p, C.byref(st), C.byref(hp), ptr(ws), ws.numel(), B, *args,
                                          ptr(L), stream_ptr(dev)), "dgg_wgan_g_phase")
             parallel.allreduce_sum_(self.G.grads)
-            self.G.adam_step(hp.lr_gen, hp.beta1, hp.beta2, hp.eps, hp.weight_decay, hp.grad_scale)
+            self._update(self.G, hp.lr_gen, hp)
         return L
 
     # ---- A11
@@ -309,7 +328,7 @@ class TrainEngine:
                                   ws.numel(), B, ptr(bps), ptr(rot9), ptr(transl), ptr(label), ptr(dk), int(seed),
                                   ptr(L), stream_ptr(dev)), "dgg_eva_phase")
         self._reduce("E")
-        E.adam_step(hp.lr_eva, hp.beta1, hp.beta2, hp.eps, hp.weight_decay, hp.grad_scale)
+        self._update(E, hp.lr_eva, hp)
         return L
 
     def eva_keep_masks(self, B):
@@ -395,6 +414,8 @@ class TrainEngine:
         are not captured.  Returns a GraphStep."""
         if parallel.is_distributed():
             raise _lib.DggError("capture_joint_step: data-parallel steps are not captured (RCCL work is enqueued eagerly)")
+        if self.muon:
+            raise _lib.DggError('capture_joint_step: only with cfg["optimizer"] = "adam" (its step number lives on the device)')
         dev = self.device
         keep = (tuple(gan_inputs), z, tuple(eva_inputs))
         for t in keep[0] + (z,) + keep[2]:
@@ -462,7 +483,7 @@ class TrainEngine:
             adam = lambda net, lr: net.adam_step_graph(lr, hp.beta1, hp.beta2, hp.eps, hp.weight_decay, hp.grad_scale)
             next_gan_inputs = None
         else:
-            adam = lambda net, lr: net.adam_step(lr, hp.beta1, hp.beta2, hp.eps, hp.weight_decay, hp.grad_scale)
+            adam = lambda net, lr: self._update(net, lr, hp)
         wg = os.environ.get("DGG_JOINT_WGRAD_STREAMS", "0") == "1" and not graph_mode
         main, s2 = self._streams(two_streams, wgrad=wg)
         if two_streams:
@@ -478,7 +499,7 @@ class TrainEngine:
         # backward.  It paid while the chain was longer (rounds 2-5: -10..-20 us per step); with the chain of round 6 its two
         # cross-stream waits cost more than the overlap gives (1.350 / 1.344 against 1.339 / 1.335 ms, one box, alternating)
         split = (two_streams and not graph_mode and os.environ.get("DGG_SPLIT_ADAM", "0") == "1"
-                 and not parallel.is_distributed())
+                 and not parallel.is_distributed() and not self.muon)
         self._arm_reducers(force=split)
         self._mark("step_begin")
         # this step's loss vector: the next ring slot (a look-ahead real pass enqueued by the previous step has already

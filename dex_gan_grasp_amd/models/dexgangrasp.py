@@ -14,7 +14,7 @@ import numpy as np
 import torch
 
 from .. import _lib, ops, parallel
-from ..engine import TrainEngine
+from ..engine import TrainEngine, optimizer_of
 from ..utils import utils
 from ..utils.train_tools import EarlyStopping
 from . import losses, networks
@@ -106,6 +106,7 @@ class DexGanGrasp(object):
         self._sync_replicas()   # every rank draws its own init (dexgangrasp.py:39-62): rank 0's wins
 
         if self.is_train:
+            optimizer_of(cfg)   # (an unknown one is refused here, not at the first step)
             self.bce_weight = cfg["bce_weight"]
             self.kl_coef = cfg["kl_coef"]
             self.transl_coef = 100.
@@ -194,6 +195,10 @@ class DexGanGrasp(object):
     def _export_adam(self, optim, module, flat):
         """Expose the fused Adam moments as a torch optimizer state (checkpoint format of
         dexgangrasp.py:662-712): state[p] = {step, exp_avg, exp_avg_sq}."""
+        for group in optim.param_groups:   # whose state it is (_import_adam); the reference's files do not have the key
+            group.pop("optimizer", None)
+            if optimizer_of(self.cfg) == "muon":
+                group["optimizer"] = "muon"
         if flat is None or flat.step == 0:
             return
         mv, vv = flat.views("m"), flat.views("v")
@@ -201,12 +206,21 @@ class DexGanGrasp(object):
             optim.state[p] = {"step": torch.tensor(float(flat.step)), "exp_avg": mv[name], "exp_avg_sq": vv[name]}
 
     def _import_adam(self, optim, module, flat):
-        """After optim.load_state_dict: copy loaded moments into the flat buffers the kernel uses."""
+        """After optim.load_state_dict: copy loaded moments into the flat buffers the kernel uses.  Muon's momentum of a hidden
+        matrix and Adam's moments are no state for each other: those of a checkpoint that the other optimiser wrote stay
+        behind, and the hidden matrices start anew (Adam: the whole network, whose step number is one)."""
         mv, vv = flat.views("m"), flat.views("v")
+        muon = optimizer_of(self.cfg) == "muon"
+        wrote_muon = optim.param_groups[0].get("optimizer") == "muon"
+        skip = () if muon == wrote_muon else flat.muon_split()[0] if muon else mv
         step = 0
         for name, p in module.named_parameters():
             st = optim.state.get(p)
-            if st:
+            if name in skip:
+                mv[name].zero_()
+                vv[name].zero_()
+                optim.state.pop(p, None)
+            elif st:
                 mv[name].copy_(st["exp_avg"].to(mv[name].device))
                 vv[name].copy_(st["exp_avg_sq"].to(vv[name].device))
                 step = max(step, int(float(st["step"])))

@@ -146,6 +146,53 @@ class ResBlock(nn.Module):
         return y
 
 
+class _GroupNormActFn(torch.autograd.Function):
+    """ops.group_norm_act_forward / _backward under autograd; keeps x and the statistics."""
+
+    @staticmethod
+    def forward(ctx, x, weight, bias, groups, eps, act, slope):
+        y, stats = ops.group_norm_act_forward(x, groups, weight, bias, eps, act, slope)
+        ctx.save_for_backward(x, weight, bias, stats)
+        ctx.args = (groups, eps, act, slope)
+        return y
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dy):
+        x, weight, bias, stats = ctx.saved_tensors
+        groups, eps, act, slope = ctx.args
+        want = ctx.needs_input_grad
+        dx, dw, db = ops.group_norm_act_backward(dy, x, groups, weight, bias, eps, act, slope, stats,
+                                                 param_grads=want[1] or want[2])
+        return dx if want[0] else None, dw if want[1] else None, db if want[2] else None, None, None, None, None
+
+
+class GroupNormAct(nn.Module):
+    """Group norm and activation in one kernel, channels last: x (N, .., C) -> act(group_norm(x)) with statistics over a sample's
+    points and a group's channels.  Stands where BatchNorm + LeakyReLU stands in a ResBlock (networks.py:29-41) when a sample
+    must not see its batch — a per-sample gradient penalty, batches of one, data-parallel shards of any size — and on
+    per-point features (N, points, C).  float32, bfloat16 or float16 in and out; weight and bias are float32.  Once
+    differentiable.  act: "leaky_relu" (`slope`), "silu" or "none"."""
+
+    def __init__(self, num_groups, num_channels, eps=1e-5, act="leaky_relu", slope=0.2, affine=True, device=None):
+        super().__init__()
+        if num_groups < 1 or num_channels < 1 or num_channels % num_groups:
+            raise _lib.DggError("GroupNormAct: %d groups do not divide %d channels" % (num_groups, num_channels))
+        self.num_groups, self.num_channels, self.eps, self.act, self.slope = num_groups, num_channels, eps, act, slope
+        self.weight = nn.Parameter(torch.ones(num_channels, device=device)) if affine else None
+        self.bias = nn.Parameter(torch.zeros(num_channels, device=device)) if affine else None
+
+    def forward(self, x):
+        if not x.is_cuda:
+            raise _lib.DggError("GroupNormAct.forward: GPU tensor required (this implementation has no CPU path)")
+        if x.dim() < 2 or x.shape[-1] != self.num_channels:
+            raise _lib.DggError("GroupNormAct: x must be (N, .., %d); got %s" % (self.num_channels, tuple(x.shape)))
+        return _GroupNormActFn.apply(x, self.weight, self.bias, self.num_groups, self.eps, self.act, self.slope)
+
+    def extra_repr(self):
+        return "%d, %d, eps=%g, act=%s" % (self.num_groups, self.num_channels, self.eps, self.act)
+
+
 def _pin_bn_counters(module):
     """BatchNorm's `num_batches_tracked` buffers stay HOST tensors whatever device the module moves to.  Nothing on the
     device reads them (momentum is 0.1: the reference only increments them, networks.py / nn.BatchNorm1d), and the train
