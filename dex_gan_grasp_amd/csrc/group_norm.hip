@@ -12,14 +12,18 @@
 // would take the wrong side for every element within its rounding error of zero.  (64-bit vector instructions run at the
 // rate of the fp32 ones here; per element they are 4 to 6 of them.)  What follows the sign is fp32, rounded once to the output type.
 //
-// Two routes, chosen by gn_run:
-//  * "unit": a group's S x D elements fit the registers of at most one wave.  L = 2^k lanes own one (n, g): one read of x,
-//    mean and centred variance by lane shuffles, no LDS, no barrier.
+// Three routes, chosen by gn_run:
+//  * "unit": a group's S x D elements fit the registers of at most one wave (backward: rows, S = 1).  L = 2^k lanes own one (n, g):
+//    one read of x, mean and centred variance by lane shuffles, no LDS, no barrier.  1024 x 512 f32 in 32 groups: 4.3 us forward,
+//    9.7 backward with dw and db (launches); 16384 x 512: 24 and 29 us (2.9 and 3.4 TB/s).
+//  * "resident": a sample's points in a block of groups fit a workgroup's registers: one read, one launch.  128 x 2048 x 256 bf16
+//    in 32 groups: 71 us forward (3.8 TB/s), 140 backward (2.9 TB/s: the arithmetic and the memory take turns, one workgroup a CU).
 //  * "tile": a workgroup owns a range of the rows of one sample and a block of channels (a thread keeps ITS channels while
 //    it walks down the rows), leaves per-channel partial sums in the workspace, and a small launch merges them in a fixed
 //    order into the groups' statistics (and dw, db); a last launch applies them.  No atomics: results do not depend on the
 //    order in which workgroups run.
 #include <initializer_list>
+#include <type_traits>
 
 #include "dgg_internal.h"
 
@@ -27,6 +31,7 @@ namespace dgg {
 namespace {
 
 constexpr int kGnThreads = 256;
+constexpr int kMergeThreads = 1024;
 constexpr int kUnitItems = 8;   // vectors of a group one lane holds, at most
 
 template <typename T, int V> struct alignas(sizeof(T) * V) Vec { T e[V]; };
@@ -86,6 +91,7 @@ struct GnArgs {
     double* part;           // tile: [N][chunks][C][2]; unit backward: float [rows of partials][C][2]
     double* chan;           // tile backward: [N][C][2], part summed over the chunks (part itself where there is one)
     double* coef;           // tile backward: [N][G][2]: mean(w dz), mean(w dz xh)
+    double* ranges;         // [ranges][C][2]: gn_param_grad
     float* dw;
     float* db;
     long long x_sn, x_ss, dy_sn, dy_ss;   // strides in elements; the channel stride is 1
@@ -166,21 +172,21 @@ __global__ __launch_bounds__(kGnThreads) void gn_unit_bwd_kernel(GnArgs a) {
     const int per = a.G < slots ? slots / a.G : 1;             // samples side by side in a workgroup
     const int g = a.G < slots ? slot % a.G : (int)(blockIdx.x % a.blocks_g) * slots + slot;
     const int side = a.G < slots ? slot / a.G : 0;
-    if (side >= per || g >= a.G) return;
+    const bool on = side < per && g < a.G;
     const int nb = (int)(blockIdx.x / a.blocks_g);
     const int nv = a.D / V;
     float w[I][V], b[I][V];
     double dw[I][V], db[I][V];
 #pragma unroll
     for (int i = 0; i < I; ++i) {
-        const long long c = (long long)g * a.D + min(lane + i * L, nv - 1) * V;
+        const long long c = (long long)min(g, a.G - 1) * a.D + min(lane + i * L, nv - 1) * V;
         load_param<V>(a.w, c, 1.f, w[i]);
         load_param<V>(a.b, c, 0.f, b[i]);
 #pragma unroll
         for (int k = 0; k < V; ++k) dw[i][k] = db[i][k] = 0.0;
     }
     const double inv = 1.0 / ((double)nv * V);
-    for (long long n = (long long)nb * per + side; n < a.N; n += (long long)a.blocks_n * per) {
+    for (long long n = on ? (long long)nb * per + side : a.N; n < a.N; n += (long long)a.blocks_n * per) {
         const T* x = (const T*)a.x + n * a.x_sn + (long long)g * a.D;
         const T* dy = (const T*)a.dy + n * a.dy_sn + (long long)g * a.D;
         const double mean = a.stats[2 * (n * a.G + g)], rstd = a.stats[2 * (n * a.G + g) + 1];
@@ -220,11 +226,29 @@ __global__ __launch_bounds__(kGnThreads) void gn_unit_bwd_kernel(GnArgs a) {
         }
     }
     if (!a.part) return;
-    float* p = (float*)a.part + 2ll * a.C * ((long long)nb * per + side);
+    // the samples side by side are added up here: 1024 x 2048 f32 in one group left 17 MB of partial sums for 25 MB of data
+    __shared__ double sh[kGnThreads * V * 2];
+    float* p = (float*)a.part + 2ll * a.C * nb;
 #pragma unroll
     for (int i = 0; i < I; ++i) {
+        if (per > 1) {
+            __syncthreads();
+#pragma unroll
+            for (int k = 0; k < V; ++k) {
+                sh[(k * 2) * kGnThreads + threadIdx.x] = dw[i][k];
+                sh[(k * 2 + 1) * kGnThreads + threadIdx.x] = db[i][k];
+            }
+            __syncthreads();
+            if (side == 0)
+                for (int y = 1; y < per; ++y)
+#pragma unroll
+                    for (int k = 0; k < V; ++k) {
+                        dw[i][k] += sh[(k * 2) * kGnThreads + threadIdx.x + y * a.G * L];
+                        db[i][k] += sh[(k * 2 + 1) * kGnThreads + threadIdx.x + y * a.G * L];
+                    }
+        }
         const int e = lane + i * L;
-        if (e < nv)
+        if (on && side == 0 && e < nv)
 #pragma unroll
             for (int k = 0; k < V; ++k) {
                 p[2 * (g * a.D + e * V + k)] = (float)dw[i][k];
@@ -317,41 +341,67 @@ __global__ __launch_bounds__(kGnThreads) void gn_tile_sum_kernel(GnArgs a) {
 }
 
 // sum of v over the workgroup, in a fixed order, for every thread
-__device__ __forceinline__ double block_sum(double v, double* sh /* kGnThreads / 64 */) {
+__device__ __forceinline__ double block_sum(double v, double* sh /* blockDim.x / 64 */) {
     v = lane_sum(v, 64);
     __syncthreads();
     if ((threadIdx.x & 63) == 0) sh[threadIdx.x >> 6] = v;
     __syncthreads();
     double s = 0.0;
-#pragma unroll
-    for (int i = 0; i < kGnThreads / 64; ++i) s += sh[i];
+    for (int i = 0; i < (int)blockDim.x / 64; ++i) s += sh[i];
     return s;
+}
+
+// The sums part[..][C][2] of one (n, g) over the row ranges, channel by channel: `use(c, p, q)` runs for each channel once, in one
+// thread (T walkers a channel, added up in order).
+template <typename Use> __device__ __forceinline__ void over_chunks(const GnArgs& a, const double* part, double* col /* 2 blockDim.x */, Use use) {
+    const int wide = min(a.D, (int)blockDim.x), T = (int)blockDim.x / wide, w = (int)threadIdx.x / wide, c0 = (int)threadIdx.x - w * wide;
+    for (int base = 0; base < a.D; base += wide) {
+        const int c = base + c0;
+        const bool on = w < T && c < a.D;
+        double p = 0.0, q = 0.0;
+        if (on) {
+            const double* o = part + 2ll * c;
+#pragma unroll 4
+            for (int ch = w; ch < a.chunks; ch += T) {
+                p += o[2ll * ch * a.C];
+                q += o[2ll * ch * a.C + 1];
+            }
+        }
+        __syncthreads();
+        col[2 * threadIdx.x] = p;
+        col[2 * threadIdx.x + 1] = q;
+        __syncthreads();
+        if (on && w == 0) {
+            for (int t = 1; t < T; ++t) {
+                p += col[2 * (t * wide + c0)];
+                q += col[2 * (t * wide + c0) + 1];
+            }
+            use(c, p, q);
+        }
+    }
 }
 
 // One workgroup per (n, g) merges the shifted sums of its channels and row ranges: with d = x - k_c,
 //   mean = (sum_c k_c + sum d / S) / D,   sum (x - mean)^2 = sum d^2 + 2 (k_c - mean) sum d + S sum_c (k_c - mean)^2
+// (a channel's sums over the ranges take the place of its first range's between the two)
 template <typename T>
-__global__ __launch_bounds__(kGnThreads) void gn_stats_kernel(GnArgs a) {
-    __shared__ double sh[kGnThreads / 64];
+__global__ __launch_bounds__(kMergeThreads) void gn_stats_kernel(GnArgs a) {
+    __shared__ double sh[kMergeThreads / 64], col[kMergeThreads * 2];
     const unsigned n = blockIdx.x / (unsigned)a.G, g = blockIdx.x - n * (unsigned)a.G;
     const T* x0 = (const T*)a.x + (long long)n * a.x_sn + (long long)g * a.D;
-    const double* part = a.part + 2ll * ((long long)n * a.chunks * a.C + (long long)g * a.D);
-    const long long items = (long long)a.D * a.chunks;
+    double* part = a.part + 2ll * ((long long)n * a.chunks * a.C + (long long)g * a.D);
     const double rs = 1.0 / (double)a.S;
     double sum = 0.0;
-    for (long long e = threadIdx.x; e < items; e += kGnThreads) {
-        const unsigned ch = (unsigned)(e / a.D), c = (unsigned)(e - (long long)ch * a.D);
-        sum += part[2ll * ((long long)ch * a.C + c)] * rs;
-        if (ch == 0) sum += (double)(float)x0[c];
-    }
+    over_chunks(a, part, col, [&](int c, double p, double q) {
+        sum += fma(p, rs, (double)(float)x0[c]);
+        part[2ll * c] = p;
+        part[2ll * c + 1] = q;
+    });
     const double mean = block_sum(sum, sh) / (double)a.D;
     double m2 = 0.0;
-    for (long long e = threadIdx.x; e < items; e += kGnThreads) {
-        const unsigned ch = (unsigned)(e / a.D), c = (unsigned)(e - (long long)ch * a.D);
-        const double* o = part + 2ll * ((long long)ch * a.C + c);
+    for (int c = threadIdx.x; c < a.D; c += blockDim.x) {   // (written by this very thread: the first walker's channels)
         const double k = (double)(float)x0[c] - mean;
-        m2 += fma(2.0 * k, o[0], o[1]) * rs;
-        if (ch == 0) m2 = fma(k, k, m2);
+        m2 = fma(k, k, fma(fma(2.0 * k, part[2ll * c], part[2ll * c + 1]), rs, m2));
     }
     const double var = block_sum(m2, sh) / (double)a.D;
     if (threadIdx.x == 0) {
@@ -447,43 +497,21 @@ __global__ __launch_bounds__(kGnThreads) void gn_tile_bwd_sum_kernel(GnArgs a) {
         }
 }
 
-// One workgroup per (n, g): the group's two means, and its channels' sums over the chunks on the way (T walkers a channel, in order)
-__global__ __launch_bounds__(kGnThreads) void gn_bwd_coef_kernel(GnArgs a) {
-    __shared__ double sh[kGnThreads / 64], col[kGnThreads * 2];
+// One workgroup per (n, g): the group's two means, and its channels' sums over the chunks on the way
+__global__ __launch_bounds__(kMergeThreads) void gn_bwd_coef_kernel(GnArgs a) {
+    __shared__ double sh[kMergeThreads / 64], col[kMergeThreads * 2];
     const unsigned n = blockIdx.x / (unsigned)a.G, g = blockIdx.x - n * (unsigned)a.G;
-    const int wide = a.D < kGnThreads ? a.D : kGnThreads, T = kGnThreads / wide, w = (int)threadIdx.x / wide, c0 = (int)threadIdx.x - w * wide;
     double s1 = 0.0, s2 = 0.0;
-    for (int base = 0; base < a.D; base += wide) {
-        const int c = base + c0;
-        const bool on = w < T && c < a.D;
-        double p = 0.0, q = 0.0;
-        if (on) {
-            const double* o = a.part + 2ll * ((long long)n * a.chunks * a.C + (long long)g * a.D + c);
-#pragma unroll 4
-            for (int ch = w; ch < a.chunks; ch += T) {
-                p += o[2ll * ch * a.C];
-                q += o[2ll * ch * a.C + 1];
-            }
+    over_chunks(a, a.part + 2ll * ((long long)n * a.chunks * a.C + (long long)g * a.D), col, [&](int c, double p, double q) {
+        const long long at = 2ll * ((long long)n * a.C + (long long)g * a.D + c);
+        if (a.chan != a.part) {
+            a.chan[at] = p;
+            a.chan[at + 1] = q;
         }
-        __syncthreads();
-        col[2 * threadIdx.x] = p;
-        col[2 * threadIdx.x + 1] = q;
-        __syncthreads();
-        if (on && w == 0) {
-            for (int t = 1; t < T; ++t) {
-                p += col[2 * (t * wide + c0)];
-                q += col[2 * (t * wide + c0) + 1];
-            }
-            const long long at = 2ll * ((long long)n * a.C + (long long)g * a.D + c);
-            if (a.chan != a.part) {
-                a.chan[at] = p;
-                a.chan[at + 1] = q;
-            }
-            const double wt = a.w ? (double)a.w[(long long)g * a.D + c] : 1.0;
-            s1 = fma(wt, q, s1);
-            s2 = fma(wt, p, s2);
-        }
-    }
+        const double wt = a.w ? (double)a.w[(long long)g * a.D + c] : 1.0;
+        s1 = fma(wt, q, s1);
+        s2 = fma(wt, p, s2);
+    });
     const double inv = 1.0 / ((double)a.S * a.D);
     s1 = block_sum(s1, sh) * inv;
     s2 = block_sum(s2, sh) * inv;
@@ -560,13 +588,17 @@ struct Res {
 
 // A vector of V elements as it lies in memory.  keep(): what has been made of it is forgotten — the compiler would rather hold the
 // unpacked fp32 values from one use to the next than unpack again, and spill them.
+template <int N> struct RawBits { typedef uint32_t Type __attribute__((ext_vector_type(N / 4))); };
+template <> struct RawBits<4> { typedef uint32_t Type; };
+template <> struct RawBits<2> { typedef uint16_t Type; };
 template <typename T, int V> struct Raw {
-    typedef uint32_t Bits __attribute__((ext_vector_type(V * sizeof(T) / 4)));
-    Bits bits;
+    typedef typename RawBits<V * sizeof(T)>::Type Bits;
+    typename std::conditional<sizeof(Bits) == 2, uint32_t, Bits>::type bits;
     __device__ __forceinline__ void load(const T* p) { bits = *reinterpret_cast<const Bits*>(p); }
     __device__ __forceinline__ void keep() { asm("" : "+v"(bits)); }
+    __device__ __forceinline__ float at(int k) const { return (float)__builtin_bit_cast(Vec<T, V>, (Bits)bits).e[k]; }
     __device__ __forceinline__ void get(float (&v)[V]) const {
-        const Vec<T, V> r = __builtin_bit_cast(Vec<T, V>, bits);
+        const Vec<T, V> r = __builtin_bit_cast(Vec<T, V>, (Bits)bits);
 #pragma unroll
         for (int k = 0; k < V; ++k) v[k] = (float)r.e[k];
     }
@@ -664,12 +696,12 @@ __global__ __launch_bounds__(kResThreads) void gn_res_bwd_kernel(GnArgs a) {
     const int c0 = ((int)t.blk * a.res_groups * t.per + t.x) * V, S = (int)a.S, g = t.x / t.per;
     const T* x = (const T*)a.x + (long long)t.n * a.x_sn + c0;
     const T* dy = (const T*)a.dy + (long long)t.n * a.dy_sn + c0;
-    Raw<T, V> rx[R], rd[R];
+    Raw<T, V> rx[R];
+    float dz[R][V];   // (kept: its activation's slope is most of the arithmetic, 128 x 2048 x 256 bf16 was bound by having it twice)
     float w[V], b[V];
-    double p[V], q[V], mean = 0.0, rstd = 0.0;
-#pragma unroll
-    for (int k = 0; k < V; ++k) p[k] = q[k] = 0.0;
+    double mean = 0.0, rstd = 0.0;
     if (t.on) {
+        Raw<T, V> rd[R];
 #pragma unroll
         for (int r = 0; r < R; ++r) {
             const long long row = min(t.ty + r * t.rows, S - 1);
@@ -682,29 +714,26 @@ __global__ __launch_bounds__(kResThreads) void gn_res_bwd_kernel(GnArgs a) {
         mean = st[0];
         rstd = st[1];
 #pragma unroll
-        for (int r = 0; r < R; ++r)
-            if (t.ty + r * t.rows < S) {
-                float v[V], d[V];
-                rx[r].get(v);
-                rd[r].get(d);
+        for (int k = 0; k < V; ++k) {   // one channel's sums at a time
+            const double sc = rstd * (double)w[k];
+            double p = 0.0, q = 0.0;
 #pragma unroll
-                for (int k = 0; k < V; ++k) {
-                    const double xh = ((double)v[k] - mean) * rstd;
-                    const double dz = (double)(d[k] * act_slope(fma(xh, (double)w[k], (double)b[k]), ACT, a.slope));
-                    p[k] = fma(dz, xh, p[k]);
-                    q[k] += dz;
+            for (int r = 0; r < R; ++r) {
+                const double d = (double)rx[r].at(k) - mean;
+                const float z = rd[r].at(k) * act_slope(fma(d, sc, (double)b[k]), ACT, a.slope);
+                dz[r][k] = z;
+                if (t.ty + r * t.rows < S) {
+                    p = fma((double)z, d, p);
+                    q += (double)z;
                 }
             }
+            sh[((int)threadIdx.x * V + k) * 2] = (float)(p * rstd);
+            sh[((int)threadIdx.x * V + k) * 2 + 1] = (float)q;
+        }
     }
     // The columns' sums over the rows — a column: one of the two sums of one channel —, fp32 from each thread, added in 64 bits: `parts`
     // threads a column, then a wave a group, which also has the group's two means from them.
     const int cols = t.tx * V * 2, parts = cols < (int)blockDim.x ? (int)blockDim.x / cols : 1;
-    if (t.on)
-#pragma unroll
-        for (int k = 0; k < V; ++k) {
-            sh[((int)threadIdx.x * V + k) * 2] = (float)p[k];
-            sh[((int)threadIdx.x * V + k) * 2 + 1] = (float)q[k];
-        }
     __syncthreads();
     const int part = parts > 1 ? (int)threadIdx.x / cols : 0;
     double sum = 0.0;
@@ -748,36 +777,35 @@ __global__ __launch_bounds__(kResThreads) void gn_res_bwd_kernel(GnArgs a) {
     if (!t.on) return;
     const double s1 = sums[2 * g], s2 = sums[2 * g + 1];
     const double inv = 1.0 / ((double)S * a.D);
-    const float f1 = (float)(s1 * inv), f2 = (float)(s2 * inv), fr = (float)rstd;
+    // dx = (rstd w) dz + ((x - mean) c2 + c1)
+    const double c1 = -rstd * (s1 * inv), c2 = -rstd * rstd * (s2 * inv);
     T* o = (T*)a.out + (long long)t.n * S * a.C + c0;
+#pragma unroll
+    for (int k = 0; k < V; ++k) w[k] = (float)(rstd * (double)w[k]);
 #pragma unroll
     for (int r = 0; r < R; ++r) {
         const int row = t.ty + r * t.rows;
         if (row >= S) break;
-        float v[V], d[V];
+        float v[V];
         rx[r].keep();
-        rd[r].keep();
         rx[r].get(v);
-        rd[r].get(d);
 #pragma unroll
-        for (int k = 0; k < V; ++k) {
-            const double xh = ((double)v[k] - mean) * rstd;
-            const float wd = w[k] * (d[k] * act_slope(fma(xh, (double)w[k], (double)b[k]), ACT, a.slope));
-            v[k] = fr * (wd - f1 - (float)xh * f2);
-        }
+        for (int k = 0; k < V; ++k) v[k] = fmaf(w[k], dz[r][k], (float)fma((double)v[k] - mean, c2, c1));
         store_vec<T, V>(o + (long long)row * a.C, v);
     }
 }
 
-// dw, db: the sums [rows][C][2] over their rows, 32 channels and 32 row walkers per workgroup
+// dw, db: the sums [rows][C][2] over their rows, 32 channels and 32 row walkers per workgroup; more than one range of rows (gridDim.y):
+// the ranges' sums, [range][C][2]
 template <typename P>
-__global__ __launch_bounds__(1024) void gn_param_grad_kernel(const P* part, long long rows, int C, float* dw, float* db) {
+__global__ __launch_bounds__(1024) void gn_param_grad_kernel(const P* part, long long rows, int C, float* dw, float* db, double* ranges) {
     __shared__ double sh[1024 * 2];
     const int col = threadIdx.x & 31, ty = threadIdx.x >> 5, c = (int)blockIdx.x * 32 + col;
+    const long long per = (rows + gridDim.y - 1) / gridDim.y, r1 = min(rows, (blockIdx.y + 1) * per);
     double p = 0.0, q = 0.0;
     if (c < C)
 #pragma unroll 8
-        for (long long r = ty; r < rows; r += 32) {
+        for (long long r = blockIdx.y * per + ty; r < r1; r += 32) {
             p += (double)part[2 * (r * C + c)];
             q += (double)part[2 * (r * C + c) + 1];
         }
@@ -789,8 +817,13 @@ __global__ __launch_bounds__(1024) void gn_param_grad_kernel(const P* part, long
             p += sh[2 * (y * 32 + col)];
             q += sh[2 * (y * 32 + col) + 1];
         }
-        dw[c] = (float)p;
-        db[c] = (float)q;
+        if (ranges) {
+            ranges[2 * ((long long)blockIdx.y * C + c)] = p;
+            ranges[2 * ((long long)blockIdx.y * C + c) + 1] = q;
+        } else {
+            dw[c] = (float)p;
+            db[c] = (float)q;
+        }
     }
 }
 
@@ -801,7 +834,7 @@ struct GnPlan {
     int res_rows, res_groups, res_blocks, res_threads;
     int items, lanes;     // unit
     int per, blocks_g, blocks_n;
-    int tx, blocks_c, chunks;
+    int tx, blocks_c, chunks, merge;   // merge: threads that merge a group's partial sums
     long long chunk_rows;
 };
 
@@ -833,10 +866,14 @@ void gn_tile_plan(GnPlan& P, long long N, long long S, int C) {
     P.chunks = (int)((S + P.chunk_rows - 1) / P.chunk_rows);
 }
 
+// A group in a part of a wave's registers: rows (S = 1) up to 8 vectors a lane, points (forward only) up to 2 — a wave walks over a
+// group's points in short accesses, and whole samples in a workgroup are faster from there on.  Unit against resident, forward, us:
+// 20000 x 2 x 16 in 2 groups 4.0 / 26.8, 4000 x 16 x 32 in 4 8.1 / 11.8, 300 x 37 x 15 in 5 (111 vectors) 4.5 / 5.5, 64 x 100 x 15 in 5
+// (300) 6.0 / 4.6, 256 x 256 x 128 in 8 (512) 30.3 / 15.0; rows 1024 x 512 in 32 4.3 / 16.9, backward 9.7 / 26.4.
 bool gn_unit_plan(GnPlan& P, long long S, int D, bool backward) {
-    if (backward ? S != 1 : S * D > 64ll * kUnitItems * P.V) return false;
+    if (S != 1 && (backward || S > 128)) return false;
     const long long nv = S * (D / P.V);
-    if (nv > 64 * kUnitItems) return false;
+    if (nv > (S == 1 ? 64 * kUnitItems : 128)) return false;
     P.lanes = 1;
     while (P.lanes < 64 && P.lanes < nv) P.lanes *= 2;
     P.items = 1;
@@ -844,10 +881,12 @@ bool gn_unit_plan(GnPlan& P, long long S, int D, bool backward) {
     return true;
 }
 
-// Resident: whole samples in registers, 16 vectors a thread (backward: of x and of dy) and 512 threads at most.
-bool gn_res_plan(GnPlan& P, long long N, long long S, int C, int G, bool backward) {
+// Resident: whole samples in registers, 16 vectors a thread (backward: of x and of dy) and 512 threads at most.  Resident against
+// tile, forward / backward, us: 32 x 2048 x 256 bf16 in 32 groups 25 / 35 against 31 / 57, 128 x 2048 x 256 71 / 140 against 102 / 185,
+// 6 x 1111 x 132 f16 in 11 9.2 / 13.5 against 12.9 / 17.9, 4 x 4096 x 64 in 8 13.9 / 20.3 against 15.4 / 19.6.
+bool gn_res_plan(GnPlan& P, long long N, long long S, int C, int G) {
     const int D = C / G;
-    if (P.V < 4 || D % P.V || S > 16 * kResThreads) return false;
+    if (S > 16 * kResThreads) return false;
     const int per = D / P.V;
     if (per > kResThreads) return false;
     // as many groups side by side as leave every thread 16 rows ..
@@ -856,7 +895,8 @@ bool gn_res_plan(GnPlan& P, long long N, long long S, int C, int G, bool backwar
     while (groups > 0 && (long long)(kResThreads / (groups * per)) * 16 < S) --groups;
     if (groups < 1) return false;
     if (groups > G) groups = G;
-    // .. but 256 workgroups at least, down to 64 bytes of a row each (and 64 workgroups whatever it takes)
+    // .. but 256 workgroups at least, down to 64 bytes of a row each (and 64 workgroups whatever it takes; 128 or 512, and 32 or 128
+    // bytes, make 3 % at most either way, 64 x 64 x 64 bf16 backward excepted: 7.8, 8.2 and 9.2 us with 32, 64 and 128 bytes)
     const int line = 64 / (P.V * P.es);
     while (groups > 1 && N * ((G + groups - 1) / groups) < 256 && ((groups / 2) * per >= line || N * ((G + groups - 1) / groups) < 64))
         groups /= 2;
@@ -877,10 +917,15 @@ void gn_unit_bwd_grid(GnPlan& P, long long N, int G) {
     const int slots = kGnThreads / P.lanes;
     P.per = G < slots ? slots / G : 1;
     P.blocks_g = G < slots ? 1 : (G + slots - 1) / slots;
-    long long nb = (N + P.per - 1) / P.per, most = 512 / P.blocks_g;
+    // (16384 x 512 f32 in 32 groups, backward: 54, 37, 30 us with 256, 512, 1024 workgroups)
+    long long nb = (N + P.per - 1) / P.per, most = 1024 / P.blocks_g;
     if (most < 1) most = 1;
     P.blocks_n = (int)(nb < most ? nb : most);
 }
+
+// Ranges of rows in the sum that makes dw and db: one where the launch is a latency or two long, else of 512 rows or more
+// (20000 samples of 2 x 16: the backward pass takes 114 us in all, 182 with one range)
+int gn_ranges(long long rows) { return rows <= 1024 ? 1 : rows < 64 * 512 ? (int)((rows + 511) / 512) : 64; }
 
 int gn_check(long long N, long long S, int C, int G, int act, int dtype, const char* who) {
     if (N < 1 || S < 1 || C < 1 || G < 1 || C % G != 0) {
@@ -911,7 +956,7 @@ int64_t gn_ws_bytes(long long N, long long S, int C, int G, int dtype, bool back
         if ((C / G) % V == 0 && gn_unit_plan(P, S, C / G, backward)) {
             if (backward) {
                 gn_unit_bwd_grid(P, N, G);
-                n = (int64_t)P.blocks_n * P.per * C * 2 * sizeof(float);
+                n = (int64_t)P.blocks_n * C * 2 * sizeof(float);
             } else {
                 n = 0;
             }
@@ -921,7 +966,16 @@ int64_t gn_ws_bytes(long long N, long long S, int C, int G, int dtype, bool back
         }
         if (n > need) need = n;
     }
-    return need;
+    return need + (backward && gn_ranges(N) > 1 ? (int64_t)gn_ranges(N) * C * 2 * sizeof(double) : 0);
+}
+
+template <typename P> void gn_param_grad(const GnArgs& a, const P* part, long long rows, hipStream_t st) {
+    const int ranges = gn_ranges(rows);
+    const dim3 grid((unsigned)((a.C + 31) / 32), ranges), block(1024);
+    hipLaunchKernelGGL((gn_param_grad_kernel<P>), grid, block, 0, st, part, rows, a.C, a.dw, a.db, ranges > 1 ? a.ranges : nullptr);
+    if (ranges > 1)
+        hipLaunchKernelGGL((gn_param_grad_kernel<double>), dim3(grid.x), block, 0, st, (const double*)a.ranges, (long long)ranges, a.C, a.dw,
+                           a.db, (double*)nullptr);
 }
 
 #define GN_ACT(act, kernel, grid)                                                                                       \
@@ -946,23 +1000,22 @@ template <typename T, int V> int gn_forward_v(const GnPlan& P, GnArgs& a, hipStr
         }
         return check_launch("group_norm forward");
     }
-    if constexpr (V >= 4)
-        if (P.res) {
-            const dim3 grid((unsigned)(a.N * P.res_blocks)), block(P.res_threads);
-            if (P.res_rows == 4) { GN_RES(a.act, gn_res_fwd_kernel, 4) }
-            else if (P.res_rows == 8) { GN_RES(a.act, gn_res_fwd_kernel, 8) }
-            else { GN_RES(a.act, gn_res_fwd_kernel, 16) }
-            return check_launch("group_norm forward");
-        }
+    if (P.res) {
+        const dim3 grid((unsigned)(a.N * P.res_blocks)), block(P.res_threads);
+        if (P.res_rows == 4) { GN_RES(a.act, gn_res_fwd_kernel, 4) }
+        else if (P.res_rows == 8) { GN_RES(a.act, gn_res_fwd_kernel, 8) }
+        else { GN_RES(a.act, gn_res_fwd_kernel, 16) }
+        return check_launch("group_norm forward");
+    }
     const dim3 grid((unsigned)(a.N * P.chunks), P.blocks_c), block(kGnThreads);
     hipLaunchKernelGGL((gn_tile_sum_kernel<T, V>), grid, block, 0, st, a);
-    hipLaunchKernelGGL((gn_stats_kernel<T>), dim3((unsigned)(a.N * a.G)), block, 0, st, a);
+    hipLaunchKernelGGL((gn_stats_kernel<T>), dim3((unsigned)(a.N * a.G)), dim3(P.merge), 0, st, a);
     GN_ACT(a.act, gn_tile_apply_kernel, grid)
     return check_launch("group_norm forward");
 }
 
 template <typename T, int V> int gn_backward_v(const GnPlan& P, GnArgs& a, hipStream_t st) {
-    const dim3 block(kGnThreads), cols((unsigned)((a.C + 31) / 32));
+    const dim3 block(kGnThreads);
     if (P.unit) {
         if (!a.dw) a.part = nullptr;
         const dim3 grid((unsigned)P.blocks_g * P.blocks_n);
@@ -972,26 +1025,21 @@ template <typename T, int V> int gn_backward_v(const GnPlan& P, GnArgs& a, hipSt
             case 4: hipLaunchKernelGGL((gn_unit_bwd_kernel<T, V, 4>), grid, block, 0, st, a); break;
             default: hipLaunchKernelGGL((gn_unit_bwd_kernel<T, V, 8>), grid, block, 0, st, a); break;
         }
-        if (a.dw)
-            hipLaunchKernelGGL((gn_param_grad_kernel<float>), cols, dim3(1024), 0, st, (const float*)a.part,
-                               (long long)P.blocks_n * P.per, a.C, a.dw, a.db);
+        if (a.dw) gn_param_grad(a, (const float*)a.part, P.blocks_n, st);
         return check_launch("group_norm backward");
     }
-    if constexpr (V >= 4)
-        if (P.res) {
-            const dim3 grid((unsigned)(a.N * P.res_blocks)), block(P.res_threads);
-            if (P.res_rows == 4) { GN_RES(a.act, gn_res_bwd_kernel, 4) }
-            else if (P.res_rows == 8) { GN_RES(a.act, gn_res_bwd_kernel, 8) }
-            else { GN_RES(a.act, gn_res_bwd_kernel, 16) }
-            if (a.dw)
-                hipLaunchKernelGGL((gn_param_grad_kernel<double>), cols, dim3(1024), 0, st, (const double*)a.chan, a.N, a.C, a.dw, a.db);
-            return check_launch("group_norm backward");
-        }
+    if (P.res) {
+        const dim3 grid((unsigned)(a.N * P.res_blocks)), block(P.res_threads);
+        if (P.res_rows == 4) { GN_RES(a.act, gn_res_bwd_kernel, 4) }
+        else if (P.res_rows == 8) { GN_RES(a.act, gn_res_bwd_kernel, 8) }
+        else { GN_RES(a.act, gn_res_bwd_kernel, 16) }
+        if (a.dw) gn_param_grad(a, (const double*)a.chan, a.N, st);
+        return check_launch("group_norm backward");
+    }
     const dim3 grid((unsigned)(a.N * P.chunks), P.blocks_c);
     GN_ACT(a.act, gn_tile_bwd_sum_kernel, grid)
-    hipLaunchKernelGGL(gn_bwd_coef_kernel, dim3((unsigned)(a.N * a.G)), block, 0, st, a);
-    if (a.dw)
-        hipLaunchKernelGGL((gn_param_grad_kernel<double>), cols, dim3(1024), 0, st, (const double*)a.chan, a.N, a.C, a.dw, a.db);
+    hipLaunchKernelGGL(gn_bwd_coef_kernel, dim3((unsigned)(a.N * a.G)), dim3(P.merge), 0, st, a);
+    if (a.dw) gn_param_grad(a, (const double*)a.chan, a.N, st);
     GN_ACT(a.act, gn_tile_bwd_apply_kernel, grid)
     return check_launch("group_norm backward");
 }
@@ -1010,7 +1058,7 @@ int gn_run(bool backward, GnArgs& a, int dtype, void* ws, size_t ws_bytes, hipSt
     P.V = gn_width(dtype, a.D, a.C, backward ? bs : fs, {a.x, a.out, backward ? a.dy : a.x});
     P.es = elem_bytes(dtype);
     P.unit = gn_unit_plan(P, a.S, a.D, backward);
-    P.res = !P.unit && gn_res_plan(P, a.N, a.S, a.C, a.G, backward);
+    P.res = !P.unit && gn_res_plan(P, a.N, a.S, a.C, a.G);
     if (P.unit) {
         a.lanes = P.lanes;
         if (backward) {
@@ -1024,14 +1072,18 @@ int gn_run(bool backward, GnArgs& a, int dtype, void* ws, size_t ws_bytes, hipSt
     } else {
         P.V = gn_width(dtype, 0, a.C, backward ? bs : fs, {a.x, a.out, backward ? a.dy : a.x});
         gn_tile_plan(P, a.N, a.S, a.C);
-        if (P.blocks_c > 65535) return DGG_ERR_INVALID;
+        P.merge = (long long)P.chunks * a.D > 1024 ? kMergeThreads : kGnThreads;
+        if (P.blocks_c > 65535) {
+            set_error_text("%s: %d channels element by element: 2^24 - 256 at most", who, a.C);
+            return DGG_ERR_INVALID;
+        }
         a.chunks = P.chunks;
         a.chunk_rows = P.chunk_rows;
         a.tx = P.tx;
     }
-    size_t need = 0;
+    size_t need = 0, ranges = backward && !P.unit && a.dw && gn_ranges(a.N) > 1 ? (size_t)gn_ranges(a.N) * a.C * 2 * sizeof(double) : 0;
     if (P.unit) {
-        need = backward && a.dw ? (size_t)P.blocks_n * P.per * a.C * 2 * sizeof(float) : 0;
+        need = backward && a.dw ? (size_t)P.blocks_n * a.C * 2 * sizeof(float) : 0;
     } else if (P.res) {
         need = backward && a.dw ? (size_t)a.N * a.C * 2 * sizeof(double) : 0;
         a.chan = (double*)ws;
@@ -1042,6 +1094,8 @@ int gn_run(bool backward, GnArgs& a, int dtype, void* ws, size_t ws_bytes, hipSt
         a.coef = (double*)((char*)ws + part + more);
         if (!a.stats) a.stats = a.coef;   // a forward without a backward keeps its statistics in the workspace
     }
+    a.ranges = (double*)((char*)ws + need);
+    need += ranges;
     if (need && (!ws || ws_bytes < need || (uintptr_t)ws % 8)) {
         set_error_text("%s: the workspace has %zu bytes, %zu (8-byte aligned) are needed", who, ws_bytes, need);
         return DGG_ERR_WORKSPACE;

@@ -601,6 +601,9 @@ __global__ __launch_bounds__(kThreads, 2) void ns_apply_kernel(const NsArgs* arg
 // A matrix whose planes fit the LDS of one workgroup (short side <= 32 and long side <= 512, or 64 and 192): the whole step in one
 // launch, 16 waves.  What bounds it is the chain of 5 barriers a step; the launches of the other route alone take 100 us.
 // The same planes in the same order and scales as there: A = X X^T in ranges of k that meet in LDS, A^2 and B X one 32 x 32 block a wave.
+// A short side of a few rows has short sums, and the planes' 22 bits are what its error consists of (12 x 512: 1.0 to 1.5e-6 of |X|
+// where fp32 products give 0.7 to 1.1e-6).  The matrix instructions are no bound here: lo lo is multiplied too, and B, whose error
+// stays the same for all of X, has a third plane (together 0.4 to 0.9e-6).
 constexpr int kSmallThreads = 1024, kPart = 32 * 36;
 
 __host__ __device__ __forceinline__ int small_splits(int mp) { return mp == 32 ? 4 : 2; }
@@ -618,7 +621,10 @@ __device__ __forceinline__ void small_multiply(const SmallFrags& x, f32x16& hh, 
     cross = __builtin_amdgcn_mfma_f32_32x32x16_f16(x.ph, x.ql, cross, 0, 0, 0);
     hh = __builtin_amdgcn_mfma_f32_32x32x16_f16(x.ph, x.qh, hh, 0, 0, 0);
     cross = __builtin_amdgcn_mfma_f32_32x32x16_f16(x.pl, x.qh, cross, 0, 0, 0);
+    cross = __builtin_amdgcn_mfma_f32_32x32x16_f16(x.pl, x.ql, cross, 0, 0, 0);
 }
+// where a third plane of its own (1 KB a block) holds what lies at `at` of the hi plane
+__device__ __forceinline__ size_t third(size_t at) { return (at >> 11 << 10) | (at & 1023); }
 __device__ __forceinline__ void zero(f32x16& hh, f32x16& cross) {
 #pragma unroll
     for (int e = 0; e < 16; ++e) hh[e] = cross[e] = 0.f;
@@ -637,6 +643,7 @@ __global__ __launch_bounds__(kSmallThreads) void ns_small_kernel(NsArgs a, NsFir
     char* A = xt + mp * np * 4;
     char* B = A + mp * mp * 4;
     float* part = (float*)(B + mp * mp * 4);
+    char* B3 = (char*)part;   // (the partial sums of A have been added up by then)
     const Global<In>* in = (const Global<In>*)M.in + (size_t)bat * M.in_stride;
     Global<float>* mom = MUON ? (Global<float>*)M.mom + (size_t)bat * M.mom_stride : nullptr;
     // U as it lies in memory, 16 elements a thread at most, through LDS (fp32 [mp][np + 4], in the place of X by columns and the start of A)
@@ -777,7 +784,12 @@ __global__ __launch_bounds__(kSmallThreads) void ns_small_kernel(NsArgs a, NsFir
 #pragma unroll
                 for (int e = 0; e < 4; ++e)
                     v[e] = fmaf(fc, hh[4 * q + e] + cross[4 * q + e], fmaf(fb, v[e], row + e == bcol ? fa : 0.f));
-                store4(B + plane_at(bcol, row, mp), v);
+                const size_t to = plane_at(bcol, row, mp);
+                store4(B + to, v);
+                float two[4];   // (as stored; what is left is exact)
+                load4(B + to, two);
+                *(half4*)(B3 + third(to)) = half4{(_Float16)(v[0] - two[0]), (_Float16)(v[1] - two[1]), (_Float16)(v[2] - two[2]),
+                                                  (_Float16)(v[3] - two[3])};
             }
         }
         __syncthreads();
@@ -788,12 +800,17 @@ __global__ __launch_bounds__(kSmallThreads) void ns_small_kernel(NsArgs a, NsFir
         if (mine)
             for (int x = 0, n = mp / 16; x < n; x += 2) {
                 SmallFrags f[2];
-#pragma unroll
-                for (int y = 0; y < 2; ++y)
-                    small_read(B + (bi * n + x + y) * 2048 + lane * 16, xt + (bj * n + x + y) * 2048 + lane * 16, f[y]);
+                half8 b3[2];
 #pragma unroll
                 for (int y = 0; y < 2; ++y) {
+                    small_read(B + (bi * n + x + y) * 2048 + lane * 16, xt + (bj * n + x + y) * 2048 + lane * 16, f[y]);
+                    b3[y] = *(const half8*)(B3 + (bi * n + x + y) * 1024 + lane * 16);
+                }
+#pragma unroll
+                for (int y = 0; y < 2; ++y) {
+                    cross = __builtin_amdgcn_mfma_f32_32x32x16_f16(b3[y], f[y].qh, cross, 0, 0, 0);
                     small_multiply(f[y], hh, cross);
+                    cross2 = __builtin_amdgcn_mfma_f32_32x32x16_f16(f[y].qh, b3[y], cross2, 0, 0, 0);
                     small_multiply({f[y].qh, f[y].ql, f[y].ph, f[y].pl}, hh2, cross2);
                 }
             }
