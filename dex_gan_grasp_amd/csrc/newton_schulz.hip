@@ -900,6 +900,15 @@ bool ns_small(const dgg_matrix& m) {
     return lo <= 32 ? hi <= 512 : lo <= 64 && hi <= 192;
 }
 
+// Whether a call's small matrices have a launch of their own: not where they find places in the launches that its other matrices
+// need anyway (30 x 2000, 100 x 2000 and 100 x 30: 129 us with a launch of its own for the last, 98 without).
+bool ns_apart(const dgg_matrix* mats, int count) {
+    int small = 0;
+    for (int i = 0; i < count; ++i) small += ns_small(mats[i]);
+    const int free = (kNsMats - (count - small) % kNsMats) % kNsMats;
+    return count == small || small > free;
+}
+
 // What both routes need to know of one matrix.
 void ns_fill(const dgg_matrix& in, const NsArgs& a, int pad, NsMat& M) {
     M.in = in.in; M.out = in.out; M.mom = in.momentum;
@@ -970,17 +979,18 @@ void ns_plan(const dgg_matrix* const* mats, int count, NsArgs& a, NsPlan& P) {
 }
 
 // up to kNsMats matrices of one route, from mats[at] on; at moves behind them
-int ns_group(const dgg_matrix* mats, int count, bool small, int& at, const dgg_matrix** group) {
+int ns_group(const dgg_matrix* mats, int count, bool apart, bool small, int& at, const dgg_matrix** group) {
     int n = 0;
     for (; at < count && n < kNsMats; ++at)
-        if (ns_small(mats[at]) == small) group[n++] = mats + at;
+        if ((apart && ns_small(mats[at])) == small) group[n++] = mats + at;
     return n;
 }
 
 int64_t ns_need(const dgg_matrix* mats, int count) {
     const dgg_matrix* group[kNsMats];
     size_t need = 256;
-    for (int at = 0, n; (n = ns_group(mats, count, false, at, group)) > 0;) {
+    const bool apart = ns_apart(mats, count);
+    for (int at = 0, n; (n = ns_group(mats, count, apart, false, at, group)) > 0;) {
         NsArgs a = {};
         NsPlan P;
         ns_plan(group, n, a, P);
@@ -996,8 +1006,8 @@ struct NsSpan {
     bool written;
 };
 
-// Two spans share no element: they lie apart, or they are column blocks of one wider buffer.
-bool ns_apart(const NsSpan& a, const NsSpan& b) {
+// Two spans share no element: they lie one behind the other, or they are column blocks of one wider buffer.
+bool ns_free(const NsSpan& a, const NsSpan& b) {
     if (a.hi <= b.lo || b.hi <= a.lo) return true;
     if (a.ld != b.ld || (a.batch > 1 && a.stride % a.ld) || (b.batch > 1 && b.stride % b.ld)) return false;
     const uintptr_t d = a.lo <= b.lo ? (b.lo - a.lo) % a.ld : (a.ld - (a.lo - b.lo) % a.ld) % a.ld;   // b's first column from a's
@@ -1030,7 +1040,7 @@ bool ns_disjoint(const dgg_matrix* mats, int count, size_t size, bool muon) {
     std::sort(spans.begin(), spans.end(), [](const NsSpan& a, const NsSpan& b) { return a.lo < b.lo; });
     for (size_t i = 0; i < spans.size(); ++i)
         for (size_t j = i + 1; j < spans.size() && spans[j].lo < spans[i].hi; ++j)
-            if ((spans[i].written || spans[j].written) && !ns_apart(spans[i], spans[j])) return false;
+            if ((spans[i].written || spans[j].written) && !ns_free(spans[i], spans[j])) return false;
     return true;
 }
 
@@ -1062,18 +1072,19 @@ int ns_run(const dgg_matrix* mats, int count, NsArgs& a, const double* coef, int
         set_error_text("%s: the workspace has %zu bytes, %lld are needed", who, ws_bytes, (long long)need);
         return DGG_ERR_WORKSPACE;
     }
-    bool apart = false;
+    bool disjoint = false;
     try {
-        apart = ns_disjoint(mats, count, sizeof(T), MUON);
+        disjoint = ns_disjoint(mats, count, sizeof(T), MUON);
     } catch (const std::exception& e) {
         set_error_text("%s: %s", who, e.what());
         return DGG_ERR_INVALID;
     }
-    if (!apart) {
+    if (!disjoint) {
         set_error_text("%s: what is written overlaps itself or another operand", who);
         return DGG_ERR_INVALID;
     }
-    for (int at = 0, n; (n = ns_group(mats, count, true, at, group)) > 0;) {
+    const bool apart = ns_apart(mats, count);
+    for (int at = 0, n; (n = ns_group(mats, count, apart, true, at, group)) > 0;) {
         NsFirst first;
         int grid = 0, lds = 0;
         for (int i = 0; i < kNsMats; ++i) {
@@ -1093,7 +1104,7 @@ int ns_run(const dgg_matrix* mats, int count, NsArgs& a, const double* coef, int
         }
         hipLaunchKernelGGL((ns_small_kernel<T, MUON>), dim3(grid), dim3(kSmallThreads), lds, st, a, first);
     }
-    for (int at = 0, n; (n = ns_group(mats, count, false, at, group)) > 0;) {
+    for (int at = 0, n; (n = ns_group(mats, count, apart, false, at, group)) > 0;) {
         ns_plan(group, n, a, P);
         const dim3 block(kThreads);
         const NsArgs* args = (const NsArgs*)ws;
