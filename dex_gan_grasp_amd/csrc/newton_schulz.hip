@@ -34,6 +34,8 @@ namespace {
 typedef _Float16 half8 __attribute__((ext_vector_type(8)));
 typedef _Float16 half2 __attribute__((ext_vector_type(2)));
 typedef _Float16 half4 __attribute__((ext_vector_type(4)));
+typedef float f32x2 __attribute__((ext_vector_type(2)));
+typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef float f32x16 __attribute__((ext_vector_type(16)));
 typedef __attribute__((address_space(3))) char lds_char;
 typedef __attribute__((address_space(3))) float lds_f32;
@@ -630,6 +632,119 @@ __device__ __forceinline__ void zero(f32x16& hh, f32x16& cross) {
     for (int e = 0; e < 16; ++e) hh[e] = cross[e] = 0.f;
 }
 
+// The four pieces of a step, for a workgroup whose X (n columns of it) lies in LDS; p: this lane's place in a fragment.
+// A = X X^T: tiles (0, 0), (0, 1), (1, 1), a range of k each, a wave each -> part[tile * splits + range][j][i], pitch 36
+__device__ __forceinline__ void small_gram(const char* xr, int np, int tiles, int splits, float* part) {
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, r = lane & 31, h = lane >> 5;
+    if (wave >= tiles * splits) return;
+    const int tile = wave / splits, ti = tile >> 1, tj = (tile + 1) >> 1, n = np / 16, per = ((n + splits - 1) / splits + 1) & ~1;
+    const int b = (wave - tile * splits) * per, e = min(b + per, n);   // (an even number of 16 k)
+    const char *p = xr + ti * n * 2048 + lane * 16, *q = xr + tj * n * 2048 + lane * 16;
+    f32x16 hh, cross;
+    zero(hh, cross);
+    for (int x = b; x < e; x += 2) {
+        SmallFrags f[2];
+        small_read(p + x * 2048, q + x * 2048, f[0]);
+        small_read(p + x * 2048 + 2048, q + x * 2048 + 2048, f[1]);
+        small_multiply(f[0], hh, cross);
+        small_multiply(f[1], hh, cross);
+    }
+    float* o = part + wave * kPart + r * 36 + 4 * h;
+#pragma unroll
+    for (int y = 0; y < 4; ++y)
+        *(float4*)(o + 8 * y) = make_float4(hh[4 * y] + cross[4 * y], hh[4 * y + 1] + cross[4 * y + 1], hh[4 * y + 2] + cross[4 * y + 2],
+                                            hh[4 * y + 3] + cross[4 * y + 3]);
+}
+// a thread's 8 elements of A (row aj, i8 .. of its tile), the ranges added up in order; threads below tiles * 128
+__device__ __forceinline__ void small_sum(const float* part, int splits, float (&v)[8]) {
+    const int tile = threadIdx.x >> 7, aj = threadIdx.x & 31, i8 = ((threadIdx.x >> 5) & 3) * 8;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v[e] = 0.f;
+    for (int sp = 0; sp < splits; ++sp) {
+        const float* o = part + (tile * splits + sp) * kPart + aj * 36 + i8;
+        const float4 lo = *(const float4*)o, hi = *(const float4*)(o + 4);
+        v[0] += lo.x; v[1] += lo.y; v[2] += lo.z; v[3] += lo.w;
+        v[4] += hi.x; v[5] += hi.y; v[6] += hi.z; v[7] += hi.w;
+    }
+}
+// planes of A from them, both triangles
+__device__ __forceinline__ void small_a(float (&v)[8], const NsScale& z, int mp, char* A) {
+    const int tile = threadIdx.x >> 7, ti = tile >> 1, tj = (tile + 1) >> 1, aj = threadIdx.x & 31, i8 = ((threadIdx.x >> 5) & 3) * 8;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v[e] = v[e] * z.sx * z.sx * z.sa;
+    store8(A + plane_at(tj * 32 + aj, ti * 32 + i8, mp), v);
+    if (ti == tj) return;
+#pragma unroll
+    for (int e = 0; e < 8; e += 2) {
+        half2 hi, lo;
+        split2(v[e], v[e + 1], hi, lo);
+        char* o = A + plane_at(ti * 32 + i8 + e, tj * 32 + aj, mp);
+        *(_Float16*)o = hi.x;
+        *(_Float16*)(o + 1024) = lo.x;
+        *(_Float16*)(o + 16) = hi.y;   // (the next row)
+        *(_Float16*)(o + 1040) = lo.y;
+    }
+}
+// B = a + b A + c A^2 in three planes, a block a wave
+__device__ __forceinline__ void small_square(const char* A, char* B, char* B3, const NsStep& S, const NsScale& z, int mp) {
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, r = lane & 31, h = lane >> 5, T = mp / 32;
+    if (wave >= T * T) return;
+    const int ti = wave / T, tj = wave - ti * T, n = mp / 16, bcol = tj * 32 + r;
+    const float ratio = z.sb / z.sa, fa = S.a * z.sb, fb = S.b * ratio, fc = S.c * ratio / z.sa;
+    f32x16 hh, cross;
+    zero(hh, cross);
+    for (int x = 0; x < n; x += 2) {
+        SmallFrags f[2];
+#pragma unroll
+        for (int y = 0; y < 2; ++y)
+            small_read(A + (ti * n + x + y) * 2048 + lane * 16, A + (tj * n + x + y) * 2048 + lane * 16, f[y]);
+        small_multiply(f[0], hh, cross);
+        small_multiply(f[1], hh, cross);
+    }
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+        const int row = ti * 32 + 8 * q + 4 * h;
+        float v[4], two[4];
+        load4(A + plane_at(bcol, row, mp), v);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[e] = fmaf(fc, hh[4 * q + e] + cross[4 * q + e], fmaf(fb, v[e], row + e == bcol ? fa : 0.f));
+        const size_t to = plane_at(bcol, row, mp);
+        store4(B + to, v);
+        load4(B + to, two);   // (as stored; what is left is exact)
+        *(half4*)(B3 + third(to)) = half4{(_Float16)(v[0] - two[0]), (_Float16)(v[1] - two[1]), (_Float16)(v[2] - two[2]),
+                                          (_Float16)(v[3] - two[3])};
+    }
+}
+// Block (bi, bj) of B X: a lane has a column's rows; ROWS: the same values with the operands exchanged, a lane has a row's columns, as X
+// by rows is written.  (One after the other: the accumulators of both do not fit beside the rest.)
+template <bool ROWS>
+__device__ __forceinline__ void small_apply(const char* B, const char* B3, const char* xt, int bi, int bj, int mp, float f, float (&v)[4][4]) {
+    const int lane = threadIdx.x & 63;
+    f32x16 hh, cross;
+    zero(hh, cross);
+    for (int x = 0, n = mp / 16; x < n; x += 2) {
+        SmallFrags g[2];
+        half8 b3[2];
+#pragma unroll
+        for (int y = 0; y < 2; ++y) {
+            const char *b = B + (bi * n + x + y) * 2048 + lane * 16, *c = xt + (bj * n + x + y) * 2048 + lane * 16;
+            if (ROWS) small_read(c, b, g[y]);
+            else small_read(b, c, g[y]);
+            b3[y] = *(const half8*)(B3 + (bi * n + x + y) * 1024 + lane * 16);
+        }
+#pragma unroll
+        for (int y = 0; y < 2; ++y) {
+            if (ROWS) cross = __builtin_amdgcn_mfma_f32_32x32x16_f16(g[y].ph, b3[y], cross, 0, 0, 0);
+            else cross = __builtin_amdgcn_mfma_f32_32x32x16_f16(b3[y], g[y].qh, cross, 0, 0, 0);
+            small_multiply(g[y], hh, cross);
+        }
+    }
+#pragma unroll
+    for (int q = 0; q < 4; ++q)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[q][e] = f * (hh[4 * q + e] + cross[4 * q + e]);
+}
+
 template <typename In, bool MUON>
 __global__ __launch_bounds__(kSmallThreads) void ns_small_kernel(NsArgs a, NsFirst first) {
     extern __shared__ char smem[];
@@ -704,141 +819,244 @@ __global__ __launch_bounds__(kSmallThreads) void ns_small_kernel(NsArgs a, NsFir
     const int bj = wave / T, bi = wave - bj * T, i = bi * 32 + 4 * h, j = bj * 32 + r;
     const long long di = M.turned ? 1 : M.ld_out, at = M.turned ? (long long)j * M.ld_out + i : (long long)i * M.ld_out + j;
     Global<float>* W = (Global<float>*)M.out + (size_t)bat * M.out_stride;
-    float w[4][4];
     for (int k = 0; k < a.steps; ++k) {
         const NsScale z = sc[k];
         const bool last = k + 1 == a.steps;
-        if (MUON && last) {   // the parameters are on their way during the last step
+        float v[4][4], x[4][4];   // x: X by rows, or (last step) the parameters
+        if (MUON && last) {   // (on their way during the step)
 #pragma unroll
             for (int q = 0; q < 4; ++q)
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
                     const int ic = min(i + 8 * q + e, M.m - 1), jc = min(j, M.n - 1);   // (beyond: not used)
-                    w[q][e] = W[M.turned ? (long long)jc * M.ld_out + ic : (long long)ic * M.ld_out + jc];
+                    x[q][e] = W[M.turned ? (long long)jc * M.ld_out + ic : (long long)ic * M.ld_out + jc];
                 }
         }
-        f32x16 hh, cross;
-        if (wave < tiles * splits) {   // A: tiles (0, 0), (0, 1), (1, 1), a range of k each
-            const int tile = wave / splits, ti = tile >> 1, tj = (tile + 1) >> 1, n = np / 16, per = ((n + splits - 1) / splits + 1) & ~1;
-            const int b = (wave - tile * splits) * per, e = min(b + per, n);   // (an even number of 16 k)
-            const char *p = xr + ti * n * 2048 + lane * 16, *q = xr + tj * n * 2048 + lane * 16;
-            zero(hh, cross);
-            for (int x = b; x < e; x += 2) {
-                SmallFrags f[2];
-                small_read(p + x * 2048, q + x * 2048, f[0]);
-                small_read(p + x * 2048 + 2048, q + x * 2048 + 2048, f[1]);
-                small_multiply(f[0], hh, cross);
-                small_multiply(f[1], hh, cross);
-            }
-            float* o = part + wave * kPart + r * 36 + 4 * h;   // [j][i]
-#pragma unroll
-            for (int y = 0; y < 4; ++y)
-                *(float4*)(o + 8 * y) = make_float4(hh[4 * y] + cross[4 * y], hh[4 * y + 1] + cross[4 * y + 1],
-                                                    hh[4 * y + 2] + cross[4 * y + 2], hh[4 * y + 3] + cross[4 * y + 3]);
+        small_gram(xr, np, tiles, splits, part);
+        __syncthreads();
+        if ((int)threadIdx.x < tiles * 128) {
+            float s[8];
+            small_sum(part, splits, s);
+            small_a(s, z, mp, A);
         }
         __syncthreads();
-        if ((int)threadIdx.x < tiles * 128) {   // 8 i of a row j a thread
-            const int tile = threadIdx.x >> 7, ti = tile >> 1, tj = (tile + 1) >> 1, aj = threadIdx.x & 31, i8 = ((threadIdx.x >> 5) & 3) * 8;
-            float v[8];
-#pragma unroll
-            for (int e = 0; e < 8; ++e) v[e] = 0.f;
-            for (int sp = 0; sp < splits; ++sp) {
-                const float* o = part + (tile * splits + sp) * kPart + aj * 36 + i8;
-                const float4 lo = *(const float4*)o, hi = *(const float4*)(o + 4);
-                v[0] += lo.x; v[1] += lo.y; v[2] += lo.z; v[3] += lo.w;
-                v[4] += hi.x; v[5] += hi.y; v[6] += hi.z; v[7] += hi.w;
-            }
-#pragma unroll
-            for (int e = 0; e < 8; ++e) v[e] = v[e] * z.sx * z.sx * z.sa;
-            store8(A + plane_at(tj * 32 + aj, ti * 32 + i8, mp), v);
-            if (ti != tj)
-#pragma unroll
-                for (int e = 0; e < 8; e += 2) {
-                    half2 hi, lo;
-                    split2(v[e], v[e + 1], hi, lo);
-                    char* o = A + plane_at(ti * 32 + i8 + e, tj * 32 + aj, mp);
-                    *(_Float16*)o = hi.x;
-                    *(_Float16*)(o + 1024) = lo.x;
-                    *(_Float16*)(o + 16) = hi.y;   // (the next row)
-                    *(_Float16*)(o + 1040) = lo.y;
-                }
-        }
+        small_square(A, B, B3, a.step[k], z, mp);
         __syncthreads();
-        if (wave < T * T) {   // B
-            const int ti = wave / T, tj = wave - ti * T, n = mp / 16, bcol = tj * 32 + r;
-            const float ratio = z.sb / z.sa, fa = a.step[k].a * z.sb, fb = a.step[k].b * ratio, fc = a.step[k].c * ratio / z.sa;
-            zero(hh, cross);
-            for (int x = 0; x < n; x += 2) {
-                SmallFrags f[2];
-#pragma unroll
-                for (int y = 0; y < 2; ++y)
-                    small_read(A + (ti * n + x + y) * 2048 + lane * 16, A + (tj * n + x + y) * 2048 + lane * 16, f[y]);
-                small_multiply(f[0], hh, cross);
-                small_multiply(f[1], hh, cross);
-            }
-#pragma unroll
-            for (int q = 0; q < 4; ++q) {
-                const int row = ti * 32 + 8 * q + 4 * h;
-                float v[4];
-                load4(A + plane_at(bcol, row, mp), v);
-#pragma unroll
-                for (int e = 0; e < 4; ++e)
-                    v[e] = fmaf(fc, hh[4 * q + e] + cross[4 * q + e], fmaf(fb, v[e], row + e == bcol ? fa : 0.f));
-                const size_t to = plane_at(bcol, row, mp);
-                store4(B + to, v);
-                float two[4];   // (as stored; what is left is exact)
-                load4(B + to, two);
-                *(half4*)(B3 + third(to)) = half4{(_Float16)(v[0] - two[0]), (_Float16)(v[1] - two[1]), (_Float16)(v[2] - two[2]),
-                                                  (_Float16)(v[3] - two[3])};
-            }
-        }
-        __syncthreads();
-        // B X, and once more with the operands exchanged: the same values lane by row, as X by rows is written
-        f32x16 hh2, cross2;
-        zero(hh, cross);
-        zero(hh2, cross2);
-        if (mine)
-            for (int x = 0, n = mp / 16; x < n; x += 2) {
-                SmallFrags f[2];
-                half8 b3[2];
-#pragma unroll
-                for (int y = 0; y < 2; ++y) {
-                    small_read(B + (bi * n + x + y) * 2048 + lane * 16, xt + (bj * n + x + y) * 2048 + lane * 16, f[y]);
-                    b3[y] = *(const half8*)(B3 + (bi * n + x + y) * 1024 + lane * 16);
-                }
-#pragma unroll
-                for (int y = 0; y < 2; ++y) {
-                    cross = __builtin_amdgcn_mfma_f32_32x32x16_f16(b3[y], f[y].qh, cross, 0, 0, 0);
-                    small_multiply(f[y], hh, cross);
-                    cross2 = __builtin_amdgcn_mfma_f32_32x32x16_f16(f[y].qh, b3[y], cross2, 0, 0, 0);
-                    small_multiply({f[y].qh, f[y].ql, f[y].ph, f[y].pl}, hh2, cross2);
-                }
-            }
         const float f = z.sx / z.sb * (last ? 1.f : z.sx_next);
+        if (mine) {
+            small_apply<false>(B, B3, xt, bi, bj, mp, f, v);
+            if (!last) small_apply<true>(B, B3, xt, bi, bj, mp, f, x);
+        }
         __syncthreads();   // everyone has read X: its place takes the next
         if (mine)
 #pragma unroll
             for (int q = 0; q < 4; ++q) {
-                float v[4], x[4];
-#pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    v[e] = f * (hh[4 * q + e] + cross[4 * q + e]);
-                    x[e] = f * (hh2[4 * q + e] + cross2[4 * q + e]);
-                }
                 if (!last) {
-                    store4(xt + plane_at(j, i + 8 * q, mp), v);
-                    store4(xr + plane_at(bi * 32 + r, bj * 32 + 8 * q + 4 * h, np), x);
+                    store4(xt + plane_at(j, i + 8 * q, mp), v[q]);
+                    store4(xr + plane_at(bi * 32 + r, bj * 32 + 8 * q + 4 * h, np), x[q]);
                     continue;
                 }
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
                     if (i + 8 * q + e >= M.m || j >= M.n) continue;
-                    if (MUON) W[at + (8 * q + e) * di] = fmaf(-step, v[e], decay * w[q][e]);
-                    else ((Global<In>*)M.out)[(size_t)bat * M.out_stride + at + (8 * q + e) * di] = (In)v[e];
+                    if (MUON) W[at + (8 * q + e) * di] = fmaf(-step, v[q][e], decay * x[q][e]);
+                    else ((Global<In>*)M.out)[(size_t)bat * M.out_stride + at + (8 * q + e) * di] = (In)v[q][e];
                 }
             }
         __syncthreads();
     }
+}
+
+// ------------------------------------------------------------------------------------------------ narrow matrices
+// A short side of up to 64 rows and a long one that one workgroup cannot hold: a workgroup owns kNarrow / mp columns of X, and a step is
+// ONE launch.  A workgroup adds up everyone's share of A = X X^T (4 KB a tile each), makes B from it — the same B in every workgroup —,
+// multiplies its columns and leaves their share of the next A.  Shares alternate between two places (a launch reads one and writes
+// the other), columns of X are read by their own workgroup alone.  What bounds it is the launches, steps + 1 of them, and the sum of the
+// shares: 12 x 4608 53 us, 64 x 4108 87 (the general route: 91 and 99); 64 x 8192, 64 workgroups, would take 112.  With half as many
+// columns again a workgroup, 12 x 4608 takes 66 us and 64 x 4108 85.
+constexpr int kNarrow = 8192, kNarrowThreads = 512, kNarrowParts = 64;
+__host__ __device__ __forceinline__ int narrow_splits(int mp) { return mp == 32 ? 8 : 2; }
+int narrow_lds(int mp) { return kNarrow * 8 + mp * mp * 8 + small_tiles(mp) * narrow_splits(mp) * kPart * 4; }
+
+// the power of two of a norm (as in ns_split_kernel)
+__device__ __forceinline__ int power_of(double norm) { return norm > 0.0 && norm < INFINITY ? 14 - ilogb(norm) : 0; }
+
+// this workgroup's share of A -> memory
+__device__ __forceinline__ void narrow_share(const float* part, int mp, Global<float>* to) {
+    if ((int)threadIdx.x >= small_tiles(mp) * 128) return;
+    const int tile = threadIdx.x >> 7, aj = threadIdx.x & 31, i8 = ((threadIdx.x >> 5) & 3) * 8;
+    float v[8];
+    small_sum(part, narrow_splits(mp), v);
+    Global<f32x4>* o = (Global<f32x4>*)(to + (tile * 32 + aj) * 32 + i8);
+    o[0] = f32x4{v[0], v[1], v[2], v[3]};
+    o[1] = f32x4{v[4], v[5], v[6], v[7]};
+}
+
+// everyone's shares of A, two elements of each of N tiles a thread -> part, as small_gram leaves one range (all loads of some shares
+// are in flight)
+template <int N> __device__ __forceinline__ void narrow_sum(const Global<float>* shares, const float* weight, int C, float* part) {
+    const int e = threadIdx.x * 2;
+    f32x2 v[N];
+#pragma unroll
+    for (int t = 0; t < N; ++t) v[t] = f32x2{0.f, 0.f};
+#pragma unroll N == 1 ? 16 : 6
+    for (int c = 0; c < C; ++c) {
+        const float f = weight[c] * weight[c];
+#pragma unroll
+        for (int t = 0; t < N; ++t) {
+            const f32x2 o = *(const Global<f32x2>*)(shares + ((size_t)c * N + t) * 1024 + e);
+            v[t].x = fmaf(f, o.x, v[t].x);
+            v[t].y = fmaf(f, o.y, v[t].y);
+        }
+    }
+#pragma unroll
+    for (int t = 0; t < N; ++t) *(f32x2*)(part + t * kPart + (e >> 5) * 36 + (e & 31)) = v[t];
+}
+
+// The columns of U (muon: M is updated on the way) as planes of U * 2^k, k of THEIR norm, and their share of the first A
+template <typename In, bool MUON>
+__global__ __launch_bounds__(kNarrowThreads) void ns_narrow_first_kernel(NsArgs a, NsFirst first) {
+    extern __shared__ char smem[];
+    __shared__ double sh[kNarrowThreads / 64];
+    if (blockIdx.x == 0)   // (for the launches that follow: ns_norm_kernel)
+        for (int i = threadIdx.x; i < (int)(sizeof(NsArgs) / 8); i += kNarrowThreads) ((Global<uint64_t>*)a.ws)[i] = ((const uint64_t*)&a)[i];
+    int local;
+    const NsMat& M = a.mat[find(first, (int)blockIdx.x, local)];
+    const int bat = local / M.parts, chunk = local - bat * M.parts, mp = M.mp, nc = kNarrow / mp, j0 = chunk * nc, wide = min(nc, M.n - j0);
+    char* xr = smem;
+    float* stage = (float*)(xr + kNarrow * 4);   // fp32 [mp][nc + 4]
+    float* part = (float*)(xr + kNarrow * 8 + mp * mp * 8);
+    const Global<In>* in = (const Global<In>*)M.in + (size_t)bat * M.in_stride;
+    Global<float>* mom = MUON ? (Global<float>*)M.mom + (size_t)bat * M.mom_stride : nullptr;
+    const int pitch = nc + 4, line = M.turned ? M.m : wide, total = M.m * wide;   // line: elements side by side in memory
+    const NsUpdate up = a.update;
+    const float per_line = 1.f / (float)line;
+    for (int e = threadIdx.x; e < mp * pitch / 4; e += kNarrowThreads) ((float4*)stage)[e] = make_float4(0.f, 0.f, 0.f, 0.f);
+    float u[16], m[16];
+#pragma unroll
+    for (int t = 0; t < 16; ++t) {
+        const int e = min((int)threadIdx.x + t * kNarrowThreads, total - 1), y = (int)(((float)e + 0.5f) * per_line), x = e - y * line;
+        const long long r = M.turned ? j0 + y : y, c = M.turned ? x : j0 + x;   // (e below 2^13: the quotient's error stays below the half)
+        u[t] = (float)in[r * M.ld_in + c];
+        if (MUON) m[t] = mom[r * M.ld_mom + c];
+    }
+    __syncthreads();
+    double s = 0.0;
+#pragma unroll
+    for (int t = 0; t < 16; ++t) {
+        const int e = (int)threadIdx.x + t * kNarrowThreads, y = (int)(((float)e + 0.5f) * per_line), x = e - y * line;
+        if (e >= total) break;
+        if (MUON) {
+            m[t] = fmaf(up.mu, m[t], up.gscale * u[t]);
+            mom[(long long)(M.turned ? j0 + y : y) * M.ld_mom + (M.turned ? x : j0 + x)] = m[t];
+            u[t] = muon_u(up, u[t], m[t]);
+        }
+        s = fma((double)u[t], (double)u[t], s);
+        stage[M.turned ? x * pitch + y : y * pitch + x] = u[t];
+    }
+    s = block_sum<kNarrowThreads>(s, sh);
+    if (threadIdx.x == 0) ((Global<double>*)(a.ws + M.part))[(size_t)bat * M.parts + chunk] = s;
+    const int k = power_of(sqrt(s));
+    char* xt = a.ws + M.xt + ((size_t)bat * M.parts + chunk) * kNarrow * 4;
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+        const int q = threadIdx.x + t * kNarrowThreads, i = q & (mp - 1), j = q / mp * 8, groups = nc / 32;
+        float w[8], v[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) w[e] = ldexpf(stage[i * pitch + j + e], k);
+        store8(xr + plane_at(i, j, nc), w);
+        const int g = (q >> 5) / groups, i8 = g * 8, col = ((q >> 5) - g * groups) * 32 + (q & 31);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[e] = ldexpf(stage[(i8 + e) * pitch + col], k);
+        store8(xt + plane_at(col, i8, mp), v);
+    }
+    __syncthreads();
+    small_gram(xr, nc, small_tiles(mp), narrow_splits(mp), part);
+    __syncthreads();
+    narrow_share(part, mp, (Global<float>*)(a.ws + M.slab) + ((size_t)bat * M.parts + chunk) * small_tiles(mp) * 1024);
+}
+
+template <typename In, bool MUON>
+__global__ __launch_bounds__(kNarrowThreads) void ns_narrow_kernel(const NsArgs* args, NsFirst first, int k) {
+    extern __shared__ char smem[];
+    __shared__ double sh[kNarrowThreads / 64];
+    __shared__ NsScale sc[kNsSteps];
+    __shared__ float weight[kNarrowParts];
+    const NsArgs& a = *args;
+    char* const ws = (char*)args;   // (they lie at its start)
+    int local;
+    const NsMat M = a.mat[find(first, (int)blockIdx.x, local)];
+    const int C = M.parts, bat = local / C, chunk = local - bat * C, mp = M.mp, T = mp / 32, nc = kNarrow / mp, j0 = chunk * nc;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, r = lane & 31, h = lane >> 5, tiles = small_tiles(mp);
+    char *xr = smem, *xt = xr + kNarrow * 4, *A = xt + kNarrow * 4, *B = A + mp * mp * 4;
+    float* part = (float*)(B + mp * mp * 4);
+    char* B3 = (char*)part;
+    char* const xt_ws = ws + M.xt + ((size_t)bat * C + chunk) * kNarrow * 4;
+    const size_t half = (size_t)M.batch * C * tiles * 1024;   // floats of one of the two places of the shares
+    const Global<float>* shares = (const Global<float>*)(ws + M.slab) + (k & 1) * half + (size_t)bat * C * tiles * 1024;
+    const bool last = k + 1 == a.steps;
+    // X, and what the last step needs of the parameters, on their way
+    f32x4 x[4];
+#pragma unroll
+    for (int q = 0; q < 4; ++q) x[q] = ((const Global<f32x4>*)xt_ws)[threadIdx.x + q * kNarrowThreads];
+    const int bj = wave / T, bi = wave - bj * T, i = bi * 32 + 4 * h, j = j0 + bj * 32 + r;
+    const long long di = M.turned ? 1 : M.ld_out, at = M.turned ? (long long)j * M.ld_out + i : (long long)i * M.ld_out + j;
+    Global<float>* W = (Global<float>*)M.out + (size_t)bat * M.out_stride;
+    const float step = M.step, decay = a.decay;
+    float v[4][4], y[4][4];   // y: X by rows, or (last step) the parameters
+    if (MUON && last) {
+#pragma unroll
+        for (int q = 0; q < 4; ++q)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const int ic = min(i + 8 * q + e, M.m - 1), jc = min(j, M.n - 1);   // (beyond: not used)
+                y[q][e] = W[M.turned ? (long long)jc * M.ld_out + ic : (long long)ic * M.ld_out + jc];
+            }
+    }
+    double s = 0.0, mine = 0.0;
+    if ((int)threadIdx.x < C) s = mine = ((const Global<double>*)(ws + M.part))[(size_t)bat * C + threadIdx.x];
+    const double norm = sqrt(block_sum<kNarrowThreads>(s, sh));
+    const int k0 = power_of(norm);
+    // the first shares are in their columns' own powers of two (a share of nothing counts as nothing, whatever its power)
+    if ((int)threadIdx.x < C) weight[threadIdx.x] = k ? 1.f : mine > 0.0 ? ldexpf(1.f, k0 - power_of(sqrt(mine))) : 0.f;
+    if (threadIdx.x == 0) scales(a, norm, k0, k, sc);
+#pragma unroll
+    for (int q = 0; q < 4; ++q) ((f32x4*)xt)[threadIdx.x + q * kNarrowThreads] = x[q];
+    __syncthreads();
+    const NsScale z = sc[k];
+    if (tiles == 1) narrow_sum<1>(shares, weight, C, part);
+    else narrow_sum<3>(shares, weight, C, part);
+    __syncthreads();
+    if ((int)threadIdx.x < tiles * 128) {
+        float s[8];
+        small_sum(part, 1, s);
+        small_a(s, z, mp, A);
+    }
+    __syncthreads();
+    small_square(A, B, B3, a.step[k], z, mp);
+    __syncthreads();
+    const float f = z.sx / z.sb * (last ? 1.f : z.sx_next) * weight[chunk];
+    small_apply<false>(B, B3, xt, bi, bj, mp, f, v);
+    if (!last) small_apply<true>(B, B3, xt, bi, bj, mp, f, y);
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+        if (!last) {
+            store4(xt_ws + plane_at(j - j0, i + 8 * q, mp), v[q]);
+            store4(xr + plane_at(bi * 32 + r, bj * 32 + 8 * q + 4 * h, nc), y[q]);
+            continue;
+        }
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            if (i + 8 * q + e >= M.m || j >= M.n) continue;
+            if (MUON) W[at + (8 * q + e) * di] = fmaf(-step, v[q][e], decay * y[q][e]);
+            else ((Global<In>*)M.out)[(size_t)bat * M.out_stride + at + (8 * q + e) * di] = (In)v[q][e];
+        }
+    }
+    if (last) return;
+    __syncthreads();
+    small_gram(xr, nc, tiles, narrow_splits(mp), part);
+    __syncthreads();
+    narrow_share(part, mp, (Global<float>*)(ws + M.slab) + ((k + 1) & 1) * half + ((size_t)bat * C + chunk) * tiles * 1024);
 }
 
 // ------------------------------------------------------------------------------------------------ host side
@@ -895,21 +1113,30 @@ int ns_check(const dgg_matrix* mats, int count, const char* who) {
     return DGG_OK;
 }
 
-bool ns_small(const dgg_matrix& m) {
+enum { kSmall, kNarrowRoute, kGeneral, kRoutes };
+
+int ns_kind(const dgg_matrix& m) {
     const int lo = m.rows < m.cols ? m.rows : m.cols, hi = m.rows < m.cols ? m.cols : m.rows;
-    return lo <= 32 ? hi <= 512 : lo <= 64 && hi <= 192;
+    if (lo <= 32 ? hi <= 512 : lo <= 64 && hi <= 192) return kSmall;
+    return lo <= 64 && hi <= (lo <= 32 ? 16384 : 6144) ? kNarrowRoute : kGeneral;   // (64 and 48 workgroups)
 }
 
-// Whether a call's small matrices have a launch of their own: not where they find places in the launches that its other matrices
-// need anyway (30 x 2000, 100 x 2000 and 100 x 30: 129 us with a launch of its own for the last, 98 without).
-bool ns_apart(const dgg_matrix* mats, int count) {
-    int small = 0;
-    for (int i = 0; i < count; ++i) small += ns_small(mats[i]);
-    const int free = (kNsMats - (count - small) % kNsMats) % kNsMats;
-    return count == small || small > free;
-}
+// The route that each kind of a call's matrices takes: a route's launches work on up to 16 matrices, and those that another kind
+// needs anyway are shared where they have the places (30 x 2000, 100 x 2000 and 100 x 30: 129 us where the last had a launch of
+// its own, 98 together).
+struct NsRoutes {
+    int of[kRoutes];
+    NsRoutes(const dgg_matrix* mats, int count) {
+        int n[kRoutes] = {0, 0, 0};
+        for (int i = 0; i < count; ++i) ++n[ns_kind(mats[i])];
+        const auto free = [](int used) { return (kNsMats - used % kNsMats) % kNsMats; };
+        for (int r = 0; r < kRoutes; ++r) of[r] = r;
+        if (n[kSmall] <= free(n[kNarrowRoute])) of[kSmall] = kNarrowRoute;
+        if (n[kSmall] + n[kNarrowRoute] <= free(n[kGeneral])) of[kSmall] = of[kNarrowRoute] = kGeneral;
+    }
+};
 
-// What both routes need to know of one matrix.
+// What every route needs to know of one matrix.
 void ns_fill(const dgg_matrix& in, const NsArgs& a, int pad, NsMat& M) {
     M.in = in.in; M.out = in.out; M.mom = in.momentum;
     M.in_stride = in.in_stride; M.out_stride = in.out_stride; M.mom_stride = in.momentum_stride;
@@ -978,19 +1205,49 @@ void ns_plan(const dgg_matrix* const* mats, int count, NsArgs& a, NsPlan& P) {
     P.bytes = at;
 }
 
+// The same of the narrow route; returns its workgroups
+int ns_narrow_plan(const dgg_matrix* const* mats, int count, NsArgs& a, NsFirst& first, int& lds, size_t& bytes) {
+    size_t at = up(sizeof(NsArgs));   // (its device copy)
+    int grid = 0;
+    lds = 0;
+    for (int i = 0; i < kNsMats; ++i) first.at[i] = 0x7fffffff;
+    for (int i = 0; i < count; ++i) {
+        NsMat& M = a.mat[i];
+        ns_fill(*mats[i], a, 32, M);
+        M.parts = ceil_div(M.n, kNarrow / M.mp);
+        const size_t wgs = (size_t)M.batch * M.parts;
+        M.xt = at;   at = up(at + wgs * kNarrow * 4);
+        M.slab = at; at = up(at + wgs * 2 * small_tiles(M.mp) * 4096);
+        M.part = at; at = up(at + wgs * 8);
+        if (narrow_lds(M.mp) > lds) lds = narrow_lds(M.mp);
+        first.at[i] = grid;
+        grid += (int)wgs;
+    }
+    bytes = at;
+    return grid;
+}
+
 // up to kNsMats matrices of one route, from mats[at] on; at moves behind them
-int ns_group(const dgg_matrix* mats, int count, bool apart, bool small, int& at, const dgg_matrix** group) {
+int ns_group(const dgg_matrix* mats, int count, const NsRoutes& routes, int route, int& at, const dgg_matrix** group) {
     int n = 0;
     for (; at < count && n < kNsMats; ++at)
-        if ((apart && ns_small(mats[at])) == small) group[n++] = mats + at;
+        if (routes.of[ns_kind(mats[at])] == route) group[n++] = mats + at;
     return n;
 }
 
 int64_t ns_need(const dgg_matrix* mats, int count) {
     const dgg_matrix* group[kNsMats];
     size_t need = 256;
-    const bool apart = ns_apart(mats, count);
-    for (int at = 0, n; (n = ns_group(mats, count, apart, false, at, group)) > 0;) {
+    const NsRoutes routes(mats, count);
+    for (int at = 0, n; (n = ns_group(mats, count, routes, kNarrowRoute, at, group)) > 0;) {
+        NsArgs a = {};
+        NsFirst first;
+        size_t bytes;
+        int lds;
+        ns_narrow_plan(group, n, a, first, lds, bytes);
+        if (bytes > need) need = bytes;
+    }
+    for (int at = 0, n; (n = ns_group(mats, count, routes, kGeneral, at, group)) > 0;) {
         NsArgs a = {};
         NsPlan P;
         ns_plan(group, n, a, P);
@@ -1044,6 +1301,13 @@ bool ns_disjoint(const dgg_matrix* mats, int count, size_t size, bool muon) {
     return true;
 }
 
+// (more than 64 KB of LDS has to be asked for, on every device that launches)
+bool ns_lds(const void* kernel, int bytes, const char* who) {
+    const hipError_t e = hipFuncSetAttribute(kernel, hipFuncAttributeMaxDynamicSharedMemorySize, bytes);
+    if (e != hipSuccess) set_error(who, e);
+    return e == hipSuccess;
+}
+
 template <typename T, bool MUON>
 int ns_run(const dgg_matrix* mats, int count, NsArgs& a, const double* coef, int steps, void* ws, size_t ws_bytes,
            hipStream_t st, const char* who) {
@@ -1083,8 +1347,8 @@ int ns_run(const dgg_matrix* mats, int count, NsArgs& a, const double* coef, int
         set_error_text("%s: what is written overlaps itself or another operand", who);
         return DGG_ERR_INVALID;
     }
-    const bool apart = ns_apart(mats, count);
-    for (int at = 0, n; (n = ns_group(mats, count, apart, true, at, group)) > 0;) {
+    const NsRoutes routes(mats, count);
+    for (int at = 0, n; (n = ns_group(mats, count, routes, kSmall, at, group)) > 0;) {
         NsFirst first;
         int grid = 0, lds = 0;
         for (int i = 0; i < kNsMats; ++i) {
@@ -1096,15 +1360,20 @@ int ns_run(const dgg_matrix* mats, int count, NsArgs& a, const double* coef, int
             first.at[i] = grid;
             grid += a.mat[i].batch;
         }
-        // (more than 64 KB of LDS has to be asked for, on every device that launches)
-        const hipError_t e = hipFuncSetAttribute((const void*)ns_small_kernel<T, MUON>, hipFuncAttributeMaxDynamicSharedMemorySize, lds);
-        if (e != hipSuccess) {
-            set_error(who, e);
-            return DGG_ERR_LAUNCH;
-        }
+        if (!ns_lds((const void*)ns_small_kernel<T, MUON>, lds, who)) return DGG_ERR_LAUNCH;
         hipLaunchKernelGGL((ns_small_kernel<T, MUON>), dim3(grid), dim3(kSmallThreads), lds, st, a, first);
     }
-    for (int at = 0, n; (n = ns_group(mats, count, apart, false, at, group)) > 0;) {
+    for (int at = 0, n; (n = ns_group(mats, count, routes, kNarrowRoute, at, group)) > 0;) {
+        NsFirst first;
+        int lds;
+        size_t bytes;
+        const dim3 grid(ns_narrow_plan(group, n, a, first, lds, bytes)), block(kNarrowThreads);
+        if (!ns_lds((const void*)ns_narrow_first_kernel<T, MUON>, lds, who) || !ns_lds((const void*)ns_narrow_kernel<T, MUON>, lds, who))
+            return DGG_ERR_LAUNCH;
+        hipLaunchKernelGGL((ns_narrow_first_kernel<T, MUON>), grid, block, lds, st, a, first);
+        for (int k = 0; k < steps; ++k) hipLaunchKernelGGL((ns_narrow_kernel<T, MUON>), grid, block, lds, st, (const NsArgs*)ws, first, k);
+    }
+    for (int at = 0, n; (n = ns_group(mats, count, routes, kGeneral, at, group)) > 0;) {
         ns_plan(group, n, a, P);
         const dim3 block(kThreads);
         const NsArgs* args = (const NsArgs*)ws;

@@ -344,3 +344,79 @@ def test_layouts_that_share_a_buffer():
         with pytest.raises(_lib.DggError):
             call()
     assert bool((w == 1).all()) and not m.any()
+
+
+# short sides up to 64 beside long ones: on both sides of what one workgroup holds (512 and 192 columns, 256 and 128 of a longer one) and
+# of the longest
+NARROW = [(1, 513), (12, 700), (32, 512), (32, 513), (32, 769), (33, 193), (64, 1024), (64, 1025), (5000, 7), (4108, 64), (32, 16384),
+          (32, 16385), (64, 6144), (64, 6145)]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("shape", NARROW, ids=lambda s: "%dx%d" % s)
+def test_narrow_matrices(shape):
+    for dtype in (torch.float32, torch.bfloat16, torch.float16):
+        g = matrix(*shape, seed=sum(shape), dtype=dtype)
+        close(ops.orthogonalize(g.cuda()), g, dtype)
+    g = matrix(*shape, seed=7)
+    out = ops.orthogonalize(g.cuda(), 10, (1.0, 0.0, 0.0)).double().cpu()      # (test_operands_keep_22_bits)
+    ref = g.double() / (g.double().norm() + EPS)
+    assert bool(((out - ref).abs() <= 11 * 2.0 ** -23 * ref.abs() + 2.0 ** -38).all())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("shape", [(20, 900), (1500, 50)], ids=lambda s: "%dx%d" % s)
+def test_narrow_scales_and_special_values(shape):
+    g = matrix(*shape, seed=4)
+    for scale in (1e-4, 1e-12, 1e-16, 1e15, 1e30):
+        close(ops.orthogonalize((g * scale).cuda()), g * scale)
+    assert not ops.orthogonalize(torch.zeros(*shape, device="cuda")).any()
+    spike = torch.zeros(*shape)
+    spike[5, 7] = -3.0                                       # every other workgroup's columns are zero
+    close(ops.orthogonalize(spike.cuda()), spike)
+    uneven = g.clone()                                       # columns whose powers of two lie far apart
+    (uneven if shape[1] > shape[0] else uneven.t())[:, :300] *= 1e-18
+    close(ops.orthogonalize(uneven.cuda()), uneven)
+    close(ops.orthogonalize((g * 1e-30).cuda(), eps=0.0), g * 1e-30, eps=0.0)
+    stack = torch.stack([g, g, g, g])
+    stack[1, -1, -1] = float("nan")
+    stack[2, 0, 3] = float("inf")
+    out = ops.orthogonalize(stack.cuda())
+    one = ops.orthogonalize(g.cuda())
+    assert torch.equal(out[0], one) and torch.equal(out[3], one) and out[1].isnan().all() and out[2].isnan().all()
+    pitch = torch.full((shape[0], shape[1] + 9), 4.0, device="cuda")
+    pitch[:, 3:3 + shape[1]] = g.cuda()
+    assert torch.equal(ops.orthogonalize(pitch[:, 3:3 + shape[1]]), one)
+    for steps in (1, 2, 9):
+        close(ops.orthogonalize(g.cuda(), steps), g, steps=steps)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("shapes", [[(20, 900), (1000, 64), (12, 512), (3, 4)], [(33, 700)] * 18, [(40, 600), (100, 130), (5, 9)],
+                                    [(8, 30)] * 17 + [(30, 800)], [(8, 30)] * 17 + [(100, 200)]],
+                         ids=["narrow and small", "more than 16", "with general ones", "small apart", "small apart, general"])
+def test_muon_step_of_narrow_and_mixed_matrices(shapes):
+    lr, mu, wd = 0.02, 0.9, 0.1
+    ws = [matrix(*s, seed=i, kind="normal") for i, s in enumerate(shapes)]
+    gs = [matrix(*s, seed=50 + i) for i, s in enumerate(shapes)]
+    ms = [matrix(*s, seed=90 + i) for i, s in enumerate(shapes)]
+    wide = [torch.full((s[0], s[1] + 5), 4.0, device="cuda") for s in shapes]
+    dw = [t[:, 2:2 + s[1]].copy_(w) for t, s, w in zip(wide, shapes, ws)]
+    dg, dm = [t.cuda() for t in gs], [t.cuda() for t in ms]
+    graph, side = torch.cuda.CUDAGraph(), [(w.clone(), m.clone()) for w, m in zip(dw, dm)]
+    with torch.cuda.graph(graph):
+        ops.muon_step([w for w, _ in side], dg, [m for _, m in side], lr, mu, weight_decay=wd)
+    for k in range(3):
+        before = [(w.cpu(), m.cpu()) for w, m in zip(dw, dm)]
+        ops.muon_step(dw, dg, dm, lr, mu, weight_decay=wd)
+        graph.replay()
+        torch.cuda.synchronize()
+        for (w, m), g, nw, nm, (gw, gm), t in zip(before, gs, dw, dm, side, wide):
+            s = w.shape
+            rw, rm, tol = muon_reference(w, g, m, lr, mu, True, wd, math.sqrt(max(1.0, s[0] / s[1])), 1.0)
+            assert bool(((nm.cpu().double() - rm).abs() <= 3 * U * (m.double().abs() + g.double().abs() + rm.abs())).all())
+            err = (nw.cpu().double() - rw).abs()
+            assert float(err.norm()) <= 2 * tol + 4 * U * float(w.norm())
+            assert bool((err <= 40 * tol / math.sqrt(w.numel()) + 4 * U * (w.double().abs() + rw.abs())).all())
+            assert torch.equal(gw, nw) and torch.equal(gm, nm), k
+            assert bool((t[:, :2] == 4).all()) and bool((t[:, 2 + s[1]:] == 4).all())
