@@ -601,7 +601,7 @@ __global__ __launch_bounds__(kThreads, 2) void ns_apply_kernel(const NsArgs* arg
 
 // ------------------------------------------------------------------------------------------------ small matrices
 // A matrix whose planes fit the LDS of one workgroup (short side <= 32 and long side <= 512, or 64 and 192): the whole step in one
-// launch, 16 waves.  What bounds it is the chain of 5 barriers a step; the launches of the other route alone take 100 us.
+// launch, 16 waves.  What bounds it is the chain of 5 barriers a step: 12 x 512 33 us, 32 x 300 31 (general route: 86 and more).
 // The same planes in the same order and scales as there: A = X X^T in ranges of k that meet in LDS, A^2 and B X one 32 x 32 block a wave.
 // A short side of a few rows has short sums, and the planes' 22 bits are what its error consists of (12 x 512: 1.0 to 1.5e-6 of |X|
 // where fp32 products give 0.7 to 1.1e-6).  The matrix instructions are no bound here: lo lo is multiplied too, and B, whose error
@@ -819,9 +819,9 @@ __global__ __launch_bounds__(kSmallThreads) void ns_small_kernel(NsArgs a, NsFir
     const int bj = wave / T, bi = wave - bj * T, i = bi * 32 + 4 * h, j = bj * 32 + r;
     const long long di = M.turned ? 1 : M.ld_out, at = M.turned ? (long long)j * M.ld_out + i : (long long)i * M.ld_out + j;
     Global<float>* W = (Global<float>*)M.out + (size_t)bat * M.out_stride;
-    for (int k = 0; k < a.steps; ++k) {
+    const auto one = [&](int k, auto is_last) {   // (the last step apart: its addresses take registers)
+        constexpr bool last = decltype(is_last)::value;
         const NsScale z = sc[k];
-        const bool last = k + 1 == a.steps;
         float v[4][4], x[4][4];   // x: X by rows, or (last step) the parameters
         if (MUON && last) {   // (on their way during the step)
 #pragma unroll
@@ -864,7 +864,9 @@ __global__ __launch_bounds__(kSmallThreads) void ns_small_kernel(NsArgs a, NsFir
                 }
             }
         __syncthreads();
-    }
+    };
+    for (int k = 0; k + 1 < a.steps; ++k) one(k, std::false_type());
+    one(a.steps - 1, std::true_type());
 }
 
 // ------------------------------------------------------------------------------------------------ narrow matrices
