@@ -43,7 +43,7 @@ typedef __attribute__((address_space(3))) half8 lds_half8;
 
 constexpr int kNsMats = 16;      // matrices (stacks of them) per launch
 constexpr int kNsSteps = 16;
-constexpr int kNsParts = 256;    // partial sums of squares per matrix, at most
+constexpr int kNsParts = 1024;   // partial sums of squares per matrix, at most
 constexpr int kThreads = 256;
 
 struct NsMat {
