@@ -220,6 +220,8 @@ def _group_norm_args(who, x, num_groups, weight, bias, act):
     if act not in _ACTS:
         raise _lib.DggError("%s: act must be one of %s; got %r" % (who, sorted(_ACTS), act))
     c = x.shape[-1]
+    if c > 1 << 24:
+        raise _lib.DggError("%s: %d channels; 2^24 at most" % (who, c))
     if num_groups < 1 or c < 1 or c % num_groups:
         raise _lib.DggError("%s: %d groups do not divide %d channels" % (who, num_groups, c))
     for name, t in (("weight", weight), ("bias", bias)):
@@ -292,9 +294,9 @@ _ADJUST = {"spectral": _lib.MUON_SPECTRAL, "match_rms": _lib.MUON_MATCH_RMS}
 
 def _coefficients(who, steps, coefficients):
     """`coefficients`: one (a, b, c) for all steps or a sequence of `steps` of them -> a C array of doubles."""
-    rows = [coefficients] * steps if len(coefficients) == 3 and not hasattr(coefficients[0], "__len__") else list(coefficients)
-    if steps < 1 or len(rows) != steps or any(len(r) != 3 for r in rows):
-        raise _lib.DggError("%s: %d steps need one (a, b, c) or one for each step; got %r" % (who, steps, coefficients))
+    rows = [coefficients] * min(steps, 17) if len(coefficients) == 3 and not hasattr(coefficients[0], "__len__") else list(coefficients)
+    if not 1 <= steps <= 16 or len(rows) != steps or any(len(r) != 3 for r in rows):
+        raise _lib.DggError("%s: 1 to 16 steps and one (a, b, c) for all or for each; got %d, %r" % (who, steps, coefficients))
     return (C.c_double * (3 * steps))(*[float(v) for r in rows for v in r])
 
 
@@ -302,9 +304,11 @@ def _matrix_rows(t):
     """A matrix or a stack (B, rows, cols) whose rows are contiguous, as (tensor, batch, rows, cols, pitch, stride)."""
     *stack, r, c = t.shape
     b = stack[0] if stack else 1
+    if max(r, c) > 1 << 20:
+        raise _lib.DggError("matrices of up to 2^20 rows and columns; got %s" % (tuple(t.shape),))
     if t.is_contiguous():
         return t, b, r, c, c, r * c
-    if t.stride(-1) != 1 and c > 1 or r > 1 and t.stride(-2) < c:
+    if t.stride(-1) != 1 and c > 1 or r > 1 and not c <= t.stride(-2) < 1 << 31:
         t = t.detach().contiguous()
     return t, b, r, c, (t.stride(-2) if r > 1 else c), (t.stride(0) if t.dim() == 3 and b > 1 else r * c)
 

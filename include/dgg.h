@@ -160,7 +160,7 @@ int dgg_resblock_backward(int fin, const float* params, float* grads, void* ws, 
  * copy); types DGG_F32 / DGG_BF16 / DGG_F16 for x, y, dy, dx alike, weight / bias (C, NULL = 1 / 0) and their gradients fp32:
  *   mean, var over the S x C/groups elements of sample n and group g;  z = weight * (x - mean) / sqrt(var + eps) + bias;
  *   y = act(z): DGG_ACT_NONE, DGG_ACT_LEAKY_RELU (`slope` for z <= 0) or DGG_ACT_SILU (z * sigmoid(z)).
- * y and dx are contiguous (N, S, C).  Statistics and z are 64-bit inside: the side of LeakyReLU's kink an element takes is the
+ * y and dx are contiguous (N, S, C) and overlap no input.  Statistics and z are 64-bit inside: the side of LeakyReLU's kink an element takes is the
  * exact one.  stats (N, groups, 2) doubles = (mean, 1 / sqrt(var + eps)): written by the forward if non-NULL, read by the
  * backward; dweight / dbias: both or none.  N * groups < 2^31, S < 2^31, C <= 2^24; N, S >= 1.  ws (8-byte aligned) of
  * dgg_group_norm_workspace_bytes(.., backward) bytes; results do not depend on the order in which workgroups run. */

@@ -266,3 +266,45 @@ def test_refusals():
                  lambda: ops.group_norm_act_backward(x, x, 4, w, w, 1e-5, "silu", 0.2, st)):
         with pytest.raises(_lib.DggError):
             call()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=["f32", "bf16"])
+@pytest.mark.parametrize("shape", [(1100, 3, 20, 5), (33000, 2, 6, 2), (1030, 8200, 1, 1), (1, 16384, 64, 1), (3, 128, 4, 4), (3, 129, 4, 4),
+                                   (40, 16, 1024, 2)], ids=lambda s: "x".join(map(str, s)))
+def test_many_samples_and_long_ones(shape, dtype):
+    """More samples than one sum of the parameters' gradients takes; samples whose partial sums a wide workgroup merges."""
+    *xs, groups = shape
+    check(*data(tuple(xs), dtype, 5)[:2], groups, *data(tuple(xs), dtype, 5)[2:])
+
+
+@pytest.mark.gpu
+def test_offsets_beyond_32_bits():
+    """Samples or points 2^31 elements apart, and tensors of more than 2^32 elements, against the same data close together."""
+    far = torch.empty((1 << 32) + (1 << 16), dtype=torch.bfloat16, device="cuda")
+    for n, s, strides in ((3, 40, (1 << 31, 64, 1)), (1, 3, (64, 1 << 31, 1)), (3, 1, (1 << 31, 64, 1))):
+        x, dy, w, b = (t.cuda() for t in data((n, s, 64), torch.bfloat16, 8))
+        xf = far.as_strided((n, s, 64), strides)
+        xf.copy_(x)
+        y, st = ops.group_norm_act_forward(x, 8, w, b)
+        yf, sf = ops.group_norm_act_forward(xf, 8, w, b)
+        assert torch.equal(y, yf) and torch.equal(st, sf)
+        for a, c in zip(ops.group_norm_act_backward(dy, x, 8, w, b, 1e-5, "leaky_relu", 0.2, st),
+                        ops.group_norm_act_backward(dy, xf, 8, w, b, 1e-5, "leaky_relu", 0.2, st)):
+            assert torch.equal(a, c)
+    for s in (1, 4):
+        n = ((1 << 32) // 1024 + 64) // s
+        x = far[:n * s * 1024].view(n, s, 1024)
+        ends = torch.cat([x[:3], x[-3:]])
+        ends.copy_(data((6, s, 1024), torch.bfloat16, 9)[0])
+        x[:3].copy_(ends[:3])
+        x[-3:].copy_(ends[3:])
+        y, st = ops.group_norm_act_forward(x, 16)
+        small, st_small = ops.group_norm_act_forward(ends, 16)
+        assert torch.equal(y[:3], small[:3]) and torch.equal(y[-3:], small[3:]) and torch.equal(st[-3:], st_small[3:])
+        dx, _, _ = ops.group_norm_act_backward(x, x, 16, None, None, 1e-5, "leaky_relu", 0.2, st, param_grads=False)
+        dx_small, _, _ = ops.group_norm_act_backward(ends, ends, 16, None, None, 1e-5, "leaky_relu", 0.2, st_small, param_grads=False)
+        assert torch.equal(dx[:3], dx_small[:3]) and torch.equal(dx[-3:], dx_small[3:])
+        del y, dx
+    del far
+    torch.cuda.empty_cache()

@@ -420,3 +420,38 @@ def test_muon_step_of_narrow_and_mixed_matrices(shapes):
             assert bool((err <= 40 * tol / math.sqrt(w.numel()) + 4 * U * (w.double().abs() + rw.abs())).all())
             assert torch.equal(gw, nw) and torch.equal(gm, nm), k
             assert bool((t[:, :2] == 4).all()) and bool((t[:, 2 + s[1]:] == 4).all())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("shape", [(1600, 1700), (1100, 700), (66, 20000)], ids=lambda s: "%dx%d" % s)
+def test_large_matrices(shape):
+    g = matrix(*shape, seed=3)
+    close(ops.orthogonalize(g.cuda()), g)
+
+
+@pytest.mark.gpu
+def test_offsets_beyond_32_bits():
+    """Matrices 2^31 elements apart; rows further apart than a pitch may be are copied, or refused where they are written."""
+    far = torch.empty((1 << 32) + (1 << 17), dtype=torch.float32, device="cuda")
+    for shape in ((20, 30), (40, 700), (70, 200)):
+        g = torch.stack([matrix(*shape, seed=s) for s in range(3)]).cuda()
+        view = far.as_strided(g.shape, (1 << 31, shape[1], 1))
+        view.copy_(g)
+        assert torch.equal(ops.orthogonalize(view), ops.orthogonalize(g))
+        w, m = torch.ones_like(g), torch.zeros_like(g)
+        ops.muon_step([w], [g], [m], 0.1)
+        view.fill_(1.0)
+        fm = torch.zeros_like(g)
+        ops.muon_step([view], [g], [fm], 0.1)
+        assert torch.equal(view, w) and torch.equal(fm, m)
+    rows = far.as_strided((3, 50), (1 << 31, 1))
+    rows.copy_(g[0, :3, :50])
+    assert torch.equal(ops.orthogonalize(rows), ops.orthogonalize(g[0, :3, :50].contiguous()))
+    with pytest.raises(_lib.DggError):
+        ops.muon_step([rows], [g[0, :3, :50]], [torch.zeros(3, 50, device="cuda")], 0.1)
+    with pytest.raises(_lib.DggError):
+        ops.orthogonalize(far[:(1 << 32) + 5].view(1, -1))
+    with pytest.raises(_lib.DggError):
+        ops.orthogonalize(g, 1 << 33)
+    del far, view, rows
+    torch.cuda.empty_cache()
