@@ -4,7 +4,7 @@ here: every function is one or two library calls on the current HIP stream."""
 from __future__ import annotations
 
 import ctypes as C
-from contextlib import nullcontext
+import functools
 
 import torch
 
@@ -183,9 +183,12 @@ def _stream(dev):
     return torch._C._cuda_getCurrentRawStream(dev.index)
 
 
-def _on(dev):
-    """The context in which kernels for `dev` are launched: launches go to the current device."""
-    return torch.cuda.device(dev) if dev.index is not None and dev.index != torch.cuda.current_device() else nullcontext()
+def _launch(dev, call, *args):
+    """call(*args) with `dev` the current device: launches go there."""
+    if dev.index == torch._C._cuda_getDevice():
+        return call(*args)
+    with torch.cuda.device(dev):
+        return call(*args)
 
 
 def _ptr(t):
@@ -224,18 +227,19 @@ def _group_norm_args(who, x, num_groups, weight, bias, act):
         raise _lib.DggError("%s: %d channels; 2^24 at most" % (who, c))
     if num_groups < 1 or c < 1 or c % num_groups:
         raise _lib.DggError("%s: %d groups do not divide %d channels" % (who, num_groups, c))
-    for name, t in (("weight", weight), ("bias", bias)):
-        if t is not None and (t.device != dev or t.dtype != torch.float32 or t.shape != (c,)):
+    for t in (weight, bias):
+        if t is not None and (t.dtype != torch.float32 or t.shape != (c,) or t.device != dev):
             raise _lib.DggError("%s: %s must be a float32 (%d,) tensor on %s; got %s %s on %s"
-                                % (who, name, c, dev, t.dtype, tuple(t.shape), t.device))
+                                % (who, "weight" if t is weight else "bias", c, dev, t.dtype, tuple(t.shape), t.device))
     return dev, (None if weight is None else weight.contiguous()), (None if bias is None else bias.contiguous())
 
 
-def _group_norm_ws(n, s, c, g, dtype, backward, dev):
+@functools.lru_cache(maxsize=4096)
+def _group_norm_bytes(n, s, c, g, dtype, backward):
     nb = lib().dgg_group_norm_workspace_bytes(n, s, c, g, dtype, backward)
     if nb < 0:
         check(nb, "dgg_group_norm_workspace_bytes")
-    return _lib.new_workspace(nb, dev) if nb else None, nb
+    return nb
 
 
 def group_norm_act_forward(x, num_groups, weight=None, bias=None, eps=1e-5, act="leaky_relu", slope=0.2):
@@ -251,11 +255,10 @@ def group_norm_act_forward(x, num_groups, weight=None, bias=None, eps=1e-5, act=
         return y, stats.zero_()
     x, n, s, c, sn, ss = _rows(x)
     dt = _DTYPES[x.dtype]
-    with _on(dev):
-        ws, nb = _group_norm_ws(n, s, c, num_groups, dt, 0, dev)
-        check(lib().dgg_group_norm_act_forward(x.data_ptr(), sn, ss, n, s, c, num_groups, _ptr(weight), _ptr(bias), eps,
-                                               _ACTS[act], slope, dt, y.data_ptr(), stats.data_ptr(), _ptr(ws), nb,
-                                               _stream(dev)), "dgg_group_norm_act_forward")
+    nb = _group_norm_bytes(n, s, c, num_groups, dt, 0)
+    ws = _lib.new_workspace(nb, dev) if nb else None
+    check(_launch(dev, lib().dgg_group_norm_act_forward, x.data_ptr(), sn, ss, n, s, c, num_groups, _ptr(weight), _ptr(bias), eps,
+                  _ACTS[act], slope, dt, y.data_ptr(), stats.data_ptr(), _ptr(ws), nb, _stream(dev)), "dgg_group_norm_act_forward")
     return y, stats
 
 
@@ -273,17 +276,18 @@ def group_norm_act_backward(dy, x, num_groups, weight, bias, eps, act, slope, st
     dx = _like(x)
     dw = db = None
     if param_grads:
-        dw, db = x.new_empty((c,), dtype=torch.float32), x.new_empty((c,), dtype=torch.float32)
+        dw = x.new_empty((c,), dtype=torch.float32) if weight is None else torch.empty_like(weight)
+        db = x.new_empty((c,), dtype=torch.float32) if bias is None else torch.empty_like(bias)
     if x.numel() == 0:
         return dx, (dw.zero_() if param_grads else None), (db.zero_() if param_grads else None)
     x, n, s, c, sn, ss = _rows(x)
     dy, _, _, _, dsn, dss = _rows(dy)
     dt = _DTYPES[x.dtype]
-    with _on(dev):
-        ws, nb = _group_norm_ws(n, s, c, num_groups, dt, 1, dev)
-        check(lib().dgg_group_norm_act_backward(dy.data_ptr(), dsn, dss, x.data_ptr(), sn, ss, n, s, c, num_groups, _ptr(weight),
-                                                _ptr(bias), _ACTS[act], slope, dt, stats.data_ptr(), dx.data_ptr(), _ptr(dw),
-                                                _ptr(db), _ptr(ws), nb, _stream(dev)), "dgg_group_norm_act_backward")
+    nb = _group_norm_bytes(n, s, c, num_groups, dt, 1)
+    ws = _lib.new_workspace(nb, dev) if nb else None
+    check(_launch(dev, lib().dgg_group_norm_act_backward, dy.data_ptr(), dsn, dss, x.data_ptr(), sn, ss, n, s, c, num_groups,
+                  _ptr(weight), _ptr(bias), _ACTS[act], slope, dt, stats.data_ptr(), dx.data_ptr(), _ptr(dw), _ptr(db), _ptr(ws), nb,
+                  _stream(dev)), "dgg_group_norm_act_backward")
     return dx, dw, db
 
 
@@ -339,10 +343,9 @@ def orthogonalize(grad, steps=5, coefficients=NS_COEFFICIENTS, eps=1e-7):
         dev = grads[0].device
         mats = (_lib.Matrix * len(work))(*[_lib.Matrix(t.data_ptr(), o.data_ptr(), None, b, st, r * c, 0, r, c, ld, c, 0, 0)
                                            for (t, b, r, c, ld, st), o in work])
-        with _on(dev):
-            ws, nb = _ns_workspace(mats, len(work), dev)
-            check(lib().dgg_orthogonalize(mats, len(work), _DTYPES[grads[0].dtype], coef, steps, eps, ws.data_ptr(), nb,
-                                          _stream(dev)), "dgg_orthogonalize")
+        ws, nb = _ns_workspace(mats, len(work), dev)
+        check(_launch(dev, lib().dgg_orthogonalize, mats, len(work), _DTYPES[grads[0].dtype], coef, steps, eps, ws.data_ptr(), nb,
+                      _stream(dev)), "dgg_orthogonalize")
     return outs[0] if single else outs
 
 
@@ -376,10 +379,9 @@ def muon_step(params, grads, momentum, lr, mu=0.95, nesterov=True, weight_decay=
     if mats:
         n = len(mats)
         mats = (_lib.Matrix * n)(*mats)
-        with _on(dev):
-            ws, nb = _ns_workspace(mats, n, dev)
-            check(lib().dgg_muon_step(mats, n, lr, mu, int(nesterov), weight_decay, _ADJUST[adjust], grad_scale, coef, steps, eps,
-                                      ws.data_ptr(), nb, _stream(dev)), "dgg_muon_step")
+        ws, nb = _ns_workspace(mats, n, dev)
+        check(_launch(dev, lib().dgg_muon_step, mats, n, lr, mu, int(nesterov), weight_decay, _ADJUST[adjust], grad_scale, coef, steps,
+                      eps, ws.data_ptr(), nb, _stream(dev)), "dgg_muon_step")
 
 
 # ------------------------------------------------------------------------------------------ small ops
