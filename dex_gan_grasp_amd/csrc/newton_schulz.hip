@@ -18,7 +18,7 @@
 // Layout.  All products are C[i][j] = sum_k P[i][k] Q[j][k] with k contiguous in both operands: A = X X^T from X stored by rows,
 // A^2 from A (symmetric), B X from B and X stored by columns.  So X is kept in both layouts.  Planes lie in the order in which the
 // matrix instruction reads them (plane_at): a product's operands go through LDS as they are, and an epilogue's lanes write 512 bytes
-// in a row.  Both sizes are padded to multiples of 64 with zeros, which stay zeros in every product.
+// in a row.  Both sizes are padded to multiples of 32 with zeros, which stay zeros in every product.
 #include <math.h>
 
 #include <algorithm>
@@ -232,7 +232,7 @@ __global__ __launch_bounds__(kThreads) void ns_split_kernel(const NsArgs* args, 
     __shared__ float t[64][65];   // [i][j] of X
     int local;
     const NsMat M = a.mat[find(first, (int)blockIdx.x, local)];
-    const int ti = M.mp / 64, tj = M.np / 64;
+    const int ti = (M.mp + 63) / 64, tj = (M.np + 63) / 64;
     const int bat = local / (ti * tj), tile = local - bat * ti * tj, i0 = tile / tj * 64, j0 = tile % tj * 64;
     const Global<T>* in = (const Global<T>*)M.in + (size_t)bat * M.in_stride;
     const Global<float>* mom = MUON ? (Global<float>*)M.mom + (size_t)bat * M.mom_stride : nullptr;
@@ -271,8 +271,8 @@ __global__ __launch_bounds__(kThreads) void ns_split_kernel(const NsArgs* args, 
             v[e] = t[row][k8 + e];
             w[e] = t[k8 + e][row];
         }
-        store8(xr + plane_at(i0 + row, j0 + k8, M.np), v);
-        store8(xt + plane_at(j0 + row, i0 + k8, M.mp), w);
+        if (i0 + row < M.mp && j0 + k8 < M.np) store8(xr + plane_at(i0 + row, j0 + k8, M.np), v);
+        if (j0 + row < M.np && i0 + k8 < M.mp) store8(xt + plane_at(j0 + row, i0 + k8, M.mp), w);
     }
 }
 
@@ -420,13 +420,14 @@ __global__ __launch_bounds__(kThreads) void ns_gram_kernel(const NsArgs* args, N
     char* const ws = (char*)args;   // (they lie at its start)
     int local;
     const NsMat M = a.mat[find(first, by_die(), local)];
-    const int t = M.mp / Pr::kTile, tiles = t * (t + 1) / 2, per = tiles * M.splits;
+    const int t = (M.mp + Pr::kTile - 1) / Pr::kTile, tiles = t * (t + 1) / 2, per = tiles * M.splits;
     const int bat = local / per, rest = local - bat * per, split = rest / tiles;
     int ti, tj;
     upper(rest - split * tiles, t, ti, tj);
     const char* x = ws + M.xr + (size_t)bat * plane_bytes(M.mp, M.np);
     Pr p;
     p.run(x, ti * Pr::kTile, M.mp, x, tj * Pr::kTile, M.mp, M.np, split * M.kblocks, min((split + 1) * M.kblocks, M.np / 32));
+    if (ti * Pr::kTile + p.i0() >= M.mp || tj * Pr::kTile + p.j0() >= M.mp) return;   // (the same for all of a wave: sizes are multiples of 32)
     if (M.splits == 1) {   // all of k: A itself, and its mirror image
         const NsScale z = scale_of(ws, M, bat, k);
         char* A = ws + M.a + (size_t)bat * plane_bytes(M.mp, M.mp);
@@ -498,20 +499,22 @@ __global__ __launch_bounds__(kThreads) void ns_square_kernel(const NsArgs* args,
     char* const ws = (char*)args;   // (they lie at its start)
     int local;
     const NsMat M = a.mat[find(first, by_die(), local)];
-    const int t = M.mp / Pr::kTile, tiles = t * (t + 1) / 2, bat = local / tiles;
+    const int t = (M.mp + Pr::kTile - 1) / Pr::kTile, tiles = t * (t + 1) / 2, bat = local / tiles;
     int ti, tj;
     upper(local - bat * tiles, t, ti, tj);
     const char* A = ws + M.a + (size_t)bat * plane_bytes(M.mp, M.mp);
     char* B = ws + M.b + (size_t)bat * plane_bytes(M.mp, M.mp);
     Pr p;
     const int i0 = ti * Pr::kTile, j0 = tj * Pr::kTile, i = i0 + p.i0(), j = j0 + p.j0();
-    const size_t at = plane_at(j, i, M.mp);   // row j, k = i: A and B are symmetric
+    const bool on = i < M.mp && j < M.mp;   // (the same for all of a wave)
+    const size_t at = on ? plane_at(j, i, M.mp) : 0;   // row j, k = i: A and B are symmetric
     float v[4][4];
 #pragma unroll
     for (int q = 0; q < 4; ++q) load4(A + at + (q >> 1) * 2048 + (q & 1) * 512, v[q]);
     const NsScale z = scale_of(ws, M, bat, k);
     const float ratio = z.sb / z.sa, fa = a.step[k].a * z.sb, fb = a.step[k].b * ratio, fc = a.step[k].c * ratio / z.sa;
     p.run(A, i0, M.mp, A, j0, M.mp, M.mp, 0, M.mp / 32);
+    if (!on) return;
 #pragma unroll
     for (int q = 0; q < 4; ++q) {
 #pragma unroll
@@ -555,7 +558,7 @@ __global__ __launch_bounds__(kThreads, 2) void ns_apply_kernel(const NsArgs* arg
 #pragma unroll
         for (int g = 0; g < F; ++g) {
             const int i = i0 + p.i0() + 32 * f, j = j0 + p.j0() + 32 * g;
-            if (i >= M.mp || j >= M.np) continue;   // (the same for all of a wave: sizes are multiples of 64)
+            if (i >= M.mp || j >= M.np) continue;   // (the same for all of a wave)
             float v[4][4];
 #pragma unroll
             for (int q = 0; q < 4; ++q)
@@ -1139,7 +1142,7 @@ struct NsRoutes {
 };
 
 // What every route needs to know of one matrix.
-void ns_fill(const dgg_matrix& in, const NsArgs& a, int pad, NsMat& M) {
+void ns_fill(const dgg_matrix& in, const NsArgs& a, NsMat& M) {
     M.in = in.in; M.out = in.out; M.mom = in.momentum;
     M.in_stride = in.in_stride; M.out_stride = in.out_stride; M.mom_stride = in.momentum_stride;
     M.ld_in = in.ld_in; M.ld_out = in.ld_out; M.ld_mom = in.ld_momentum;
@@ -1147,8 +1150,8 @@ void ns_fill(const dgg_matrix& in, const NsArgs& a, int pad, NsMat& M) {
     M.turned = in.rows > in.cols;
     M.m = M.turned ? in.cols : in.rows;
     M.n = M.turned ? in.rows : in.cols;
-    M.mp = ceil_div(M.m, pad) * pad;
-    M.np = ceil_div(M.n, pad) * pad;
+    M.mp = ceil_div(M.m, 32) * 32;
+    M.np = ceil_div(M.n, 32) * 32;
     const double f = a.adjust == DGG_MUON_SPECTRAL ? sqrt(fmax(1.0, (double)in.rows / in.cols)) : 0.2 * sqrt((double)M.n);
     M.step = (float)(a.lr * f);
 }
@@ -1175,10 +1178,10 @@ void ns_plan(const dgg_matrix* const* mats, int count, NsArgs& a, NsPlan& P) {
     for (int i = 0; i < count; ++i) {
         const dgg_matrix& in = *mats[i];
         NsMat& M = a.mat[i];
-        ns_fill(in, a, 64, M);
+        ns_fill(in, a, M);
         M.parts = ceil_div((long long)M.m * M.n, kThreads * 16);
         if (M.parts > kNsParts) M.parts = kNsParts;
-        const int t = M.mp / 64, tiles = t * (t + 1) / 2;
+        const int t = ceil_div(M.mp, 64), tiles = t * (t + 1) / 2;
         // two workgroups a CU share the k of A = X X^T, 256 k or more each (192 .. 768 workgroups: 26.8, 21.8 (256), 19.6 (512), 19.0 us
         // for the generator's matrices, 10.8 .. 11.6 for 512 x 4620; 128 x 128 tiles: 18.9 and 11.6)
         int splits = ceil_div(512, (long long)tiles * M.batch);
@@ -1197,7 +1200,7 @@ void ns_plan(const dgg_matrix* const* mats, int count, NsArgs& a, NsPlan& P) {
         M.part = at; at = up(at + b * M.parts * 8);
         M.scal = at; at = up(at + b * kNsSteps * sizeof(NsScale));
         const int n32 = M.mp / 32;
-        const int blocks[kPhases] = {M.parts, t * (M.np / 64), tiles * M.splits, M.splits > 1 ? n32 * (n32 + 1) / 2 : 0, tiles,
+        const int blocks[kPhases] = {M.parts, t * ceil_div(M.np, 64), tiles * M.splits, M.splits > 1 ? n32 * (n32 + 1) / 2 : 0, tiles,
                                        ceil_div(M.mp, 64 * P.f_apply) * ceil_div(M.np, 64 * P.f_apply)};
         for (int k = 0; k < kPhases; ++k) {
             P.first[k].at[i] = P.grid[k];
@@ -1215,7 +1218,7 @@ int ns_narrow_plan(const dgg_matrix* const* mats, int count, NsArgs& a, NsFirst&
     for (int i = 0; i < kNsMats; ++i) first.at[i] = 0x7fffffff;
     for (int i = 0; i < count; ++i) {
         NsMat& M = a.mat[i];
-        ns_fill(*mats[i], a, 32, M);
+        ns_fill(*mats[i], a, M);
         M.parts = ceil_div(M.n, kNarrow / M.mp);
         const size_t wgs = (size_t)M.batch * M.parts;
         M.xt = at;   at = up(at + wgs * kNarrow * 4);
@@ -1356,7 +1359,7 @@ int ns_run(const dgg_matrix* mats, int count, NsArgs& a, const double* coef, int
         for (int i = 0; i < kNsMats; ++i) {
             first.at[i] = 0x7fffffff;
             if (i >= n) continue;
-            ns_fill(*group[i], a, 32, a.mat[i]);
+            ns_fill(*group[i], a, a.mat[i]);
             const int bytes = small_lds(a.mat[i].mp, a.mat[i].np);
             if (bytes > lds) lds = bytes;
             first.at[i] = grid;
