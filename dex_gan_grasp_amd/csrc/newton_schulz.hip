@@ -1306,7 +1306,8 @@ bool ns_disjoint(const dgg_matrix* mats, int count, size_t size, bool muon) {
     return true;
 }
 
-// (more than 64 KB of LDS has to be asked for, on every device that launches)
+// More than 64 KB of LDS has to be asked for, on every device that launches: always the most a kernel may need, so that another
+// thread's call does not lower it in between.
 bool ns_lds(const void* kernel, int bytes, const char* who) {
     const hipError_t e = hipFuncSetAttribute(kernel, hipFuncAttributeMaxDynamicSharedMemorySize, bytes);
     if (e != hipSuccess) set_error(who, e);
@@ -1365,7 +1366,7 @@ int ns_run(const dgg_matrix* mats, int count, NsArgs& a, const double* coef, int
             first.at[i] = grid;
             grid += a.mat[i].batch;
         }
-        if (!ns_lds((const void*)ns_small_kernel<T, MUON>, lds, who)) return DGG_ERR_LAUNCH;
+        if (!ns_lds((const void*)ns_small_kernel<T, MUON>, small_lds(64, 192), who)) return DGG_ERR_LAUNCH;
         hipLaunchKernelGGL((ns_small_kernel<T, MUON>), dim3(grid), dim3(kSmallThreads), lds, st, a, first);
     }
     for (int at = 0, n; (n = ns_group(mats, count, routes, kNarrowRoute, at, group)) > 0;) {
@@ -1373,7 +1374,8 @@ int ns_run(const dgg_matrix* mats, int count, NsArgs& a, const double* coef, int
         int lds;
         size_t bytes;
         const dim3 grid(ns_narrow_plan(group, n, a, first, lds, bytes)), block(kNarrowThreads);
-        if (!ns_lds((const void*)ns_narrow_first_kernel<T, MUON>, lds, who) || !ns_lds((const void*)ns_narrow_kernel<T, MUON>, lds, who))
+        if (!ns_lds((const void*)ns_narrow_first_kernel<T, MUON>, narrow_lds(64), who) ||
+            !ns_lds((const void*)ns_narrow_kernel<T, MUON>, narrow_lds(64), who))
             return DGG_ERR_LAUNCH;
         hipLaunchKernelGGL((ns_narrow_first_kernel<T, MUON>), grid, block, lds, st, a, first);
         for (int k = 0; k < steps; ++k) hipLaunchKernelGGL((ns_narrow_kernel<T, MUON>), grid, block, lds, st, (const NsArgs*)ws, first, k);

@@ -349,3 +349,40 @@ def test_a_captured_block_step():
         torch.cuda.synchronize()
         for a, b in zip([mine[0], mine[1], mine[2].weight, mine[2].bias] + mine[3], [eager[0], eager[1], eager[2].weight, eager[2].bias] + eager[3]):
             assert torch.equal(a, b), k
+
+
+@pytest.mark.gpu
+def test_calls_from_several_threads_at_once():
+    """Each thread on a stream of its own, all routes of both operators: every result as on one stream."""
+    import threading
+    shapes = [(20, 30), (64, 190), (20, 900), (64, 1300), (100, 200), (200, 300)]
+    gs = [TO.matrix(*s, seed=i).cuda() for i, s in enumerate(shapes)]
+    xs = [(TG.data((n, s, c), torch.float32, 3)[0].cuda(), g) for n, s, c, g in ((64, 1, 512, 32), (4, 300, 64, 8), (2, 9000, 4, 1))]
+    want = [ops.orthogonalize(g) for g in gs], [ops.group_norm_act_forward(x, g) for x, g in xs]
+    back = [ops.group_norm_act_backward(x, x, g, None, None, 1e-5, "leaky_relu", 0.2, y[1]) for (x, g), y in zip(xs, want[1])]
+    torch.cuda.synchronize()
+    bad = []
+
+    def run(turn):
+        try:
+            stream = torch.cuda.Stream()
+            with torch.cuda.stream(stream):
+                for k in range(6):
+                    order = [(turn + k + i) % len(gs) for i in range(len(gs))]
+                    got = {i: ops.orthogonalize(gs[i]) for i in order}
+                    for (x, g), (y, st), b in zip(xs, want[1], back):
+                        gy, gst = ops.group_norm_act_forward(x, g)
+                        gb = ops.group_norm_act_backward(x, x, g, None, None, 1e-5, "leaky_relu", 0.2, gst)
+                        if not (torch.equal(gy, y) and torch.equal(gst, st) and all(torch.equal(p, q) for p, q in zip(gb, b))):
+                            bad.append(("group norm", turn, k, tuple(x.shape)))
+                    bad.extend(("orthogonalize", turn, k, shapes[i]) for i, o in got.items() if not torch.equal(o, want[0][i]))
+        except Exception as e:
+            bad.append((turn, repr(e)))
+
+    threads = [threading.Thread(target=run, args=(t,)) for t in range(4)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    torch.cuda.synchronize()
+    assert not bad, bad[:5]
