@@ -22,7 +22,6 @@
 //    it walks down the rows), leaves per-channel partial sums in the workspace, and a small launch merges them in a fixed
 //    order into the groups' statistics (and dw, db); a last launch applies them.  No atomics: results do not depend on the
 //    order in which workgroups run.
-#include <initializer_list>
 #include <type_traits>
 
 #include "dgg_internal.h"
@@ -34,7 +33,11 @@ constexpr int kGnThreads = 256;
 constexpr int kMergeThreads = 1024;
 constexpr int kUnitItems = 8;   // vectors of a group one lane holds, at most
 
-template <typename T, int V> struct alignas(sizeof(T) * V) Vec { T e[V]; };
+// V elements of memory, one access at any address that an element may have (global memory is accessed unaligned): rows of any pitch
+template <typename T, int V> struct Vec { T e[V]; };
+template <int N> struct Bits { typedef uint32_t Type __attribute__((ext_vector_type(N / 4))); };
+template <> struct Bits<4> { typedef uint32_t Type; };
+template <> struct Bits<2> { typedef uint16_t Type; };
 
 template <typename T, int V> __device__ __forceinline__ void load_vec(const T* p, float (&v)[V]) {
     const Vec<T, V> r = *reinterpret_cast<const Vec<T, V>*>(p);
@@ -47,6 +50,14 @@ template <typename T, int V> __device__ __forceinline__ void store_vec(T* p, con
     for (int i = 0; i < V; ++i) r.e[i] = (T)v[i];   // the one rounding to the output type (nearest even)
     *reinterpret_cast<Vec<T, V>*>(p) = r;
 }
+
+// Vector v of a group of `width` >= V channels: its first channel, and how many of its elements belong to the vector before it.  EVEN: V
+// divides the width; else the last vector ends with the group, and what it shares with the one before is the same in both.
+template <int V, bool EVEN> struct Span {
+    int at, skip;
+    __device__ __forceinline__ Span(int v, int width) : at(EVEN ? v * V : min(v * V, width - V)), skip(EVEN ? 0 : v * V - at) {}
+};
+__host__ __device__ __forceinline__ int vectors(int width, int V) { return (width + V - 1) / V; }
 
 // 1 / (1 + exp(-z)) by the hardware's exp2 and reciprocal (1 unit in the last place each).  The exponent is formed in 64 bits and
 // rounded once, so the result is off by (|z| + 6) 2^-24 of itself at most.  (With expf and a division, 30 instructions an element,
@@ -114,39 +125,42 @@ __device__ __forceinline__ double lane_sum(double v, int lanes) {
 }
 
 // ------------------------------------------------------------------------------------------------ unit route
-template <typename T, int V, int I>
+template <typename T, int V, bool EVEN, int I>
 __global__ __launch_bounds__(kGnThreads) void gn_unit_fwd_kernel(GnArgs a) {
     const int L = a.lanes, lane = threadIdx.x & (L - 1);
     const long long u = ((long long)blockIdx.x * kGnThreads + threadIdx.x) / L;
     if (u >= a.N * a.G) return;   // whole groups of L lanes leave together: the shuffles below stay inside a group
     const unsigned n = (unsigned)u / (unsigned)a.G, g = (unsigned)u - n * (unsigned)a.G;
-    const int dv = a.D / V, nv = (int)a.S * dv;
+    const int dv = vectors(a.D, V), nv = (int)a.S * dv;
     const T* x = (const T*)a.x + (long long)n * a.x_sn + (long long)g * a.D;
     float v[I][V], w[I][V], b[I][V];
     double sum = 0.0;
 #pragma unroll
     for (int i = 0; i < I; ++i) {   // (lanes beyond the end: the last vector once more, not used)
-        const int e = min(lane + i * L, nv - 1), s = a.S == 1 ? 0 : e / dv, cv = (e - s * dv) * V;
+        const int e = min(lane + i * L, nv - 1), s = a.S == 1 ? 0 : e / dv, cv = Span<V, EVEN>(e - s * dv, a.D).at;
         load_vec<T, V>(x + (long long)s * a.x_ss + cv, v[i]);
         load_param<V>(a.w, (long long)g * a.D + cv, 1.f, w[i]);
         load_param<V>(a.b, (long long)g * a.D + cv, 0.f, b[i]);
     }
+    const auto skip = [&](int i) {   // elements of this lane's vector i that are not its own
+        const int e = lane + i * L, s = a.S == 1 ? 0 : e / dv;
+        return e < nv ? Span<V, EVEN>(e - s * dv, a.D).skip : V;
+    };
 #pragma unroll
     for (int i = 0; i < I; ++i)
-        if (lane + i * L < nv)
 #pragma unroll
-            for (int k = 0; k < V; ++k) sum += (double)v[i][k];
-    const double count = (double)nv * V;
+        for (int k = 0; k < V; ++k)
+            if (k >= skip(i)) sum += (double)v[i][k];
+    const double count = (double)a.S * a.D;
     const double mean = lane_sum(sum, L) / count;   // (a constant group's mean is exact: z = bias there, not beside it)
     double m2 = 0.0;
 #pragma unroll
     for (int i = 0; i < I; ++i)
-        if (lane + i * L < nv)
 #pragma unroll
-            for (int k = 0; k < V; ++k) {
-                const double d = (double)v[i][k] - mean;
-                m2 = fma(d, d, m2);
-            }
+        for (int k = 0; k < V; ++k) {
+            const double d = (double)v[i][k] - mean;
+            if (k >= skip(i)) m2 = fma(d, d, m2);
+        }
     const double rstd = 1.0 / sqrt(lane_sum(m2, L) / count + a.eps);
     if (a.stats && lane == 0) {
         a.stats[2 * u] = mean;
@@ -156,7 +170,7 @@ __global__ __launch_bounds__(kGnThreads) void gn_unit_fwd_kernel(GnArgs a) {
     for (int i = 0; i < I; ++i) {
         const int e = lane + i * L;
         if (e >= nv) continue;
-        const int s = a.S == 1 ? 0 : e / dv, c = (int)g * a.D + (e - s * dv) * V;
+        const int s = a.S == 1 ? 0 : e / dv, c = (int)g * a.D + Span<V, EVEN>(e - s * dv, a.D).at;
         float y[V];
 #pragma unroll
         for (int k = 0; k < V; ++k) y[k] = act_value(fma((double)v[i][k] - mean, rstd * (double)w[i][k], (double)b[i][k]), a.act, a.slope);
@@ -166,7 +180,7 @@ __global__ __launch_bounds__(kGnThreads) void gn_unit_fwd_kernel(GnArgs a) {
 
 // Backward for S = 1 (rows): a lane keeps its channels while it walks over the samples n, so that dw and db need no
 // exchange between lanes; every workgroup row leaves one partial (64-bit sums, stored as fp32) per channel.
-template <typename T, int V, int I>
+template <typename T, int V, bool EVEN, int I>
 __global__ __launch_bounds__(kGnThreads) void gn_unit_bwd_kernel(GnArgs a) {
     const int L = a.lanes, lane = threadIdx.x & (L - 1), slot = threadIdx.x / L, slots = kGnThreads / L;
     const int per = a.G < slots ? slots / a.G : 1;             // samples side by side in a workgroup
@@ -174,18 +188,18 @@ __global__ __launch_bounds__(kGnThreads) void gn_unit_bwd_kernel(GnArgs a) {
     const int side = a.G < slots ? slot / a.G : 0;
     const bool on = side < per && g < a.G;
     const int nb = (int)(blockIdx.x / a.blocks_g);
-    const int nv = a.D / V;
+    const int nv = vectors(a.D, V);
     float w[I][V], b[I][V];
     double dw[I][V], db[I][V];
 #pragma unroll
     for (int i = 0; i < I; ++i) {
-        const long long c = (long long)min(g, a.G - 1) * a.D + min(lane + i * L, nv - 1) * V;
+        const long long c = (long long)min(g, a.G - 1) * a.D + Span<V, EVEN>(min(lane + i * L, nv - 1), a.D).at;
         load_param<V>(a.w, c, 1.f, w[i]);
         load_param<V>(a.b, c, 0.f, b[i]);
 #pragma unroll
         for (int k = 0; k < V; ++k) dw[i][k] = db[i][k] = 0.0;
     }
-    const double inv = 1.0 / ((double)nv * V);
+    const double inv = 1.0 / (double)a.D;
     for (long long n = on ? (long long)nb * per + side : a.N; n < a.N; n += (long long)a.blocks_n * per) {
         const T* x = (const T*)a.x + n * a.x_sn + (long long)g * a.D;
         const T* dy = (const T*)a.dy + n * a.dy_sn + (long long)g * a.D;
@@ -193,26 +207,29 @@ __global__ __launch_bounds__(kGnThreads) void gn_unit_bwd_kernel(GnArgs a) {
         float xv[I][V], dv[I][V];
 #pragma unroll
         for (int i = 0; i < I; ++i) {
-            const int e = min(lane + i * L, nv - 1);
-            load_vec<T, V>(x + e * V, xv[i]);
-            load_vec<T, V>(dy + e * V, dv[i]);
+            const int at = Span<V, EVEN>(min(lane + i * L, nv - 1), a.D).at;
+            load_vec<T, V>(x + at, xv[i]);
+            load_vec<T, V>(dy + at, dv[i]);
         }
         double s1 = 0.0, s2 = 0.0;
 #pragma unroll
-        for (int i = 0; i < I; ++i)
-            if (lane + i * L < nv)
+        for (int i = 0; i < I; ++i) {
+            const int skip = lane + i * L < nv ? Span<V, EVEN>(lane + i * L, a.D).skip : V;
 #pragma unroll
-                for (int k = 0; k < V; ++k) {
-                    const double xh = ((double)xv[i][k] - mean) * rstd;
-                    const double dz = (double)(dv[i][k] * act_slope(fma(xh, (double)w[i][k], (double)b[i][k]), a.act, a.slope));
+            for (int k = 0; k < V; ++k) {
+                const double xh = ((double)xv[i][k] - mean) * rstd;
+                const double dz = (double)(dv[i][k] * act_slope(fma(xh, (double)w[i][k], (double)b[i][k]), a.act, a.slope));
+                const double wd = dz * w[i][k];
+                if (k >= skip) {
                     dw[i][k] = fma(dz, xh, dw[i][k]);
                     db[i][k] += dz;
-                    const double wd = dz * w[i][k];
                     s1 += wd;
                     s2 = fma(wd, xh, s2);
-                    xv[i][k] = (float)xh;
-                    dv[i][k] = (float)wd;
                 }
+                xv[i][k] = (float)xh;
+                dv[i][k] = (float)wd;
+            }
+        }
         const double m1 = lane_sum(s1, L) * inv, m2 = lane_sum(s2, L) * inv;
         const float f1 = (float)m1, f2 = (float)m2, fr = (float)rstd;
 #pragma unroll
@@ -222,7 +239,7 @@ __global__ __launch_bounds__(kGnThreads) void gn_unit_bwd_kernel(GnArgs a) {
             float o[V];
 #pragma unroll
             for (int k = 0; k < V; ++k) o[k] = fr * (dv[i][k] - f1 - xv[i][k] * f2);
-            store_vec<T, V>((T*)a.out + n * a.C + g * a.D + e * V, o);
+            store_vec<T, V>((T*)a.out + n * a.C + g * a.D + Span<V, EVEN>(e, a.D).at, o);
         }
     }
     if (!a.part) return;
@@ -248,12 +265,14 @@ __global__ __launch_bounds__(kGnThreads) void gn_unit_bwd_kernel(GnArgs a) {
                     }
         }
         const int e = lane + i * L;
+        const Span<V, EVEN> at(e, a.D);
         if (on && side == 0 && e < nv)
 #pragma unroll
-            for (int k = 0; k < V; ++k) {
-                p[2 * (g * a.D + e * V + k)] = (float)dw[i][k];
-                p[2 * (g * a.D + e * V + k) + 1] = (float)db[i][k];
-            }
+            for (int k = 0; k < V; ++k)
+                if (k >= at.skip) {
+                    p[2 * (g * a.D + at.at + k)] = (float)dw[i][k];
+                    p[2 * (g * a.D + at.at + k) + 1] = (float)db[i][k];
+                }
     }
 }
 
@@ -588,17 +607,15 @@ struct Res {
 
 // A vector of V elements as it lies in memory.  keep(): what has been made of it is forgotten — the compiler would rather hold the
 // unpacked fp32 values from one use to the next than unpack again, and spill them.
-template <int N> struct RawBits { typedef uint32_t Type __attribute__((ext_vector_type(N / 4))); };
-template <> struct RawBits<4> { typedef uint32_t Type; };
-template <> struct RawBits<2> { typedef uint16_t Type; };
 template <typename T, int V> struct Raw {
-    typedef typename RawBits<V * sizeof(T)>::Type Bits;
-    typename std::conditional<sizeof(Bits) == 2, uint32_t, Bits>::type bits;
-    __device__ __forceinline__ void load(const T* p) { bits = *reinterpret_cast<const Bits*>(p); }
+    typedef typename Bits<V * sizeof(T)>::Type Reg;
+    typedef Reg Mem __attribute__((aligned(sizeof(T))));
+    typename std::conditional<sizeof(Reg) == 2, uint32_t, Reg>::type bits;
+    __device__ __forceinline__ void load(const T* p) { bits = *reinterpret_cast<const Mem*>(p); }
     __device__ __forceinline__ void keep() { asm("" : "+v"(bits)); }
-    __device__ __forceinline__ float at(int k) const { return (float)__builtin_bit_cast(Vec<T, V>, (Bits)bits).e[k]; }
+    __device__ __forceinline__ float at(int k) const { return (float)__builtin_bit_cast(Vec<T, V>, (Reg)bits).e[k]; }
     __device__ __forceinline__ void get(float (&v)[V]) const {
-        const Vec<T, V> r = __builtin_bit_cast(Vec<T, V>, (Bits)bits);
+        const Vec<T, V> r = __builtin_bit_cast(Vec<T, V>, (Reg)bits);
 #pragma unroll
         for (int k = 0; k < V; ++k) v[k] = (float)r.e[k];
     }
@@ -835,22 +852,19 @@ struct GnPlan {
     int items, lanes;     // unit
     int per, blocks_g, blocks_n;
     int tx, blocks_c, chunks, merge;   // merge: threads that merge a group's partial sums
+    size_t part, more, ranges;         // tile: bytes of the partial sums and of the channels' sums; where gn_param_grad's begin
     long long chunk_rows;
 };
 
 int elem_bytes(int dtype) { return dtype == DGG_F32 ? 4 : 2; }
 
-// The widest access (at most 16 bytes) that every row allows; unit: that a group's row also divides into.
-int gn_width(int dtype, int unit_d, int C, std::initializer_list<long long> strides, std::initializer_list<const void*> ptrs) {
-    const int es = elem_bytes(dtype);
-    for (int V = 16 / es; V > 1; V >>= 1) {
-        if (V == 2) continue;   // no 2-element kernels: rows that allow no more go element by element
-        bool ok = C % V == 0 && (unit_d == 0 || unit_d % V == 0);
-        for (long long s : strides) ok = ok && s % V == 0;
-        for (const void* p : ptrs) ok = ok && ((uintptr_t)p % (V * es)) == 0;
-        if (ok) return V;
-    }
-    return 1;
+// The widest access, of at most 16 bytes, that divides a range of channels (two elements: one at a time); `fits`: that is no wider than
+// it.  The unit route lets a group's last vector overlap the one before it: 4096 x 515 bf16 in 5 groups 13.8 -> 7.7 us forward, 22.4 -> 17.2
+// backward, 20000 x 105 f32 in 7 17.1 -> 8.8 and 22.6 -> 15.3; in the others the masks cost more than the accesses (64 x 4096 x 33 bf16
+// in 11, tile: 27 us element by element, 44 with overlapping vectors).
+int gn_width(int dtype, int width, bool fits) {
+    const int W = 16 / elem_bytes(dtype);
+    return (fits ? width >= W : width % W == 0) ? W : (fits ? width >= 4 : width % 4 == 0) ? 4 : 1;
 }
 
 void gn_tile_plan(GnPlan& P, long long N, long long S, int C) {
@@ -872,7 +886,7 @@ void gn_tile_plan(GnPlan& P, long long N, long long S, int C) {
 // (300) 6.0 / 4.6, 256 x 256 x 128 in 8 (512) 30.3 / 15.0; rows 1024 x 512 in 32 4.3 / 16.9, backward 9.7 / 26.4.
 bool gn_unit_plan(GnPlan& P, long long S, int D, bool backward) {
     if (S != 1 && (backward || S > 128)) return false;
-    const long long nv = S * (D / P.V);
+    const long long nv = S * vectors(D, P.V);
     if (nv > (S == 1 ? 64 * kUnitItems : 128)) return false;
     P.lanes = 1;
     while (P.lanes < 64 && P.lanes < nv) P.lanes *= 2;
@@ -885,9 +899,8 @@ bool gn_unit_plan(GnPlan& P, long long S, int D, bool backward) {
 // tile, forward / backward, us: 32 x 2048 x 256 bf16 in 32 groups 25 / 35 against 31 / 57, 128 x 2048 x 256 71 / 140 against 102 / 185,
 // 6 x 1111 x 132 f16 in 11 9.2 / 13.5 against 12.9 / 17.9, 4 x 4096 x 64 in 8 13.9 / 20.3 against 15.4 / 19.6.
 bool gn_res_plan(GnPlan& P, long long N, long long S, int C, int G) {
-    const int D = C / G;
     if (S > 16 * kResThreads) return false;
-    const int per = D / P.V;
+    const int per = C / G / P.V;
     if (per > kResThreads) return false;
     // as many groups side by side as leave every thread 16 rows ..
     int groups = (int)(16ll * kResThreads / (S * per));
@@ -945,28 +958,32 @@ int gn_check(long long N, long long S, int C, int G, int act, int dtype, const c
     return DGG_OK;
 }
 
-// What both directions need at most, for whatever alignment the tensors turn out to have.
-int64_t gn_ws_bytes(long long N, long long S, int C, int G, int dtype, bool backward) {
-    int64_t need = 0;
-    for (int V : {16 / elem_bytes(dtype), 4, 1}) {
-        if (C % V) continue;
-        GnPlan P;
-        P.V = V;
-        int64_t n = 0;
-        if ((C / G) % V == 0 && gn_unit_plan(P, S, C / G, backward)) {
-            if (backward) {
-                gn_unit_bwd_grid(P, N, G);
-                n = (int64_t)P.blocks_n * C * 2 * sizeof(float);
-            } else {
-                n = 0;
-            }
-        } else {
-            gn_tile_plan(P, N, S, C);
-            n = (int64_t)N * (P.chunks + (backward && P.chunks > 1)) * C * 2 * sizeof(double) + (int64_t)N * G * 2 * sizeof(double);
-        }
-        if (n > need) need = n;
+// The route of a call, its launches and the workspace it needs (part and more: see gn_run).
+size_t gn_plan(GnPlan& P, long long N, long long S, int C, int G, int dtype, bool backward, bool grads) {
+    const int D = C / G;
+    P.es = elem_bytes(dtype);
+    P.V = gn_width(dtype, D, true);
+    P.unit = gn_unit_plan(P, S, D, backward);
+    if (!P.unit) P.V = gn_width(dtype, D, false);
+    P.res = !P.unit && gn_res_plan(P, N, S, C, G);
+    P.part = P.more = 0;
+    size_t need = 0;
+    if (P.unit) {
+        if (backward) gn_unit_bwd_grid(P, N, G);
+        need = grads ? (size_t)P.blocks_n * C * 2 * sizeof(float) : 0;
+    } else if (P.res) {
+        need = grads ? (size_t)N * C * 2 * sizeof(double) : 0;
+    } else {
+        P.V = gn_width(dtype, C, false);
+        gn_tile_plan(P, N, S, C);
+        P.merge = (long long)P.chunks * D > 1024 ? kMergeThreads : kGnThreads;
+        const size_t chan = (size_t)N * C * 2 * sizeof(double);
+        P.part = chan * P.chunks;
+        P.more = backward && P.chunks > 1 ? chan : 0;
+        need = P.part + P.more + (size_t)N * G * 2 * sizeof(double);
     }
-    return need + (backward && gn_ranges(N) > 1 ? (int64_t)gn_ranges(N) * C * 2 * sizeof(double) : 0);
+    P.ranges = need;   // where gn_param_grad's partial sums begin
+    return need + (grads && !P.unit && gn_ranges(N) > 1 ? (size_t)gn_ranges(N) * C * 2 * sizeof(double) : 0);
 }
 
 template <typename P> void gn_param_grad(const GnArgs& a, const P* part, long long rows, hipStream_t st) {
@@ -983,6 +1000,17 @@ template <typename P> void gn_param_grad(const GnArgs& a, const P* part, long lo
     else if (act == DGG_ACT_SILU) hipLaunchKernelGGL((kernel<T, V, DGG_ACT_SILU>), grid, block, 0, st, a);              \
     else hipLaunchKernelGGL((kernel<T, V, DGG_ACT_NONE>), grid, block, 0, st, a);
 
+#define GN_UNIT_I(kernel, EVEN)                                                                                                \
+    switch (P.items) {                                                                                                        \
+        case 1: hipLaunchKernelGGL((kernel<T, V, EVEN, 1>), grid, block, 0, st, a); break;                                     \
+        case 2: hipLaunchKernelGGL((kernel<T, V, EVEN, 2>), grid, block, 0, st, a); break;                                     \
+        case 4: hipLaunchKernelGGL((kernel<T, V, EVEN, 4>), grid, block, 0, st, a); break;                                     \
+        default: hipLaunchKernelGGL((kernel<T, V, EVEN, 8>), grid, block, 0, st, a); break;                                    \
+    }
+#define GN_UNIT(kernel)                                                                                                       \
+    if (V == 1 || a.D % V == 0) { GN_UNIT_I(kernel, true) }                                                                   \
+    else { GN_UNIT_I(kernel, (V == 1)) }
+
 #define GN_RES(act, kernel, R)                                                                                             \
     if (act == DGG_ACT_LEAKY_RELU) hipLaunchKernelGGL((kernel<T, V, R, DGG_ACT_LEAKY_RELU>), grid, block, 0, st, a);       \
     else if (act == DGG_ACT_SILU) hipLaunchKernelGGL((kernel<T, V, R, DGG_ACT_SILU>), grid, block, 0, st, a);              \
@@ -992,12 +1020,7 @@ template <typename T, int V> int gn_forward_v(const GnPlan& P, GnArgs& a, hipStr
     if (P.unit) {
         const long long threads = a.N * a.G * P.lanes;
         const dim3 grid((unsigned)((threads + kGnThreads - 1) / kGnThreads)), block(kGnThreads);
-        switch (P.items) {
-            case 1: hipLaunchKernelGGL((gn_unit_fwd_kernel<T, V, 1>), grid, block, 0, st, a); break;
-            case 2: hipLaunchKernelGGL((gn_unit_fwd_kernel<T, V, 2>), grid, block, 0, st, a); break;
-            case 4: hipLaunchKernelGGL((gn_unit_fwd_kernel<T, V, 4>), grid, block, 0, st, a); break;
-            default: hipLaunchKernelGGL((gn_unit_fwd_kernel<T, V, 8>), grid, block, 0, st, a); break;
-        }
+        GN_UNIT(gn_unit_fwd_kernel)
         return check_launch("group_norm forward");
     }
     if (P.res) {
@@ -1019,12 +1042,7 @@ template <typename T, int V> int gn_backward_v(const GnPlan& P, GnArgs& a, hipSt
     if (P.unit) {
         if (!a.dw) a.part = nullptr;
         const dim3 grid((unsigned)P.blocks_g * P.blocks_n);
-        switch (P.items) {
-            case 1: hipLaunchKernelGGL((gn_unit_bwd_kernel<T, V, 1>), grid, block, 0, st, a); break;
-            case 2: hipLaunchKernelGGL((gn_unit_bwd_kernel<T, V, 2>), grid, block, 0, st, a); break;
-            case 4: hipLaunchKernelGGL((gn_unit_bwd_kernel<T, V, 4>), grid, block, 0, st, a); break;
-            default: hipLaunchKernelGGL((gn_unit_bwd_kernel<T, V, 8>), grid, block, 0, st, a); break;
-        }
+        GN_UNIT(gn_unit_bwd_kernel)
         if (a.dw) gn_param_grad(a, (const float*)a.part, P.blocks_n, st);
         return check_launch("group_norm backward");
     }
@@ -1053,53 +1071,38 @@ template <typename T> int gn_dispatch(bool backward, const GnPlan& P, GnArgs& a,
 
 int gn_run(bool backward, GnArgs& a, int dtype, void* ws, size_t ws_bytes, hipStream_t st, const char* who) {
     a.D = a.C / a.G;
-    GnPlan P;
-    std::initializer_list<long long> fs = {a.x_sn, a.x_ss}, bs = {a.x_sn, a.x_ss, a.dy_sn, a.dy_ss};
-    P.V = gn_width(dtype, a.D, a.C, backward ? bs : fs, {a.x, a.out, backward ? a.dy : a.x});
-    P.es = elem_bytes(dtype);
-    P.unit = gn_unit_plan(P, a.S, a.D, backward);
-    P.res = !P.unit && gn_res_plan(P, a.N, a.S, a.C, a.G);
+    GnPlan P = {};
+    const size_t need = gn_plan(P, a.N, a.S, a.C, a.G, dtype, backward, backward && a.dw);
+    if (need && (!ws || ws_bytes < need || (uintptr_t)ws % 8)) {
+        set_error_text("%s: the workspace has %zu bytes, %zu (8-byte aligned) are needed", who, ws_bytes, need);
+        return DGG_ERR_WORKSPACE;
+    }
+    const int es = elem_bytes(dtype);
+    if ((uintptr_t)a.x % es || (uintptr_t)a.out % es || (uintptr_t)a.dy % es) {
+        set_error_text("%s: a tensor that does not begin at an element's address", who);
+        return DGG_ERR_INVALID;
+    }
+    a.chan = (double*)ws;
     if (P.unit) {
         a.lanes = P.lanes;
-        if (backward) {
-            gn_unit_bwd_grid(P, a.N, a.G);
-            a.blocks_g = P.blocks_g;
-            a.blocks_n = P.blocks_n;
-        }
+        a.blocks_g = P.blocks_g;
+        a.blocks_n = P.blocks_n;
     } else if (P.res) {
         a.res_groups = P.res_groups;
         a.blocks_g = P.res_blocks;
     } else {
-        P.V = gn_width(dtype, 0, a.C, backward ? bs : fs, {a.x, a.out, backward ? a.dy : a.x});
-        gn_tile_plan(P, a.N, a.S, a.C);
-        P.merge = (long long)P.chunks * a.D > 1024 ? kMergeThreads : kGnThreads;
         if (P.blocks_c > 65535) {
-            set_error_text("%s: %d channels element by element: 2^24 - 256 at most", who, a.C);
+            set_error_text("%s: %d channels: 2^24 - 256 at most", who, a.C);
             return DGG_ERR_INVALID;
         }
         a.chunks = P.chunks;
         a.chunk_rows = P.chunk_rows;
         a.tx = P.tx;
-    }
-    size_t need = 0, ranges = backward && !P.unit && a.dw && gn_ranges(a.N) > 1 ? (size_t)gn_ranges(a.N) * a.C * 2 * sizeof(double) : 0;
-    if (P.unit) {
-        need = backward && a.dw ? (size_t)P.blocks_n * a.C * 2 * sizeof(float) : 0;
-    } else if (P.res) {
-        need = backward && a.dw ? (size_t)a.N * a.C * 2 * sizeof(double) : 0;
-        a.chan = (double*)ws;
-    } else {
-        const size_t chan = (size_t)a.N * a.C * 2 * sizeof(double), part = chan * P.chunks, more = backward && P.chunks > 1 ? chan : 0;
-        need = part + more + (size_t)a.N * a.G * 2 * sizeof(double);
-        a.chan = (double*)((char*)ws + (more ? part : 0));
-        a.coef = (double*)((char*)ws + part + more);
+        a.chan = (double*)((char*)ws + (P.more ? P.part : 0));
+        a.coef = (double*)((char*)ws + P.part + P.more);
         if (!a.stats) a.stats = a.coef;   // a forward without a backward keeps its statistics in the workspace
     }
-    a.ranges = (double*)((char*)ws + need);
-    need += ranges;
-    if (need && (!ws || ws_bytes < need || (uintptr_t)ws % 8)) {
-        set_error_text("%s: the workspace has %zu bytes, %zu (8-byte aligned) are needed", who, ws_bytes, need);
-        return DGG_ERR_WORKSPACE;
-    }
+    a.ranges = (double*)((char*)ws + P.ranges);
     a.part = (double*)ws;
     return dtype == DGG_F32 ? gn_dispatch<float>(backward, P, a, st)
          : dtype == DGG_BF16 ? gn_dispatch<__bf16>(backward, P, a, st) : gn_dispatch<_Float16>(backward, P, a, st);
@@ -1114,7 +1117,8 @@ extern "C" {
 
 int64_t dgg_group_norm_workspace_bytes(int64_t N, int64_t S, int C, int groups, int dtype, int backward) {
     const int rc = gn_check(N, S, C, groups, DGG_ACT_NONE, dtype, "dgg_group_norm_workspace_bytes");
-    return rc != DGG_OK ? rc : gn_ws_bytes(N, S, C, groups, dtype, backward != 0);
+    GnPlan P = {};
+    return rc != DGG_OK ? rc : (int64_t)gn_plan(P, N, S, C, groups, dtype, backward != 0, backward != 0);
 }
 
 int dgg_group_norm_act_forward(const void* x, int64_t x_stride_n, int64_t x_stride_s, int64_t N, int64_t S, int C, int groups,

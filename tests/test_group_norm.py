@@ -308,3 +308,28 @@ def test_offsets_beyond_32_bits():
         del y, dx
     del far
     torch.cuda.empty_cache()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16], ids=["f32", "bf16", "f16"])
+@pytest.mark.parametrize("shape", [(6, 1, 35, 7), (50, 1, 99, 11), (9, 1, 39, 3), (4, 1, 31, 1), (70, 1, 515, 5), (3, 1, 2049, 1), (9, 7, 35, 7),
+                                   (3, 40, 26, 2), (2, 200, 24, 3), (2, 3000, 64, 4), (2, 9000, 12, 1), (2, 400, 516, 3)],
+                         ids=lambda s: "x".join(map(str, s)))
+def test_groups_and_addresses_that_no_vector_divides(shape, dtype):
+    """Groups whose last vector overlaps the one before it; rows of odd pitch that begin one element into a 16-byte line, and what lies
+    beside them."""
+    n, s, c, groups = shape
+    x, dy, w, b = data((n, s, c), dtype, 12)
+    check(x, dy, groups, w, b, act="silu")
+    pitch = c + 3 + c % 2
+    wide = [torch.full((n, s, pitch), 7.0, dtype=dtype, device="cuda") for _ in range(2)]
+    xv, dyv = (t[:, :, 1:1 + c] for t in wide)
+    xv.copy_(x)
+    dyv.copy_(dy)
+    check(xv, dyv, groups, w, b)
+    flat = torch.full((n * s * c + 5,), 7.0, dtype=dtype, device="cuda")
+    odd = flat[1:1 + n * s * c].view(n, s, c)
+    odd.copy_(x)
+    y, st = ops.group_norm_act_forward(odd, groups, w.cuda(), b.cuda())
+    assert torch.equal(y, ops.group_norm_act_forward(x.cuda(), groups, w.cuda(), b.cuda())[0])
+    assert all(bool((t[:, :, 0] == 7).all() and (t[:, :, 1 + c:] == 7).all()) for t in wide) and bool((flat[-4:] == 7).all())
