@@ -858,13 +858,16 @@ struct GnPlan {
 
 int elem_bytes(int dtype) { return dtype == DGG_F32 ? 4 : 2; }
 
-// The widest access, of at most 16 bytes, that divides a range of channels (two elements: one at a time); `fits`: that is no wider than
-// it.  The unit route lets a group's last vector overlap the one before it: 4096 x 515 bf16 in 5 groups 13.8 -> 7.7 us forward, 22.4 -> 17.2
-// backward, 20000 x 105 f32 in 7 17.1 -> 8.8 and 22.6 -> 15.3; in the others the masks cost more than the accesses (64 x 4096 x 33 bf16
-// in 11, tile: 27 us element by element, 44 with overlapping vectors).
+// The widest access, of at most 16 bytes, that divides a range of channels (256 x 256 x 34 bf16 in 17 groups with two elements instead
+// of one: 11.6 -> 9.3 us forward, 18.6 -> 15.1 backward); `fits`: that is no wider than it.  The unit route lets a group's last vector
+// overlap the one before it: 4096 x 515 bf16 in 5 groups 13.8 -> 7.7 us forward, 22.4 -> 17.2 backward, 20000 x 105 f32 in 7 17.1 -> 8.8
+// and 22.6 -> 15.3; in the others the masks cost more than the accesses (64 x 4096 x 33 bf16 in 11, tile: 27 us element by element, 44
+// with overlapping vectors).
 int gn_width(int dtype, int width, bool fits) {
     const int W = 16 / elem_bytes(dtype);
-    return (fits ? width >= W : width % W == 0) ? W : (fits ? width >= 4 : width % 4 == 0) ? 4 : 1;
+    for (int V = W; V > 1; V /= 2)
+        if (fits ? width >= V : width % V == 0) return V;
+    return 1;
 }
 
 void gn_tile_plan(GnPlan& P, long long N, long long S, int C) {
@@ -1066,6 +1069,7 @@ template <typename T> int gn_dispatch(bool backward, const GnPlan& P, GnArgs& a,
     constexpr int W = 16 / sizeof(T);
     if (P.V == W) return backward ? gn_backward_v<T, W>(P, a, st) : gn_forward_v<T, W>(P, a, st);
     if (W > 4 && P.V == 4) return backward ? gn_backward_v<T, 4>(P, a, st) : gn_forward_v<T, 4>(P, a, st);
+    if (P.V == 2) return backward ? gn_backward_v<T, 2>(P, a, st) : gn_forward_v<T, 2>(P, a, st);
     return backward ? gn_backward_v<T, 1>(P, a, st) : gn_forward_v<T, 1>(P, a, st);
 }
 
