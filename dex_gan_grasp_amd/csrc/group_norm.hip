@@ -288,23 +288,33 @@ __device__ __forceinline__ Tile tile_of(const GnArgs& a, int vecs, int by) {
     return t;
 }
 
-// sums a per-thread (p, q)[V] over the workgroup's rows in a fixed order; row 0 of each column holds the result
+// Adds up the entries of n threads `stride` apart, y = 0 .. n - 1 the thread's own number among them, halving n: the first has the sum, in a
+// fixed order.  sh: [N][blockDim.x], entry k of thread t at k * blockDim.x + t; every thread of the workgroup calls it.
+template <int N> __device__ __forceinline__ void fold(double* sh, int y, int n, int stride) {
+    __syncthreads();
+    while (n > 1) {
+        const int h = (n + 1) / 2;
+        if (y < n - h)
+#pragma unroll
+            for (int k = 0; k < N; ++k) sh[k * blockDim.x + threadIdx.x] += sh[k * blockDim.x + threadIdx.x + h * stride];
+        n = h;
+        __syncthreads();
+    }
+}
+
+// sums a per-thread (p, q)[V] over the workgroup's rows; row 0 of each column holds the result
 template <int V> __device__ __forceinline__ void column_sum(double (&p)[V], double (&q)[V], const GnArgs& a, const Tile& t) {
-    __shared__ double sh[kGnThreads * 2];
+    __shared__ double sh[2 * V * kGnThreads];
+#pragma unroll
     for (int k = 0; k < V; ++k) {
-        __syncthreads();
-        sh[2 * threadIdx.x] = p[k];
-        sh[2 * threadIdx.x + 1] = q[k];
-        __syncthreads();
-        if (t.on && t.ty == 0) {
-            double s = 0.0, r = 0.0;
-            for (int y = 0; y < t.rows; ++y) {
-                s += sh[2 * (y * a.tx + threadIdx.x)];
-                r += sh[2 * (y * a.tx + threadIdx.x) + 1];
-            }
-            p[k] = s;
-            q[k] = r;
-        }
+        sh[2 * k * kGnThreads + threadIdx.x] = p[k];
+        sh[(2 * k + 1) * kGnThreads + threadIdx.x] = q[k];
+    }
+    fold<2 * V>(sh, t.ty < t.rows ? t.ty : t.rows, t.rows, a.tx);
+#pragma unroll
+    for (int k = 0; k < V; ++k) {
+        p[k] = sh[2 * k * kGnThreads + threadIdx.x];
+        q[k] = sh[(2 * k + 1) * kGnThreads + threadIdx.x];
     }
 }
 
@@ -387,16 +397,10 @@ template <typename Use> __device__ __forceinline__ void over_chunks(const GnArgs
             }
         }
         __syncthreads();
-        col[2 * threadIdx.x] = p;
-        col[2 * threadIdx.x + 1] = q;
-        __syncthreads();
-        if (on && w == 0) {
-            for (int t = 1; t < T; ++t) {
-                p += col[2 * (t * wide + c0)];
-                q += col[2 * (t * wide + c0) + 1];
-            }
-            use(c, p, q);
-        }
+        col[threadIdx.x] = p;
+        col[blockDim.x + threadIdx.x] = q;
+        fold<2>(col, w < T ? w : T, T, wide);
+        if (on && w == 0) use(c, col[threadIdx.x], col[blockDim.x + threadIdx.x]);
     }
 }
 
@@ -874,9 +878,9 @@ void gn_tile_plan(GnPlan& P, long long N, long long S, int C) {
     const int vecs = C / P.V;
     P.blocks_c = (vecs + kGnThreads - 1) / kGnThreads;
     P.tx = (vecs + P.blocks_c - 1) / P.blocks_c;
-    // about 2048 workgroups, of at least 64 rows each (the partial sums stay small beside the data)
+    // about 2048 workgroups, of at least 64 rows each and two for every thread (the partial sums stay small beside the data)
     long long want = 2048 / (N * P.blocks_c);
-    const long long most = (S + 63) / 64;
+    const long long least = 2 * (kGnThreads / P.tx) > 64 ? 2 * (kGnThreads / P.tx) : 64, most = (S + least - 1) / least;
     if (want > most) want = most;
     if (want < 1) want = 1;
     P.chunk_rows = (S + want - 1) / want;
