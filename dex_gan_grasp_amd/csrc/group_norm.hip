@@ -767,17 +767,26 @@ __global__ __launch_bounds__(kResThreads) void gn_res_bwd_kernel(GnArgs a) {
         __syncthreads();
     }
     const int lane = threadIdx.x & 63, waves = blockDim.x >> 6, groups = t.tx / t.per, n = parts > 1 ? parts : t.rows;
+    int side = 1;   // channels side by side in a wave; the lanes that are left share a channel's rows
+    while (side < a.D && side < 64) side *= 2;
+    const int e0 = lane & (side - 1), y0 = lane / side, ystep = 64 / side;
     for (int j = threadIdx.x >> 6; j < groups; j += waves) {
         double s1 = 0.0, s2 = 0.0;
-        for (int e = lane; e < t.per * V; e += 64) {
-            const int ch = j * t.per * V + e;
+        for (int base = 0; base < a.D; base += side) {
+            const int e = base + e0;
             double u = 0.0, v = 0.0;
-            for (int y = 0; y < n; ++y) {
-                const float2 o = *reinterpret_cast<const float2*>(sh + y * cols + 2 * ch);
-                u += (double)o.x;
-                v += (double)o.y;
+            if (e < a.D)
+                for (int y = y0; y < n; y += ystep) {
+                    const float2 o = *reinterpret_cast<const float2*>(sh + y * cols + 2 * (j * a.D + e));
+                    u += (double)o.x;
+                    v += (double)o.y;
+                }
+            for (int o = side; o < 64; o *= 2) {
+                u += __shfl_xor(u, o);
+                v += __shfl_xor(v, o);
             }
-            const long long c = (long long)t.blk * a.res_groups * t.per * V + ch;
+            if (e >= a.D || y0) continue;
+            const long long c = ((long long)t.blk * a.res_groups + j) * a.D + e;
             if (a.dw) {
                 double* o = a.chan + 2ll * ((long long)t.n * a.C + c);
                 o[0] = u;
@@ -863,10 +872,10 @@ struct GnPlan {
 int elem_bytes(int dtype) { return dtype == DGG_F32 ? 4 : 2; }
 
 // The widest access, of at most 16 bytes, that divides a range of channels (256 x 256 x 34 bf16 in 17 groups with two elements instead
-// of one: 11.6 -> 9.3 us forward, 18.6 -> 15.1 backward); `fits`: that is no wider than it.  The unit route lets a group's last vector
-// overlap the one before it: 4096 x 515 bf16 in 5 groups 13.8 -> 7.7 us forward, 22.4 -> 17.2 backward, 20000 x 105 f32 in 7 17.1 -> 8.8
-// and 22.6 -> 15.3; in the others the masks cost more than the accesses (64 x 4096 x 33 bf16 in 11, tile: 27 us element by element, 44
-// with overlapping vectors).
+// of one: 11.6 -> 9.3 us forward, 18.6 -> 15.1 backward); `fits`: that is no wider than it.  For rows the unit route lets a group's last
+// vector overlap the one before it: 4096 x 515 bf16 in 5 groups 13.8 -> 7.7 us forward, 22.4 -> 17.2 backward, 20000 x 105 f32 in 7 17.1
+// -> 8.8 and 22.6 -> 15.3; elsewhere the masks cost more than the accesses (64 x 4096 x 33 bf16 in 11, tile: 27 us element by element, 44
+// with overlapping vectors; 3000 x 9 x 33 in 11, unit: 11 and 15).
 int gn_width(int dtype, int width, bool fits) {
     const int W = 16 / elem_bytes(dtype);
     for (int V = W; V > 1; V /= 2)
@@ -878,10 +887,13 @@ void gn_tile_plan(GnPlan& P, long long N, long long S, int C) {
     const int vecs = C / P.V;
     P.blocks_c = (vecs + kGnThreads - 1) / kGnThreads;
     P.tx = (vecs + P.blocks_c - 1) / P.blocks_c;
-    // about 2048 workgroups, of at least 64 rows each and two for every thread (the partial sums stay small beside the data)
-    long long want = 2048 / (N * P.blocks_c);
-    const long long least = 2 * (kGnThreads / P.tx) > 64 ? 2 * (kGnThreads / P.tx) : 64, most = (S + least - 1) / least;
-    if (want > most) want = most;
+    // about 2048 workgroups, of at least 64 rows each and two for every thread (the partial sums stay small beside the data), or
+    // about 512 of at least 8 and two (2 x 269 x 666 f16 in 18 groups, forward and backward: 46 -> 28 us)
+    const long long rows = 2 * (kGnThreads / P.tx), least = rows > 64 ? rows : 64, few = rows > 8 ? rows : 8;
+    long long want = 2048 / (N * P.blocks_c), less = 512 / (N * P.blocks_c);
+    if (want > (S + least - 1) / least) want = (S + least - 1) / least;
+    if (less > (S + few - 1) / few) less = (S + few - 1) / few;
+    if (want < less) want = less;
     if (want < 1) want = 1;
     P.chunk_rows = (S + want - 1) / want;
     P.chunks = (int)((S + P.chunk_rows - 1) / P.chunk_rows);
@@ -969,7 +981,7 @@ int gn_check(long long N, long long S, int C, int G, int act, int dtype, const c
 size_t gn_plan(GnPlan& P, long long N, long long S, int C, int G, int dtype, bool backward, bool grads) {
     const int D = C / G;
     P.es = elem_bytes(dtype);
-    P.V = gn_width(dtype, D, true);
+    P.V = gn_width(dtype, D, S == 1);
     P.unit = gn_unit_plan(P, S, D, backward);
     if (!P.unit) P.V = gn_width(dtype, D, false);
     P.res = !P.unit && gn_res_plan(P, N, S, C, G);
