@@ -887,10 +887,10 @@ void gn_tile_plan(GnPlan& P, long long N, long long S, int C) {
     const int vecs = C / P.V;
     P.blocks_c = (vecs + kGnThreads - 1) / kGnThreads;
     P.tx = (vecs + P.blocks_c - 1) / P.blocks_c;
-    // about 2048 workgroups, of at least 64 rows each and two for every thread (the partial sums stay small beside the data), or
+    // about 1024 workgroups (2048: 9 x 61743 x 16 bf16 35 instead of 26 us forward), of at least 64 rows each and two for every thread (the partial sums stay small beside the data), or
     // about 512 of at least 8 and two (2 x 269 x 666 f16 in 18 groups, forward and backward: 46 -> 28 us)
     const long long rows = 2 * (kGnThreads / P.tx), least = rows > 64 ? rows : 64, few = rows > 8 ? rows : 8;
-    long long want = 2048 / (N * P.blocks_c), less = 512 / (N * P.blocks_c);
+    long long want = 1024 / (N * P.blocks_c), less = 512 / (N * P.blocks_c);
     if (want > (S + least - 1) / least) want = (S + least - 1) / least;
     if (less > (S + few - 1) / few) less = (S + few - 1) / few;
     if (want < less) want = less;
@@ -899,14 +899,11 @@ void gn_tile_plan(GnPlan& P, long long N, long long S, int C) {
     P.chunks = (int)((S + P.chunk_rows - 1) / P.chunk_rows);
 }
 
-// A group in a part of a wave's registers: rows (S = 1) up to 8 vectors a lane, points (forward only) up to 2 — a wave walks over a
-// group's points in short accesses, and whole samples in a workgroup are faster from there on.  Unit against resident, forward, us:
-// 20000 x 2 x 16 in 2 groups 4.0 / 26.8, 4000 x 16 x 32 in 4 8.1 / 11.8, 300 x 37 x 15 in 5 (111 vectors) 4.5 / 5.5, 64 x 100 x 15 in 5
-// (300) 6.0 / 4.6, 256 x 256 x 128 in 8 (512) 30.3 / 15.0; rows 1024 x 512 in 32 4.3 / 16.9, backward 9.7 / 26.4.
+// A group in a part of a wave's registers, 8 vectors a lane at most; backward: rows (S = 1).
 bool gn_unit_plan(GnPlan& P, long long S, int D, bool backward) {
-    if (S != 1 && (backward || S > 128)) return false;
+    if (S != 1 && (backward || S > 64 * kUnitItems)) return false;
     const long long nv = S * vectors(D, P.V);
-    if (nv > (S == 1 ? 64 * kUnitItems : 128)) return false;
+    if (nv > 64 * kUnitItems) return false;
     P.lanes = 1;
     while (P.lanes < 64 && P.lanes < nv) P.lanes *= 2;
     P.items = 1;
@@ -984,7 +981,16 @@ size_t gn_plan(GnPlan& P, long long N, long long S, int C, int G, int dtype, boo
     P.V = gn_width(dtype, D, S == 1);
     P.unit = gn_unit_plan(P, S, D, backward);
     if (!P.unit) P.V = gn_width(dtype, D, false);
-    P.res = !P.unit && gn_res_plan(P, N, S, C, G);
+    P.res = (S > 1 || !P.unit) && gn_res_plan(P, N, S, C, G);
+    // Points that fit both go to the units unless those take 1.5 times the resident route's threads (a lane with a vector costs 8 ns a
+    // thousand, a thread with its rows 12 to 17).  Unit against resident, forward, us: 20000 x 2 x 16 bf16 in 2 groups 3.8 / 26, 4000 x 16 x 32
+    // f32 in 4 8.0 / 11.5, 3000 x 9 x 33 bf16 in 11 11 / 19, 300 x 37 x 15 f32 in 5 4.5 / 5.4, 64 x 100 x 15 in 5 6.0 / 4.6, 1779 x 6 x 459 bf16
+    // in 51 50 / 37, 256 x 256 x 128 in 8 30 / 15; rows 1024 x 512 f32 in 32 4.3 / 16.9, backward 9.7 / 26.4.
+    if (P.unit && P.res) {
+        const long long lanes = N * G * P.lanes * P.items, threads = N * P.res_blocks * P.res_threads;
+        P.unit = 2 * lanes <= 3 * threads;
+        P.res = !P.unit;
+    }
     P.part = P.more = 0;
     size_t need = 0;
     if (P.unit) {
