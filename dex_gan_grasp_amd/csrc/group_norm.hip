@@ -887,8 +887,9 @@ void gn_tile_plan(GnPlan& P, long long N, long long S, int C) {
     const int vecs = C / P.V;
     P.blocks_c = (vecs + kGnThreads - 1) / kGnThreads;
     P.tx = (vecs + P.blocks_c - 1) / P.blocks_c;
-    // about 1024 workgroups (2048: 9 x 61743 x 16 bf16 35 instead of 26 us forward), of at least 64 rows each and two for every thread (the partial sums stay small beside the data), or
-    // about 512 of at least 8 and two (2 x 269 x 666 f16 in 18 groups, forward and backward: 46 -> 28 us)
+    // about 1024 workgroups (2048: 9 x 61743 x 16 bf16 35 instead of 26 us forward), of at least 64 rows each and two for every thread
+    // (the partial sums stay small beside the data), or about 512 of at least 8 and two (2 x 269 x 666 f16 in 18 groups, forward and
+    // backward: 46 -> 28 us)
     const long long rows = 2 * (kGnThreads / P.tx), least = rows > 64 ? rows : 64, few = rows > 8 ? rows : 8;
     long long want = 1024 / (N * P.blocks_c), less = 512 / (N * P.blocks_c);
     if (want > (S + least - 1) / least) want = (S + least - 1) / least;
