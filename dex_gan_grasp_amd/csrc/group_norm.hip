@@ -13,7 +13,7 @@
 // rate of the fp32 ones here; per element they are 4 to 6 of them.)  What follows the sign is fp32, rounded once to the output type.
 //
 // Three routes, chosen by gn_run:
-//  * "unit": a group's S x D elements fit the registers of at most one wave (backward: rows, S = 1).  L = 2^k lanes own one (n, g):
+//  * "unit": a group's S x D elements fit the registers of at most one wave.  L = 2^k lanes own one (n, g):
 //    one read of x, mean and centred variance by lane shuffles, no LDS, no barrier.  1024 x 512 f32 in 32 groups: 4.3 us forward,
 //    9.7 backward with dw and db (launches); 16384 x 512: 24 and 29 us (2.9 and 3.4 TB/s).
 //  * "resident": a sample's points in a block of groups fit a workgroup's registers: one read, one launch.  128 x 2048 x 256 bf16
@@ -124,6 +124,20 @@ __device__ __forceinline__ double lane_sum(double v, int lanes) {
     return v;
 }
 
+// Adds up the entries of n threads `stride` apart, y = 0 .. n - 1 the thread's own number among them, halving n: the first has the sum, in a
+// fixed order.  sh: [N][blockDim.x], entry k of thread t at k * blockDim.x + t; every thread of the workgroup calls it.
+template <int N> __device__ __forceinline__ void fold(double* sh, int y, int n, int stride) {
+    __syncthreads();
+    while (n > 1) {
+        const int h = (n + 1) / 2;
+        if (y < n - h)
+#pragma unroll
+            for (int k = 0; k < N; ++k) sh[k * blockDim.x + threadIdx.x] += sh[k * blockDim.x + threadIdx.x + h * stride];
+        n = h;
+        __syncthreads();
+    }
+}
+
 // ------------------------------------------------------------------------------------------------ unit route
 template <typename T, int V, bool EVEN, int I>
 __global__ __launch_bounds__(kGnThreads) void gn_unit_fwd_kernel(GnArgs a) {
@@ -178,9 +192,9 @@ __global__ __launch_bounds__(kGnThreads) void gn_unit_fwd_kernel(GnArgs a) {
     }
 }
 
-// Backward for S = 1 (rows): a lane keeps its channels while it walks over the samples n, so that dw and db need no
-// exchange between lanes; every workgroup row leaves one partial (64-bit sums, stored as fp32) per channel.
-template <typename T, int V, bool EVEN, int I>
+// Backward: a lane keeps its channels while it walks over the samples n, so that dw and db need no exchange between lanes until the
+// end; every workgroup row leaves one partial (64-bit sums, stored as fp32) per channel.  POINTS: S > 1, a lane has a vector of a point.
+template <typename T, int V, bool EVEN, int I, bool POINTS>
 __global__ __launch_bounds__(kGnThreads) void gn_unit_bwd_kernel(GnArgs a) {
     const int L = a.lanes, lane = threadIdx.x & (L - 1), slot = threadIdx.x / L, slots = kGnThreads / L;
     const int per = a.G < slots ? slots / a.G : 1;             // samples side by side in a workgroup
@@ -188,18 +202,20 @@ __global__ __launch_bounds__(kGnThreads) void gn_unit_bwd_kernel(GnArgs a) {
     const int side = a.G < slots ? slot / a.G : 0;
     const bool on = side < per && g < a.G;
     const int nb = (int)(blockIdx.x / a.blocks_g);
-    const int nv = vectors(a.D, V);
+    const int per_row = vectors(a.D, V), nv = POINTS ? (int)a.S * per_row : per_row;
+    const auto point = [&](int e) { return POINTS ? e / per_row : 0; };
+    const auto span = [&](int e) { return Span<V, EVEN>(e - point(e) * per_row, a.D); };
     float w[I][V], b[I][V];
     double dw[I][V], db[I][V];
 #pragma unroll
     for (int i = 0; i < I; ++i) {
-        const long long c = (long long)min(g, a.G - 1) * a.D + Span<V, EVEN>(min(lane + i * L, nv - 1), a.D).at;
+        const long long c = (long long)min(g, a.G - 1) * a.D + span(min(lane + i * L, nv - 1)).at;
         load_param<V>(a.w, c, 1.f, w[i]);
         load_param<V>(a.b, c, 0.f, b[i]);
 #pragma unroll
         for (int k = 0; k < V; ++k) dw[i][k] = db[i][k] = 0.0;
     }
-    const double inv = 1.0 / (double)a.D;
+    const double inv = 1.0 / (POINTS ? (double)a.S * a.D : (double)a.D);
     for (long long n = on ? (long long)nb * per + side : a.N; n < a.N; n += (long long)a.blocks_n * per) {
         const T* x = (const T*)a.x + n * a.x_sn + (long long)g * a.D;
         const T* dy = (const T*)a.dy + n * a.dy_sn + (long long)g * a.D;
@@ -207,45 +223,61 @@ __global__ __launch_bounds__(kGnThreads) void gn_unit_bwd_kernel(GnArgs a) {
         float xv[I][V], dv[I][V];
 #pragma unroll
         for (int i = 0; i < I; ++i) {
-            const int at = Span<V, EVEN>(min(lane + i * L, nv - 1), a.D).at;
-            load_vec<T, V>(x + at, xv[i]);
-            load_vec<T, V>(dy + at, dv[i]);
+            const int e = min(lane + i * L, nv - 1), at = span(e).at;
+            load_vec<T, V>(x + (POINTS ? point(e) * a.x_ss : 0) + at, xv[i]);
+            load_vec<T, V>(dy + (POINTS ? point(e) * a.dy_ss : 0) + at, dv[i]);
         }
         double s1 = 0.0, s2 = 0.0;
 #pragma unroll
         for (int i = 0; i < I; ++i) {
-            const int skip = lane + i * L < nv ? Span<V, EVEN>(lane + i * L, a.D).skip : V;
+            const int skip = lane + i * L < nv ? span(lane + i * L).skip : V;
 #pragma unroll
             for (int k = 0; k < V; ++k) {
-                const double xh = ((double)xv[i][k] - mean) * rstd;
-                const double dz = (double)(dv[i][k] * act_slope(fma(xh, (double)w[i][k], (double)b[i][k]), a.act, a.slope));
-                const double wd = dz * w[i][k];
+                const double d = (double)xv[i][k] - mean, xh = d * rstd;
+                dv[i][k] *= act_slope(fma(d, rstd * (double)w[i][k], (double)b[i][k]), a.act, a.slope);
+                const double dz = (double)dv[i][k], wd = dz * (double)w[i][k];
                 if (k >= skip) {
                     dw[i][k] = fma(dz, xh, dw[i][k]);
                     db[i][k] += dz;
                     s1 += wd;
                     s2 = fma(wd, xh, s2);
                 }
-                xv[i][k] = (float)xh;
-                dv[i][k] = (float)wd;
             }
         }
-        const double m1 = lane_sum(s1, L) * inv, m2 = lane_sum(s2, L) * inv;
-        const float f1 = (float)m1, f2 = (float)m2, fr = (float)rstd;
+        // dx = (rstd w) dz + ((x - mean) c2 + c1), as in the resident route: a sample's gradients do not depend on how many there are
+        const double c1 = -rstd * (lane_sum(s1, L) * inv), c2 = -rstd * rstd * (lane_sum(s2, L) * inv);
 #pragma unroll
         for (int i = 0; i < I; ++i) {
             const int e = lane + i * L;
             if (e >= nv) continue;
             float o[V];
 #pragma unroll
-            for (int k = 0; k < V; ++k) o[k] = fr * (dv[i][k] - f1 - xv[i][k] * f2);
-            store_vec<T, V>((T*)a.out + n * a.C + g * a.D + Span<V, EVEN>(e, a.D).at, o);
+            for (int k = 0; k < V; ++k)
+                o[k] = fmaf((float)(rstd * (double)w[i][k]), dv[i][k], (float)fma((double)xv[i][k] - mean, c2, c1));
+            store_vec<T, V>((T*)a.out + (POINTS ? n * a.S + point(e) : n) * a.C + g * a.D + span(e).at, o);
         }
     }
     if (!a.part) return;
     // the samples side by side are added up here: 1024 x 2048 f32 in one group left 17 MB of partial sums for 25 MB of data
     __shared__ double sh[kGnThreads * V * 2];
     float* p = (float*)a.part + 2ll * a.C * nb;
+    if constexpr (POINTS) {   // first over the points, then over the samples
+#pragma unroll
+        for (int k = 0; k < V; ++k) {
+            sh[(k * 2) * kGnThreads + threadIdx.x] = dw[0][k];
+            sh[(k * 2 + 1) * kGnThreads + threadIdx.x] = db[0][k];
+        }
+        const int s = point(lane), first = lane < per_row;
+        fold<2 * V>(sh, on && s < a.S ? s : (int)a.S, (int)a.S, per_row);
+        fold<2 * V>(sh, on && first ? side : per, per, a.G * L);
+        if (!on || side || !first) return;
+#pragma unroll
+        for (int k = 0; k < V; ++k) {
+            p[2 * (g * a.D + lane * V + k)] = (float)sh[(k * 2) * kGnThreads + threadIdx.x];
+            p[2 * (g * a.D + lane * V + k) + 1] = (float)sh[(k * 2 + 1) * kGnThreads + threadIdx.x];
+        }
+        return;
+    }
 #pragma unroll
     for (int i = 0; i < I; ++i) {
         if (per > 1) {
@@ -265,7 +297,7 @@ __global__ __launch_bounds__(kGnThreads) void gn_unit_bwd_kernel(GnArgs a) {
                     }
         }
         const int e = lane + i * L;
-        const Span<V, EVEN> at(e, a.D);
+        const Span<V, EVEN> at = span(e);
         if (on && side == 0 && e < nv)
 #pragma unroll
             for (int k = 0; k < V; ++k)
@@ -286,20 +318,6 @@ __device__ __forceinline__ Tile tile_of(const GnArgs& a, int vecs, int by) {
     t.vx = by * a.tx + (int)threadIdx.x - t.ty * a.tx;
     t.on = t.ty < t.rows && t.vx < vecs;
     return t;
-}
-
-// Adds up the entries of n threads `stride` apart, y = 0 .. n - 1 the thread's own number among them, halving n: the first has the sum, in a
-// fixed order.  sh: [N][blockDim.x], entry k of thread t at k * blockDim.x + t; every thread of the workgroup calls it.
-template <int N> __device__ __forceinline__ void fold(double* sh, int y, int n, int stride) {
-    __syncthreads();
-    while (n > 1) {
-        const int h = (n + 1) / 2;
-        if (y < n - h)
-#pragma unroll
-            for (int k = 0; k < N; ++k) sh[k * blockDim.x + threadIdx.x] += sh[k * blockDim.x + threadIdx.x + h * stride];
-        n = h;
-        __syncthreads();
-    }
 }
 
 // sums a per-thread (p, q)[V] over the workgroup's rows; row 0 of each column holds the result
@@ -900,11 +918,12 @@ void gn_tile_plan(GnPlan& P, long long N, long long S, int C) {
     P.chunks = (int)((S + P.chunk_rows - 1) / P.chunk_rows);
 }
 
-// A group in a part of a wave's registers, 8 vectors a lane at most; backward: rows (S = 1).
+// A group in a part of a wave's registers, 8 vectors a lane at most; points backward: one.
 bool gn_unit_plan(GnPlan& P, long long S, int D, bool backward) {
-    if (S != 1 && (backward || S > 64 * kUnitItems)) return false;
+    const int most = 64 * (backward && S != 1 ? 1 : kUnitItems);
+    if (S > most) return false;
     const long long nv = S * vectors(D, P.V);
-    if (nv > 64 * kUnitItems) return false;
+    if (nv > most) return false;
     P.lanes = 1;
     while (P.lanes < 64 && P.lanes < nv) P.lanes *= 2;
     P.items = 1;
@@ -954,7 +973,7 @@ void gn_unit_bwd_grid(GnPlan& P, long long N, int G) {
 }
 
 // Ranges of rows in the sum that makes dw and db: one where the launch is a latency or two long, else of 512 rows or more
-// (20000 samples of 2 x 16: the backward pass takes 114 us in all, 182 with one range)
+// (20000 samples of 2 x 16, resident: the backward pass takes 114 us in all, 182 with one range)
 int gn_ranges(long long rows) { return rows <= 1024 ? 1 : rows < 64 * 512 ? (int)((rows + 511) / 512) : 64; }
 
 int gn_check(long long N, long long S, int C, int G, int act, int dtype, const char* who) {
@@ -984,12 +1003,14 @@ size_t gn_plan(GnPlan& P, long long N, long long S, int C, int G, int dtype, boo
     if (!P.unit) P.V = gn_width(dtype, D, false);
     P.res = (S > 1 || !P.unit) && gn_res_plan(P, N, S, C, G);
     // Points that fit both go to the units unless those take 1.5 times the resident route's threads (a lane with a vector costs 8 ns a
-    // thousand, a thread with its rows 12 to 17).  Unit against resident, forward, us: 20000 x 2 x 16 bf16 in 2 groups 3.8 / 26, 4000 x 16 x 32
-    // f32 in 4 8.0 / 11.5, 3000 x 9 x 33 bf16 in 11 11 / 19, 300 x 37 x 15 f32 in 5 4.5 / 5.4, 64 x 100 x 15 in 5 6.0 / 4.6, 1779 x 6 x 459 bf16
-    // in 51 50 / 37, 256 x 256 x 128 in 8 30 / 15; rows 1024 x 512 f32 in 32 4.3 / 16.9, backward 9.7 / 26.4.
+    // thousand, a thread with its rows 12 to 17), backward where there are samples for every slot too.  Unit against resident, us, forward:
+    // 20000 x 2 x 16 bf16 in 2 groups 3.8 / 26, 4000 x 16 x 32 f32 in 4 8.0 / 11.5, 3000 x 9 x 33 bf16 in 11 11 / 19, 300 x 37 x 15 f32 in 5
+    // 4.5 / 5.4, 64 x 100 x 15 in 5 6.0 / 4.6, 1779 x 6 x 459 bf16 in 51 50 / 37, 256 x 256 x 128 in 8 30 / 15; backward: 20000 x 2 x 16 14 /
+    // 123, 4096 x 4 x 256 in 32 20 / 92, 4000 x 16 x 32 19 / 29, 64 x 64 x 64 in 8 12.4 / 9.3; rows 1024 x 512 f32 in 32 4.3 / 16.9 and 9.7 /
+    // 26.4.
     if (P.unit && P.res) {
         const long long lanes = N * G * P.lanes * P.items, threads = N * P.res_blocks * P.res_threads;
-        P.unit = 2 * lanes <= 3 * threads;
+        P.unit = 2 * lanes <= 3 * threads && !(backward && N * P.res_blocks < 512);
         P.res = !P.unit;
     }
     P.part = P.more = 0;
@@ -1033,6 +1054,16 @@ template <typename P> void gn_param_grad(const GnArgs& a, const P* part, long lo
         case 4: hipLaunchKernelGGL((kernel<T, V, EVEN, 4>), grid, block, 0, st, a); break;                                     \
         default: hipLaunchKernelGGL((kernel<T, V, EVEN, 8>), grid, block, 0, st, a); break;                                    \
     }
+#define GN_UNIT_ROWS_I(EVEN)                                                                                                  \
+    switch (P.items) {                                                                                                        \
+        case 1: hipLaunchKernelGGL((gn_unit_bwd_kernel<T, V, EVEN, 1, false>), grid, block, 0, st, a); break;                  \
+        case 2: hipLaunchKernelGGL((gn_unit_bwd_kernel<T, V, EVEN, 2, false>), grid, block, 0, st, a); break;                  \
+        case 4: hipLaunchKernelGGL((gn_unit_bwd_kernel<T, V, EVEN, 4, false>), grid, block, 0, st, a); break;                  \
+        default: hipLaunchKernelGGL((gn_unit_bwd_kernel<T, V, EVEN, 8, false>), grid, block, 0, st, a); break;                 \
+    }
+#define GN_UNIT_ROWS                                                                                                          \
+    if (V == 1 || a.D % V == 0) { GN_UNIT_ROWS_I(true) }                                                                      \
+    else { GN_UNIT_ROWS_I((V == 1)) }
 #define GN_UNIT(kernel)                                                                                                       \
     if (V == 1 || a.D % V == 0) { GN_UNIT_I(kernel, true) }                                                                   \
     else { GN_UNIT_I(kernel, (V == 1)) }
@@ -1068,7 +1099,8 @@ template <typename T, int V> int gn_backward_v(const GnPlan& P, GnArgs& a, hipSt
     if (P.unit) {
         if (!a.dw) a.part = nullptr;
         const dim3 grid((unsigned)P.blocks_g * P.blocks_n);
-        GN_UNIT(gn_unit_bwd_kernel)
+        if (a.S == 1) { GN_UNIT_ROWS }
+        else hipLaunchKernelGGL((gn_unit_bwd_kernel<T, V, true, 1, true>), grid, block, 0, st, a);
         if (a.dw) gn_param_grad(a, (const float*)a.part, P.blocks_n, st);
         return check_launch("group_norm backward");
     }

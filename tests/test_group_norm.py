@@ -333,3 +333,22 @@ def test_groups_and_addresses_that_no_vector_divides(shape, dtype):
     y, st = ops.group_norm_act_forward(odd, groups, w.cuda(), b.cuda())
     assert torch.equal(y, ops.group_norm_act_forward(x.cuda(), groups, w.cuda(), b.cuda())[0])
     assert all(bool((t[:, :, 0] == 7).all() and (t[:, :, 1 + c:] == 7).all()) for t in wide) and bool((flat[-4:] == 7).all())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=["f32", "bf16"])
+@pytest.mark.parametrize("shape", [(1100, 5, 64, 4), (600, 32, 64, 32), (700, 9, 24, 3), (5000, 2, 2, 1), (513, 64, 4, 4), (520, 3, 21, 1), (1030, 33, 8, 1)],
+                         ids=lambda s: "x".join(map(str, s)))
+def test_many_small_samples(shape, dtype):
+    """A few points each: a group in a part of a wave in both directions, samples side by side."""
+    n, s, c, groups = shape
+    x, dy, w, b = data((n, s, c), dtype, 21)
+    _, dx, _, _ = check(x, dy, groups, w, b, act="silu")
+    wide = [torch.full((n, s, c + 5), 7.0, dtype=dtype, device="cuda") for _ in range(2)]
+    xv, dyv = (t[:, :, 3:3 + c] for t in wide)
+    xv.copy_(x)
+    dyv.copy_(dy)
+    check(xv, dyv, groups, None, b)
+    st = ops.group_norm_act_forward(xv, groups, w.cuda(), b.cuda(), act="silu")[1]
+    only = ops.group_norm_act_backward(dyv, xv, groups, w.cuda(), b.cuda(), 1e-5, "silu", 0.2, st, param_grads=False)
+    assert torch.equal(only[0], dx) and only[1] is None and only[2] is None
