@@ -31,7 +31,6 @@ namespace {
 
 constexpr int kGnThreads = 256;
 constexpr int kMergeThreads = 1024;
-constexpr int kUnitItems = 8;   // vectors of a group one lane holds, at most
 
 // V elements of memory, one access at any address that an element may have (global memory is accessed unaligned): rows of any pitch
 template <typename T, int V> struct Vec { T e[V]; };
@@ -124,6 +123,23 @@ __device__ __forceinline__ double lane_sum(double v, int lanes) {
     return v;
 }
 
+// sum of v over the workgroup, in a fixed order, for every thread
+__device__ __forceinline__ double block_sum(double v, double* sh /* blockDim.x / 64 */) {
+    v = lane_sum(v, 64);
+    __syncthreads();
+    if ((threadIdx.x & 63) == 0) sh[threadIdx.x >> 6] = v;
+    __syncthreads();
+    double s = 0.0;
+    for (int i = 0; i < (int)blockDim.x / 64; ++i) s += sh[i];
+    return s;
+}
+
+// a lane's value summed over the lanes of its group: `lanes` of a wave, or (WIDE) the workgroup
+template <bool WIDE> __device__ __forceinline__ double group_sum(double v, int lanes, double* sh /* WIDE: blockDim.x / 64 */) {
+    if constexpr (WIDE) return block_sum(v, sh);
+    else return lane_sum(v, lanes);
+}
+
 // Adds up the entries of n threads `stride` apart, y = 0 .. n - 1 the thread's own number among them, halving n: the first has the sum, in a
 // fixed order.  sh: [N][blockDim.x], entry k of thread t at k * blockDim.x + t; every thread of the workgroup calls it.
 template <int N> __device__ __forceinline__ void fold(double* sh, int y, int n, int stride) {
@@ -139,9 +155,10 @@ template <int N> __device__ __forceinline__ void fold(double* sh, int y, int n, 
 }
 
 // ------------------------------------------------------------------------------------------------ unit route
-template <typename T, int V, bool EVEN, int I>
+template <typename T, int V, bool EVEN, int I, bool WIDE>
 __global__ __launch_bounds__(kGnThreads) void gn_unit_fwd_kernel(GnArgs a) {
-    const int L = a.lanes, lane = threadIdx.x & (L - 1);
+    __shared__ double wide[WIDE ? kGnThreads / 64 : 1];
+    const int L = WIDE ? kGnThreads : a.lanes, lane = threadIdx.x & (L - 1);
     const long long u = ((long long)blockIdx.x * kGnThreads + threadIdx.x) / L;
     if (u >= a.N * a.G) return;   // whole groups of L lanes leave together: the shuffles below stay inside a group
     const unsigned n = (unsigned)u / (unsigned)a.G, g = (unsigned)u - n * (unsigned)a.G;
@@ -166,7 +183,7 @@ __global__ __launch_bounds__(kGnThreads) void gn_unit_fwd_kernel(GnArgs a) {
         for (int k = 0; k < V; ++k)
             if (k >= skip(i)) sum += (double)v[i][k];
     const double count = (double)a.S * a.D;
-    const double mean = lane_sum(sum, L) / count;   // (a constant group's mean is exact: z = bias there, not beside it)
+    const double mean = group_sum<WIDE>(sum, L, wide) / count;   // (a constant group's mean is exact: z = bias there, not beside it)
     double m2 = 0.0;
 #pragma unroll
     for (int i = 0; i < I; ++i)
@@ -175,7 +192,7 @@ __global__ __launch_bounds__(kGnThreads) void gn_unit_fwd_kernel(GnArgs a) {
             const double d = (double)v[i][k] - mean;
             if (k >= skip(i)) m2 = fma(d, d, m2);
         }
-    const double rstd = 1.0 / sqrt(lane_sum(m2, L) / count + a.eps);
+    const double rstd = 1.0 / sqrt(group_sum<WIDE>(m2, L, wide) / count + a.eps);
     if (a.stats && lane == 0) {
         a.stats[2 * u] = mean;
         a.stats[2 * u + 1] = rstd;
@@ -194,9 +211,10 @@ __global__ __launch_bounds__(kGnThreads) void gn_unit_fwd_kernel(GnArgs a) {
 
 // Backward: a lane keeps its channels while it walks over the samples n, so that dw and db need no exchange between lanes until the
 // end; every workgroup row leaves one partial (64-bit sums, stored as fp32) per channel.  POINTS: S > 1, a lane has a vector of a point.
-template <typename T, int V, bool EVEN, int I, bool POINTS>
+template <typename T, int V, bool EVEN, int I, bool WIDE, bool POINTS>
 __global__ __launch_bounds__(kGnThreads) void gn_unit_bwd_kernel(GnArgs a) {
-    const int L = a.lanes, lane = threadIdx.x & (L - 1), slot = threadIdx.x / L, slots = kGnThreads / L;
+    __shared__ double wide[WIDE ? kGnThreads / 64 : 1];
+    const int L = WIDE ? kGnThreads : a.lanes, lane = threadIdx.x & (L - 1), slot = threadIdx.x / L, slots = kGnThreads / L;
     const int per = a.G < slots ? slots / a.G : 1;             // samples side by side in a workgroup
     const int g = a.G < slots ? slot % a.G : (int)(blockIdx.x % a.blocks_g) * slots + slot;
     const int side = a.G < slots ? slot / a.G : 0;
@@ -234,7 +252,7 @@ __global__ __launch_bounds__(kGnThreads) void gn_unit_bwd_kernel(GnArgs a) {
 #pragma unroll
             for (int k = 0; k < V; ++k) {
                 const double d = (double)xv[i][k] - mean, xh = d * rstd;
-                dv[i][k] *= act_slope(fma(d, rstd * (double)w[i][k], (double)b[i][k]), a.act, a.slope);
+                dv[i][k] *= act_slope(fma(xh, (double)w[i][k], (double)b[i][k]), a.act, a.slope);
                 const double dz = (double)dv[i][k], wd = dz * (double)w[i][k];
                 if (k >= skip) {
                     dw[i][k] = fma(dz, xh, dw[i][k]);
@@ -245,7 +263,8 @@ __global__ __launch_bounds__(kGnThreads) void gn_unit_bwd_kernel(GnArgs a) {
             }
         }
         // dx = (rstd w) dz + ((x - mean) c2 + c1), as in the resident route: a sample's gradients do not depend on how many there are
-        const double c1 = -rstd * (lane_sum(s1, L) * inv), c2 = -rstd * rstd * (lane_sum(s2, L) * inv);
+        const double c1 = -rstd * (group_sum<WIDE>(s1, L, wide) * inv), c2 = -rstd * rstd * (group_sum<WIDE>(s2, L, wide) * inv);
+        const float fr = (float)rstd;
 #pragma unroll
         for (int i = 0; i < I; ++i) {
             const int e = lane + i * L;
@@ -253,13 +272,13 @@ __global__ __launch_bounds__(kGnThreads) void gn_unit_bwd_kernel(GnArgs a) {
             float o[V];
 #pragma unroll
             for (int k = 0; k < V; ++k)
-                o[k] = fmaf((float)(rstd * (double)w[i][k]), dv[i][k], (float)fma((double)xv[i][k] - mean, c2, c1));
+                o[k] = fmaf(fr * w[i][k], dv[i][k], (float)fma((double)xv[i][k] - mean, c2, c1));
             store_vec<T, V>((T*)a.out + (POINTS ? n * a.S + point(e) : n) * a.C + g * a.D + span(e).at, o);
         }
     }
     if (!a.part) return;
     // the samples side by side are added up here: 1024 x 2048 f32 in one group left 17 MB of partial sums for 25 MB of data
-    __shared__ double sh[kGnThreads * V * 2];
+    __shared__ double sh[WIDE ? 1 : kGnThreads * V * 2];
     float* p = (float*)a.part + 2ll * a.C * nb;
     if constexpr (POINTS) {   // first over the points, then over the samples
 #pragma unroll
@@ -280,7 +299,7 @@ __global__ __launch_bounds__(kGnThreads) void gn_unit_bwd_kernel(GnArgs a) {
     }
 #pragma unroll
     for (int i = 0; i < I; ++i) {
-        if (per > 1) {
+        if (!WIDE && per > 1) {
             __syncthreads();
 #pragma unroll
             for (int k = 0; k < V; ++k) {
@@ -385,17 +404,6 @@ __global__ __launch_bounds__(kGnThreads) void gn_tile_sum_kernel(GnArgs a) {
             o[0] = p[k];
             o[1] = q[k];
         }
-}
-
-// sum of v over the workgroup, in a fixed order, for every thread
-__device__ __forceinline__ double block_sum(double v, double* sh /* blockDim.x / 64 */) {
-    v = lane_sum(v, 64);
-    __syncthreads();
-    if ((threadIdx.x & 63) == 0) sh[threadIdx.x >> 6] = v;
-    __syncthreads();
-    double s = 0.0;
-    for (int i = 0; i < (int)blockDim.x / 64; ++i) s += sh[i];
-    return s;
 }
 
 // The sums part[..][C][2] of one (n, g) over the row ranges, channel by channel: `use(c, p, q)` runs for each channel once, in one
@@ -829,7 +837,7 @@ __global__ __launch_bounds__(kResThreads) void gn_res_bwd_kernel(GnArgs a) {
     const double c1 = -rstd * (s1 * inv), c2 = -rstd * rstd * (s2 * inv);
     T* o = (T*)a.out + (long long)t.n * S * a.C + c0;
 #pragma unroll
-    for (int k = 0; k < V; ++k) w[k] = (float)(rstd * (double)w[k]);
+    for (int k = 0; k < V; ++k) w[k] *= (float)rstd;
 #pragma unroll
     for (int r = 0; r < R; ++r) {
         const int row = t.ty + r * t.rows;
@@ -918,14 +926,14 @@ void gn_tile_plan(GnPlan& P, long long N, long long S, int C) {
     P.chunks = (int)((S + P.chunk_rows - 1) / P.chunk_rows);
 }
 
-// A group in a part of a wave's registers, 8 vectors a lane at most; points backward: one.
+// A group in the registers of a part of a wave, 4 vectors a lane at most (points backward: one), or, rows, of a workgroup, 32 elements a thread
+// at most (8192 x 4096 bf16 in one group: 107 us forward and 754 backward with 8 vectors a lane of a wave, which spills, 62 and 78 so).
 bool gn_unit_plan(GnPlan& P, long long S, int D, bool backward) {
-    const int most = 64 * (backward && S != 1 ? 1 : kUnitItems);
-    if (S > most) return false;
-    const long long nv = S * vectors(D, P.V);
-    if (nv > most) return false;
+    const long long nv = S * (long long)vectors(D, P.V), most = S == 1 ? 256ll * (32 / P.V > 8 ? 8 : 32 / P.V) : backward ? 64 : 256;
+    if (S > most || nv > most) return false;
     P.lanes = 1;
-    while (P.lanes < 64 && P.lanes < nv) P.lanes *= 2;
+    if (nv > 256) P.lanes = kGnThreads;
+    else while (P.lanes < 64 && P.lanes < nv) P.lanes *= 2;
     P.items = 1;
     while (P.items * P.lanes < nv) P.items *= 2;
     return true;
@@ -1047,26 +1055,21 @@ template <typename P> void gn_param_grad(const GnArgs& a, const P* part, long lo
     else if (act == DGG_ACT_SILU) hipLaunchKernelGGL((kernel<T, V, DGG_ACT_SILU>), grid, block, 0, st, a);              \
     else hipLaunchKernelGGL((kernel<T, V, DGG_ACT_NONE>), grid, block, 0, st, a);
 
-#define GN_UNIT_I(kernel, EVEN)                                                                                                \
-    switch (P.items) {                                                                                                        \
-        case 1: hipLaunchKernelGGL((kernel<T, V, EVEN, 1>), grid, block, 0, st, a); break;                                     \
-        case 2: hipLaunchKernelGGL((kernel<T, V, EVEN, 2>), grid, block, 0, st, a); break;                                     \
-        case 4: hipLaunchKernelGGL((kernel<T, V, EVEN, 4>), grid, block, 0, st, a); break;                                     \
-        default: hipLaunchKernelGGL((kernel<T, V, EVEN, 8>), grid, block, 0, st, a); break;                                    \
-    }
-#define GN_UNIT_ROWS_I(EVEN)                                                                                                  \
-    switch (P.items) {                                                                                                        \
-        case 1: hipLaunchKernelGGL((gn_unit_bwd_kernel<T, V, EVEN, 1, false>), grid, block, 0, st, a); break;                  \
-        case 2: hipLaunchKernelGGL((gn_unit_bwd_kernel<T, V, EVEN, 2, false>), grid, block, 0, st, a); break;                  \
-        case 4: hipLaunchKernelGGL((gn_unit_bwd_kernel<T, V, EVEN, 4, false>), grid, block, 0, st, a); break;                  \
-        default: hipLaunchKernelGGL((gn_unit_bwd_kernel<T, V, EVEN, 8, false>), grid, block, 0, st, a); break;                 \
-    }
-#define GN_UNIT_ROWS                                                                                                          \
-    if (V == 1 || a.D % V == 0) { GN_UNIT_ROWS_I(true) }                                                                      \
-    else { GN_UNIT_ROWS_I((V == 1)) }
-#define GN_UNIT(kernel)                                                                                                       \
-    if (V == 1 || a.D % V == 0) { GN_UNIT_I(kernel, true) }                                                                   \
-    else { GN_UNIT_I(kernel, (V == 1)) }
+// items: 1, 2, 4 vectors a lane of a wave; 2, 4, 8 (16 bits: 4) widest ones a thread of a workgroup
+#define GN_UNIT_I(kernel, EVEN, ...)                                                                                          \
+    if (P.lanes == kGnThreads) {                                                                                              \
+        if constexpr (V == 16 / (int)sizeof(T)) {                                                                             \
+            if (P.items == 2) hipLaunchKernelGGL((kernel<T, V, EVEN, 2, true __VA_ARGS__>), grid, block, 0, st, a);            \
+            else if (P.items == 4 || V == 8) hipLaunchKernelGGL((kernel<T, V, EVEN, 4, true __VA_ARGS__>), grid, block, 0, st, a); \
+            else hipLaunchKernelGGL((kernel<T, V, EVEN, V == 8 ? 4 : 8, true __VA_ARGS__>), grid, block, 0, st, a);            \
+        }                                                                                                                     \
+    } else if (P.items == 1) hipLaunchKernelGGL((kernel<T, V, EVEN, 1, false __VA_ARGS__>), grid, block, 0, st, a);            \
+    else if (P.items == 2) hipLaunchKernelGGL((kernel<T, V, EVEN, 2, false __VA_ARGS__>), grid, block, 0, st, a);              \
+    else hipLaunchKernelGGL((kernel<T, V, EVEN, 4, false __VA_ARGS__>), grid, block, 0, st, a);
+#define GN_COMMA ,
+#define GN_UNIT(kernel, ...)                                                                                                  \
+    if (V == 1 || a.D % V == 0) { GN_UNIT_I(kernel, true, __VA_ARGS__) }                                                      \
+    else { GN_UNIT_I(kernel, (V == 1), __VA_ARGS__) }
 
 #define GN_RES(act, kernel, R)                                                                                             \
     if (act == DGG_ACT_LEAKY_RELU) hipLaunchKernelGGL((kernel<T, V, R, DGG_ACT_LEAKY_RELU>), grid, block, 0, st, a);       \
@@ -1077,7 +1080,7 @@ template <typename T, int V> int gn_forward_v(const GnPlan& P, GnArgs& a, hipStr
     if (P.unit) {
         const long long threads = a.N * a.G * P.lanes;
         const dim3 grid((unsigned)((threads + kGnThreads - 1) / kGnThreads)), block(kGnThreads);
-        GN_UNIT(gn_unit_fwd_kernel)
+        GN_UNIT(gn_unit_fwd_kernel, )
         return check_launch("group_norm forward");
     }
     if (P.res) {
@@ -1099,8 +1102,8 @@ template <typename T, int V> int gn_backward_v(const GnPlan& P, GnArgs& a, hipSt
     if (P.unit) {
         if (!a.dw) a.part = nullptr;
         const dim3 grid((unsigned)P.blocks_g * P.blocks_n);
-        if (a.S == 1) { GN_UNIT_ROWS }
-        else hipLaunchKernelGGL((gn_unit_bwd_kernel<T, V, true, 1, true>), grid, block, 0, st, a);
+        if (a.S == 1) { GN_UNIT(gn_unit_bwd_kernel, GN_COMMA false) }
+        else hipLaunchKernelGGL((gn_unit_bwd_kernel<T, V, true, 1, false, true>), grid, block, 0, st, a);
         if (a.dw) gn_param_grad(a, (const float*)a.part, P.blocks_n, st);
         return check_launch("group_norm backward");
     }

@@ -352,3 +352,18 @@ def test_many_small_samples(shape, dtype):
     st = ops.group_norm_act_forward(xv, groups, w.cuda(), b.cuda(), act="silu")[1]
     only = ops.group_norm_act_backward(dyv, xv, groups, w.cuda(), b.cuda(), 1e-5, "silu", 0.2, st, param_grads=False)
     assert torch.equal(only[0], dx) and only[1] is None and only[2] is None
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=["f32", "bf16"])
+@pytest.mark.parametrize("shape", [(5, 1, 1025, 1), (300, 1, 2048, 2), (70, 1, 4101, 1), (3, 1, 8192, 1), (3, 1, 8193, 1), (1030, 1, 2050, 2), (2, 1, 12001, 1)],
+                         ids=lambda s: "x".join(map(str, s)))
+def test_long_rows(shape, dtype):
+    """A group in a workgroup's registers, on both sides of what fits."""
+    n, s, c, groups = shape
+    x, dy, w, b = data((n, s, c), dtype, 31)
+    check(x, dy, groups, w, b, act="silu")
+    wide = torch.full((n, s, c + 3), 7.0, dtype=dtype, device="cuda")
+    xv = wide[:, :, 1:1 + c]
+    xv.copy_(x)
+    check(xv, dy, groups, w, None)
