@@ -236,7 +236,7 @@ def test_refusals_without_a_gpu():
         ops.group_norm_act_forward(torch.zeros(2, 8), 2)
     lib = _lib.lib()
     ws = lib.dgg_group_norm_workspace_bytes
-    assert ws(32, 2048, 256, 32, _lib.BF16, 0) > 0 and ws(32, 1, 512, 32, _lib.F32, 0) >= 0
+    assert ws(32, 2048, 256, 32, _lib.BF16, 1) > 0 and ws(4, 100000, 8, 2, _lib.F32, 0) > 0 and ws(32, 1, 512, 32, _lib.F32, 0) >= 0
     for bad in ((0, 1, 8, 2, 0, 0), (1, 0, 8, 2, 0, 0), (1, 1, 9, 2, 0, 0), (1, 1, 8, 0, 0, 0), (1, 1, 8, 2, 3, 0), (1 << 31, 1, 8, 2, 0, 0)):
         assert ws(*bad) == -1, bad
     f, b = lib.dgg_group_norm_act_forward, lib.dgg_group_norm_act_backward
@@ -244,6 +244,8 @@ def test_refusals_without_a_gpu():
     fwd = [one, 8, 8, 4, 1, 8, 2, None, None, 1e-5, 1, 0.2, 0, one, None, None, 0, None]
     for k, v in ((0, None), (13, None), (1, -1), (9, -1.0), (9, float("nan")), (10, 3), (12, 7), (6, 3)):
         assert f(*[v if i == k else a for i, a in enumerate(fwd)]) == -1, (k, v)
+    for k in (0, 13):                                                          # not an element's address
+        assert f(*[one + 2 if i == k else a for i, a in enumerate(fwd)]) == -1, k
     points = [one, 800, 8, 4, 100000, 8, 2, None, None, 1e-5, 1, 0.2, 0, one, None, None, 0, None]
     assert f(*points) == -3 and b"workspace" in lib.dgg_last_error()           # this size needs one
     bwd = [one, 8, 8, one, 8, 8, 4, 1, 8, 2, None, None, 1, 0.2, 0, one, one, None, None, None, 0, None]
