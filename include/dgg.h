@@ -156,8 +156,8 @@ int dgg_resblock_backward(int fin, const float* params, float* grads, void* ws, 
 
 /* Group normalisation with an activation over channels-last data — the batch-independent form of a ResBlock's BatchNorm +
  * LeakyReLU (networks.py:43-56 normalises over the batch instead).  x: N samples of S points (rows) of C channels, the channel
- * stride is 1, samples and points `*_stride_n` / `*_stride_s` ELEMENTS apart (a column block of a wider product needs no
- * copy); types DGG_F32 / DGG_BF16 / DGG_F16 for x, y, dy, dx alike, weight / bias (C, NULL = 1 / 0) and their gradients fp32:
+ * stride is 1, samples and points `*_stride_n` / `*_stride_s` ELEMENTS apart, at any element's address (a column block of a
+ * wider product needs no copy); types DGG_F32 / DGG_BF16 / DGG_F16 for x, y, dy, dx alike, weight / bias (C, NULL = 1 / 0) and their gradients fp32:
  *   mean, var over the S x C/groups elements of sample n and group g;  z = weight * (x - mean) / sqrt(var + eps) + bias;
  *   y = act(z): DGG_ACT_NONE, DGG_ACT_LEAKY_RELU (`slope` for z <= 0) or DGG_ACT_SILU (z * sigmoid(z)).
  * y and dx are contiguous (N, S, C) and overlap no input.  Statistics and z are 64-bit inside: the side of LeakyReLU's kink an element takes is the
