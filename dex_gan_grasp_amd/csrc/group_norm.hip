@@ -12,16 +12,16 @@
 // would take the wrong side for every element within its rounding error of zero.  (64-bit vector instructions run at the
 // rate of the fp32 ones here; per element they are 4 to 6 of them.)  What follows the sign is fp32, rounded once to the output type.
 //
-// Three routes, chosen by gn_run:
-//  * "unit": a group's S x D elements fit the registers of at most one wave.  L = 2^k lanes own one (n, g):
-//    one read of x, mean and centred variance by lane shuffles, no LDS, no barrier.  1024 x 512 f32 in 32 groups: 4.3 us forward,
-//    9.7 backward with dw and db (launches); 16384 x 512: 24 and 29 us (2.9 and 3.4 TB/s).
+// Three routes, chosen by gn_plan:
+//  * "unit": a group's S x D elements fit the registers of at most one wave, or, long rows, of a workgroup.  L = 2^k lanes own one
+//    (n, g): one read of x, mean and centred variance by lane shuffles.  1024 x 512 f32 in 32 groups: 4.2 us forward, 9.7 backward with dw
+//    and db (launches); 16384 x 512: 22 and 28 us (3.0 and 3.6 TB/s); 8192 x 4096 bf16 in one group 62 and 78.
 //  * "resident": a sample's points in a block of groups fit a workgroup's registers: one read, one launch.  128 x 2048 x 256 bf16
-//    in 32 groups: 71 us forward (3.8 TB/s), 140 backward (2.9 TB/s: the arithmetic and the memory take turns, one workgroup a CU).
+//    in 32 groups: 71 us forward (3.8 TB/s), 136 backward (3.0 TB/s: the arithmetic and the memory take turns, one workgroup a CU).
 //  * "tile": a workgroup owns a range of the rows of one sample and a block of channels (a thread keeps ITS channels while
 //    it walks down the rows), leaves per-channel partial sums in the workspace, and a small launch merges them in a fixed
 //    order into the groups' statistics (and dw, db); a last launch applies them.  No atomics: results do not depend on the
-//    order in which workgroups run.
+//    order in which workgroups run.  30 x 1000 x 1020 bf16 in 60 groups: 58 and 82 us (x is read twice, dy too).
 #include <type_traits>
 
 #include "dgg_internal.h"
