@@ -31,6 +31,7 @@ namespace {
 
 constexpr int kGnThreads = 256;
 constexpr int kMergeThreads = 1024;
+constexpr int kGnFew = 8;   // elements of a group, at most, whose dx may be what cancellation leaves (grad_few)
 
 // V elements of memory, one access at any address that an element may have (global memory is accessed unaligned): rows of any pitch
 template <typename T, int V> struct Vec { T e[V]; };
@@ -78,6 +79,12 @@ __device__ __forceinline__ float act_slope(double z, int act, float slope) {
         return s * (1.f + zf * (1.f - s));
     }
     return 1.f;
+}
+
+// dx in a group of up to kGnFew elements, d = x - mean, m1 = mean(w dz), k2 = -rstd mean(w dz xh): the three terms cancel — to 0 for one
+// element, to eps / (var + eps) of them for two —, so they are added up in 64 bits and rounded once; one element gives exactly 0.
+__device__ __forceinline__ float grad_few(double d, float dz, float w, double rstd, double m1, double k2) {
+    return (float)(rstd * fma(d, k2, fma((double)w, (double)dz, -m1)));
 }
 
 // V consecutive channels of weight or bias, or what stands for one that is not there (one branch for all of them)
@@ -234,6 +241,7 @@ __global__ __launch_bounds__(kGnThreads) void gn_unit_bwd_kernel(GnArgs a) {
         for (int k = 0; k < V; ++k) dw[i][k] = db[i][k] = 0.0;
     }
     const double inv = 1.0 / (POINTS ? (double)a.S * a.D : (double)a.D);
+    const bool few = !WIDE && (POINTS ? a.S * a.D : a.D) <= kGnFew;
     for (long long n = on ? (long long)nb * per + side : a.N; n < a.N; n += (long long)a.blocks_n * per) {
         const T* x = (const T*)a.x + n * a.x_sn + (long long)g * a.D;
         const T* dy = (const T*)a.dy + n * a.dy_sn + (long long)g * a.D;
@@ -262,8 +270,10 @@ __global__ __launch_bounds__(kGnThreads) void gn_unit_bwd_kernel(GnArgs a) {
                 }
             }
         }
-        // dx = (rstd w) dz + ((x - mean) c2 + c1), as in the resident route: a sample's gradients do not depend on how many there are
-        const double c1 = -rstd * (group_sum<WIDE>(s1, L, wide) * inv), c2 = -rstd * rstd * (group_sum<WIDE>(s2, L, wide) * inv);
+        // dx = rstd ((w dz - m1) + (x - mean) k2).  Groups of more than a few elements: rstd w and the rest are rounded to fp32 and joined by
+        // one fma (8192 x 4096 bf16 backward 66 us, 75 all in 64 bits)
+        const double m1 = group_sum<WIDE>(s1, L, wide) * inv, k2 = -rstd * (group_sum<WIDE>(s2, L, wide) * inv);
+        const double c1 = -rstd * m1, c2 = rstd * k2;
         const float fr = (float)rstd;
 #pragma unroll
         for (int i = 0; i < I; ++i) {
@@ -271,8 +281,10 @@ __global__ __launch_bounds__(kGnThreads) void gn_unit_bwd_kernel(GnArgs a) {
             if (e >= nv) continue;
             float o[V];
 #pragma unroll
-            for (int k = 0; k < V; ++k)
-                o[k] = fmaf(fr * w[i][k], dv[i][k], (float)fma((double)xv[i][k] - mean, c2, c1));
+            for (int k = 0; k < V; ++k) {
+                const double d = (double)xv[i][k] - mean;
+                o[k] = few ? grad_few(d, dv[i][k], w[i][k], rstd, m1, k2) : fmaf(fr * w[i][k], dv[i][k], (float)fma(d, c2, c1));
+            }
             store_vec<T, V>((T*)a.out + (POINTS ? n * a.S + point(e) : n) * a.C + g * a.D + span(e).at, o);
         }
     }
@@ -746,7 +758,9 @@ __global__ __launch_bounds__(kResThreads) void gn_res_bwd_kernel(GnArgs a) {
     Raw<T, V> rx[R];
     float dz[R][V];   // (kept: its activation's slope is most of the arithmetic, 128 x 2048 x 256 bf16 was bound by having it twice)
     float w[V], b[V];
-    double mean = 0.0, rstd = 0.0;
+    double mean = 0.0, rstd = 0.0, few1 = 0.0, few2 = 0.0;
+    constexpr bool kFew = V * (R == 4 ? 2 : R / 2 + 1) <= kGnFew;   // D >= V, and the fewest points that give a thread R rows
+    const bool few = kFew && S * a.D <= kGnFew;
     if (t.on) {
         Raw<T, V> rd[R];
 #pragma unroll
@@ -776,7 +790,15 @@ __global__ __launch_bounds__(kResThreads) void gn_res_bwd_kernel(GnArgs a) {
             }
             sh[((int)threadIdx.x * V + k) * 2] = (float)(p * rstd);
             sh[((int)threadIdx.x * V + k) * 2 + 1] = (float)q;
+            if constexpr (kFew) {
+                few1 = fma((double)w[k], q, few1);
+                few2 = fma((double)w[k], p * rstd, few2);
+            }
         }
+    }
+    if (few) {   // the threads' 64-bit sums, in the place of the groups'
+        sums[threadIdx.x] = few1;
+        sums[kResThreads + threadIdx.x] = few2;
     }
     // The columns' sums over the rows — a column: one of the two sums of one channel —, fp32 from each thread, added in 64 bits: `parts`
     // threads a column, then a wave a group, which also has the group's two means from them.
@@ -824,18 +846,48 @@ __global__ __launch_bounds__(kResThreads) void gn_res_bwd_kernel(GnArgs a) {
         }
         s1 = lane_sum(s1, 64);
         s2 = lane_sum(s2, 64);
-        if (lane == 0) {
+        if (lane == 0 && !few) {
             sums[2 * j] = s1;
             sums[2 * j + 1] = s2;
+        }
+    }
+    if (few) {   // a thread a group adds up its few threads'
+        few1 = few2 = 0.0;
+        if ((int)threadIdx.x < groups)
+            for (int y = 0; y < min(t.rows, S); ++y)
+                for (int e = 0; e < t.per; ++e) {
+                    few1 += sums[y * t.tx + (int)threadIdx.x * t.per + e];
+                    few2 += sums[kResThreads + y * t.tx + (int)threadIdx.x * t.per + e];
+                }
+        __syncthreads();
+        if ((int)threadIdx.x < groups) {
+            sums[2 * threadIdx.x] = few1;
+            sums[2 * threadIdx.x + 1] = few2;
         }
     }
     __syncthreads();
     if (!t.on) return;
     const double s1 = sums[2 * g], s2 = sums[2 * g + 1];
     const double inv = 1.0 / ((double)S * a.D);
-    // dx = (rstd w) dz + ((x - mean) c2 + c1)
-    const double c1 = -rstd * (s1 * inv), c2 = -rstd * rstd * (s2 * inv);
     T* o = (T*)a.out + (long long)t.n * S * a.C + c0;
+    if constexpr (kFew)
+        if (few) {
+            const double m1 = s1 * inv, k2 = -rstd * (s2 * inv);
+#pragma unroll
+            for (int r = 0; r < R; ++r) {
+                const int row = t.ty + r * t.rows;
+                if (row >= S) break;
+                float v[V];
+                rx[r].get(v);
+#pragma unroll
+                for (int k = 0; k < V; ++k) v[k] = grad_few((double)v[k] - mean, dz[r][k], w[k], rstd, m1, k2);
+                store_vec<T, V>(o + (long long)row * a.C, v);
+            }
+            return;
+        }
+    // dx = (rstd w) dz + ((x - mean) c2 + c1), rstd w and the sum in brackets rounded to fp32 (32 x 2048 x 256 bf16 29 us, 31 with all of it
+    // in 64 bits, for which there are not enough registers)
+    const double c1 = -rstd * (s1 * inv), c2 = -rstd * rstd * (s2 * inv);
 #pragma unroll
     for (int k = 0; k < V; ++k) w[k] *= (float)rstd;
 #pragma unroll

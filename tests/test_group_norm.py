@@ -369,3 +369,44 @@ def test_long_rows(shape, dtype):
     xv = wide[:, :, 1:1 + c]
     xv.copy_(x)
     check(xv, dy, groups, w, None)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16], ids=["f32", "bf16", "f16"])
+@pytest.mark.parametrize("c", [1, 7, 64, 515])
+def test_groups_of_one_element_have_no_gradient(c, dtype):
+    """One point and one channel a group: xh is 0 whatever x is, so dx is exactly 0 — the difference of w dz and its own mean."""
+    for n, act in ((1, "none"), (33, "leaky_relu"), (3000, "silu")):
+        x, dy, w, b = (t.cuda() for t in data((n, 1, c), dtype, 40 + n))
+        y, st = ops.group_norm_act_forward(x, c, w, b, 1e-5, act)
+        for ww, bb in ((w, b), (None, None)):
+            dx, dw, _ = ops.group_norm_act_backward(dy, x, c, ww, bb, 1e-5, act, 0.2, st)
+            assert not dx.any(), (n, act, float(dx.abs().max()))
+            assert not dw.any()
+
+
+# (N, S, C, groups): groups of two to eight elements, rows and points, few samples and many, a last workgroup with fewer groups
+SMALL_GROUPS = [(40, 1, 6, 3), (3000, 1, 12, 4), (7, 1, 64, 16), (9, 1, 35, 5), (5, 1, 8, 1), (3, 2, 8, 8), (600, 2, 4, 4), (2, 2, 6, 2), (2000, 3, 2, 1),
+                (5, 2, 33, 11), (1, 1, 2, 1), (2, 8, 16, 16), (1, 4, 16, 8), (700, 4, 512, 256), (1100, 8, 96, 96), (2, 2, 2052, 513), (3, 7, 515, 515),
+                (1, 2, 8192, 2048)]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16], ids=["f32", "bf16", "f16"])
+@pytest.mark.parametrize("shape", SMALL_GROUPS, ids=lambda s: "x".join(map(str, s)))
+def test_dx_of_small_groups_is_rounded_once(shape, dtype):
+    """In a group of a few elements the three terms of dx cancel nearly (two elements: to eps / (var + eps) of them), so they have to be
+    added up in 64 bits.  Without an activation dz is dy, every sum and product is a 64-bit one (2^-40 of the terms is far above what the
+    roundings of 2^-53 make of 8 of them with x within a few deviations of 0), and what is left is the rounding to fp32 and that to
+    the output type."""
+    n, s, c, g = shape
+    x, dy, w, b = data((n, s, c), dtype, 50 + n)
+    for ww in (w, None):
+        xd, dyd, wd = x.cuda(), dy.cuda(), None if ww is None else ww.cuda()
+        y, st = ops.group_norm_act_forward(xd, g, wd, None, 1e-5, "none")
+        dx, _, _ = ops.group_norm_act_backward(dyd, xd, g, wd, None, 1e-5, "none", 0.2, st)
+        r = reference(x, dy, g, ww, None, 1e-5, "none", 0.2)
+        xh = (r["z"] / (torch.ones(c) if ww is None else ww).double().view(g, -1)).abs()
+        wdz = (dy.double().reshape(r["dx"].shape) * (torch.ones(c) if ww is None else ww).double().view(g, -1)).abs()
+        terms = r["rstd"] * (wdz + wdz.mean((1, 3), keepdim=True) + xh * (wdz * xh).mean((1, 3), keepdim=True))
+        close(dx, r["dx"], half_step(dtype, r["dx"]) + U * r["dx"].abs() + 2.0 ** -40 * terms, "dx")
