@@ -79,7 +79,7 @@ struct NsArgs {
     NsMat mat[kNsMats];
     char* ws;
     NsUpdate update;
-    float decay;
+    float decay;             // lr wd
     int adjust;
     double lr, eps;
     int steps;
@@ -134,6 +134,13 @@ template <int N> __device__ __forceinline__ double block_sum(double v, double* s
 
 // u of the muon step from the gradient and the momentum AFTER its update
 __device__ __forceinline__ float muon_u(const NsUpdate& a, float g, float m) { return a.nesterov ? fmaf(a.mu, m, a.gscale * g) : m; }
+
+// W of the muon step.  What is taken off — lr f x and lr wd w — is added up before the one rounding against w: lr wd is often below the
+// spacing of fp32 under 1 (5e-8 for the trainers' lr 1e-4 and wd 5e-4), where 1 - lr wd as a factor would be 1.7 times too much decay or
+// none at all.  (An infinite parameter stays one.)
+__device__ __forceinline__ float muon_w(float w, float x, float step, float decay) {
+    return fabsf(w) < INFINITY ? w - fmaf(step, x, decay * w) : fmaf(-step, x, (1.f - decay) * w);
+}
 
 // ------------------------------------------------------------------------------------------------ norm
 // sum of squares in 64 bits, one partial a workgroup (muon: M is updated on the way).  Rows without gaps are one long row.
@@ -589,7 +596,7 @@ __global__ __launch_bounds__(kThreads, 2) void ns_apply_kernel(const NsArgs* arg
                     for (int q = 0; q < 4; ++q)
 #pragma unroll
                         for (int e = 0; e < 4; ++e)
-                            if (i + 8 * q + e < M.m && j < M.n) W[(8 * q + e) * di] = fmaf(-step, v[q][e], decay * w[q][e]);
+                            if (i + 8 * q + e < M.m && j < M.n) W[(8 * q + e) * di] = muon_w(w[q][e], v[q][e], step, decay);
                 } else {
                     Global<Out>* o = (Global<Out>*)M.out + at;
 #pragma unroll
@@ -862,7 +869,7 @@ __global__ __launch_bounds__(kSmallThreads) void ns_small_kernel(NsArgs a, NsFir
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
                     if (i + 8 * q + e >= M.m || j >= M.n) continue;
-                    if (MUON) W[at + (8 * q + e) * di] = fmaf(-step, v[q][e], decay * x[q][e]);
+                    if (MUON) W[at + (8 * q + e) * di] = muon_w(x[q][e], v[q][e], step, decay);
                     else ((Global<In>*)M.out)[(size_t)bat * M.out_stride + at + (8 * q + e) * di] = (In)v[q][e];
                 }
             }
@@ -1053,7 +1060,7 @@ __global__ __launch_bounds__(kNarrowThreads) void ns_narrow_kernel(const NsArgs*
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
             if (i + 8 * q + e >= M.m || j >= M.n) continue;
-            if (MUON) W[at + (8 * q + e) * di] = fmaf(-step, v[q][e], decay * y[q][e]);
+            if (MUON) W[at + (8 * q + e) * di] = muon_w(y[q][e], v[q][e], step, decay);
             else ((Global<In>*)M.out)[(size_t)bat * M.out_stride + at + (8 * q + e) * di] = (In)v[q][e];
         }
     }
@@ -1454,7 +1461,7 @@ int dgg_muon_step(const dgg_matrix* mats, int count, double lr, double momentum,
     a.update = {(float)momentum, (float)grad_scale, nesterov != 0};
     a.lr = lr;
     a.adjust = adjust;
-    a.decay = (float)(1.0 - lr * weight_decay);
+    a.decay = (float)(lr * weight_decay);
     a.eps = eps;
     return ns_run<float, true>(mats, count, a, coefficients, steps, ws, ws_bytes, (hipStream_t)stream, who);
 }

@@ -455,3 +455,38 @@ def test_offsets_beyond_32_bits():
         ops.orthogonalize(g, 1 << 33)
     del far, view, rows
     torch.cuda.empty_cache()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("shape", [(32, 500), (60, 2000), (512, 1025), (700, 300)], ids=lambda s: "%dx%d" % s)
+def test_a_small_weight_decay_is_the_one_asked_for(shape):
+    """lr wd = 5e-8 and half of it — the trainers' defaults — lie below the spacing of fp32 under 1: the parameters move by it on average,
+    beside the update that rounds each of them one way or the other.  sum sign(w) (w - w' - update) / sum |w| is lr wd, off by
+      the rounding of w' (one, so at most half a step of it; over n parameters six times the root mean square of a step / sqrt 12: the
+        update, many steps long and the same function of no parameter, spreads it evenly),
+      the update's own error, |error|_F <= lr f tol, so sqrt(n) lr f tol in the sum."""
+    w = matrix(*shape, seed=1, kind="normal")
+    g = matrix(*shape, seed=2, kind="normal")
+    for lr in (1e-4, 0.5e-4):
+        wd = 5e-4
+        p, m = w.cuda(), torch.zeros(shape, device="cuda")
+        ops.muon_step([p], [g.cuda()], [m], lr, 0.0, True, wd, adjust="match_rms")
+        ref, tol = reference(g)
+        f = 0.2 * math.sqrt(max(shape))
+        new = p.cpu().double()
+        total = float(w.double().abs().sum())
+        decay = float((w.double().sign() * (w.double() - new - lr * f * ref)).sum()) / total
+        step = torch.ldexp(torch.ones(shape, dtype=torch.float64), torch.frexp(new)[1] - 24)
+        allowed = (6 * float(((step ** 2).sum() / 12).sqrt()) + math.sqrt(w.numel()) * lr * f * tol) / total
+        assert allowed < 0.12 * lr * wd, (allowed, lr * wd)
+        assert abs(decay - lr * wd) <= allowed, (decay / (lr * wd), allowed / (lr * wd))
+
+
+@pytest.mark.gpu
+def test_infinite_parameters_stay_infinite():
+    for shape in ((20, 30), (30, 900), (100, 130)):
+        w = torch.ones(shape, device="cuda")
+        w[3, 4], w[5, 6] = float("inf"), -float("inf")
+        for wd in (0.0, 0.1):
+            ops.muon_step([w], [matrix(*shape, seed=3).cuda()], [torch.zeros(shape, device="cuda")], 0.1, weight_decay=wd)
+            assert w[3, 4] == float("inf") and w[5, 6] == -float("inf") and int(w.isfinite().sum()) == w.numel() - 2
