@@ -945,7 +945,10 @@ struct GnPlan {
     int tx, blocks_c, chunks, merge;   // merge: threads that merge a group's partial sums
     size_t part, more, ranges;         // tile: bytes of the partial sums and of the channels' sums; where gn_param_grad's begin
     long long chunk_rows;
+    bool fits;                         // false: a launch would need kGnMost threads or more
 };
+
+constexpr long long kGnMost = (1ll << 32) - 1024;   // threads of a launch: below 2^32 when rounded up to whole workgroups
 
 int elem_bytes(int dtype) { return dtype == DGG_F32 ? 4 : 2; }
 
@@ -1019,7 +1022,7 @@ bool gn_res_plan(GnPlan& P, long long N, long long S, int C, int G) {
     rows = P.res_threads / tx;
     const long long most = (S + rows - 1) / rows;
     P.res_rows = most <= 4 ? 4 : most <= 8 ? 8 : 16;
-    return N * P.res_blocks < 0x7fffffff;
+    return (long long)P.res_blocks * P.res_threads < kGnMost;   // (of one sample: gn_launches)
 }
 
 void gn_unit_bwd_grid(GnPlan& P, long long N, int G) {
@@ -1074,6 +1077,7 @@ size_t gn_plan(GnPlan& P, long long N, long long S, int C, int G, int dtype, boo
         P.res = !P.unit;
     }
     P.part = P.more = 0;
+    P.fits = true;
     size_t need = 0;
     if (P.unit) {
         if (backward) gn_unit_bwd_grid(P, N, G);
@@ -1084,6 +1088,7 @@ size_t gn_plan(GnPlan& P, long long N, long long S, int C, int G, int dtype, boo
         P.V = gn_width(dtype, C, false);
         gn_tile_plan(P, N, S, C);
         P.merge = (long long)P.chunks * D > 1024 ? kMergeThreads : kGnThreads;
+        P.fits = N * P.chunks * kGnThreads < kGnMost && N * G * P.merge < kGnMost && P.blocks_c <= 65535;
         const size_t chan = (size_t)N * C * 2 * sizeof(double);
         P.part = chan * P.chunks;
         P.more = backward && P.chunks > 1 ? chan : 0;
@@ -1100,6 +1105,22 @@ template <typename P> void gn_param_grad(const GnArgs& a, const P* part, long lo
     if (ranges > 1)
         hipLaunchKernelGGL((gn_param_grad_kernel<double>), dim3(grid.x), block, 0, st, (const double*)a.ranges, (long long)ranges, a.C, a.dw,
                            a.db, (double*)nullptr);
+}
+
+// launch(samples of a call): all of them, or, where they need `threads` each and kGnMost together, ranges of them in turn
+template <typename Launch> void gn_launches(const GnArgs& a, long long threads, int es, Launch launch) {
+    const long long most = kGnMost / threads;
+    if (a.N <= most) return launch(a);
+    for (long long n = 0; n < a.N; n += most) {
+        GnArgs r = a;
+        r.N = a.N - n < most ? a.N - n : most;
+        r.x = (const char*)a.x + n * a.x_sn * es;
+        r.dy = a.dy ? (const char*)a.dy + n * a.dy_sn * es : nullptr;
+        r.out = (char*)a.out + n * a.S * a.C * es;
+        r.stats = a.stats ? a.stats + 2 * n * a.G : nullptr;
+        r.chan = a.dw ? a.chan + 2 * n * a.C : nullptr;
+        launch(r);
+    }
 }
 
 #define GN_ACT(act, kernel, grid)                                                                                       \
@@ -1130,16 +1151,19 @@ template <typename P> void gn_param_grad(const GnArgs& a, const P* part, long lo
 
 template <typename T, int V> int gn_forward_v(const GnPlan& P, GnArgs& a, hipStream_t st) {
     if (P.unit) {
-        const long long threads = a.N * a.G * P.lanes;
-        const dim3 grid((unsigned)((threads + kGnThreads - 1) / kGnThreads)), block(kGnThreads);
-        GN_UNIT(gn_unit_fwd_kernel, )
+        gn_launches(a, (long long)a.G * P.lanes, sizeof(T), [&](const GnArgs& a) {
+            const dim3 grid((unsigned)((a.N * a.G * P.lanes + kGnThreads - 1) / kGnThreads)), block(kGnThreads);
+            GN_UNIT(gn_unit_fwd_kernel, )
+        });
         return check_launch("group_norm forward");
     }
     if (P.res) {
-        const dim3 grid((unsigned)(a.N * P.res_blocks)), block(P.res_threads);
-        if (P.res_rows == 4) { GN_RES(a.act, gn_res_fwd_kernel, 4) }
-        else if (P.res_rows == 8) { GN_RES(a.act, gn_res_fwd_kernel, 8) }
-        else { GN_RES(a.act, gn_res_fwd_kernel, 16) }
+        gn_launches(a, (long long)P.res_blocks * P.res_threads, sizeof(T), [&](const GnArgs& a) {
+            const dim3 grid((unsigned)(a.N * P.res_blocks)), block(P.res_threads);
+            if (P.res_rows == 4) { GN_RES(a.act, gn_res_fwd_kernel, 4) }
+            else if (P.res_rows == 8) { GN_RES(a.act, gn_res_fwd_kernel, 8) }
+            else { GN_RES(a.act, gn_res_fwd_kernel, 16) }
+        });
         return check_launch("group_norm forward");
     }
     const dim3 grid((unsigned)(a.N * P.chunks), P.blocks_c), block(kGnThreads);
@@ -1160,10 +1184,12 @@ template <typename T, int V> int gn_backward_v(const GnPlan& P, GnArgs& a, hipSt
         return check_launch("group_norm backward");
     }
     if (P.res) {
-        const dim3 grid((unsigned)(a.N * P.res_blocks)), block(P.res_threads);
-        if (P.res_rows == 4) { GN_RES(a.act, gn_res_bwd_kernel, 4) }
-        else if (P.res_rows == 8) { GN_RES(a.act, gn_res_bwd_kernel, 8) }
-        else { GN_RES(a.act, gn_res_bwd_kernel, 16) }
+        gn_launches(a, (long long)P.res_blocks * P.res_threads, sizeof(T), [&](const GnArgs& a) {
+            const dim3 grid((unsigned)(a.N * P.res_blocks)), block(P.res_threads);
+            if (P.res_rows == 4) { GN_RES(a.act, gn_res_bwd_kernel, 4) }
+            else if (P.res_rows == 8) { GN_RES(a.act, gn_res_bwd_kernel, 8) }
+            else { GN_RES(a.act, gn_res_bwd_kernel, 16) }
+        });
         if (a.dw) gn_param_grad(a, (const double*)a.chan, a.N, st);
         return check_launch("group_norm backward");
     }
@@ -1183,10 +1209,17 @@ template <typename T> int gn_dispatch(bool backward, const GnPlan& P, GnArgs& a,
     return backward ? gn_backward_v<T, 1>(P, a, st) : gn_forward_v<T, 1>(P, a, st);
 }
 
+int gn_refuse(long long N, long long S, int C, int G, const char* who) {
+    set_error_text("%s: %lld samples of %lld points of %d channels in %d groups need a launch of 2^32 threads or of more than 65535 blocks of "
+                   "channels", who, N, S, C, G);
+    return DGG_ERR_INVALID;
+}
+
 int gn_run(bool backward, GnArgs& a, int dtype, void* ws, size_t ws_bytes, hipStream_t st, const char* who) {
     a.D = a.C / a.G;
     GnPlan P = {};
     const size_t need = gn_plan(P, a.N, a.S, a.C, a.G, dtype, backward, backward && a.dw);
+    if (!P.fits) return gn_refuse(a.N, a.S, a.C, a.G, who);
     if (need && (!ws || ws_bytes < need || (uintptr_t)ws % 8)) {
         set_error_text("%s: the workspace has %zu bytes, %zu (8-byte aligned) are needed", who, ws_bytes, need);
         return DGG_ERR_WORKSPACE;
@@ -1205,10 +1238,6 @@ int gn_run(bool backward, GnArgs& a, int dtype, void* ws, size_t ws_bytes, hipSt
         a.res_groups = P.res_groups;
         a.blocks_g = P.res_blocks;
     } else {
-        if (P.blocks_c > 65535) {
-            set_error_text("%s: %d channels: 2^24 - 256 at most", who, a.C);
-            return DGG_ERR_INVALID;
-        }
         a.chunks = P.chunks;
         a.chunk_rows = P.chunk_rows;
         a.tx = P.tx;
@@ -1231,8 +1260,10 @@ extern "C" {
 
 int64_t dgg_group_norm_workspace_bytes(int64_t N, int64_t S, int C, int groups, int dtype, int backward) {
     const int rc = gn_check(N, S, C, groups, DGG_ACT_NONE, dtype, "dgg_group_norm_workspace_bytes");
+    if (rc != DGG_OK) return rc;
     GnPlan P = {};
-    return rc != DGG_OK ? rc : (int64_t)gn_plan(P, N, S, C, groups, dtype, backward != 0, backward != 0);
+    const size_t need = gn_plan(P, N, S, C, groups, dtype, backward != 0, backward != 0);
+    return P.fits ? (int64_t)need : gn_refuse(N, S, C, groups, "dgg_group_norm_workspace_bytes");
 }
 
 int dgg_group_norm_act_forward(const void* x, int64_t x_stride_n, int64_t x_stride_s, int64_t N, int64_t S, int C, int groups,

@@ -162,7 +162,8 @@ int dgg_resblock_backward(int fin, const float* params, float* grads, void* ws, 
  *   y = act(z): DGG_ACT_NONE, DGG_ACT_LEAKY_RELU (`slope` for z <= 0) or DGG_ACT_SILU (z * sigmoid(z)).
  * y and dx are contiguous (N, S, C) and overlap no input.  Statistics and z are 64-bit inside: the side of LeakyReLU's kink an element takes is the
  * exact one.  stats (N, groups, 2) doubles = (mean, 1 / sqrt(var + eps)): written by the forward if non-NULL, read by the
- * backward; dweight / dbias: both or none.  N * groups < 2^31, S < 2^31, C <= 2^24; N, S >= 1.  ws (8-byte aligned) of
+ * backward; dweight / dbias: both or none.  N * groups < 2^31, S < 2^31, C <= 2^24; N, S >= 1; groups of
+ * 8192 and more elements of a sample: N * groups < 2^22 is always taken, more only where no launch needs 2^32 threads (DGG_ERR_INVALID).  ws (8-byte aligned) of
  * dgg_group_norm_workspace_bytes(.., backward) bytes; results do not depend on the order in which workgroups run. */
 enum { DGG_F32 = 0, DGG_BF16 = 1, DGG_F16 = 2 };
 enum { DGG_ACT_NONE = 0, DGG_ACT_LEAKY_RELU = 1, DGG_ACT_SILU = 2 };

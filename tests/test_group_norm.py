@@ -410,3 +410,39 @@ def test_dx_of_small_groups_is_rounded_once(shape, dtype):
         wdz = (dy.double().reshape(r["dx"].shape) * (torch.ones(c) if ww is None else ww).double().view(g, -1)).abs()
         terms = r["rstd"] * (wdz + wdz.mean((1, 3), keepdim=True) + xh * (wdz * xh).mean((1, 3), keepdim=True))
         close(dx, r["dx"], half_step(dtype, r["dx"]) + U * r["dx"].abs() + 2.0 ** -40 * terms, "dx")
+
+
+def test_launches_beyond_2_32_threads_are_refused_without_a_gpu():
+    lib = _lib.lib()
+    ws = lib.dgg_group_norm_workspace_bytes
+    for shape in ((1 << 24, 9000, 1, 1), (1 << 20, 9000, 16, 16), (1, 9000, (1 << 24) - 1, 1)):
+        for backward in (0, 1):
+            assert ws(*shape, _lib.BF16, backward) == -1 and b"2^32" in lib.dgg_last_error(), shape
+        n, s, c, g = shape
+        one = 4096   # never read: the checks come first
+        assert lib.dgg_group_norm_act_forward(one, s * c, c, n, s, c, g, None, None, 1e-5, 1, 0.2, _lib.BF16, one, None, one, 1 << 62, None) == -1
+    assert ws((1 << 22) - 1, 9000, 1, 1, _lib.BF16, 1) > 0 and ws((1 << 26) + 5, 33, 1, 1, _lib.BF16, 0) == 0
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("n,s,first", [((1 << 26) + 5, 33, ((1 << 32) - 1024) // 64), ((1 << 24) + 3, 300, ((1 << 32) - 1024) // 320)],
+                         ids=["part of a wave", "workgroup"])
+def test_more_samples_than_a_launch_has_threads(n, s, first):
+    """2^32 threads and more go in several launches: samples at both ends and where a second launch begins (`first`, in the forward pass)."""
+    x = torch.empty((n, s, 1), dtype=torch.bfloat16, device="cuda").normal_(generator=torch.Generator("cuda").manual_seed(1))
+    dy = torch.zeros_like(x)
+    at = torch.tensor([0, 1, 2, first - 2, first - 1, first, first + 1, n // 2, n - 2, n - 1], device="cuda")
+    small, dsmall, w, b = data((len(at), s, 1), torch.bfloat16, 60)
+    x[at], dy[at] = small.cuda(), dsmall.cuda()
+    y, st = ops.group_norm_act_forward(x, 1, w.cuda(), b.cuda())
+    r = reference(small, dsmall, 1, w, b, 1e-5, "leaky_relu", 0.2)
+    close(y[at], r["y"], half_step(x.dtype, r["y"]) + (8 + r["z"].abs()) * U * r["y"].abs(), "y")
+    close(st[at][..., 1], r["rstd"].reshape(-1, 1), 1e-12 * r["rstd"].reshape(-1, 1), "rstd")
+    assert bool((st[..., 1] > 0.25).all()) and not bool((st[..., 1] > 1e3).any())       # every sample has its own
+    del y
+    dx, dw, db = ops.group_norm_act_backward(dy, x, 1, w.cuda(), b.cuda(), 1e-5, "leaky_relu", 0.2, st)
+    close(dx[at], r["dx"], half_step(x.dtype, r["dx"]) + r["dx_tol"], "dx")
+    close(dw, r["dw"], r["dw_tol"] + U * r["dw"].abs(), "dweight")                        # dy is zero in every other sample
+    close(db, r["db"], r["db_tol"] + U * r["db"].abs(), "dbias")
+    del x, dy, dx, st
+    torch.cuda.empty_cache()
