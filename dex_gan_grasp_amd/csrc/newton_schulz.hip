@@ -1239,18 +1239,39 @@ int ns_narrow_plan(const dgg_matrix* const* mats, int count, NsArgs& a, NsFirst&
     return grid;
 }
 
-// up to kNsMats matrices of one route, from mats[at] on; at moves behind them
+// Threads of a launch: below 2^32 (from there on a grid may be cut short without an error).  A matrix needs at most a workgroup for each
+// 64 x 64 of its elements in every launch; up to 1024 more where the general route shares A's k between workgroups (ns_plan: 512) and sums.
+constexpr long long kNsMost = (1ll << 32) - 1024ll * kNsMats * kThreads - 1;
+long long ns_threads(const dgg_matrix& m, int route) {
+    const int lo = m.rows < m.cols ? m.rows : m.cols, hi = m.rows < m.cols ? m.cols : m.rows;
+    if (route == kSmall) return (long long)m.batch * kSmallThreads;
+    if (route == kNarrowRoute) return (long long)m.batch * ceil_div(hi, kNarrow / (lo <= 32 ? 32 : 64)) * kNarrowThreads;
+    return (long long)m.batch * ceil_div(lo, 64) * ceil_div(hi, 64) * kThreads;
+}
+
+// up to kNsMats matrices of one route that a launch has the threads for, from mats[at] on; at moves behind them
 int ns_group(const dgg_matrix* mats, int count, const NsRoutes& routes, int route, int& at, const dgg_matrix** group) {
     int n = 0;
-    for (; at < count && n < kNsMats; ++at)
-        if (routes.of[ns_kind(mats[at])] == route) group[n++] = mats + at;
+    long long threads = 0;
+    for (; at < count && n < kNsMats; ++at) {
+        if (routes.of[ns_kind(mats[at])] != route) continue;
+        threads += ns_threads(mats[at], route);
+        if (n > 0 && threads > kNsMost) break;
+        group[n++] = mats + at;
+    }
     return n;
 }
 
-int64_t ns_need(const dgg_matrix* mats, int count) {
+int64_t ns_need(const dgg_matrix* mats, int count, const char* who) {
     const dgg_matrix* group[kNsMats];
     size_t need = 256;
     const NsRoutes routes(mats, count);
+    for (int i = 0; i < count; ++i)
+        if (ns_threads(mats[i], routes.of[ns_kind(mats[i])]) > kNsMost) {
+            set_error_text("%s: matrix %d: a stack of %lld of %d x %d needs a launch of 2^32 threads or more", who, i, (long long)mats[i].batch,
+                           mats[i].rows, mats[i].cols);
+            return DGG_ERR_INVALID;
+        }
     for (int at = 0, n; (n = ns_group(mats, count, routes, kNarrowRoute, at, group)) > 0;) {
         NsArgs a = {};
         NsFirst first;
@@ -1344,7 +1365,8 @@ int ns_run(const dgg_matrix* mats, int count, NsArgs& a, const double* coef, int
     a.steps = steps;
     NsPlan P;
     const dgg_matrix* group[kNsMats];
-    int64_t need = ns_need(mats, count);
+    const int64_t need = ns_need(mats, count, who);
+    if (need < 0) return (int)need;
     if ((int64_t)ws_bytes < need) {
         set_error_text("%s: the workspace has %zu bytes, %lld are needed", who, ws_bytes, (long long)need);
         return DGG_ERR_WORKSPACE;
@@ -1416,7 +1438,7 @@ int ns_run(const dgg_matrix* mats, int count, NsArgs& a, const double* coef, int
 
 int64_t ns_ws(const dgg_matrix* mats, int count, const char* who) {
     const int rc = ns_check(mats, count, who);
-    return rc != DGG_OK ? rc : ns_need(mats, count);
+    return rc != DGG_OK ? rc : ns_need(mats, count, who);
 }
 
 }  // namespace

@@ -490,3 +490,32 @@ def test_infinite_parameters_stay_infinite():
         for wd in (0.0, 0.1):
             ops.muon_step([w], [matrix(*shape, seed=3).cuda()], [torch.zeros(shape, device="cuda")], 0.1, weight_decay=wd)
             assert w[3, 4] == float("inf") and w[5, 6] == -float("inf") and int(w.isfinite().sum()) == w.numel() - 2
+
+
+def test_stacks_beyond_2_32_threads_are_refused_without_a_gpu():
+    lib = _lib.lib()
+    for kw in (dict(batch=1 << 18, rows=1, cols=16384), dict(batch=1 << 12, rows=1 << 20, cols=1), dict(batch=1 << 11, rows=2, cols=1 << 20)):
+        mats = (_lib.Matrix * 2)()
+        for m, d in zip(mats, (dict(batch=1, rows=8, cols=8), kw)):
+            for k, v in dict(in_=4096, out=4096, momentum=4096, ld_in=1 << 20, ld_out=1 << 20, ld_momentum=1 << 20, **d).items():
+                setattr(m, k, v)
+        assert lib.dgg_orthogonalize_workspace_bytes(mats, 2) == -1 and b"2^32" in lib.dgg_last_error(), kw
+    mats[1].batch = (1 << 20) // 2      # half of the threads' limit
+    mats[1].rows = mats[1].cols = 65
+    assert lib.dgg_orthogonalize_workspace_bytes(mats, 2) > 0
+
+
+@pytest.mark.gpu
+def test_stacks_that_need_more_than_one_launch():
+    """Five stacks of 2^20 matrices of one element: 1024 threads a matrix are 5 x 2^30."""
+    gen = torch.Generator("cuda").manual_seed(1)
+    gs = [torch.empty(1 << 20, 1, 1, device="cuda").uniform_(0.5, 2.0, generator=gen) for _ in range(5)]
+    gs[4].neg_()
+    ref, tol = reference(torch.ones(1, 1))              # (eps, 2e-7 of the smallest, makes less of a difference than the other roundings)
+    ref, tol = ref.item(), 20 * tol
+    for g, o in zip(gs, ops.orthogonalize(gs)):
+        assert bool(((o * g.sign() - ref).abs() <= tol).all())
+    ws, ms = [torch.ones_like(g) for g in gs], [torch.zeros_like(g) for g in gs]
+    ops.muon_step(ws, gs, ms, 0.5, 0.0)
+    for w, m, g in zip(ws, ms, gs):
+        assert bool(((w - (1 - 0.5 * ref * g.sign())).abs() <= tol).all()) and torch.equal(m, g)
