@@ -362,7 +362,7 @@ def muon_step(params, grads, momentum, lr, mu=0.95, nesterov=True, weight_decay=
     if adjust not in _ADJUST:
         raise _lib.DggError("%s: adjust must be one of %s; got %r" % (who, sorted(_ADJUST), adjust))
     coef = _coefficients(who, steps, coefficients)
-    mats, keep = [], []
+    mats, keep, written = [], [], []
     dev = _dev(params[0]) if params else None
     for w, g, m in zip(params, grads, momentum):
         for t in (w, g, m):
@@ -375,6 +375,7 @@ def muon_step(params, grads, momentum, lr, mu=0.95, nesterov=True, weight_decay=
         if wt is not w or mt is not m:
             raise _lib.DggError("%s: parameters and momentum are updated in place: their rows must be contiguous and apart" % who)
         keep.append(gt)
+        written += (w, m)
         mats.append(_lib.Matrix(gt.data_ptr(), w.data_ptr(), m.data_ptr(), b, sg, sw, sm, r, c, ldg, ldw, ldm, 0))
     if mats:
         n = len(mats)
@@ -382,6 +383,8 @@ def muon_step(params, grads, momentum, lr, mu=0.95, nesterov=True, weight_decay=
         ws, nb = _ns_workspace(mats, n, dev)
         check(_launch(dev, lib().dgg_muon_step, mats, n, lr, mu, int(nesterov), weight_decay, _ADJUST[adjust], grad_scale, coef, steps,
                       eps, ws.data_ptr(), nb, _stream(dev)), "dgg_muon_step")
+        # autograd learns that they were written: a graph that still needs their old values raises in its backward pass
+        torch.autograd.graph.increment_version([t for t in written if not t.is_inference()])
 
 
 # ------------------------------------------------------------------------------------------ small ops

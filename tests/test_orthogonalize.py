@@ -519,3 +519,25 @@ def test_stacks_that_need_more_than_one_launch():
     ops.muon_step(ws, gs, ms, 0.5, 0.0)
     for w, m, g in zip(ws, ms, gs):
         assert bool(((w - (1 - 0.5 * ref * g.sign())).abs() <= tol).all()) and torch.equal(m, g)
+
+
+@pytest.mark.gpu
+def test_autograd_knows_what_a_muon_step_wrote():
+    w = torch.randn(20, 30, device="cuda", requires_grad=True)
+    m = torch.zeros(20, 30, device="cuda")
+    loss = (w * w).sum()
+    g, = torch.autograd.grad(loss, w, retain_graph=True)
+    versions = w._version, m._version, g._version
+    ops.muon_step([w], [g], [m], 0.1)
+    assert w._version > versions[0] and m._version > versions[1] and g._version == versions[2]
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        torch.autograd.grad(loss, w)
+    (w * w).sum().backward()
+    assert torch.equal(w.grad, 2 * w.detach())
+    flat = torch.zeros(2, 20, 30, device="cuda")        # a view's base, and what has no versions
+    ops.muon_step([flat[0]], [g], [m], 0.1)
+    assert flat._version > 0
+    with torch.inference_mode():
+        w = torch.ones(20, 30, device="cuda")
+        ops.muon_step([w], [g], [torch.zeros_like(w)], 0.1)
+    assert bool((w != 1).any())
