@@ -1289,19 +1289,32 @@ int64_t ns_need(const dgg_matrix* mats, int count, const char* who) {
     return (int64_t)need;
 }
 
-// What one matrix or stack covers in memory (bytes), for the check below.
+// What one matrix or stack covers in memory (bytes), for the check below: rows `row` wide and `ld` apart, matrices `one` long and `stride`
+// apart.  A stack of single rows is one matrix.
 struct NsSpan {
-    uintptr_t lo, hi, ld, stride, row;
-    int batch;
+    uintptr_t lo, hi, ld, stride, row, one;
+    int rows, batch;
     bool written;
 };
 
-// Two spans share no element: they lie one behind the other, or they are column blocks of one wider buffer.
+// Every element of `a` lies in one of the places lo + k period + [0, length); do those of b, moved to them by multiples of the period,
+// lie between two such places?
+bool ns_between(const NsSpan& a, uintptr_t period, uintptr_t length, const NsSpan& b) {
+    uintptr_t wide = b.hi - b.lo;   // what b covers once its own repetitions by multiples of the period are left out
+    if (b.batch == 1 || b.stride % period == 0) wide = b.rows == 1 || b.ld % period == 0 ? b.row : b.one;
+    const uintptr_t d = a.lo <= b.lo ? (b.lo - a.lo) % period : (period - (a.lo - b.lo) % period) % period;
+    return d >= length && d + wide <= period;
+}
+
+// Two spans share no element: they lie one behind the other, or one lies in the gaps between the rows or the matrices of the other
+// (column blocks of one wider buffer, stacks that alternate).
 bool ns_free(const NsSpan& a, const NsSpan& b) {
     if (a.hi <= b.lo || b.hi <= a.lo) return true;
-    if (a.ld != b.ld || (a.batch > 1 && a.stride % a.ld) || (b.batch > 1 && b.stride % b.ld)) return false;
-    const uintptr_t d = a.lo <= b.lo ? (b.lo - a.lo) % a.ld : (a.ld - (a.lo - b.lo) % a.ld) % a.ld;   // b's first column from a's
-    return d >= a.row && d + b.row <= a.ld;
+    const auto gaps = [](const NsSpan& p, const NsSpan& q) {
+        return (p.rows > 1 && (p.batch == 1 || p.stride % p.ld == 0) && ns_between(p, p.ld, p.row, q)) ||
+               (p.batch > 1 && p.stride > 0 && ns_between(p, p.stride, p.one, q));
+    };
+    return gaps(a, b) || gaps(b, a);
 }
 
 // What a call writes is written once and read by nothing else in it, only an output may be its own matrix' input: launches read an
@@ -1318,8 +1331,9 @@ bool ns_disjoint(const dgg_matrix* mats, int count, size_t size, bool muon) {
                 const bool beside = stride >= m.cols && (uintptr_t)(m.batch - 1) * stride * size + row <= (uintptr_t)ld * size;
                 if (!behind && !beside) return false;
             }
-            spans.push_back({lo, lo + (uintptr_t)(m.batch - 1) * stride * size + one, (uintptr_t)ld * size, (uintptr_t)stride * size,
-                             row, (int)m.batch, written});
+            const uintptr_t hi = lo + (uintptr_t)(m.batch - 1) * stride * size + one, pitch = (uintptr_t)(m.rows > 1 ? ld : stride) * size;
+            if (m.rows > 1) spans.push_back({lo, hi, pitch, (uintptr_t)stride * size, row, one, m.rows, (int)m.batch, written});
+            else spans.push_back({lo, hi, pitch, 0, row, hi - lo, pitch ? (int)m.batch : 1, 1, written});
             return true;
         };
         const bool same = !muon && m.in == m.out && m.ld_in == m.ld_out && (m.batch == 1 || m.in_stride == m.out_stride);

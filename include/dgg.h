@@ -271,8 +271,9 @@ int dgg_adam_l2(float* params, const float* grads, float* m, float* v, int64_t n
  * `mats` (host): any number of entries, each a stack of `batch` matrices of one shape; all of them share the launches (16 entries
  * at a time).  Rows lie ld_* >= cols elements apart, the matrices of a stack *_stride elements.  Products are fp32-accurate
  * (two fp16 planes an operand, fp32 accumulators) for every type.  A NaN or infinity makes its own matrix NaN, no other; a zero
- * matrix stays zero (eps > 0).  What is written may overlap nothing else that the call reads or writes (column blocks of one
- * wider buffer are apart): DGG_ERR_INVALID.  The coefficients must keep the iterates bounded for singular values in [0, 1]: DGG_ERR_INVALID
+ * matrix stays zero (eps > 0).  What is written may overlap nothing else that the call reads or writes: DGG_ERR_INVALID (column
+ * blocks of one wider buffer and stacks whose matrices alternate are apart; layouts with no common pitch or stride have to lie one behind the
+ * other).  The coefficients must keep the iterates bounded for singular values in [0, 1]: DGG_ERR_INVALID
  * otherwise.  Short side <= 16384, long side <= 2^20, a stack <= 2^32 elements
  * and no more than a launch has threads for (2^32: 2^18 matrices of 1 x 16384 are too many): DGG_ERR_INVALID.  ws: dgg_orthogonalize_workspace_bytes, 256-byte
  * aligned, one per stream in flight. */

@@ -541,3 +541,52 @@ def test_autograd_knows_what_a_muon_step_wrote():
         w = torch.ones(20, 30, device="cuda")
         ops.muon_step([w], [g], [torch.zeros_like(w)], 0.1)
     assert bool((w != 1).any())
+
+
+@pytest.mark.gpu
+def test_stacks_that_alternate_and_single_rows_are_apart():
+    """Stacks whose matrices alternate in one buffer, a matrix between those of a stack, rows of a buffer beside a column block of it."""
+    g = torch.stack([matrix(20, 30, s) for s in range(4)]).cuda()
+    want = [torch.ones(20, 30, device="cuda") for _ in range(4)]
+    for i in range(4):
+        ops.muon_step([want[i]], [g[i]], [torch.zeros(20, 30, device="cuda")], 0.1)
+    both, mom = torch.ones(2, 2, 20, 30, device="cuda"), torch.zeros(2, 2, 20, 30, device="cuda")
+    ops.muon_step([both[:, 0], both[:, 1]], [g[:2], g[2:]], [mom[:, 1], mom[:, 0]], 0.1)      # (both's and mom's own, crosswise)
+    for i in range(4):
+        assert torch.equal(both[i % 2, i // 2], want[i]) and torch.equal(mom[i % 2, 1 - i // 2], g[i])
+    gaps = torch.ones(2, 2, 20, 30, device="cuda")
+    ops.muon_step([gaps[:, 0], gaps[0, 1]], [g[:2], g[2]], [torch.zeros(2, 20, 30, device="cuda"), torch.zeros(20, 30, device="cuda")], 0.1)
+    assert torch.equal(gaps[0, 0], want[0]) and torch.equal(gaps[1, 0], want[1]) and torch.equal(gaps[0, 1], want[2])
+    assert bool((gaps[1, 1] == 1).all())
+    wide = torch.ones(20, 50, device="cuda")
+    ops.muon_step([wide[:, :30], wide[4:5, 30:], wide[7:8, 30:]], [g[0], g[1][:1, :20], g[2][:1, :20]],
+                  [torch.zeros(20, 30, device="cuda"), torch.zeros(1, 20, device="cuda"), torch.zeros(1, 20, device="cuda")], 0.1)
+    assert torch.equal(wide[:, :30], want[0]) and int((wide[:, 30:] != 1).sum(1).gt(0).sum()) == 2
+    rows = torch.ones(6, 2, 30, device="cuda")             # stacks of single rows
+    ops.muon_step([rows[:, :1], rows[:, 1:]], [g[0][:6, None], g[1][:6, None]], [torch.zeros(6, 1, 30, device="cuda") for _ in range(2)], 0.1)
+    assert bool((rows != 1).any(-1).all())
+
+
+def test_alternating_stacks_that_overlap_are_refused_without_a_gpu():
+    lib, C = _lib.lib(), _lib.C
+    coef = (C.c_double * 15)(*(COEF * 5))
+    base = 1 << 20
+
+    def call(a, b):      # outputs of two stacks of 8 x 8, everything else apart
+        arr = (_lib.Matrix * 2)()
+        for i, (m, kw) in enumerate(zip(arr, (a, b))):
+            d = dict(in_=(4 + i) * base, out=2 * base, momentum=(6 + i) * base, batch=2, rows=8, cols=8, ld_in=8, ld_out=8, ld_momentum=8,
+                     in_stride=64, out_stride=128, momentum_stride=64)
+            for k, v in {**d, **kw}.items():
+                setattr(m, k, v)
+        n = lib.dgg_orthogonalize_workspace_bytes(arr, 2)
+        return lib.dgg_muon_step(arr, 2, 0.1, 0.9, 1, 0.0, 0, 1.0, coef, 5, 1e-7, 4096, n, None)
+
+    at = 2 * base
+    for bad in (({}, dict(out=at + 252)), ({}, dict(out=at + 260)), ({}, dict(out=at + 256, out_stride=129)), ({}, dict(out=at + 256, ld_out=9)),
+                ({}, dict(out=at + 256, batch=3, out_stride=64)), ({}, dict(out=at + 128, batch=1)), ({}, dict(out=at + 260, batch=1)),
+                (dict(ld_out=16, out_stride=16 * 8), dict(batch=1, rows=1, out=at + 16 * 4 * 3 + 4)),
+                (dict(ld_out=16, out_stride=16 * 8), dict(batch=1, rows=1, out=at + 16 * 4 * 3 + 36)),
+                (dict(rows=1, out_stride=8), dict(rows=1, out=at + 28, out_stride=16))):
+        assert call(*bad) == -1 and b"overlaps" in lib.dgg_last_error(), bad
+        assert call(*bad[::-1]) == -1 and b"overlaps" in lib.dgg_last_error(), bad
