@@ -1128,21 +1128,26 @@ template <typename Launch> void gn_launches(const GnArgs& a, long long threads, 
     else if (act == DGG_ACT_SILU) hipLaunchKernelGGL((kernel<T, V, DGG_ACT_SILU>), grid, block, 0, st, a);              \
     else hipLaunchKernelGGL((kernel<T, V, DGG_ACT_NONE>), grid, block, 0, st, a);
 
-// items: 1, 2, 4 vectors a lane of a wave; 2, 4, 8 (16 bits: 4) widest ones a thread of a workgroup
-#define GN_UNIT_I(kernel, EVEN, ...)                                                                                          \
+// items: 1, 2, 4 vectors a lane of a wave (MANY: more than 1 only there); 2, 4, 8 (16 bits: 4) widest ones a thread of a workgroup
+#define GN_UNIT_I(kernel, EVEN, MANY, ...)                                                                                    \
     if (P.lanes == kGnThreads) {                                                                                              \
         if constexpr (V == 16 / (int)sizeof(T)) {                                                                             \
             if (P.items == 2) hipLaunchKernelGGL((kernel<T, V, EVEN, 2, true __VA_ARGS__>), grid, block, 0, st, a);            \
             else if (P.items == 4 || V == 8) hipLaunchKernelGGL((kernel<T, V, EVEN, 4, true __VA_ARGS__>), grid, block, 0, st, a); \
             else hipLaunchKernelGGL((kernel<T, V, EVEN, V == 8 ? 4 : 8, true __VA_ARGS__>), grid, block, 0, st, a);            \
         }                                                                                                                     \
-    } else if (P.items == 1) hipLaunchKernelGGL((kernel<T, V, EVEN, 1, false __VA_ARGS__>), grid, block, 0, st, a);            \
-    else if (P.items == 2) hipLaunchKernelGGL((kernel<T, V, EVEN, 2, false __VA_ARGS__>), grid, block, 0, st, a);              \
-    else hipLaunchKernelGGL((kernel<T, V, EVEN, 4, false __VA_ARGS__>), grid, block, 0, st, a);
+    } else if constexpr (MANY) {                                                                                              \
+        if (P.items == 1) hipLaunchKernelGGL((kernel<T, V, EVEN, 1, false __VA_ARGS__>), grid, block, 0, st, a);               \
+        else if (P.items == 2) hipLaunchKernelGGL((kernel<T, V, EVEN, 2, false __VA_ARGS__>), grid, block, 0, st, a);          \
+        else hipLaunchKernelGGL((kernel<T, V, EVEN, 4, false __VA_ARGS__>), grid, block, 0, st, a);                            \
+    } else hipLaunchKernelGGL((kernel<T, V, EVEN, 1, false __VA_ARGS__>), grid, block, 0, st, a);
 #define GN_COMMA ,
-#define GN_UNIT(kernel, ...)                                                                                                  \
-    if (V == 1 || a.D % V == 0) { GN_UNIT_I(kernel, true, __VA_ARGS__) }                                                      \
-    else { GN_UNIT_I(kernel, (V == 1), __VA_ARGS__) }
+// POINTS: S > 1 may come here, whose accesses divide the channels.  Rows have narrow accesses only where a group is narrower than a wide one:
+// two vectors, in two lanes
+#define GN_UNIT(kernel, POINTS, ...)                                                                                          \
+    constexpr bool widest = V == 16 / (int)sizeof(T);                                                                         \
+    if (V == 1 || a.D % V == 0) { GN_UNIT_I(kernel, true, widest || POINTS, __VA_ARGS__) }                                    \
+    else { GN_UNIT_I(kernel, (V == 1), widest || (V == 1 && POINTS), __VA_ARGS__) }
 
 #define GN_RES(act, kernel, R)                                                                                             \
     if (act == DGG_ACT_LEAKY_RELU) hipLaunchKernelGGL((kernel<T, V, R, DGG_ACT_LEAKY_RELU>), grid, block, 0, st, a);       \
@@ -1153,7 +1158,7 @@ template <typename T, int V> int gn_forward_v(const GnPlan& P, GnArgs& a, hipStr
     if (P.unit) {
         gn_launches(a, (long long)a.G * P.lanes, sizeof(T), [&](const GnArgs& a) {
             const dim3 grid((unsigned)((a.N * a.G * P.lanes + kGnThreads - 1) / kGnThreads)), block(kGnThreads);
-            GN_UNIT(gn_unit_fwd_kernel, )
+            GN_UNIT(gn_unit_fwd_kernel, true, )
         });
         return check_launch("group_norm forward");
     }
@@ -1178,7 +1183,7 @@ template <typename T, int V> int gn_backward_v(const GnPlan& P, GnArgs& a, hipSt
     if (P.unit) {
         if (!a.dw) a.part = nullptr;
         const dim3 grid((unsigned)P.blocks_g * P.blocks_n);
-        if (a.S == 1) { GN_UNIT(gn_unit_bwd_kernel, GN_COMMA false) }
+        if (a.S == 1) { GN_UNIT(gn_unit_bwd_kernel, false, GN_COMMA false) }
         else hipLaunchKernelGGL((gn_unit_bwd_kernel<T, V, true, 1, false, true>), grid, block, 0, st, a);
         if (a.dw) gn_param_grad(a, (const float*)a.part, P.blocks_n, st);
         return check_launch("group_norm backward");
