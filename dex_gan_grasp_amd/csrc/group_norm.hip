@@ -10,18 +10,20 @@
 // Arithmetic.  Statistics are accumulated in 64 bits, and so is the pre-activation z = (x - mean) rstd w + b: its
 // SIGN decides which side of LeakyReLU's kink an element lies on, i.e. a factor 1 / slope in its gradient, and an fp32 z
 // would take the wrong side for every element within its rounding error of zero.  (64-bit vector instructions run at the
-// rate of the fp32 ones here; per element they are 4 to 6 of them.)  What follows the sign is fp32, rounded once to the output type.
+// rate of the fp32 ones here; per element they are 4 to 6 of them.)  What follows the sign is fp32, rounded once to the output
+// type; dx of a group of a few elements is 64-bit to the end (grad_few).  SiLU and no activation have no such sign: they share
+// the arithmetic, which keeps x - mean exact for data far from zero, at the price of those instructions.
 //
-// Three routes, chosen by gn_plan:
+// Three routes, chosen by gn_plan (us of a call's launches in a graph, inputs that change from pass to pass):
 //  * "unit": a group's S x D elements fit the registers of at most one wave, or, long rows, of a workgroup.  L = 2^k lanes own one
-//    (n, g): one read of x, mean and centred variance by lane shuffles.  1024 x 512 f32 in 32 groups: 4.2 us forward, 9.7 backward with dw
-//    and db (launches); 16384 x 512: 22 and 28 us (3.0 and 3.6 TB/s); 8192 x 4096 bf16 in one group 62 and 78.
+//    (n, g): one read of x, mean and centred variance by lane shuffles.  1024 x 512 f32 in 32 groups: 3.5 us forward, 8.8 backward with dw
+//    and db (launches); 16384 x 512: 19 and 27 us (3.5 and 3.7 TB/s); 8192 x 4096 bf16 in one group 50 and 72.
 //  * "resident": a sample's points in a block of groups fit a workgroup's registers: one read, one launch.  128 x 2048 x 256 bf16
-//    in 32 groups: 71 us forward (3.8 TB/s), 136 backward (3.0 TB/s: the arithmetic and the memory take turns, one workgroup a CU).
+//    in 32 groups: 69 us forward (3.9 TB/s), 128 backward (3.2 TB/s: the arithmetic and the memory take turns, one workgroup a CU).
 //  * "tile": a workgroup owns a range of the rows of one sample and a block of channels (a thread keeps ITS channels while
 //    it walks down the rows), leaves per-channel partial sums in the workspace, and a small launch merges them in a fixed
 //    order into the groups' statistics (and dw, db); a last launch applies them.  No atomics: results do not depend on the
-//    order in which workgroups run.  30 x 1000 x 1020 bf16 in 60 groups: 58 and 82 us (x is read twice, dy too).
+//    order in which workgroups run.  30 x 1000 x 1020 bf16 in 60 groups: 50 and 87 us (x is read twice, dy too).
 #include <type_traits>
 
 #include "dgg_internal.h"
@@ -60,7 +62,8 @@ template <int V, bool EVEN> struct Span {
 __host__ __device__ __forceinline__ int vectors(int width, int V) { return (width + V - 1) / V; }
 
 // 1 / (1 + exp(-z)) by the hardware's exp2 and reciprocal (1 unit in the last place each).  The exponent is formed in 64 bits and
-// rounded once, so the result is off by (|z| + 6) 2^-24 of itself at most.  (With expf and a division, 30 instructions an element,
+// rounded once, so from z = -87 on the result is off by (|z| + 6) 2^-24 of itself at most; below, where it leaves fp32's normal numbers, it
+// may be 0 (off by 2e-38).  (With expf and a division, 30 instructions an element,
 // a forward pass over 64 M bf16 elements was bound by them: 77 us for the launch that moves 268 MB.)
 __device__ __forceinline__ float sigmoid(double z) {
     return __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f((float)(z * -1.4426950408889634)));
@@ -217,7 +220,8 @@ __global__ __launch_bounds__(kGnThreads) void gn_unit_fwd_kernel(GnArgs a) {
 }
 
 // Backward: a lane keeps its channels while it walks over the samples n, so that dw and db need no exchange between lanes until the
-// end; every workgroup row leaves one partial (64-bit sums, stored as fp32) per channel.  POINTS: S > 1, a lane has a vector of a point.
+// end; every workgroup row leaves one partial per channel (64-bit sums, stored as fp32: 2^-24 of a partial for half the bytes).
+// POINTS: S > 1, a lane has a vector of a point.
 template <typename T, int V, bool EVEN, int I, bool WIDE, bool POINTS>
 __global__ __launch_bounds__(kGnThreads) void gn_unit_bwd_kernel(GnArgs a) {
     __shared__ double wide[WIDE ? kGnThreads / 64 : 1];
@@ -800,8 +804,9 @@ __global__ __launch_bounds__(kResThreads) void gn_res_bwd_kernel(GnArgs a) {
         sums[threadIdx.x] = few1;
         sums[kResThreads + threadIdx.x] = few2;
     }
-    // The columns' sums over the rows — a column: one of the two sums of one channel —, fp32 from each thread, added in 64 bits: `parts`
-    // threads a column, then a wave a group, which also has the group's two means from them.
+    // The columns' sums over the rows — a column: one of the two sums of one channel —, fp32 from each thread (2^-24 of its
+    // sum, for 32 KB of LDS instead of 64 with 8 channels a thread), added in 64 bits: `parts` threads a column, then a wave a group,
+    // which also has the group's two means from them.
     const int cols = t.tx * V * 2, parts = cols < (int)blockDim.x ? (int)blockDim.x / cols : 1;
     __syncthreads();
     const int part = parts > 1 ? (int)threadIdx.x / cols : 0;
@@ -995,8 +1000,8 @@ bool gn_unit_plan(GnPlan& P, long long S, int D, bool backward) {
 }
 
 // Resident: whole samples in registers, 16 vectors a thread (backward: of x and of dy) and 512 threads at most.  Resident against
-// tile, forward / backward, us: 32 x 2048 x 256 bf16 in 32 groups 25 / 35 against 31 / 57, 128 x 2048 x 256 71 / 140 against 102 / 185,
-// 6 x 1111 x 132 f16 in 11 9.2 / 13.5 against 12.9 / 17.9, 4 x 4096 x 64 in 8 13.9 / 20.3 against 15.4 / 19.6.
+// tile, forward / backward, us: 32 x 2048 x 256 bf16 in 32 groups 21 / 29 against 29 / 47, 128 x 2048 x 256 69 / 128 against 102 / 190,
+// 5 x 1237 x 132 f16 in 11 8.5 / 12.2 against 13.4 / 16.5, 4 x 4096 x 64 f32 in 8 10.8 / 14.5 against 12.2 / 15.2.
 bool gn_res_plan(GnPlan& P, long long N, long long S, int C, int G) {
     if (S > 16 * kResThreads) return false;
     const int per = C / G / P.V;
@@ -1035,8 +1040,9 @@ void gn_unit_bwd_grid(GnPlan& P, long long N, int G) {
     P.blocks_n = (int)(nb < most ? nb : most);
 }
 
-// Ranges of rows in the sum that makes dw and db: one where the launch is a latency or two long, else of 512 rows or more
-// (20000 samples of 2 x 16, resident: the backward pass takes 114 us in all, 182 with one range)
+// Ranges of rows in the sum that makes dw and db (resident and tile: a row a sample; the unit route has 1024 at most): one where the launch
+// is a latency or two long, else of 512 rows or more (20000 x 100 x 16 bf16 in 2 groups: the backward pass takes 166 us in all, 231 with one
+// range; 4096 x 100 x 64 in 4 77 and 90)
 int gn_ranges(long long rows) { return rows <= 1024 ? 1 : rows < 64 * 512 ? (int)((rows + 511) / 512) : 64; }
 
 int gn_check(long long N, long long S, int C, int G, int act, int dtype, const char* who) {

@@ -170,9 +170,9 @@ class _GroupNormActFn(torch.autograd.Function):
 class GroupNormAct(nn.Module):
     """Group norm and activation in one kernel, channels last: x (N, .., C) -> act(group_norm(x)) with statistics over a sample's
     points and a group's channels.  Stands where BatchNorm + LeakyReLU stands in a ResBlock (networks.py:29-41) when a sample
-    must not see its batch — a per-sample gradient penalty, batches of one, data-parallel shards of any size — and on
-    per-point features (N, points, C).  float32, bfloat16 or float16 in and out; weight and bias are float32.  Once
-    differentiable.  act: "leaky_relu" (`slope`), "silu" or "none"."""
+    must not see its batch — batches of one, data-parallel shards of any size — and on per-point features (N, points, C).
+    float32, bfloat16 or float16 in and out; weight and bias are float32.  Once differentiable: not for a gradient penalty,
+    which needs the second derivative.  act: "leaky_relu" (`slope`), "silu" or "none"."""
 
     def __init__(self, num_groups, num_channels, eps=1e-5, act="leaky_relu", slope=0.2, affine=True, device=None):
         super().__init__()

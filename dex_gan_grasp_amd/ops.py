@@ -354,7 +354,8 @@ def muon_step(params, grads, momentum, lr, mu=0.95, nesterov=True, weight_decay=
     """One Muon step over lists of float32 matrices (or stacks of them), params and momentum in place:
         M <- mu M + grad_scale G;   U = grad_scale G + mu M (nesterov) or M;   W <- (1 - lr weight_decay) W - lr f orthogonalize(U)
     with f = sqrt(max(1, rows / cols)) (adjust="spectral") or 0.2 sqrt(max(rows, cols)) ("match_rms").  A gradient may be
-    broadcast; parameters and momenta are written, so none of them may overlap another tensor of the call."""
+    broadcast; parameters and momenta are written (their version counters advance), so none of them may overlap another tensor
+    of the call."""
     who = "muon_step"
     params, grads, momentum = list(params), list(grads), list(momentum)
     if not (len(params) == len(grads) == len(momentum)):

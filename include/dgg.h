@@ -157,14 +157,16 @@ int dgg_resblock_backward(int fin, const float* params, float* grads, void* ws, 
 /* Group normalisation with an activation over channels-last data — the batch-independent form of a ResBlock's BatchNorm +
  * LeakyReLU (networks.py:43-56 normalises over the batch instead).  x: N samples of S points (rows) of C channels, the channel
  * stride is 1, samples and points `*_stride_n` / `*_stride_s` ELEMENTS apart, at any element's address (a column block of a
- * wider product needs no copy); types DGG_F32 / DGG_BF16 / DGG_F16 for x, y, dy, dx alike, weight / bias (C, NULL = 1 / 0) and their gradients fp32:
+ * wider product needs no copy); types DGG_F32 / DGG_BF16 / DGG_F16 for x, y, dy, dx alike, weight / bias (C, NULL = 1 / 0) and
+ * their gradients fp32:
  *   mean, var over the S x C/groups elements of sample n and group g;  z = weight * (x - mean) / sqrt(var + eps) + bias;
  *   y = act(z): DGG_ACT_NONE, DGG_ACT_LEAKY_RELU (`slope` for z <= 0) or DGG_ACT_SILU (z * sigmoid(z)).
- * y and dx are contiguous (N, S, C) and overlap no input.  Statistics and z are 64-bit inside: the side of LeakyReLU's kink an element takes is the
- * exact one.  stats (N, groups, 2) doubles = (mean, 1 / sqrt(var + eps)): written by the forward if non-NULL, read by the
- * backward; dweight / dbias: both or none.  N * groups < 2^31, S < 2^31, C <= 2^24; N, S >= 1; groups of
- * 8192 and more elements of a sample: N * groups < 2^22 is always taken, more only where no launch needs 2^32 threads (DGG_ERR_INVALID).  ws (8-byte aligned) of
- * dgg_group_norm_workspace_bytes(.., backward) bytes; results do not depend on the order in which workgroups run. */
+ * y and dx are contiguous (N, S, C) and overlap no input.  Statistics and z are 64-bit inside: the side of LeakyReLU's kink an
+ * element takes is that of a 64-bit z.  stats (N, groups, 2) doubles = (mean, 1 / sqrt(var + eps)): written by the forward if
+ * non-NULL, read by the backward; dweight / dbias: both or none.  N * groups < 2^31, S < 2^31, C <= 2^24; N, S >= 1; groups of
+ * 8192 and more elements of a sample: N * groups < 2^22 and C <= 2^24 - 256 are always taken, more only where no launch needs
+ * 2^32 threads (DGG_ERR_INVALID).  ws (8-byte aligned) of dgg_group_norm_workspace_bytes(.., backward) bytes; results do not depend on the
+ * order in which workgroups run. */
 enum { DGG_F32 = 0, DGG_BF16 = 1, DGG_F16 = 2 };
 enum { DGG_ACT_NONE = 0, DGG_ACT_LEAKY_RELU = 1, DGG_ACT_SILU = 2 };
 int64_t dgg_group_norm_workspace_bytes(int64_t N, int64_t S, int C, int groups, int dtype, int backward);
@@ -260,23 +262,23 @@ int dgg_bce(const float* p, const float* labels, float target_const, int B, floa
 int dgg_adam_l2(float* params, const float* grads, float* m, float* v, int64_t n, int step, double lr,
                 double beta1, double beta2, double eps, double weight_decay, double grad_scale, void* stream);
 
-/* Orthogonalisation of matrices by Newton-Schulz products, and the Muon step — beside dgg_adam_l2 the optimiser for a network's
- * hidden matrices (everything else stays with Adam).
- * dgg_orthogonalize:  X_0 = in / (|in|_F + eps);  X <- a X + (b A + c A^2) X with A = X X^T (over the shorter side), `steps` times
- *   with the k-th (a, b, c) of `coefficients` (host, steps x 3);  out = X.  in / out of one type (DGG_F32 / BF16 / F16); a matrix
- *   taller than wide is treated as its transpose.  out may be in, of the same pitch and stride.
- * dgg_muon_step (fp32, in place):  M <- momentum M + grad_scale G;  U = grad_scale G + momentum M (nesterov != 0) or M;
- *   W <- (1 - lr weight_decay) W - lr f X,  X the orthogonalised U and f = sqrt(max(1, rows / cols)) (DGG_MUON_SPECTRAL) or
- *   0.2 sqrt(max(rows, cols)) (DGG_MUON_MATCH_RMS: updates of Adam's size).  G = `in`, W = `out`, M = `momentum`.
- * `mats` (host): any number of entries, each a stack of `batch` matrices of one shape; all of them share the launches (16 entries
- * at a time).  Rows lie ld_* >= cols elements apart, the matrices of a stack *_stride elements.  Products are fp32-accurate
- * (two fp16 planes an operand, fp32 accumulators) for every type.  A NaN or infinity makes its own matrix NaN, no other; a zero
- * matrix stays zero (eps > 0).  What is written may overlap nothing else that the call reads or writes: DGG_ERR_INVALID (column
- * blocks of one wider buffer and stacks whose matrices alternate are apart; layouts with no common pitch or stride have to lie one behind the
- * other).  The coefficients must keep the iterates bounded for singular values in [0, 1]: DGG_ERR_INVALID
- * otherwise.  Short side <= 16384, long side <= 2^20, a stack <= 2^32 elements
- * and no more than a launch has threads for (2^32: 2^18 matrices of 1 x 16384 are too many): DGG_ERR_INVALID.  ws: dgg_orthogonalize_workspace_bytes, 256-byte
- * aligned, one per stream in flight. */
+/* Orthogonalisation of matrices by Newton-Schulz products, and the Muon step — beside dgg_adam_l2 the optimiser for a
+ * network's hidden matrices (everything else stays with Adam).
+ * dgg_orthogonalize:  X_0 = in / (|in|_F + eps);  X <- a X + (b A + c A^2) X with A = X X^T (over the shorter side), `steps`
+ *   times with the k-th (a, b, c) of `coefficients` (host, steps x 3);  out = X.  in / out of one type (DGG_F32 / BF16 / F16);
+ *   a matrix taller than wide is treated as its transpose.  out may be in, of the same pitch and stride.
+ * dgg_muon_step (fp32, in place):  M <- momentum M + grad_scale G;  U = grad_scale G + momentum M (nesterov != 0) or M; W <-
+ *   (1 - lr weight_decay) W - lr f X,  X the orthogonalised U and f = sqrt(max(1, rows / cols)) (DGG_MUON_SPECTRAL) or 0.2
+ *   sqrt(max(rows, cols)) (DGG_MUON_MATCH_RMS: updates of Adam's size).  G = `in`, W = `out`, M = `momentum`.
+ * `mats` (host): any number of entries, each a stack of `batch` matrices of one shape; all of them share the launches (16
+ * entries at a time).  Rows lie ld_* >= cols elements apart, the matrices of a stack *_stride elements.  Operands are taken to
+ * 22 bits (two fp16 planes each) and products summed in fp32, for every type: errors of the size that fp32 products make.  A
+ * NaN or infinity makes its own matrix NaN, no other; a zero matrix stays zero (eps > 0).  What is written may overlap nothing
+ * else that the call reads or writes: DGG_ERR_INVALID (column blocks of one wider buffer and stacks whose matrices alternate
+ * are apart; layouts with no common pitch or stride have to lie one behind the other).  The coefficients must keep the
+ * iterates bounded for singular values in [0, 1]: DGG_ERR_INVALID otherwise.  Short side <= 16384, long side <= 2^20, a stack
+ * <= 2^32 elements and no more than a launch has threads for (2^32: 2^18 matrices of 1 x 16384 are too many): DGG_ERR_INVALID.
+ * ws: dgg_orthogonalize_workspace_bytes, 256-byte aligned, one per stream in flight. */
 typedef struct {
     const void* in;        /* device */
     void* out;             /* device */
