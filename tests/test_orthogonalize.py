@@ -590,3 +590,20 @@ def test_alternating_stacks_that_overlap_are_refused_without_a_gpu():
                 (dict(rows=1, out_stride=8), dict(rows=1, out=at + 28, out_stride=16))):
         assert call(*bad) == -1 and b"overlaps" in lib.dgg_last_error(), bad
         assert call(*bad[::-1]) == -1 and b"overlaps" in lib.dgg_last_error(), bad
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("shape,dtype", [((512, 4620), torch.bfloat16), ((24, 257, 771), torch.float32), ((512, 256), torch.float16), ((64, 4108), torch.float32),
+                                         ((12, 512), torch.float32)], ids=["wide bf16", "stack f32", "tall f16", "narrow f32", "small f32"])
+def test_a_call_repeats_itself_bit_for_bit(shape, dtype):
+    """No result depends on the order of workgroups or on what a workspace held before, beside another stream's work."""
+    g = torch.randn(shape, generator=torch.Generator().manual_seed(7)).to(dtype).cuda()
+    want = ops.orthogonalize(g)
+    side, a = torch.cuda.Stream(), torch.randn(1024, 1024, device="cuda")
+    side.wait_stream(torch.cuda.current_stream())
+    for k in range(20):
+        with torch.cuda.stream(side):
+            a = a @ a.clamp(-1e-3, 1e-3)
+        torch.full((1 << (14 + k % 12),), float("nan"), device="cuda")      # what the allocator hands out next
+        assert torch.equal(ops.orthogonalize(g), want), k
+    torch.cuda.synchronize()
